@@ -1,0 +1,418 @@
+// Pages of a cache: token rows into pages and back, rows copied in the pools of many layers at once, and the bookkeeping
+// of forked, freed and compacted sequences (gfx950).  Everything here moves bytes or counts: the copies are bound by HBM,
+// the bookkeeping by the latency of a launch.
+//
+// The bookkeeping is deterministic: ranks come from scans in index order, reference counts from commutative integer
+// updates.  Parts that need an order over all pages run in one workgroup (a scan over 4096 pages is one step of it); what
+// follows from their result (table rows, page copies) runs over the whole chip in a second launch.
+#include "common.h"
+
+namespace kda355 {
+namespace {
+
+constexpr int ROW = KDA355_LATENT_ROW, LAT = KDA355_LATENT_DIM;
+constexpr int ROW_Q = ROW / 8, LAT_Q = LAT / 8;  // 16-byte pieces of a cache row, of its latent part
+constexpr int TOK_THREADS = 256;
+constexpr int SCAN_THREADS = 1024;
+constexpr int COPY_THREADS = 256, COPY_PER = 4;   // 16 KiB a workgroup
+constexpr int MAX_PAIRS = 1 << 23;                // rows of a launch: 256 threads each, below 2^32 in all
+constexpr int FREED = INT32_MIN;                  // count of a page freed in this call, until the stack has it
+
+// ------------------------------------------------------------------------------------------------ token rows
+__global__ void __launch_bounds__(TOK_THREADS) append_kernel(KdaLatentTokensArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * TOK_THREADS + threadIdx.x;
+    const int64_t t = i / ROW_Q;
+    const int c = (int)(i - t * ROW_Q);
+    if (t >= a.T) return;
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.pages * a.page_size) return;
+    const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+    const uint16_t* src = c < LAT_Q ? static_cast<const uint16_t*>(a.latent) + t * a.latent_row + c * 8
+                                    : static_cast<const uint16_t*>(a.k_pe) + t * a.pe_row + (c - LAT_Q) * 8;
+    uint16_t* dst = static_cast<uint16_t*>(a.cache) + page * a.page_stride + off * ROW + c * 8;
+    *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
+}
+
+__global__ void __launch_bounds__(TOK_THREADS) gather_kernel(KdaLatentTokensArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * TOK_THREADS + threadIdx.x;
+    const int64_t t = i / ROW_Q;
+    const int c = (int)(i - t * ROW_Q);
+    if (t >= a.T) return;
+    int lo = 0, hi = a.N;  // the sequence of row t: the last n with cu[n] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= t) lo = mid; else hi = mid;
+    }
+    if (t < a.cu[lo] || t >= a.cu[lo + 1]) return;
+    const int64_t j = t - a.cu[lo], p = j / a.page_size;
+    u32x4 x = {0, 0, 0, 0};
+    if (p < a.table_width) {
+        const int64_t page = a.block_table[lo * a.table_stride + p];
+        if (page >= 0 && page < a.pages)
+            x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.cache) + page * a.page_stride +
+                                                (j - p * a.page_size) * ROW + c * 8);
+    }
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + t * a.out_row + c * 8) = x;
+}
+
+// ------------------------------------------------------------------------------------------------ row copies
+// one 16 KiB segment of row src -> row dst of one pool
+__device__ __forceinline__ void copy_segment(const KdaPool& p, int64_t src, int64_t dst, int seg) {
+    if (src < 0 || src >= p.slots || dst < 0 || dst >= p.slots || src == dst) return;
+    const char* s = static_cast<const char*>(p.base) + src * p.slot_stride;
+    char* d = static_cast<char*>(p.base) + dst * p.slot_stride;
+    const int64_t b0 = (int64_t)seg * COPY_THREADS * COPY_PER * 16 + threadIdx.x * 16;
+    u32x4 x[COPY_PER];
+#pragma unroll
+    for (int i = 0; i < COPY_PER; ++i) {
+        const int64_t b = b0 + i * COPY_THREADS * 16;
+        if (b < p.row_bytes) x[i] = *reinterpret_cast<const u32x4*>(s + b);
+    }
+#pragma unroll
+    for (int i = 0; i < COPY_PER; ++i) {
+        const int64_t b = b0 + i * COPY_THREADS * 16;
+        if (b < p.row_bytes) *reinterpret_cast<u32x4*>(d + b) = x[i];
+    }
+}
+
+__global__ void __launch_bounds__(COPY_THREADS) copy_rows_kernel(KdaPagesArgs a) {
+    copy_segment(a.pool[blockIdx.z], a.src[blockIdx.x], a.dst[blockIdx.x], blockIdx.y);
+}
+
+// ------------------------------------------------------------------------------------------------ scans
+// exclusive prefix sum over the workgroup's threads; total in every thread
+__device__ __forceinline__ int block_scan(int x, int* sw, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int s = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(s, d);
+        if (lane >= d) s += y;
+    }
+    __syncthreads();  // sw free again
+    if (lane == 63) sw[w] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < SCAN_THREADS / 64; ++i) {
+        const int v = sw[i];
+        if (i < w) before += v;
+        total += v;
+    }
+    return before + s - x;
+}
+
+// words that another thread of the workgroup wrote in this launch: past the vector L1
+__device__ __forceinline__ int load_fresh(const int32_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ------------------------------------------------------------------------------------------------ fork
+__device__ __forceinline__ int row_len(const KdaPagesArgs& a, int row) {
+    const int64_t most = (int64_t)a.table_width * a.page_size;
+    const int64_t n = a.seq_lens[row];
+    return (int)(n < 0 ? 0 : n > most ? most : n);
+}
+
+// pair i -> workspace[i] = page to copy from (-1: none), workspace[n + i] = page taken (-1: none needed, -2: no page
+// left, -3: pair skipped).  The stack and its height follow.
+__global__ void __launch_bounds__(SCAN_THREADS) fork_take_kernel(KdaPagesArgs a) {
+    __shared__ int sw[SCAN_THREADS / 64];
+    int top = a.num_free[0];
+    top = top < 0 ? 0 : top > a.pages ? a.pages : top;
+    int taken = 0;
+    for (int i0 = 0; i0 < a.n; i0 += SCAN_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int par = -1, len = 0, ok = 0, tail = 0;
+        if (i < a.n) {
+            par = a.src[i];
+            const int child = a.dst[i];
+            ok = par >= 0 && par < a.rows && child >= 0 && child < a.rows && par != child;
+            if (ok) len = row_len(a, par);
+            tail = ok && len % a.page_size != 0;
+        }
+        int total;
+        const int rank = taken + block_scan(tail, sw, total);
+        if (i < a.n) {
+            int from = -1, to = ok ? -1 : -3;
+            if (tail) {
+                to = -2;
+                if (rank < top) {
+                    const int page = a.free_pages[top - 1 - rank];
+                    a.free_pages[top - 1 - rank] = -1;
+                    if (page >= 0 && page < a.pages) {
+                        to = page;
+                        from = a.block_table[par * a.table_stride + len / a.page_size];
+                    }
+                }
+            }
+            a.workspace[i] = from;
+            a.workspace[a.n + i] = to;
+        }
+        taken += total;
+    }
+    if (threadIdx.x == 0) a.num_free[0] = top - (taken < top ? taken : top);
+}
+
+// blockIdx.z < num_pools: a segment of the copied page; the last z: the child's row of the table
+__global__ void __launch_bounds__(COPY_THREADS) fork_rows_kernel(KdaPagesArgs a) {
+    const int i = blockIdx.x;
+    const int to = a.workspace[a.n + i];
+    if ((int)blockIdx.z < a.num_pools) {
+        if (to >= 0) copy_segment(a.pool[blockIdx.z], a.workspace[i], to, blockIdx.y);
+        return;
+    }
+    if (blockIdx.y != 0 || to == -3) return;
+    const int par = a.src[i], child = a.dst[i];
+    const int len = to == -2 ? 0 : row_len(a, par);
+    const int full = len / a.page_size;
+    const int32_t* from = a.block_table + par * a.table_stride;
+    int32_t* row = a.block_table + child * a.table_stride;
+    for (int j = threadIdx.x; j < a.table_width; j += COPY_THREADS) {
+        int page = -1;
+        if (j < full) {
+            page = from[j];
+            if (page >= 0 && page < a.pages) atomicAdd(a.ref_counts + page, 1);
+        } else if (j == full && to >= 0) {
+            page = to;
+            a.ref_counts[page] = 1;
+        }
+        row[j] = page;
+    }
+    if (threadIdx.x == 0) a.seq_lens[child] = len;
+}
+
+// ------------------------------------------------------------------------------------------------ free
+__global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a) {
+    const int r = a.src[blockIdx.x];
+    if (r < 0 || r >= a.rows) return;
+    const int used = (row_len(a, r) + a.page_size - 1) / a.page_size;
+    int32_t* row = a.block_table + r * a.table_stride;
+    for (int j = threadIdx.x; j < a.table_width; j += COPY_THREADS) {
+        const int page = row[j];
+        if (j < used && page >= 0 && page < a.pages) {
+            int32_t* ref = a.ref_counts + page;
+            int cur = load_fresh(ref);
+            while (cur > 0) {  // the last holder marks the page; a count already at zero stays
+                const int seen = atomicCAS(ref, cur, cur == 1 ? FREED : cur - 1);
+                if (seen == cur) break;
+                cur = seen;
+            }
+        }
+        row[j] = -1;
+    }
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) a.seq_lens[r] = 0;
+}
+
+__global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a) {
+    __shared__ int sw[SCAN_THREADS / 64];
+    int top = a.num_free[0];
+    top = top < 0 ? 0 : top > a.pages ? a.pages : top;
+    for (int hi = a.pages; hi > 0; hi -= 4 * SCAN_THREADS) {  // four pages a thread, the highest first
+        int mine[4], count = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = hi - 1 - 4 * (int)threadIdx.x - k;
+            mine[k] = p >= 0 && a.ref_counts[p] == FREED;
+            count += mine[k];
+        }
+        int total;
+        int at = top + block_scan(count, sw, total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (mine[k]) {
+                const int p = hi - 1 - 4 * (int)threadIdx.x - k;
+                a.ref_counts[p] = 0;
+                if (at < a.pages) a.free_pages[at] = p;
+                ++at;
+            }
+        top += total;
+    }
+    if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
+}
+
+// ------------------------------------------------------------------------------------------------ compact
+// workspace: remap [pages] | sources [pages / 2] | destinations [pages / 2], padded with -1
+__global__ void __launch_bounds__(SCAN_THREADS) compact_plan_kernel(KdaPagesArgs a) {
+    __shared__ int sw[SCAN_THREADS / 64];
+    const int pages = a.pages, half = pages / 2;
+    int32_t* remap = a.workspace;
+    int32_t* msrc = remap + pages;
+    int32_t* mdst = msrc + half;
+    int mine = 0, live;
+    for (int p = threadIdx.x; p < pages; p += SCAN_THREADS) mine += a.ref_counts[p] > 0;
+    block_scan(mine, sw, live);
+    int holes = 0, movers = 0;
+    for (int p0 = 0; p0 < pages; p0 += SCAN_THREADS) {
+        const int p = p0 + threadIdx.x;
+        const bool held = p < pages && a.ref_counts[p] > 0;
+        const int hole = p < live && !held, mover = held && p >= live;  // (live <= pages)
+        int total;
+        const int rank = block_scan(hole | (mover << 16), sw, total);  // at most 1024 of either in a step
+        if (hole) mdst[holes + (rank & 0xffff)] = p;
+        if (mover) msrc[movers + (rank >> 16)] = p;
+        if (p < pages) remap[p] = p;
+        holes += total & 0xffff;
+        movers += total >> 16;
+    }
+    __syncthreads();  // the lists are written (holes == movers, at most pages / 2)
+    for (int i = threadIdx.x; i < half; i += SCAN_THREADS) {
+        if (i < movers) {
+            const int s = load_fresh(msrc + i), d = load_fresh(mdst + i);
+            remap[s] = d;
+            a.ref_counts[d] = a.ref_counts[s];
+            a.ref_counts[s] = 0;
+        } else {
+            msrc[i] = -1;
+            mdst[i] = -1;
+        }
+    }
+    for (int j = threadIdx.x; j < pages; j += SCAN_THREADS) a.free_pages[j] = j < pages - live ? pages - 1 - j : -1;
+    if (threadIdx.x == 0) a.num_free[0] = pages - live;
+}
+
+__global__ void __launch_bounds__(COPY_THREADS) compact_move_kernel(KdaPagesArgs a) {
+    const int half = a.pages / 2;
+    if ((int)blockIdx.z < a.num_pools) {
+        if ((int)blockIdx.x >= half) return;
+        copy_segment(a.pool[blockIdx.z], a.workspace[a.pages + blockIdx.x], a.workspace[a.pages + half + blockIdx.x],
+                     blockIdx.y);
+        return;
+    }
+    if (blockIdx.y != 0) return;
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
+        for (int j = threadIdx.x; j < a.table_width; j += COPY_THREADS) {
+            int32_t* e = a.block_table + r * a.table_stride + j;
+            const int page = *e;
+            if (page >= 0 && page < a.pages) *e = a.workspace[page];
+        }
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
+    return KDA355_ELAUNCH;
+}
+
+int check_tokens(const KdaLatentTokensArgs* a, const char* what) {
+    KDA_CHECK_ARG(a != nullptr, "%s: null args", what);
+    KDA_CHECK_ARG(a->T >= 0 && a->pages >= 1 && a->page_size >= 1, "%s: T=%lld pages=%lld page_size=%d", what,
+                  (long long)a->T, (long long)a->pages, a->page_size);
+    KDA_CHECK_ARG(a->T < (1ll << 25), "%s: %lld token rows in one call (less than 2^25)", what, (long long)a->T);
+    KDA_CHECK_ARG(a->cache, "%s: a required pointer is null", what);
+    KDA_CHECK_ARG(aligned(a->cache, 16) && a->page_stride % 8 == 0 && a->page_stride >= (int64_t)a->page_size * ROW,
+                  "%s: cache pages must be dense and 16-byte aligned", what);
+    return 0;
+}
+
+// segments of the longest row; every pool checked
+int check_pools(const KdaPagesArgs* a, const char* what, int* segs) {
+    KDA_CHECK_ARG(a->num_pools >= 0 && a->num_pools <= KDA355_MAX_POOLS, "%s: num_pools=%d", what, a->num_pools);
+    int64_t most = 0;
+    for (int i = 0; i < a->num_pools; ++i) {
+        const KdaPool& p = a->pool[i];
+        KDA_CHECK_ARG(p.base && p.slots >= 0, "%s: pool %d is empty", what, i);
+        KDA_CHECK_ARG(aligned(p.base, 16) && p.row_bytes > 0 && p.row_bytes % 16 == 0 && p.slot_stride % 16 == 0 &&
+                          p.slot_stride >= p.row_bytes,
+                      "%s: the rows of pool %d must be 16-byte aligned and a multiple of 16 bytes", what, i);
+        most = p.row_bytes > most ? p.row_bytes : most;
+    }
+    const int64_t per = COPY_THREADS * COPY_PER * 16, n = (most + per - 1) / per;
+    KDA_CHECK_ARG(n <= 65535, "%s: rows of %lld bytes are too long", what, (long long)most);
+    *segs = n < 1 ? 1 : (int)n;
+    return 0;
+}
+
+int check_table(const KdaPagesArgs* a, const char* what, bool lens) {
+    KDA_CHECK_ARG(a->rows >= 1 && a->table_width >= 1 && a->pages >= 1 && a->pages < 2 * MAX_PAIRS && a->page_size >= 1,
+                  "%s: rows=%d table_width=%d pages=%d page_size=%d", what, a->rows, a->table_width, a->pages, a->page_size);
+    KDA_CHECK_ARG((int64_t)a->table_width * a->page_size < (1ll << 31), "%s: a table row spans 2^31 tokens or more", what);
+    KDA_CHECK_ARG(a->table_stride >= a->table_width, "%s: table_stride < table_width", what);
+    KDA_CHECK_ARG(a->block_table && a->ref_counts && a->free_pages && a->num_free && (!lens || a->seq_lens),
+                  "%s: a required pointer is null", what);
+    return 0;
+}
+
+}  // namespace
+}  // namespace kda355
+
+using namespace kda355;
+
+extern "C" int kda355_latent_append_launch(const KdaLatentTokensArgs* a, kda355_stream_t stream) {
+    if (const int rc = check_tokens(a, "latent_append")) return rc;
+    if (a->T == 0) return 0;
+    KDA_CHECK_ARG(a->latent && a->k_pe && a->slots, "latent_append: a required pointer is null");
+    KDA_CHECK_ARG(aligned(a->latent, 16) && aligned(a->k_pe, 16) && a->latent_row % 8 == 0 && a->pe_row % 8 == 0,
+                  "latent_append: latent and k_pe rows must be 16-byte aligned");
+    const int64_t wgs = (a->T * ROW_Q + TOK_THREADS - 1) / TOK_THREADS;
+    hipLaunchKernelGGL(append_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
+    return launched("latent_append");
+}
+
+extern "C" int kda355_latent_gather_launch(const KdaLatentTokensArgs* a, kda355_stream_t stream) {
+    if (const int rc = check_tokens(a, "latent_gather")) return rc;
+    if (a->T == 0 || a->N == 0) return 0;
+    KDA_CHECK_ARG(a->N > 0 && a->table_width >= 1 && a->table_stride >= a->table_width, "latent_gather: N=%d table_width=%d",
+                  a->N, a->table_width);
+    KDA_CHECK_ARG(a->block_table && a->cu && a->out, "latent_gather: a required pointer is null");
+    KDA_CHECK_ARG(aligned(a->out, 16) && a->out_row % 8 == 0, "latent_gather: out rows must be 16-byte aligned");
+    const int64_t wgs = (a->T * ROW_Q + TOK_THREADS - 1) / TOK_THREADS;
+    hipLaunchKernelGGL(gather_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
+    return launched("latent_gather");
+}
+
+extern "C" int kda355_copy_rows_launch(const KdaPagesArgs* a, kda355_stream_t stream) {
+    KDA_CHECK_ARG(a != nullptr, "copy_rows: null args");
+    int segs;
+    if (const int rc = check_pools(a, "copy_rows", &segs)) return rc;
+    KDA_CHECK_ARG(a->n >= 0 && a->n < MAX_PAIRS, "copy_rows: n=%d", a->n);
+    if (a->n == 0 || a->num_pools == 0) return 0;
+    KDA_CHECK_ARG(a->src && a->dst, "copy_rows: a required pointer is null");
+    hipLaunchKernelGGL(copy_rows_kernel, dim3(a->n, segs, a->num_pools), dim3(COPY_THREADS), 0,
+                       reinterpret_cast<hipStream_t>(stream), *a);
+    return launched("copy_rows");
+}
+
+extern "C" int kda355_fork_pages_launch(const KdaPagesArgs* a, kda355_stream_t stream) {
+    KDA_CHECK_ARG(a != nullptr, "fork_pages: null args");
+    int segs;
+    if (const int rc = check_pools(a, "fork_pages", &segs)) return rc;
+    if (const int rc = check_table(a, "fork_pages", true)) return rc;
+    KDA_CHECK_ARG(a->n >= 0 && a->n < MAX_PAIRS, "fork_pages: n=%d", a->n);
+    if (a->n == 0) return 0;
+    KDA_CHECK_ARG(a->src && a->dst && a->workspace, "fork_pages: a required pointer is null");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(fork_take_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+    hipLaunchKernelGGL(fork_rows_kernel, dim3(a->n, segs, a->num_pools + 1), dim3(COPY_THREADS), 0, s, *a);
+    return launched("fork_pages");
+}
+
+extern "C" int kda355_free_pages_launch(const KdaPagesArgs* a, kda355_stream_t stream) {
+    KDA_CHECK_ARG(a != nullptr, "free_pages: null args");
+    if (const int rc = check_table(a, "free_pages", true)) return rc;
+    KDA_CHECK_ARG(a->n >= 0 && a->n < MAX_PAIRS, "free_pages: n=%d", a->n);
+    if (a->n == 0) return 0;
+    KDA_CHECK_ARG(a->src, "free_pages: a required pointer is null");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(free_rows_kernel, dim3(a->n), dim3(COPY_THREADS), 0, s, *a);
+    hipLaunchKernelGGL(free_push_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+    return launched("free_pages");
+}
+
+extern "C" int kda355_compact_pages_launch(const KdaPagesArgs* a, kda355_stream_t stream) {
+    KDA_CHECK_ARG(a != nullptr, "compact_pages: null args");
+    int segs;
+    if (const int rc = check_pools(a, "compact_pages", &segs)) return rc;
+    if (const int rc = check_table(a, "compact_pages", false)) return rc;
+    KDA_CHECK_ARG(a->workspace, "compact_pages: a required pointer is null");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+    const int half = a->pages / 2;
+    hipLaunchKernelGGL(compact_move_kernel, dim3(half < 1 ? 1 : half, segs, a->num_pools + 1), dim3(COPY_THREADS), 0, s, *a);
+    return launched("compact_pages");
+}

@@ -93,6 +93,51 @@ class KdaPrefillArgs(ctypes.Structure):
     ]
 
 
+class KdaLatentPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", P), ("k", P), ("v", P), ("k_pe", P), ("out", P), ("lse", P), ("cu_q", P), ("cu_k", P),
+        ("q_row", I64), ("q_head", I64), ("k_row", I64), ("k_head", I64), ("v_row", I64), ("v_head", I64),
+        ("pe_row", I64), ("out_row", I64), ("out_head", I64), ("Tq", I64), ("Tk", I64),
+        ("N", I32), ("H", I32), ("dtype", I32), ("flags", U32), ("scale", F32), ("reserved", I32),
+    ]
+
+
+class KdaLatentDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_latent", P), ("q_pe", P), ("cache", P), ("block_table", P), ("seq_lens", P), ("prefix_table", P),
+        ("prefix_len", P), ("out", P), ("lse", P), ("workspace", P),
+        ("ql_row", I64), ("ql_head", I64), ("qp_row", I64), ("qp_head", I64), ("out_row", I64), ("out_head", I64),
+        ("page_stride", I64), ("pages", I64), ("table_stride", I64), ("workspace_bytes", I64),
+        ("B", I32), ("S", I32), ("H", I32), ("page_size", I32), ("table_width", I32), ("prefix_width", I32),
+        ("dtype", I32), ("num_cus", I32), ("scale", F32), ("flags", U32),
+    ]
+
+
+class KdaLatentTokensArgs(ctypes.Structure):
+    _fields_ = [
+        ("latent", P), ("k_pe", P), ("cache", P), ("slots", P), ("block_table", P), ("cu", P), ("out", P),
+        ("latent_row", I64), ("pe_row", I64), ("out_row", I64), ("page_stride", I64), ("pages", I64),
+        ("table_stride", I64), ("T", I64),
+        ("page_size", I32), ("table_width", I32), ("N", I32), ("reserved", I32),
+    ]
+
+
+class KdaPool(ctypes.Structure):
+    _fields_ = [("base", P), ("row_bytes", I64), ("slot_stride", I64), ("slots", I64)]
+
+
+MAX_POOLS = 24  # KDA355_MAX_POOLS
+
+
+class KdaPagesArgs(ctypes.Structure):
+    _fields_ = [
+        ("pool", KdaPool * MAX_POOLS), ("num_pools", I32), ("n", I32),
+        ("src", P), ("dst", P), ("block_table", P), ("seq_lens", P), ("ref_counts", P), ("free_pages", P),
+        ("num_free", P), ("workspace", P), ("table_stride", I64),
+        ("rows", I32), ("table_width", I32), ("pages", I32), ("page_size", I32),
+    ]
+
+
 _lib = None
 _noalloc = None
 
@@ -117,6 +162,15 @@ def lib():
         L.kda355_prefill_workspace_bytes.restype = I64
         L.kda355_prefill_launch.argtypes = [ctypes.POINTER(KdaPrefillArgs), P]
         L.kda355_prefill_launch.restype = ctypes.c_int
+        for name, args in (("latent_prefill", KdaLatentPrefillArgs), ("latent_decode", KdaLatentDecodeArgs),
+                           ("latent_append", KdaLatentTokensArgs), ("latent_gather", KdaLatentTokensArgs),
+                           ("copy_rows", KdaPagesArgs), ("fork_pages", KdaPagesArgs), ("free_pages", KdaPagesArgs),
+                           ("compact_pages", KdaPagesArgs)):
+            f = getattr(L, f"kda355_{name}_launch")
+            f.argtypes = [ctypes.POINTER(args), P]
+            f.restype = ctypes.c_int
+        L.kda355_latent_decode_workspace_bytes.argtypes = [ctypes.POINTER(KdaLatentDecodeArgs)]
+        L.kda355_latent_decode_workspace_bytes.restype = I64
         L.kda355_last_error.restype = ctypes.c_char_p
         L.kda355_version.restype = ctypes.c_int
         _lib = L
@@ -152,6 +206,9 @@ def exported_symbols():
     """Names declared in include/kda355.h that the library must export."""
     return ["kda355_recurrent_launch", "kda355_spec_commit_launch", "kda355_decode_launch", "kda355_prefill_plan",
             "kda355_prefill_workspace_bytes", "kda355_prefill_launch", "kda355_prefill_launch_noalloc",
+            "kda355_latent_prefill_launch", "kda355_latent_decode_workspace_bytes", "kda355_latent_decode_launch",
+            "kda355_latent_append_launch", "kda355_latent_gather_launch", "kda355_copy_rows_launch",
+            "kda355_fork_pages_launch", "kda355_free_pages_launch", "kda355_compact_pages_launch",
             "kda355_last_error", "kda355_version"]
 
 

@@ -1,0 +1,231 @@
+"""Latent attention and its paged cache (host side of kda355_latent_*): the attention layers that stand between the KDA
+layers of a hybrid model.  No counterpart in the reference, which holds KDA layers only.
+
+Every token leaves one latent vector of 512 values and a positional part of 64 that all heads share (rotated or not, as the
+model has it).  A cache is [pages, page_size, 576] bf16 or fp16: token rows (latent | positional part) dense within a page,
+any page stride; page numbers outside the cache are holes whose tokens take no part.
+
+    latent_append(latent, k_pe, cache, slots)                              # token rows into their pages
+    rows = latent_gather(cache, block_table, cu_seqlens, out)              # and back, dense
+    o = latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k)          # expanded form, packed sequences
+    o = latent_decode(q_latent, q_pe, cache, block_table, seq_lens)        # absorbed form, S tokens a sequence
+    o = latent_decode(..., prefix_table=pages, prefix_len=n)               # the same behind one shared prefix
+
+The expanded form takes keys and values as the up-projection leaves them (views with any token and head stride), the
+absorbed form queries that carry the key up-projection, and returns outputs in the latent space.  The default scale is
+192^-1/2 for both.  Lengths and tables stay on the device: nothing is read back, so every call can be captured in a HIP
+graph and replayed with other lengths, tables and data.
+
+Errors: TypeError for a wrong dtype or device, ValueError for a wrong shape or stride.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .recurrent import _need
+
+LATENT, PE, HEAD = 512, 64, 128
+ROW = LATENT + PE
+SCALE = (HEAD + PE) ** -0.5
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_cus = {}
+
+
+def _stream(device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _num_cus(device):
+    n = _cus.get(device)
+    if n is None:
+        n = _cus[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
+
+
+def _first(name, t):
+    """(device, dtype) of the tensor that the others have to match."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"kda355: {name} must be a tensor")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"kda355: {name} must be bfloat16 or float16, got {t.dtype}")
+    if t.device.type != "cuda":
+        raise TypeError("kda355: tensors must be on a GPU")
+    return t.device, t.dtype
+
+
+def _rows(name, t, shape, dtype, device):
+    """The tensor has this shape and a dense last dimension; returns its other strides."""
+    _need(name, t, dtype, device)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"kda355: {name} must be {list(shape)}, got {list(t.shape)}")
+    st = t.stride()
+    if shape[-1] > 1 and st[-1] != 1:
+        raise ValueError(f"kda355: the last dimension of {name} must be dense")
+    # the stride of a dimension of one is never used: any value is valid there, odd ones too
+    return [s if n > 1 else 0 for s, n in zip(st[:-1], shape)]
+
+
+def _index(name, t, shape, device, dtype=torch.int32):
+    _need(name, t, dtype, device)
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"kda355: {name} must be a contiguous {dtype} {list(shape)} tensor, got {list(t.shape)}")
+
+
+def _table(name, t, device):
+    """Row stride of a [rows, width] int32 page table with dense rows."""
+    _need(name, t, torch.int32, device)
+    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"kda355: {name} must be [rows, width >= 1] with dense rows, got {list(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _cache(cache, dtype, device):
+    """(pages, page_size, page stride) of a cache."""
+    _need("cache", cache, dtype, device)
+    if cache.dim() != 3 or cache.shape[2] != ROW or cache.shape[0] < 1 or cache.shape[1] < 1:
+        raise ValueError(f"kda355: cache must be [pages, page_size, {ROW}], got {list(cache.shape)}")
+    pages, size, _ = cache.shape
+    if cache.stride(2) != 1 or (size > 1 and cache.stride(1) != ROW):
+        raise ValueError("kda355: cache must be dense within a page")
+    return pages, size, cache.stride(0) if pages > 1 else size * ROW
+
+
+def _lse_ptr(lse, shape, device):
+    if lse is None:
+        return None
+    _index("lse", lse, shape, device, torch.float32)
+    return lse.data_ptr()
+
+
+def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal=True, *, out=None, lse=None):
+    """The expanded form over packed sequences: q [Tq, H, 192] (128 | 64), k and v [Tk, H, 128], k_pe [Tk, 64] shared by the
+    heads.  cu_seqlens_q / cu_seqlens_k int32 [N + 1] on the device; the queries are the last tokens of their sequences, so
+    with `causal` query i of Lq sees keys j <= i + Lk - Lq.  Returns out [Tq, H, 128]; `lse` (fp32 [Tq, H]) receives the
+    logarithms of the softmax sums, for joining with the attention over other keys.  A query that sees no key gets zeros and
+    -inf, and keys it does not see never reach it, whatever they hold."""
+    dev, dt = _first("q", q)
+    if q.dim() != 3 or q.shape[2] != HEAD + PE:
+        raise ValueError(f"kda355: q must be [Tq, H, {HEAD + PE}], got {list(q.shape)}")
+    Tq, H = q.shape[0], q.shape[1]
+    Tk = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else 0
+    q_st = _rows("q", q, (Tq, H, HEAD + PE), dt, dev)
+    k_st = _rows("k", k, (Tk, H, HEAD), dt, dev)
+    v_st = _rows("v", v, (Tk, H, HEAD), dt, dev)
+    pe_st = _rows("k_pe", k_pe, (Tk, PE), dt, dev)
+    N = cu_seqlens_q.numel() - 1 if isinstance(cu_seqlens_q, torch.Tensor) else 0
+    if isinstance(cu_seqlens_q, torch.Tensor) and N < 0:
+        raise ValueError("kda355: cu_seqlens_q must have at least one entry")
+    _index("cu_seqlens_q", cu_seqlens_q, (N + 1,), dev)
+    _index("cu_seqlens_k", cu_seqlens_k, (N + 1,), dev)
+    if out is None:
+        out = torch.empty(Tq, H, HEAD, dtype=dt, device=dev)
+    o_st = _rows("out", out, (Tq, H, HEAD), dt, dev)
+    a = _lib.KdaLatentPrefillArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(), _lse_ptr(lse, (Tq, H), dev),
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *q_st, *k_st, *v_st, *pe_st, *o_st, Tq, Tk, N, H, _DTYPES[dt],
+        1 if causal else 0, SCALE if scale is None else float(scale), 0)
+    _lib.check(_lib.lib().kda355_latent_prefill_launch(ctypes.byref(a), _stream(dev)), "latent_prefill")
+    return out
+
+
+def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, out=None, lse=None, prefix_table=None,
+                  prefix_len=None, workspace=None):
+    """The absorbed form over the paged cache: q_latent [B * S, H, 512] and q_pe [B * S, H, 64], S tokens a sequence (row
+    n * S + s), block_table int32 [B, width], seq_lens int32 [B] the cached tokens of each sequence, its S new ones among
+    them (token s sees j < seq_lens[n] - (S - 1 - s)).  Returns out [B * S, H, 512] in the latent space; `lse` (fp32
+    [B * S, H]) as in latent_prefill.
+
+    prefix_table (int32 [width]) and prefix_len (int32 [1]) name the pages of a prefix that all B sequences share and see in
+    front of their own tokens; it is read once for the whole batch.  block_table and seq_lens then hold what follows it.
+
+    workspace: uint8 tensor of latent_decode_workspace_bytes(...); by default one is taken from torch's allocator for the
+    call.  Calls that may overlap need workspaces of their own."""
+    dev, dt = _first("q_latent", q_latent)
+    if q_latent.dim() != 3 or q_latent.shape[2] != LATENT:
+        raise ValueError(f"kda355: q_latent must be [B * S, H, {LATENT}], got {list(q_latent.shape)}")
+    T, H = q_latent.shape[0], q_latent.shape[1]
+    ql_st = _rows("q_latent", q_latent, (T, H, LATENT), dt, dev)
+    qp_st = _rows("q_pe", q_pe, (T, H, PE), dt, dev)
+    pages, size, page_stride = _cache(cache, dt, dev)
+    table_stride = _table("block_table", block_table, dev)
+    B = block_table.shape[0]
+    _index("seq_lens", seq_lens, (B,), dev)
+    if T % B if B else T:
+        raise ValueError(f"kda355: {T} rows of q_latent are not B x S for B = {B}")
+    S = max(1, T // B) if B else 1
+    if B and T < B:
+        raise ValueError("kda355: q_latent must hold at least one token a sequence")
+    width = 0
+    if (prefix_table is None) != (prefix_len is None):
+        raise ValueError("kda355: pass prefix_table and prefix_len together")
+    if prefix_table is not None:
+        width = prefix_table.numel() if isinstance(prefix_table, torch.Tensor) else 0
+        _index("prefix_table", prefix_table, (max(1, width),), dev)
+        _index("prefix_len", prefix_len, (1,), dev)
+    if out is None:
+        out = torch.empty(T, H, LATENT, dtype=dt, device=dev)
+    o_st = _rows("out", out, (T, H, LATENT), dt, dev)
+    a = _lib.KdaLatentDecodeArgs(
+        q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        prefix_table.data_ptr() if width else None, prefix_len.data_ptr() if width else None, out.data_ptr(),
+        _lse_ptr(lse, (T, H), dev), None, *ql_st, *qp_st, *o_st, page_stride, pages, table_stride, 0, B, S, H, size,
+        block_table.shape[1], width, _DTYPES[dt], _num_cus(dev), SCALE if scale is None else float(scale), 0)
+    L = _lib.lib()
+    need = L.kda355_latent_decode_workspace_bytes(ctypes.byref(a))
+    if need < 0:
+        _lib.check(int(need), "latent_decode")
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    else:
+        _need("workspace", workspace, torch.uint8, dev)
+        if not workspace.is_contiguous() or workspace.numel() < need:
+            raise ValueError(f"kda355: workspace must be contiguous with >= {need} bytes")
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _lib.check(L.kda355_latent_decode_launch(ctypes.byref(a), _stream(dev)), "latent_decode")
+    return out
+
+
+def latent_decode_workspace_bytes(B, S, H, page_size, table_width, prefix_width=0, *, num_cus=256):
+    """Bytes of device workspace that latent_decode() needs for these sizes (host only)."""
+    a = _lib.KdaLatentDecodeArgs(B=B, S=S, H=H, page_size=page_size, table_width=table_width, prefix_width=prefix_width,
+                                 num_cus=num_cus)
+    need = _lib.lib().kda355_latent_decode_workspace_bytes(ctypes.byref(a))
+    if need < 0:
+        _lib.check(int(need), "latent_decode_workspace_bytes")
+    return int(need)
+
+
+def latent_append(latent, k_pe, cache, slots):
+    """cache row slots[t] (= page * page_size + offset, int64 [T]) <- latent [T, 512] | k_pe [T, 64]; slots outside the cache
+    (padding: -1) are skipped.  The cache is written in place and returned."""
+    dev, dt = _first("latent", latent)
+    T = latent.shape[0] if latent.dim() else 0
+    l_st = _rows("latent", latent, (T, LATENT), dt, dev)
+    p_st = _rows("k_pe", k_pe, (T, PE), dt, dev)
+    pages, size, page_stride = _cache(cache, dt, dev)
+    _index("slots", slots, (T,), dev, torch.int64)
+    a = _lib.KdaLatentTokensArgs(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), None, None, None,
+                                 *l_st, *p_st, 0, page_stride, pages, 0, T, size, 0, 0, 0)
+    _lib.check(_lib.lib().kda355_latent_append_launch(ctypes.byref(a), _stream(dev)), "latent_append")
+    return cache
+
+
+def latent_gather(cache, block_table, cu_seqlens, out):
+    """out [T, 576] row cu_seqlens[n] + j <- token j of sequence n (block_table int32 [N, width], cu_seqlens int32 [N + 1] on
+    the device); tokens in holes or past the table give zero rows, rows of `out` past the last sequence stay as they are."""
+    dev, dt = _first("cache", cache)
+    pages, size, page_stride = _cache(cache, dt, dev)
+    table_stride = _table("block_table", block_table, dev)
+    N = block_table.shape[0]
+    _index("cu_seqlens", cu_seqlens, (N + 1,), dev)
+    T = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() else 0
+    o_st = _rows("out", out, (T, ROW), dt, dev)
+    a = _lib.KdaLatentTokensArgs(None, None, cache.data_ptr(), None, block_table.data_ptr(), cu_seqlens.data_ptr(),
+                                 out.data_ptr(), 0, 0, *o_st, page_stride, pages, table_stride, T, size,
+                                 block_table.shape[1], N, 0)
+    _lib.check(_lib.lib().kda355_latent_gather_launch(ctypes.byref(a), _stream(dev)), "latent_gather")
+    return out

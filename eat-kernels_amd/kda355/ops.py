@@ -17,6 +17,9 @@ registered ops with mutation annotations and fake implementations instead of opa
   fused_recurrent_kda  vLLM's fused_recurrent_kda on a state pool as the Kimi layer calls it
                        (kda/mi350x/benchmark/vllm_reference/kda.py:488-502).
   spec_commit          copies each sequence's accepted per-token state into its pool row.
+  latent_*             latent attention and its paged cache (kda355/latent.py), `out` given by the caller.
+  copy_rows, fork_pages, free_pages, compact_pages
+                       pages of a cache (kda355/pages.py).
 
 Every op is implemented for the CUDA dispatch key only and calls the HIP kernels of libkda355.so; on CPU tensors the
 dispatcher raises.  Importing this module registers the ops once per process.
@@ -33,6 +36,8 @@ from .decode import decode as _decode_fn, decode_batch as _decode_batch
 # looked up by their full names
 _prefill = importlib.import_module(__package__ + ".prefill")
 _recurrent = importlib.import_module(__package__ + ".recurrent")
+_latent = importlib.import_module(__package__ + ".latent")
+_pages = importlib.import_module(__package__ + ".pages")
 
 D = 128
 NAMESPACE = "kda355"
@@ -66,6 +71,28 @@ SCHEMAS = {
     "spec_commit":
         "spec_commit(Tensor scratch, Tensor scratch_indices, Tensor(a!) pool, Tensor pool_indices, "
         "Tensor num_accepted_tokens, bool slot0_reserved=True) -> ()",
+    "latent_prefill":
+        "latent_prefill(Tensor q, Tensor k, Tensor v, Tensor k_pe, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
+        "Tensor(a!) out, float? scale=None, bool causal=True, Tensor(b!)? lse=None) -> ()",
+    "latent_decode":
+        "latent_decode(Tensor q_latent, Tensor q_pe, Tensor cache, Tensor block_table, Tensor seq_lens, "
+        "Tensor(a!) out, float? scale=None, Tensor(b!)? lse=None, Tensor? prefix_table=None, "
+        "Tensor? prefix_len=None, Tensor(c!)? workspace=None) -> ()",
+    "latent_append":
+        "latent_append(Tensor latent, Tensor k_pe, Tensor(a!) cache, Tensor slots) -> ()",
+    "latent_gather":
+        "latent_gather(Tensor cache, Tensor block_table, Tensor cu_seqlens, Tensor(a!) out) -> ()",
+    "copy_rows":
+        "copy_rows(Tensor(a!)[] pools, Tensor src, Tensor dst) -> ()",
+    "fork_pages":
+        "fork_pages(Tensor(a!)[] pools, Tensor(b!) block_table, Tensor(c!) seq_lens, Tensor(d!) ref_counts, "
+        "Tensor(e!) free_pages, Tensor(f!) num_free, Tensor parents, Tensor children, int page_size) -> ()",
+    "free_pages":
+        "free_pages(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor(c!) ref_counts, Tensor(d!) free_pages, "
+        "Tensor(e!) num_free, Tensor rows, int page_size) -> ()",
+    "compact_pages":
+        "compact_pages(Tensor(a!)[] pools, Tensor(b!) block_table, Tensor(c!) ref_counts, Tensor(d!) free_pages, "
+        "Tensor(e!) num_free) -> ()",
 }
 
 
@@ -203,6 +230,24 @@ def _spec_commit_op(scratch, scratch_indices, pool, pool_indices, num_accepted_t
     _recurrent.spec_commit(scratch, scratch_indices, pool, pool_indices, num_accepted_tokens, slot0_reserved)
 
 
+def _latent_prefill_op(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, out, scale=None, causal=True, lse=None):
+    _latent.latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale, causal, out=out, lse=lse)
+
+
+def _latent_decode_op(q_latent, q_pe, cache, block_table, seq_lens, out, scale=None, lse=None, prefix_table=None,
+                      prefix_len=None, workspace=None):
+    _latent.latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out=out, lse=lse,
+                          prefix_table=prefix_table, prefix_len=prefix_len, workspace=workspace)
+
+
+def _latent_append_op(latent, k_pe, cache, slots):
+    _latent.latent_append(latent, k_pe, cache, slots)
+
+
+def _latent_gather_op(cache, block_table, cu_seqlens, out):
+    _latent.latent_gather(cache, block_table, cu_seqlens, out)
+
+
 _IMPLS = {
     "fused_kda_decode": _fused_kda_decode,
     "fused_kda_prefill": _fused_kda_prefill,
@@ -210,6 +255,14 @@ _IMPLS = {
     "decode": _decode_op,
     "fused_recurrent_kda": _fused_recurrent_op,
     "spec_commit": _spec_commit_op,
+    "latent_prefill": _latent_prefill_op,
+    "latent_decode": _latent_decode_op,
+    "latent_append": _latent_append_op,
+    "latent_gather": _latent_gather_op,
+    "copy_rows": _pages.copy_rows,
+    "fork_pages": _pages.fork_pages,
+    "free_pages": _pages.free_pages,
+    "compact_pages": _pages.compact_pages,
 }
 
 

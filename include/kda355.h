@@ -285,6 +285,148 @@ int kda355_prefill_launch(const KdaPrefillArgs* args, kda355_stream_t stream);
 #define KDA355_NOALLOC_SCRATCH_BYTES (256ull << 20)
 int kda355_prefill_launch_noalloc(const KdaPrefillArgs* args, kda355_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------ latent attention */
+
+/*
+ * The attention layers between the KDA layers of a hybrid model: every token leaves one latent vector of 512 values and
+ * a positional part of 64 (rotated or not, as the model has it) that all heads share.  Head dims: 128 + 64 for q and k,
+ * 128 for v.  No counterpart in the reference, which holds KDA layers only.
+ *
+ * Cache: [pages, page_size, 576] in 16-bit elements, the token rows (latent | positional part) dense within a page, any
+ * page stride.  Page numbers outside [0, pages) are holes: their tokens are never read and take no part.
+ */
+#define KDA355_LATENT_DIM 512
+#define KDA355_LATENT_PE 64
+#define KDA355_LATENT_ROW 576
+#define KDA355_DTYPE_BF16 0
+#define KDA355_DTYPE_FP16 1
+#define KDA355_LATENT_CAUSAL 1u
+
+/*
+ * Expanded form over N packed sequences: sequence n has queries [cu_q[n], cu_q[n + 1]) and keys [cu_k[n], cu_k[n + 1]).
+ * With its lengths Lq and Lk and KDA355_LATENT_CAUSAL, query i sees keys j <= i + Lk - Lq (the queries are the last
+ * tokens); without, all of them.  z = scale (q[:128] . k + q[128:] . k_pe);  out = softmax(z) v;  lse = log sum e^z.  A
+ * query that sees no key gets zeros and an lse of -inf.  Keys that a query does not see never reach its output, whatever
+ * they hold.  Sums and softmax statistics are fp32.
+ */
+typedef struct KdaLatentPrefillArgs {
+    const void* q;       /* [Tq, H, 192], strides in elements */
+    const void* k;       /* [Tk, H, 128] */
+    const void* v;       /* [Tk, H, 128] */
+    const void* k_pe;    /* [Tk, 64] */
+    void* out;           /* [Tq, H, 128] */
+    float* lse;          /* [Tq, H] dense, natural logarithm, or NULL */
+    const int32_t* cu_q; /* [N + 1] on the device, not decreasing, within [0, Tq] (clamped to it) */
+    const int32_t* cu_k; /* [N + 1], the same for Tk */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, pe_row, out_row, out_head;
+    int64_t Tq, Tk;
+    int32_t N, H, dtype;
+    uint32_t flags;      /* KDA355_LATENT_CAUSAL or 0 */
+    float scale;
+    int32_t reserved;
+} KdaLatentPrefillArgs;
+
+int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* args, kda355_stream_t stream);
+
+/*
+ * Absorbed form over the paged cache, B sequences x S tokens (row n * S + s is token s of sequence n): with c_j the latent
+ * and r_j the positional part of cached token j, z = scale (q_latent . c_j + q_pe . r_j);  out = sum softmax(z) c_j.
+ * seq_lens[n] cached tokens, the S new ones among them: token s sees j < seq_lens[n] - (S - 1 - s).  seq_lens is clamped
+ * to [0, table_width * page_size].
+ * With prefix_table, every sequence first sees the prefix_len[0] tokens of those pages (all S tokens see all of them),
+ * then its own; the prefix is read once for all rows.  A row that sees nothing gets zeros and an lse of -inf.
+ */
+typedef struct KdaLatentDecodeArgs {
+    const void* q_latent;        /* [B * S, H, 512], strides in elements */
+    const void* q_pe;            /* [B * S, H, 64] */
+    const void* cache;           /* [pages, page_size, 576] */
+    const int32_t* block_table;  /* [B, table_width], row stride table_stride */
+    const int32_t* seq_lens;     /* [B] */
+    const int32_t* prefix_table; /* [prefix_width] or NULL */
+    const int32_t* prefix_len;   /* [1] (with prefix_table) */
+    void* out;                   /* [B * S, H, 512] */
+    float* lse;                  /* [B * S, H] dense, or NULL */
+    void* workspace;             /* kda355_latent_decode_workspace_bytes(args), 256-byte aligned; nothing in it has to
+                                    start at zero, launches that may overlap need their own */
+    int64_t ql_row, ql_head, qp_row, qp_head, out_row, out_head;
+    int64_t page_stride, pages, table_stride, workspace_bytes;
+    int32_t B, S, H, page_size, table_width, prefix_width;
+    int32_t dtype, num_cus;      /* num_cus: workgroups the launch fills (0: 256) */
+    float scale;
+    uint32_t flags;              /* 0 */
+} KdaLatentDecodeArgs;
+
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL. */
+int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArgs* args);
+int kda355_latent_decode_launch(const KdaLatentDecodeArgs* args, kda355_stream_t stream);
+
+/*
+ * Token rows into pages and back.  append: cache row slots[t] (page * page_size + offset) <- latent[t] | k_pe[t]; slots
+ * outside [0, pages * page_size) are skipped (two tokens of one slot: either may stay).  gather: out[cu[n] + j] <- token
+ * j of sequence n, for j < cu[n + 1] - cu[n]; tokens of holes or past the table give zero rows.
+ */
+typedef struct KdaLatentTokensArgs {
+    const void* latent;          /* append: [T, 512] */
+    const void* k_pe;            /* append: [T, 64] */
+    void* cache;                 /* [pages, page_size, 576] */
+    const int64_t* slots;        /* append: [T] */
+    const int32_t* block_table;  /* gather: [N, table_width] */
+    const int32_t* cu;           /* gather: [N + 1] on the device, clamped to [0, T] */
+    void* out;                   /* gather: [T, 576], row stride out_row */
+    int64_t latent_row, pe_row, out_row, page_stride, pages, table_stride, T;
+    int32_t page_size, table_width, N, reserved;
+} KdaLatentTokensArgs;
+
+int kda355_latent_append_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
+int kda355_latent_gather_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------ pages of a cache */
+
+/*
+ * Page bookkeeping on the device: sequences are rows of block_table (entries outside [0, pages) are holes), a page holds
+ * page_size tokens and ref_counts[page] sequences hold it.  free_pages[0 .. num_free[0]) is a stack of the pages nobody
+ * holds, the next one at its top; entries past it are -1.  Nothing is read back to the host, so the calls can be captured;
+ * results do not depend on timing.  No counterpart in the reference (its caller manages slots on the host).
+ *
+ * A pool is one layer's tensor [slots, ...] with dense rows of row_bytes (a multiple of 16) at 16-byte aligned addresses.
+ */
+#define KDA355_MAX_POOLS 24
+typedef struct KdaPool {
+    void* base;
+    int64_t row_bytes, slot_stride; /* bytes */
+    int64_t slots;
+} KdaPool;
+
+typedef struct KdaPagesArgs {
+    KdaPool pool[KDA355_MAX_POOLS];
+    int32_t num_pools, n;        /* n: pairs / rows given */
+    const int32_t* src;          /* copy: [n] rows;  fork: [n] parents;  free: [n] rows */
+    const int32_t* dst;          /* copy: [n] rows;  fork: [n] children */
+    int32_t* block_table;        /* [rows, table_width], row stride table_stride */
+    int32_t* seq_lens;           /* [rows] */
+    int32_t* ref_counts;         /* [pages] */
+    int32_t* free_pages;         /* [pages] */
+    int32_t* num_free;           /* [1] */
+    int32_t* workspace;          /* fork: 2 n words;  compact: 2 pages + 2 words */
+    int64_t table_stride;
+    int32_t rows, table_width, pages, page_size;
+} KdaPagesArgs;
+
+/* pool[dst[i]] <- pool[src[i]] in every pool; pairs with a row outside a pool are skipped there.  No dst may be another
+   pair's src or dst. */
+int kda355_copy_rows_launch(const KdaPagesArgs* args, kda355_stream_t stream);
+/* Sequence dst[i] becomes a copy of src[i], in the order of i: its full pages are shared, a part-filled last page is copied
+   in every pool to a page taken from the stack.  Where the stack is empty, the child gets length 0 and no pages.  What the
+   child row held before is overwritten, not released.  Pairs outside [0, rows) are skipped; children must differ from one
+   another and from every parent. */
+int kda355_fork_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
+/* Sequences src[i] (all different) give up the pages of their seq_lens tokens; rows become holes, lengths 0.  Pages that
+   nobody holds any more go onto the stack, the highest first. */
+int kda355_free_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
+/* With L pages held: the i-th held page at or above L moves into the i-th free one below L, in every pool; tables, counts
+   and the stack (pages - 1 down to L, so that L is taken next) follow. */
+int kda355_compact_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------------ misc */
 
 /* Human-readable reason of the last KDA355_EINVAL / KDA355_ELAUNCH on the calling thread ("" if none). */
