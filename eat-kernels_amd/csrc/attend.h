@@ -1,0 +1,142 @@
+// What the latent attention kernels share (gfx950, wave64): element types, the 32x32x16 MFMA, loads straight into LDS, the
+// running softmax of a 32-row tile, and values that a query does not see.
+//
+// A wave holds 32 query rows and computes transposed tiles: scores S^T [keys x rows] = K Q^T and outputs O^T [values x rows]
+// = V^T P^T, so that a query row is a lane (l % 32, both halves h = l / 32) throughout: the softmax of a row runs down the
+// lane's own registers and across the two halves once, and P^T leaves the scores' registers as the second product's operand
+// without passing through LDS.  Register r of a 32 x 32 result holds row (r & 3) + 8 (r >> 2) + 4 h; operand element e of a
+// lane is the k index 8 h + e.  The second product's k order is free, so element e of its 16-key step s stands for key
+// 16 s + 4 h + (e & 3) + 8 (e >> 2), which is the scores' own order; V is read in the same order.
+#pragma once
+#include "common.h"
+
+namespace kda355 {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// Element types.  The weights p = 2^(z - m + B) of a row are rounded to the type for the second product.  m is a past
+// maximum that z may exceed by SLACK before it is raised (raising it rescales the whole accumulator), so p <= 2^(B + SLACK).
+// bf16 has fp32's range: B = 0.  fp16 ends at 2^16 and loses precision below 2^-14: B = 9 keeps full precision for keys
+// down to 2^-23 of the maximum.
+struct Bf16 {
+    static constexpr float B = 0.f, SLACK = 8.f;
+    static constexpr uint32_t EXP = 0x7f807f80u, EXP_ONE = 0x00800080u, ONE = 0x3f80u;
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) { return f2bf2(x, y); }
+};
+struct Fp16 {
+    static constexpr float B = 9.f, SLACK = 6.f;
+    static constexpr uint32_t EXP = 0x7c007c00u, EXP_ONE = 0x04000400u, ONE = 0x3c00u;
+    static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2_t));
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ LDS
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
+
+// 64 lanes x 16 bytes from global memory into 1 KiB of LDS at byte `lds` (wave-uniform), lane l's piece at lds + 16 l.  Lane
+// offsets at or past the descriptor's size read as zeros.  In asm, because the compiler would wait for every such load
+// before any read of LDS; whoever reads the data waits with wait_loads() and a barrier.
+constexpr uint32_t LDS_ZERO = 0x80000000u;  // a lane offset that is out of range for every descriptor below
+__device__ __forceinline__ void load_to_lds(uint32_t lds, u32x4 rsrc, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+                 : "memory");
+}
+__device__ __forceinline__ u32x4 tile_rsrc(const void* base) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
+                 0x7fffffffu, 0x00020000u};
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // all but the N youngest loads of this wave have arrived
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
+    return *(__attribute__((address_space(3))) const u32x4*)(lds_byte*)(uintptr_t)at;
+}
+// transposed read: of 16 lanes, lane i gives the address of 4 elements; lane i receives element i % 4.. column i of the
+// 4 x 16 matrix whose row r are the elements at lanes 4 r .. 4 r + 3
+__device__ __forceinline__ u32x2 lds_read_tr(uint32_t at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_byte*)(uintptr_t)at));
+}
+
+// Token rows of 16-byte pieces in LDS: piece c of token t stands at c ^ f(t), f(t) = 4 (t & 3) + ((t >> 2) & 3), within
+// each 16 pieces.  Rows are a multiple of 256 bytes (all 64 banks), so the piece position alone picks the banks: 16 lanes
+// that read one piece of 16 consecutive tokens, and 16 lanes of a transposed read (4 consecutive pieces of 4 consecutive
+// tokens), both touch all 16 positions.
+__device__ __forceinline__ int swz16(int t) { return ((t & 3) << 2) | ((t >> 2) & 3); }
+// rows of 8 pieces (two tokens a bank sweep): c ^ ((t >> 1) & 7)
+__device__ __forceinline__ int swz8(int t) { return (t >> 1) & 7; }
+
+// ------------------------------------------------------------------------------------------------ lanes
+// the other half wave's value of the same row
+__device__ __forceinline__ float other_half(float x) {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return __uint_as_float((threadIdx.x & 32) ? r.x : r.y);
+}
+__device__ __forceinline__ float max_halves(float x) {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// ------------------------------------------------------------------------------------------------ running softmax
+// State of a lane's row: mo = m - B in log2 units, l = this half's sum of the weights.  Starts far below any score but
+// finite, so that hidden scores (-inf) give weights of 0 and never a NaN.
+constexpr float M_START = -1e30f;
+
+// ------------------------------------------------------------------------------------------------ values nobody sees
+// A product with weight 0 is not 0 where the value is infinite or NaN.  In tiles where some rows see a key and others do
+// not, values that are not finite are taken out of the matrix product and added afterwards for the rows that see them:
+// counts of visible +inf (or NaN) and -inf (or NaN) values come from two more products of 0 / 1 operands.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(u32x4 a) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f |= (a[i] & T::EXP) + T::EXP_ONE;  // the exponent's carry reaches the half's top bit
+    return __builtin_amdgcn_ballot_w64((f & 0x80008000u) != 0) != 0;
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_hidden(u32x4 v, u32x4 p, f32x16 acc) {
+    if (!any_nonfinite<T>(v)) return T::mfma(v, p, acc);
+    constexpr uint32_t E = T::EXP & 0xffffu;
+    u32x4 fin, pos, neg, vis;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t f = 0, ps = 0, ng = 0, vs = 0;
+#pragma unroll
+        for (int s = 0; s < 32; s += 16) {
+            const uint32_t x = (v[i] >> s) & 0xffffu, w = (p[i] >> s) & 0xffffu;
+            const bool special = (x & E) == E, nan = special && (x & 0x7fffu) != E, minus = x >> 15;
+            f |= (special ? 0u : x) << s;
+            ps |= (special && (nan || !minus) ? T::ONE : 0u) << s;
+            ng |= (special && (nan || minus) ? T::ONE : 0u) << s;
+            vs |= (w ? T::ONE : 0u) << s;
+        }
+        fin[i] = f; pos[i] = ps; neg[i] = ng; vis[i] = vs;
+    }
+    acc = T::mfma(fin, p, acc);
+    const f32x16 zero = {};
+    const f32x16 up = T::mfma(pos, vis, zero), down = T::mfma(neg, vis, zero);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        if (up[r] > 0.5f) acc[r] += INFINITY;
+        if (down[r] > 0.5f) acc[r] -= INFINITY;
+    }
+    return acc;
+}
+
+}  // namespace kda355

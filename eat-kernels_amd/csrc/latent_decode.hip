@@ -1,4 +1,4 @@
-// Latent attention (gfx950): the expanded form over packed sequences and the absorbed form over a paged cache.
+// Latent attention, absorbed form over a paged cache (gfx950).
 //
 // One workgroup of 4 wave64 per (query row, head).  Each wave walks every fourth key with the row's dot product spread over
 // its lanes and an online softmax (running maximum m, sum l and accumulator in fp32); the waves' parts are joined in LDS:
@@ -59,29 +59,6 @@ __device__ __forceinline__ void finish(Acc<NV>& c, void* out, int64_t at, float*
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) prefill_kernel(KdaLatentPrefillArgs a) {
-    const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int n = 0;
-    while (n < a.N && a.cu_q[n + 1] <= t) ++n;
-    if (n == a.N || t < a.cu_q[n]) return;
-    const int64_t k0 = min(max((int64_t)a.cu_k[n], (int64_t)0), a.Tk);
-    const int64_t Lk = max(min((int64_t)a.cu_k[n + 1], a.Tk) - k0, (int64_t)0), Lq = min((int64_t)a.cu_q[n + 1], a.Tq) - a.cu_q[n];
-    const int64_t seen = (a.flags & KDA355_LATENT_CAUSAL) ? min(Lk, t - a.cu_q[n] + Lk - Lq + 1) : Lk;
-    float q[3];
-    for (int i = 0; i < 3; ++i) q[i] = up<T>(a.q, t * a.q_row + h * a.q_head + lane + 64 * i) * a.scale;
-    Acc<2> c;
-    for (int64_t j = w; j < seen; j += WAVES) {
-        const int64_t kb = (k0 + j) * a.k_row + h * a.k_head + lane, vb = (k0 + j) * a.v_row + h * a.v_head + lane;
-        const float z = sum64(q[0] * up<T>(a.k, kb) + q[1] * up<T>(a.k, kb + 64) +
-                              q[2] * up<T>(a.k_pe, (k0 + j) * a.pe_row + lane));
-        const float v[2] = {up<T>(a.v, vb), up<T>(a.v, vb + 64)};
-        c.add(z, v);
-    }
-    finish<T>(c, a.out, t * a.out_row + h * a.out_head, a.lse ? a.lse + t * a.H + h : nullptr);
-}
-
-template <typename T>
 __global__ void __launch_bounds__(256) decode_kernel(KdaLatentDecodeArgs a) {
     const int64_t t = blockIdx.x;
     const int h = blockIdx.y, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -136,28 +113,6 @@ int check_decode_sizes(const KdaLatentDecodeArgs* a) {
 }  // namespace kda355
 
 using namespace kda355;
-
-extern "C" int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* a, kda355_stream_t stream) {
-    KDA_CHECK_ARG(a != nullptr, "latent_prefill: null args");
-    KDA_CHECK_ARG(a->N >= 0 && a->H >= 1 && a->Tq >= 0 && a->Tk >= 0, "latent_prefill: N=%d H=%d Tq=%lld Tk=%lld", a->N, a->H,
-                  (long long)a->Tq, (long long)a->Tk);
-    KDA_CHECK_ARG(a->dtype == KDA355_DTYPE_BF16 || a->dtype == KDA355_DTYPE_FP16, "latent_prefill: dtype %d", a->dtype);
-    KDA_CHECK_ARG((a->flags & ~KDA355_LATENT_CAUSAL) == 0, "latent_prefill: unknown flags 0x%x", a->flags);
-    if (a->N == 0 || a->Tq == 0) return 0;
-    KDA_CHECK_ARG(a->Tq < (1ll << 31) && a->Tk < (1ll << 31) && a->H <= 65535, "latent_prefill: too many tokens or heads");
-    KDA_CHECK_ARG(a->q && a->out && a->cu_q && a->cu_k && (a->Tk == 0 || (a->k && a->v && a->k_pe)),
-                  "latent_prefill: a required pointer is null");
-    KDA_CHECK_ARG(rows16(a->q, a->q_row, a->q_head) && rows16(a->k, a->k_row, a->k_head) && rows16(a->v, a->v_row, a->v_head) &&
-                      rows16(a->k_pe, a->pe_row) && rows16(a->out, a->out_row, a->out_head),
-                  "latent_prefill: rows must be 16-byte aligned");
-    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((uint32_t)a->Tq, a->H);
-    if (a->dtype == KDA355_DTYPE_BF16)
-        hipLaunchKernelGGL(prefill_kernel<__bf16>, grid, dim3(256), 0, s, *a);
-    else
-        hipLaunchKernelGGL(prefill_kernel<_Float16>, grid, dim3(256), 0, s, *a);
-    return launched("latent_prefill");
-}
 
 extern "C" int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArgs* a) {
     if (const int rc = check_decode_sizes(a)) return rc;

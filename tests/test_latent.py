@@ -79,7 +79,8 @@ BAD = [("latent_prefill", _prefill_args, kw, msg) for kw, msg in [
     (dict(N=-1), b"N=-1"), (dict(H=0), b"H=0"), (dict(Tq=-1), b"Tq"), (dict(dtype=2), b"dtype"), (dict(flags=2), b"flags"),
     (dict(q=0), b"null"), (dict(k=0), b"null"), (dict(cu_k=0), b"null"), (dict(q=FAKE + 8), b"aligned"),
     (dict(k_row=260), b"aligned"), (dict(v_head=4), b"aligned"), (dict(pe_row=65), b"aligned"), (dict(out_head=4), b"aligned"),
-    (dict(Tk=1 << 31), b"too many"), (dict(H=65536), b"too many")]]
+    (dict(Tk=1 << 30), b"2^30"), (dict(Tq=1 << 30), b"2^30"), (dict(scale=0.0), b"positive"), (dict(scale=-1.0), b"positive"),
+    (dict(scale=float("nan")), b"positive"), (dict(k_row=(1 << 23) + 8), b"2^23"), (dict(H=1 << 23), b"grid")]]
 BAD += [("latent_decode", _decode_args, kw, msg) for kw, msg in [
     (dict(B=-1), b"B=-1"), (dict(S=0), b"S=0"), (dict(H=0), b"H=0"), (dict(page_size=0), b"page_size"),
     (dict(table_width=1 << 30), b"2^31"), (dict(prefix_width=1 << 30), b"2^31"), (dict(B=1 << 20, S=1 << 10, H=2), b"too large"),
