@@ -27,6 +27,7 @@ struct Bf16 {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) { return f2bf2(x, y); }
+    static __device__ __forceinline__ float up(uint16_t x) { return bf2f(x); }
 };
 struct Fp16 {
     static constexpr float B = 9.f, SLACK = 6.f;
@@ -37,18 +38,20 @@ struct Fp16 {
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2_t));
     }
+    static __device__ __forceinline__ float up(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
 };
 
 // ------------------------------------------------------------------------------------------------ LDS
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
 
-// 64 lanes x 16 bytes from global memory into 1 KiB of LDS at byte `lds` (wave-uniform), lane l's piece at lds + 16 l.  Lane
-// offsets at or past the descriptor's size read as zeros.  In asm, because the compiler would wait for every such load
+// 64 lanes x 16 bytes from global memory into 1 KiB of LDS at byte `lds` (wave-uniform), lane l's piece at lds + 16 l, from
+// byte voff (a lane's) + soff (the wave's).  Lane offsets at or past the descriptor's size read as zeros.  In asm, because the compiler would wait for every such load
 // before any read of LDS; whoever reads the data waits with wait_loads() and a barrier.
 constexpr uint32_t LDS_ZERO = 0x80000000u;  // a lane offset that is out of range for every descriptor below
-__device__ __forceinline__ void load_to_lds(uint32_t lds, u32x4 rsrc, uint32_t voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+__device__ __forceinline__ void load_to_lds(uint32_t lds, u32x4 rsrc, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+                 "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(soff))
                  : "memory");
 }
 __device__ __forceinline__ u32x4 tile_rsrc(const void* base) {
@@ -100,43 +103,22 @@ constexpr float M_START = -1e30f;
 
 // ------------------------------------------------------------------------------------------------ values nobody sees
 // A product with weight 0 is not 0 where the value is infinite or NaN.  In tiles where some rows see a key and others do
-// not, values that are not finite are taken out of the matrix product and added afterwards for the rows that see them:
-// counts of visible +inf (or NaN) and -inf (or NaN) values come from two more products of 0 / 1 operands.
+// not, values that are not finite are taken out of the matrix product; a kernel that met one adds it to the rows that see
+// it once its key loop is done (a positive weight leaves such a value as it is).
 template <typename T>
-__device__ __forceinline__ bool any_nonfinite(u32x4 a) {
+__device__ __forceinline__ bool nonfinite(u32x4 a) {
     uint32_t f = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f |= (a[i] & T::EXP) + T::EXP_ONE;  // the exponent's carry reaches the half's top bit
-    return __builtin_amdgcn_ballot_w64((f & 0x80008000u) != 0) != 0;
+    return (f & 0x80008000u) != 0;
 }
+// the finite values, zeros in place of the others
 template <typename T>
-__device__ __forceinline__ f32x16 mfma_hidden(u32x4 v, u32x4 p, f32x16 acc) {
-    if (!any_nonfinite<T>(v)) return T::mfma(v, p, acc);
+__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
     constexpr uint32_t E = T::EXP & 0xffffu;
-    u32x4 fin, pos, neg, vis;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t f = 0, ps = 0, ng = 0, vs = 0;
-#pragma unroll
-        for (int s = 0; s < 32; s += 16) {
-            const uint32_t x = (v[i] >> s) & 0xffffu, w = (p[i] >> s) & 0xffffu;
-            const bool special = (x & E) == E, nan = special && (x & 0x7fffu) != E, minus = x >> 15;
-            f |= (special ? 0u : x) << s;
-            ps |= (special && (nan || !minus) ? T::ONE : 0u) << s;
-            ng |= (special && (nan || minus) ? T::ONE : 0u) << s;
-            vs |= (w ? T::ONE : 0u) << s;
-        }
-        fin[i] = f; pos[i] = ps; neg[i] = ng; vis[i] = vs;
-    }
-    acc = T::mfma(fin, p, acc);
-    const f32x16 zero = {};
-    const f32x16 up = T::mfma(pos, vis, zero), down = T::mfma(neg, vis, zero);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        if (up[r] > 0.5f) acc[r] += INFINITY;
-        if (down[r] > 0.5f) acc[r] -= INFINITY;
-    }
-    return acc;
+    for (int i = 0; i < 4; ++i) v[i] &= ((v[i] & E) == E ? 0u : 0xffffu) | ((v[i] >> 16 & E) == E ? 0u : 0xffff0000u);
+    return v;
 }
 
 }  // namespace kda355

@@ -79,28 +79,34 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     const uint16_t* vh = static_cast<const uint16_t*>(a.v) + k0 * a.v_row + h * a.v_head;
     const uint16_t* ph = static_cast<const uint16_t*>(a.k_pe) + k0 * a.pe_row;
     const uint32_t lds = lds_offset(sm);
-    const int lt = 16 * w + (lane >> 4);                         // + 4 i: this lane's token in k / v load i
-    const uint32_t piece = (lane & 15) ^ ((lane >> 4) << 2);     // ^ i: the piece it fetches (swz16 of that token)
-    const int pt = 16 * w + (lane >> 3);                         // + 8 i: in load i of the shared part
+    uint32_t koff[4], voff[4], poff[2];  // byte offsets of this lane's pieces (k / v load i: tokens 16 w + 4 i ..; swz16)
+    const int lt = 16 * w + (lane >> 4), pt = 16 * w + (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t piece = ((lane & 15) ^ ((lane >> 4) << 2) ^ i) * 16;
+        koff[i] = (uint32_t)lt * (uint32_t)(2 * a.k_row) + piece;
+        voff[i] = (uint32_t)lt * (uint32_t)(2 * a.v_row) + piece;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) poff[i] = (uint32_t)pt * (uint32_t)(2 * a.pe_row) + ((lane & 7) ^ swz8(pt + 8 * i)) * 16;
+    const uint32_t kstep = 8 * (uint32_t)a.k_row, vstep = 8 * (uint32_t)a.v_row, pstep = 16 * (uint32_t)a.pe_row;
     auto load_tile = [&](int j, int buf) {
         const int t0 = j * BN, left = Lk - t0;
         const u32x4 kr = tile_rsrc(kh + (int64_t)t0 * a.k_row), vr = tile_rsrc(vh + (int64_t)t0 * a.v_row),
                     pr = tile_rsrc(ph + (int64_t)t0 * a.pe_row);
-        const uint32_t base = lds + buf * TILE_BYTES;
+        const uint32_t base = lds + buf * TILE_BYTES + 16 * w * (HD * 2), pbase = lds + buf * TILE_BYTES + TILE_PE + 16 * w * (PE * 2);
+        auto issue = [&](auto whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = lt + 4 * i;
-            const uint32_t p16 = (piece ^ i) * 16;
-            load_to_lds(base + (16 * w + 4 * i) * (HD * 2), kr, t < left ? (uint32_t)t * (uint32_t)(2 * a.k_row) + p16 : LDS_ZERO);
-            load_to_lds(base + TILE_V + (16 * w + 4 * i) * (HD * 2), vr,
-                        t < left ? (uint32_t)t * (uint32_t)(2 * a.v_row) + p16 : LDS_ZERO);
-        }
+            for (int i = 0; i < 4; ++i) {
+                const bool in = whole || lt + 4 * i < left;
+                load_to_lds(base + 4 * i * (HD * 2), kr, in ? koff[i] : LDS_ZERO, i * kstep);
+                load_to_lds(base + TILE_V + 4 * i * (HD * 2), vr, in ? voff[i] : LDS_ZERO, i * vstep);
+            }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = pt + 8 * i;
-            load_to_lds(base + TILE_PE + (16 * w + 8 * i) * (PE * 2), pr,
-                        t < left ? (uint32_t)t * (uint32_t)(2 * a.pe_row) + ((lane & 7) ^ swz8(t)) * 16 : LDS_ZERO);
-        }
+            for (int i = 0; i < 2; ++i)
+                load_to_lds(pbase + 8 * i * (PE * 2), pr, whole || pt + 8 * i < left ? poff[i] : LDS_ZERO, i * pstep);
+        };
+        if (left >= BN) issue(std::true_type{}); else issue(std::false_type{});
     };
 
     // ---- LDS read addresses (byte offsets within a tile; key step, value tile and key block are xors and constants)
@@ -118,6 +124,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     const float sc = a.scale * 1.44269504088896f;
     f32x16 acc[4] = {};
     float mo = M_START, l = 0.f;
+    bool special = false;
     const int seen = min(Lk, min(m0 + BM, Lq) + shift);        // keys that any row of the workgroup sees
     const int mine = min(Lk, min(m0 + 32 * w + 32, Lq) + shift);  // ... of this wave
     const int full = min(Lk, m0 + 32 * w + 1 + shift);         // keys that every row of this wave sees
@@ -131,14 +138,25 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         const int t0 = j * BN;
         if (t0 >= mine) continue;  // wave-uniform; the barrier is at the top
         const uint32_t tb = lds + (j & 1) * TILE_BYTES;
+        // ---- scores: 24 steps (key step i of 12, key block b of 2), the operands of the next four read while four run
         f32x16 s[2] = {};
+        auto key = [&](int x) {
+            const int i = x >> 1, b = x & 1;
+            return i < 8 ? lds_read16((tb + ka + b * 32 * HD * 2) ^ (i << 5)) : lds_read16((tb + pa + b * 32 * PE * 2) ^ ((i - 8) << 5));
+        };
+        u32x4 kf[2][4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int x = 0; x < 4; ++x) kf[0][x] = key(x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[b] = T::mfma(lds_read16((tb + ka + b * 32 * HD * 2) ^ (i << 5)), q[i], s[b]);
+        for (int g = 0; g < 6; ++g) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (g < 5)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b] = T::mfma(lds_read16((tb + pa + b * 32 * PE * 2) ^ (i << 5)), q[8 + i], s[b]);
+                for (int x = 0; x < 4; ++x) kf[(g + 1) & 1][x] = key(4 * g + 4 + x);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[x & 1] = T::mfma(kf[g & 1][x], q[2 * g + (x >> 1)], s[x & 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
         const bool masked = t0 + BN > full;  // some row of the wave does not see some key of the tile
         if (masked) {
             const int last = min(row + shift, Lk - 1) - t0 - 4 * half;
@@ -174,18 +192,46 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
                 p[2 * b + (r >> 3)][(r >> 1) & 3] = T::pack(x, y);
             }
         // ---- values
-        auto values = [&](auto hidden) {
+        auto value = [&](int k, int d) {
+            const u32x2 v0 = lds_read_tr(((tb + va[0]) ^ (d << 6)) + k * 16 * HD * 2);
+            const u32x2 v1 = lds_read_tr(((tb + va[1]) ^ (d << 6)) + k * 16 * HD * 2);
+            return u32x4{v0.x, v0.y, v1.x, v1.y};
+        };
+        u32x4 vf[2][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+        for (int d = 0; d < 4; ++d) vf[0][d] = value(0, d);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (k < 3)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) vf[(k + 1) & 1][d] = value(k + 1, d);
+            if (masked)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const u32x2 v0 = lds_read_tr(((tb + va[0]) ^ (d << 6)) + k * 16 * HD * 2);
-                    const u32x2 v1 = lds_read_tr(((tb + va[1]) ^ (d << 6)) + k * 16 * HD * 2);
-                    const u32x4 v = {v0.x, v0.y, v1.x, v1.y};
-                    acc[d] = hidden ? mfma_hidden<T>(v, p[k], acc[d]) : T::mfma(v, p[k], acc[d]);
+                    special |= nonfinite<T>(vf[k & 1][d]);
+                    vf[k & 1][d] = finite_part<T>(vf[k & 1][d]);
                 }
-        };
-        if (masked) values(std::true_type{}); else values(std::false_type{});
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] = T::mfma(vf[k & 1][d], p[k], acc[d]);
+        }
+    }
+
+    if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the keys that not every row sees
+        const int last = min(row + shift, Lk - 1);
+#pragma unroll 1
+        for (int j = max(full, 0) & ~(BN - 1); j < mine; ++j) {
+            const uint16_t* vr = vh + (int64_t)j * a.v_row + 4 * half;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = T::up(vr[32 * d + 8 * g + e]);
+                        if (j <= last && !(fabsf(x) < INFINITY)) acc[d][4 * g + e] += x;
+                    }
+        }
     }
 
     // ---- o = acc / l
