@@ -1,112 +1,558 @@
-// Latent attention, absorbed form over a paged cache (gfx950).
+// Latent attention, absorbed form over a paged cache (gfx950): all heads of a sequence read the same 576-wide token rows, whose
+// first 512 values are keys and values at once.
 //
-// One workgroup of 4 wave64 per (query row, head).  Each wave walks every fourth key with the row's dot product spread over
-// its lanes and an online softmax (running maximum m, sum l and accumulator in fp32); the waves' parts are joined in LDS:
-// o = sum_w e^(m_w - m) acc_w / sum_w e^(m_w - m) l_w.
-#include "common.h"
+// The query rows (token, head) of a sequence are taken in groups of up to 64 (two row tiles of 32) and the keys in tiles of 64.
+// The work is cut along the keys: a launch of about one workgroup a CU, each with an equal run of key tiles through the packed
+// sequences (all groups of a sequence side by side, so that their reads of the same keys meet in one L2), and with a shared
+// prefix some of the workgroups walk its tiles for groups of all rows of the batch.  Every workgroup finds its run from the
+// lengths on the device.  A run that holds a sequence whole writes its output; parts are left in the workspace in fp32 and
+// joined by a second kernel:  o = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s.
+//
+// Token rows come straight into LDS (72 KiB a tile, the next one under way while one is computed).  Of the 4 waves, wave w
+// computes the scores of row tile w % 2 with keys 32 (w / 2) .. + 31 of the tile (its queries in 144 registers), and then
+// values 128 w .. 128 w + 127 of all rows and keys, with the other waves' weights read from LDS.
+#include "attend.h"
 
 namespace kda355 {
 namespace {
 
-constexpr int LAT = KDA355_LATENT_DIM, ROW = KDA355_LATENT_ROW;
-constexpr int WAVES = 4;
+constexpr int LAT = KDA355_LATENT_DIM, ROW = KDA355_LATENT_ROW, PE = KDA355_LATENT_PE;
+constexpr int ROW_BYTES = ROW * 2, LAT_BYTES = LAT * 2, PE_BYTES = PE * 2;
+constexpr int WAVES = 4, THREADS = WAVES * 64;
+constexpr int BN = 64;                                  // keys of a tile
+constexpr int RT = 2, MAX_ROWS = 32 * RT;               // row tiles, query rows of a group
+constexpr uint32_t MIN_TILES = 1;                       // least run of a workgroup
+constexpr int SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;  // workspace of 32 rows: accumulators, (m, l) of each row
 
-template <typename T>
-__device__ __forceinline__ float up(const void* base, int64_t i) { return (float)reinterpret_cast<const T*>(base)[i]; }
-
-__device__ __forceinline__ float sum64(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
-}
-
-template <int NV>
-struct Acc {
-    float m = -INFINITY, l = 0.f, a[NV] = {};
-    __device__ __forceinline__ void add(float z, const float (&v)[NV]) {
-        const float mn = fmaxf(m, z);
-        const float f = m == -INFINITY ? 0.f : __expf(m - mn);
-        const float p = z == -INFINITY ? 0.f : __expf(z - mn);
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) a[i] = a[i] * f + p * v[i];
-        m = mn;
+struct Groups {
+    int rows, groups;  // rows of a group, groups
+    static Groups of(int64_t n) {
+        const int64_t g = (n + MAX_ROWS - 1) / MAX_ROWS;
+        const int64_t r = g ? (n + 32 * g - 1) / (32 * g) * 32 : 32;  // in tiles of 32, about equal
+        return {(int)r, (int)((n + r - 1) / r)};
     }
 };
+struct Plan {
+    Groups own, pre;       // of a sequence's rows; of all rows of the batch, for the prefix (no groups: no prefix)
+    int grid;
+    int64_t pre_slots;     // workspace: prefix parts, then the sequences'
+};
 
-// joins the waves' parts; out elements lane + 64 i
-template <typename T, int NV>
-__device__ __forceinline__ void finish(Acc<NV>& c, void* out, int64_t at, float* lse) {
-    __shared__ float sm[WAVES], sl[WAVES], sa[WAVES][NV * 64];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// ------------------------------------------------------------------------------------------------ who does what
+struct Cut {
+    uint32_t own, pre, run;  // key tiles of all sequences, of the prefix; tiles of a workgroup
+    uint32_t pre_wgs, own_wgs;
+};
+__device__ __forceinline__ int tokens_of(int len, int width, int page_size) { return min(max(len, 0), width * page_size); }
+__device__ __forceinline__ uint32_t tiles_of(const KdaLatentDecodeArgs& a, int n) {
+    return ((uint32_t)tokens_of(a.seq_lens[n], a.table_width, a.page_size) + BN - 1) / BN;
+}
+__device__ __forceinline__ uint32_t cdiv(uint32_t x, uint32_t y) { return x / y + (x % y != 0); }
+
+// The shortest run (to 1.6 %) with which the grid covers everything, the same in every wave: the lanes try 64 candidates.
+__device__ __forceinline__ Cut cut(const KdaLatentDecodeArgs& a, const Plan& p, uint32_t own) {
+    Cut c;
+    c.own = own;
+    c.pre = p.pre.groups ? ((uint32_t)tokens_of(a.prefix_len[0], a.prefix_width, a.page_size) + BN - 1) / BN : 0;
+    c.pre = __builtin_amdgcn_readfirstlane(c.pre);
+    const uint32_t most = max(max(c.own, c.pre), MIN_TILES);  // one run a group: always fits
+    const double all = (double)p.pre.groups * c.pre + (double)p.own.groups * c.own;
+    const uint32_t lo = min(max((uint32_t)__builtin_ceil(all / p.grid), MIN_TILES), most);
+    const int lane = threadIdx.x & 63;
+    const double f = lane < 32 ? 1.0 + lane / 64.0 : 1.5 * (double)exp2f((lane - 31) * 0.25f);
+    const uint32_t r = lane == 63 ? most : (uint32_t)fmin(__builtin_ceil(lo * f), (double)most);
+    const uint64_t wgs = (uint64_t)p.pre.groups * cdiv(c.pre, r) + (uint64_t)p.own.groups * cdiv(c.own, r);
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(wgs <= (uint32_t)p.grid) | 1ull << 63);
+    c.run = __builtin_amdgcn_readlane(r, l);
+    c.pre_wgs = __builtin_amdgcn_readfirstlane(p.pre.groups * cdiv(c.pre, c.run));
+    c.own_wgs = __builtin_amdgcn_readfirstlane(p.own.groups * cdiv(c.own, c.run));
+    return c;
+}
+__device__ __forceinline__ uint32_t sum_wave(uint32_t x) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) sa[w][lane + 64 * i] = c.a[i];
-    if (lane == 0) {
-        sm[w] = c.m;
-        sl[w] = c.l;
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return __builtin_amdgcn_readfirstlane(x);
+}
+struct At { int n; uint32_t before; };
+// the sequence that holds tile u of all (u < their sum), and the tiles before it
+__device__ __forceinline__ At sequence_of(const KdaLatentDecodeArgs& a, uint32_t u) {
+    const int lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (int n0 = 0; n0 < a.B; n0 += 64) {
+        const uint32_t t = n0 + lane < a.B ? tiles_of(a, n0 + lane) : 0;
+        uint32_t s = t;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t y = __shfl_up(s, d);
+            if (lane >= d) s += y;
+        }
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + s > u);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            return {n0 + l, before + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(t, l)};
+        }
+        before += __builtin_amdgcn_readlane(s, 63);
     }
-    __syncthreads();
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < WAVES; ++j) m = fmaxf(m, sm[j]);
-    for (int j = 0; j < WAVES; ++j) l += sm[j] == -INFINITY ? 0.f : sl[j] * __expf(sm[j] - m);
-    for (int e = threadIdx.x; e < NV * 64; e += WAVES * 64) {
-        float o = 0.f;
-        for (int j = 0; j < WAVES; ++j)
-            if (sm[j] != -INFINITY) o += sa[j][e] * __expf(sm[j] - m);
-        reinterpret_cast<T*>(out)[at + e] = (T)(l > 0.f ? o / l : 0.f);
-    }
-    if (lse && threadIdx.x == 0) *lse = l > 0.f ? m + __logf(l) : -INFINITY;
+    return {a.B, before};
 }
 
+// ------------------------------------------------------------------------------------------------ LDS
+constexpr int TILE_PE = BN * LAT_BYTES, TILE_BYTES = TILE_PE + BN * PE_BYTES;  // latent rows | positional parts
+constexpr int LDS_P = 2 * TILE_BYTES;                // weights: [row tile][16-key step][lane] 16 bytes
+constexpr int LDS_MAX = LDS_P + RT * 4 * 1024;       // a tile's maxima [wave][32], at the end the sums of rows
+constexpr int LDS_FLAG = LDS_MAX + WAVES * 128;      // does wave w's tile raise the maximum
+constexpr int LDS_PAGES = LDS_FLAG + 256;            // page numbers of a tile's tokens: [wave][tile % 2][64]
+constexpr int LDS_BYTES = LDS_PAGES + WAVES * 2 * 256;
+static_assert(LDS_BYTES <= 160 * 1024, "");
+
 template <typename T>
-__global__ void __launch_bounds__(256) decode_kernel(KdaLatentDecodeArgs a) {
-    const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int n = (int)(t / a.S), s = (int)(t - (int64_t)n * a.S);
-    float q[9];
-    for (int i = 0; i < 8; ++i) q[i] = up<T>(a.q_latent, t * a.ql_row + h * a.ql_head + lane + 64 * i) * a.scale;
-    q[8] = up<T>(a.q_pe, t * a.qp_row + h * a.qp_head + lane) * a.scale;
-    Acc<8> c;
-    auto walk = [&](const int32_t* table, int width, int64_t len, int64_t hidden) {
-        len = min(max(len, (int64_t)0), (int64_t)width * a.page_size) - hidden;
-        for (int64_t j = w; j < len; j += WAVES) {
-            const int64_t page = table[j / a.page_size];
-            if (page < 0 || page >= a.pages) continue;
-            const int64_t b = page * a.page_stride + (j % a.page_size) * ROW + lane;
-            float v[8], z = q[8] * up<T>(a.cache, b + LAT);
-            for (int i = 0; i < 8; ++i) {
-                v[i] = up<T>(a.cache, b + 64 * i);
-                z += q[i] * v[i];
-            }
-            c.add(sum64(z), v);
+__global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
+    __shared__ __align__(1024) unsigned char sm[LDS_BYTES];
+    const uint32_t lds = lds_offset(sm);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int c = lane & 31, half = lane >> 5;
+
+    uint32_t own = 0;
+    for (int n = lane; n < a.B; n += 64) own += tiles_of(a, n);
+    const Cut cu = cut(a, p, sum_wave(own));
+    const uint32_t wgs = cu.pre_wgs + cu.own_wgs;
+    if (blockIdx.x >= wgs) return;
+    const uint32_t task = xcd_task(blockIdx.x, wgs);  // neighbours read the same keys: on one XCD
+    const bool prefix = task < cu.pre_wgs;
+    const Groups gr = prefix ? p.pre : p.own;
+    const uint32_t id = __builtin_amdgcn_readfirstlane(prefix ? task : task - cu.pre_wgs);
+    const uint32_t piece = __builtin_amdgcn_readfirstlane(id / gr.groups);
+    const int g = __builtin_amdgcn_readfirstlane(id - piece * gr.groups);
+    const uint32_t end = min((piece + 1) * cu.run, prefix ? cu.pre : cu.own);
+    uint32_t u = piece * cu.run;
+    At at = {0, 0};
+    if (!prefix) at = sequence_of(a, u);
+
+    const float sc = a.scale * 1.44269504088896f;
+    const int64_t page_bytes = a.page_stride * 2;
+    const char* const cache = static_cast<const char*>(a.cache);
+    const int rt = w & 1, kh = w >> 1;  // the wave's scores: row tile, keys 32 kh ..
+    // LDS read addresses within a tile: key 32 kh + c (scores), values as in the second product (attend.h)
+    const uint32_t ka = (32 * kh + c) * LAT_BYTES + ((half ^ swz16(c)) << 4);
+    const uint32_t pa = TILE_PE + (32 * kh + c) * PE_BYTES + ((half ^ swz8(c)) << 4);
+    uint32_t va[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int i16 = lane & 15, t = 4 * half + 8 * x + (i16 >> 2);
+        const int e = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+        va[x] = t * LAT_BYTES + w * 256 + ((e ^ swz16(t)) << 4) + (i16 & 1) * 8;
+    }
+
+    while (u < end) {
+        // ---- the segment: key tiles [t0, t1) of one key sequence, for rows [r0, r1) of the batch
+        int n = 0, tokens, r0, r1;
+        uint32_t t0, t1, whole;
+        const int32_t* table;
+        int width;
+        if (prefix) {
+            tokens = tokens_of(a.prefix_len[0], a.prefix_width, a.page_size);
+            table = a.prefix_table, width = a.prefix_width;
+            r0 = g * gr.rows, r1 = min(r0 + gr.rows, a.B * a.S * a.H);
+            t0 = u, t1 = end, whole = 0;
+            u = end;
+        } else {
+            n = at.n;
+            tokens = tokens_of(a.seq_lens[n], a.table_width, a.page_size);
+            table = a.block_table + n * a.table_stride, width = a.table_width;
+            const int rows = a.S * a.H;
+            r0 = n * rows + g * gr.rows, r1 = min(r0 + gr.rows, (n + 1) * rows);
+            const uint32_t tiles = ((uint32_t)tokens + BN - 1) / BN;
+            t0 = u - at.before, t1 = min(tiles, end - at.before);
+            whole = t0 == 0 && t1 == tiles && cu.pre == 0;
+            u = at.before + t1;
+            if (t1 == tiles) at = {n + 1, at.before + tiles};
         }
+        tokens = __builtin_amdgcn_readfirstlane(tokens);
+        if (t0 >= t1) continue;  // a sequence without tokens
+        const int tiles = (r1 - r0 + 31) / 32;              // row tiles
+        const int row = r0 + 32 * rt + c;                   // this lane's row in the wave's scores
+        const bool active = rt < tiles;
+        // tokens that a row sees: all for the prefix, all but the draft tokens after its own for a sequence
+        const int hidden = prefix ? 0 : a.S - 1 + n * a.S;  // (minus the row's token)
+        auto sees = [&](int r) { return prefix ? tokens : tokens - (hidden - r / a.H); };
+        const int first = __builtin_amdgcn_readfirstlane(sees(r0)), last = __builtin_amdgcn_readfirstlane(sees(r1 - 1));
+        const int mine = sees(min(row, r1 - 1));
+        const uint32_t stop = min(t1, last > 0 ? ((uint32_t)last + BN - 1) / BN : 0u);
+
+        // ---- queries: operand registers, straight from memory (rows past the end repeat the last one)
+        u32x4 q[36];
+        if (active) {
+            const int r = min(row, r1 - 1), t = r / a.H, h = r - t * a.H;
+            const uint16_t* ql = static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head + 8 * half;
+            const uint16_t* qp = static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head + 8 * half;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) q[i] = *reinterpret_cast<const u32x4*>(ql + 16 * i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[32 + i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
+        }
+
+        // ---- loads
+        const u32x4 table_rsrc = [&] {
+            u32x4 r = tile_rsrc(table);
+            r[2] = __builtin_amdgcn_readfirstlane(width) * 4;  // entries past the table read as zeros (and are past `last`)
+            return r;
+        }();
+        const uint32_t pages_at = lds + LDS_PAGES + w * 512;
+        auto load_pages = [&](uint32_t tile) {  // the page numbers of a tile's tokens
+            const uint32_t tok = tile * BN + lane;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
+                             __builtin_amdgcn_readfirstlane(pages_at + (tile & 1) * 256)),
+                         "v"(tok / (uint32_t)a.page_size * 4), "s"(table_rsrc)
+                         : "memory");
+        };
+        // tile -> buffer; returns which of its tokens are there (in the tokens that the group sees, not in a hole)
+        auto load_tile = [&](uint32_t tile, uint32_t buf) {
+            const uint32_t tok = tile * BN + lane;
+            const int page = *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 1) * 256 + lane * 4);
+            const bool in = tok < (uint32_t)last && page >= 0 && page < a.pages;
+            const uint64_t there = __builtin_amdgcn_ballot_w64(in);
+            const int64_t at_byte = in ? page * page_bytes + (int64_t)(tok % (uint32_t)a.page_size) * ROW_BYTES : 0;
+            const uint32_t lo = (uint32_t)at_byte, hi = (uint32_t)(at_byte >> 32);
+            const uint32_t base = lds + buf * TILE_BYTES;
+            // wave w brings tokens 16 w .. 16 w + 15, a token's 64 latent pieces at a time (swz16)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = 16 * w + i;
+                const uint64_t b = (uint64_t)__builtin_amdgcn_readlane(hi, t) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, t);
+                u32x4 rs = tile_rsrc(cache + b);
+                rs[2] = there >> t & 1 ? LAT_BYTES : 0;  // a token that is not there reads as zeros
+                load_to_lds(base + t * LAT_BYTES, rs, (uint32_t)(lane ^ swz16(i)) << 4, 0);
+            }
+            // positional parts, 8 lanes a token; one that is not there reads the cache's first row (its scores are replaced)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * w + 8 * i + (lane >> 3);
+                const uint64_t b = (uint64_t)(uint32_t)__shfl((int)hi, t) << 32 | (uint32_t)__shfl((int)lo, t);
+                const char* src = cache + b + LAT_BYTES + (((lane & 7) ^ swz8(t)) << 4);
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                                 __builtin_amdgcn_readfirstlane(base + TILE_PE + (16 * w + 8 * i) * PE_BYTES)),
+                             "v"(src)
+                             : "memory");
+            }
+            return there;
+        };
+
+        f32x16 acc[RT][4] = {};  // [row tile][32 values]
+        float mo[RT] = {M_START, M_START}, l = 0.f;
+        bool special = false;
+        uint64_t there = 0;
+        if (t0 < stop) {
+            load_pages(t0);
+            load_pages(t0 + 1);
+            wait_loads<0>();
+#pragma unroll
+            for (int i = 0; i < 36; ++i) asm volatile("" : "+v"(q[i]));  // the queries are there too: no later wait for them
+            there = load_tile(t0, t0 & 1);
+        }
+        for (uint32_t tile = t0; tile < stop; ++tile) {
+            wait_loads<0>();
+            lds_barrier();  // the tile is whole, and every wave is done with the one before it
+            const uint64_t now = there;
+            if (tile + 1 < stop) {
+                there = load_tile(tile + 1, (tile + 1) & 1);
+                load_pages(tile + 2);
+            }
+            const uint32_t tb = lds + (tile & 1) * TILE_BYTES;
+            const int k0 = (int)(tile * BN);
+            const bool mixed = k0 + BN > first;  // some row does not see some token of the tile
+            f32x16 s = {};
+            auto weights = [&](float m) {  // of this tile, relative to m; returns their sum
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    u32x4 pk;
+#pragma unroll
+                    for (int r = 0; r < 8; r += 2) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[8 * k + r], sc, -m));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[8 * k + r + 1], sc, -m));
+                        sum += x + y;
+                        pk[r >> 1] = T::pack(x, y);
+                    }
+                    *reinterpret_cast<u32x4*>(sm + LDS_P + (rt * 4 + 2 * kh + k) * 1024 + lane * 16) = pk;
+                }
+                return sum;
+            };
+            float sum = 0.f;
+            if (active) {
+                // ---- scores: 36 steps, the operands of the next four read while four run
+                auto key = [&](int i) {
+                    return i < 32 ? lds_read16(((tb + ka) ^ ((i & 7) << 5)) + (i >> 3) * 256)
+                                  : lds_read16((tb + pa) ^ ((i - 32) << 5));
+                };
+                u32x4 kf[2][4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) kf[0][x] = key(x);
+#pragma unroll
+                for (int i = 0; i < 9; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i < 8)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) kf[(i + 1) & 1][x] = key(4 * i + 4 + x);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s = T::mfma(kf[i & 1][x], q[4 * i + x], s);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (mixed || now != ~0ull) {
+                    const int left = mine - k0 - 32 * kh;
+                    const uint32_t vis = ((uint32_t)(now >> (32 * kh)) & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u)) >> (4 * half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (!(vis >> ((r & 3) + 8 * (r >> 2)) & 1)) s[r] = -INFINITY;
+                }
+                // ---- running softmax: weights relative to a past maximum, which is raised below only when some row of
+                // the wave exceeds it by SLACK (the result is the same for any reference)
+                float mx = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                mx = max_halves(mx) * sc;
+                const float m = rt ? mo[1] : mo[0];
+                const bool raise = __builtin_amdgcn_ballot_w64(mx - m > T::B + T::SLACK) != 0;
+                if (half == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + c) * 4) = mx;
+                if (lane == 0) *reinterpret_cast<int*>(sm + LDS_FLAG + w * 4) = raise;
+                sum = weights(m);
+            } else if (lane == 0) {
+                *reinterpret_cast<int*>(sm + LDS_FLAG + w * 4) = 0;
+            }
+            lds_barrier();  // weights, maxima and flags of all waves
+            const u32x4 fl = *reinterpret_cast<const u32x4*>(sm + LDS_FLAG);
+            if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3])) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    if (!__builtin_amdgcn_readfirstlane(fl[r] | fl[r + RT])) continue;
+                    const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (r * 32 + c) * 4);
+                    const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + ((r + RT) * 32 + c) * 4);
+                    const float mn = fmaxf(mo[r], fmaxf(m0, m1) - T::B);
+                    const float f = __builtin_amdgcn_exp2f(mo[r] - mn);
+                    mo[r] = mn;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                    if (r == rt) {
+                        l *= f;
+                        sum = weights(mn);
+                    }
+                }
+                lds_barrier();  // the weights anew
+            }
+            l += sum;
+            // ---- values: the wave's 128 of every row, 16 keys a step, the next step's operands read while one runs
+            auto value = [&](int k, int d) {
+                const u32x2 v0 = lds_read_tr(((tb + va[0]) ^ (d << 6)) + k * 16 * LAT_BYTES);
+                const u32x2 v1 = lds_read_tr(((tb + va[1]) ^ (d << 6)) + k * 16 * LAT_BYTES);
+                return u32x4{v0.x, v0.y, v1.x, v1.y};
+            };
+            auto weight = [&](int r, int k) { return lds_read16(lds + LDS_P + (r * 4 + k) * 1024 + lane * 16); };
+            u32x4 vf[2][4], pf[2][RT];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) vf[0][d] = value(0, d);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) pf[0][r] = weight(r, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (k < 3) {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) vf[(k + 1) & 1][d] = value(k + 1, d);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) pf[(k + 1) & 1][r] = weight(r, k + 1);
+                }
+                if (mixed)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        special |= nonfinite<T>(vf[k & 1][d]);
+                        vf[k & 1][d] = finite_part<T>(vf[k & 1][d]);
+                    }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) acc[r][d] = T::mfma(vf[k & 1][d], pf[k & 1][r], acc[r][d]);
+            }
+        }
+
+        if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the tokens that not every row sees
+#pragma unroll 1
+            for (int j = max(first, (int)(t0 * BN)); j < min(last, (int)(stop * BN)); ++j) {
+                const int page = table[j / a.page_size];
+                if (page < 0 || page >= a.pages) continue;
+                const uint16_t* vr = reinterpret_cast<const uint16_t*>(cache + page * page_bytes) + (int64_t)(j % a.page_size) * ROW +
+                                     128 * w + 4 * half;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int i = r0 + 32 * r + c;
+                    const bool seen = i < r1 && j < sees(min(i, r1 - 1));
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float x = T::up(vr[32 * d + 8 * (e >> 2) + (e & 3)]);
+                            if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] += x;
+                        }
+                }
+            }
+        }
+
+        // ---- results: the two waves of a row tile have summed half of its keys each
+        l = sum_halves(l);
+        if (half == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + c) * 4) = l;
+        lds_barrier();
+        float ls[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            ls[r] = *reinterpret_cast<const float*>(sm + LDS_MAX + (r * 32 + c) * 4) +
+                    *reinterpret_cast<const float*>(sm + LDS_MAX + ((r + RT) * 32 + c) * 4);
+        lds_barrier();  // free for the next segment
+        if (whole) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int i = r0 + 32 * r + c;
+                if (i >= r1) break;
+                const float inv = ls[r] > 0.f ? 1.f / ls[r] : 0.f;
+                const int t = i / a.H, h = i - t * a.H;
+                uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 128 * w + 4 * half;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<u32x2*>(o + 32 * d + 2 * e) =
+                            ls[r] == 0.f ? u32x2{0u, 0u}
+                                         : u32x2{T::pack(acc[r][d][e] * inv, acc[r][d][e + 1] * inv),
+                                                 T::pack(acc[r][d][e + 2] * inv, acc[r][d][e + 3] * inv)};
+                if (a.lse && w == 0 && half == 0)
+                    a.lse[i] = ls[r] == 0.f ? -INFINITY : (mo[r] + __builtin_amdgcn_logf(ls[r])) * 0.69314718055995f;
+            }
+        } else {
+            // the part's slot; piece + n names a sequence's parts uniquely, since both only grow along the tiles
+            const int64_t slot_bytes = (int64_t)(gr.rows / 32) * SLOT_TILE;
+            const int64_t slot = prefix ? (int64_t)id : ((int64_t)piece + n) * gr.groups + g;
+            char* out = static_cast<char*>(a.workspace) + (prefix ? 0 : p.pre_slots * (p.pre.rows / 32) * SLOT_TILE) + slot * slot_bytes;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                if (r0 + 32 * r + c >= r1) break;
+                char* o = out + r * SLOT_TILE + w * 16384 + lane * 16;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<f32x4*>(o + (d * 4 + e) * 1024) =
+                            f32x4{acc[r][d][4 * e], acc[r][d][4 * e + 1], acc[r][d][4 * e + 2], acc[r][d][4 * e + 3]};
+                if (w == 0 && half == 0) *reinterpret_cast<f32x2*>(out + r * SLOT_TILE + SLOT_ACC + c * 8) = f32x2{mo[r], ls[r]};
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ joining the parts
+// One workgroup for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
+// v, v + 4, ... and the waves' sums meet in LDS.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) join_kernel(KdaLatentDecodeArgs a, Plan p) {
+    __shared__ float sm_m[WAVES][32], sm_l[WAVES][32];
+    __shared__ f32x4 sm_a[WAVES][4][64];
+    const int tid = threadIdx.x, v = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int c = lane & 31, half = lane >> 5;
+    const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
+    const int rt = blockIdx.y >> 4, block = blockIdx.y & 15;  // value block: values 32 block ..
+    uint32_t own = 0, before = 0;
+    for (int i = lane; i < a.B; i += 64) {
+        const uint32_t t = tiles_of(a, i);
+        own += t;
+        if (i < n) before += t;
+    }
+    const Cut cu = cut(a, p, sum_wave(own));
+    before = sum_wave(before);
+    const uint32_t tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, n));
+    const uint32_t p0 = before / cu.run, p1 = tiles ? (before + tiles - 1) / cu.run + 1 : p0;
+    const uint32_t parts = p1 - p0, pre_parts = cu.pre ? cdiv(cu.pre, cu.run) : 0;
+    if (pre_parts == 0 && parts == 1) return;  // written by the workgroup that had it whole
+    const int rows = a.S * a.H;
+    const int rq = g * p.own.rows + 32 * rt;  // within the sequence
+    if (rq >= rows) return;
+    const int r = n * rows + rq + c;
+    const bool valid = rq + c < rows && 32 * rt < p.own.rows;
+
+    float m = M_START, l = 0.f;
+    f32x4 acc[4] = {};
+    auto add = [&](const char* slot_tile, int cc) {
+        const f32x2 ml = *reinterpret_cast<const f32x2*>(slot_tile + SLOT_ACC + cc * 8);
+        f32x4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = *reinterpret_cast<const f32x4*>(slot_tile + (block * 4 + e) * 1024 + (32 * half + cc) * 16);
+        const float mn = fmaxf(m, ml.x);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+        m = mn;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f0 + x[e] * f1;
     };
-    if (a.prefix_table) walk(a.prefix_table, a.prefix_width, a.prefix_len[0], 0);
-    walk(a.block_table + n * a.table_stride, a.table_width, a.seq_lens[n], a.S - 1 - s);
-    finish<T>(c, a.out, t * a.out_row + h * a.out_head, a.lse ? a.lse + t * a.H + h : nullptr);
+    if (valid) {
+        const char* ws = static_cast<const char*>(a.workspace);
+        const int64_t own_bytes = (int64_t)(p.own.rows / 32) * SLOT_TILE, pre_bytes = (int64_t)(p.pre.rows / 32) * SLOT_TILE;
+        const char* own_ws = ws + p.pre_slots * pre_bytes + g * own_bytes + rt * SLOT_TILE;
+        for (uint32_t i = v; i < parts; i += WAVES) add(own_ws + ((int64_t)p0 + i + n) * p.own.groups * own_bytes, c);
+        if (pre_parts) {
+            const int gp = r / p.pre.rows, rp = r - gp * p.pre.rows;
+            const char* pre_ws = ws + gp * pre_bytes + (rp >> 5) * SLOT_TILE;
+            for (uint32_t i = v; i < pre_parts; i += WAVES) add(pre_ws + (int64_t)i * p.pre.groups * pre_bytes, rp & 31);
+        }
+    }
+    if (half == 0) {
+        sm_m[v][c] = m;
+        sm_l[v][c] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sm_a[v][e][lane] = acc[e];
+    __syncthreads();
+    if (!valid) return;
+    float M = M_START, L = 0.f, f[WAVES];
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) M = fmaxf(M, sm_m[i][c]);
+    f32x4 o = {};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        f[i] = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
+        L += sm_l[i][c] * f[i];
+        o += sm_a[i][v][lane] * f[i];  // wave v finishes values 8 v .. 8 v + 7 of the block
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const int t = r / a.H, h = r - t * a.H;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 32 * block + 8 * v + 4 * half;
+    *reinterpret_cast<u32x2*>(out) = L == 0.f ? u32x2{0u, 0u} : u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+    if (a.lse && block == 0 && v == 0 && half == 0) a.lse[r] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.69314718055995f;
 }
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 // rows of 16-byte pieces: aligned base, strides in multiples of 8 elements
 bool rows16(const void* p, int64_t s0, int64_t s1 = 0) { return aligned(p, 16) && s0 % 8 == 0 && s1 % 8 == 0; }
 
-int launched(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return 0;
-    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
-    return KDA355_ELAUNCH;
-}
-
 int check_decode_sizes(const KdaLatentDecodeArgs* a) {
     KDA_CHECK_ARG(a != nullptr, "latent_decode: null args");
     KDA_CHECK_ARG(a->B >= 0 && a->S >= 1 && a->H >= 1 && a->page_size >= 1 && a->table_width >= 0 && a->prefix_width >= 0 &&
-                      a->num_cus >= 0,
+                      a->num_cus >= 0 && a->num_cus <= 65536,
                   "latent_decode: B=%d S=%d H=%d page_size=%d table_width=%d prefix_width=%d num_cus=%d", a->B, a->S, a->H,
                   a->page_size, a->table_width, a->prefix_width, a->num_cus);
-    KDA_CHECK_ARG((int64_t)a->B * a->S * a->H < (1ll << 31), "latent_decode: B * S * H is too large");
-    KDA_CHECK_ARG((int64_t)a->table_width * a->page_size < (1ll << 31) && (int64_t)a->prefix_width * a->page_size < (1ll << 31),
+    KDA_CHECK_ARG((int64_t)a->S * a->H < (1ll << 31) && (int64_t)a->B * a->S * a->H < (1ll << 29) && a->B < (1 << 22),
+                  "latent_decode: B * S * H is too large");
+    const int64_t span = (int64_t)a->table_width * a->page_size;
+    KDA_CHECK_ARG(span < (1ll << 31) && (int64_t)a->prefix_width * a->page_size < (1ll << 31),
                   "latent_decode: a table spans 2^31 tokens or more");
+    KDA_CHECK_ARG(a->table_width < (1 << 28) && a->prefix_width < (1 << 28), "latent_decode: a table of 2^28 pages or more");
+    KDA_CHECK_ARG(a->B * (span / BN + 1) < (1ll << 31), "latent_decode: the tables span 2^36 tokens or more");
     return 0;
+}
+
+Plan plan_of(const KdaLatentDecodeArgs* a) {
+    Plan p;
+    p.own = Groups::of((int64_t)a->S * a->H);
+    p.pre = a->prefix_width ? Groups::of((int64_t)a->B * a->S * a->H) : Groups{32, 0};
+    const int cus = a->num_cus ? a->num_cus : 256;
+    p.grid = cus > p.own.groups + p.pre.groups ? cus : p.own.groups + p.pre.groups;
+    p.pre_slots = p.pre.groups ? p.grid : 0;
+    return p;
 }
 
 }  // namespace
@@ -116,7 +562,10 @@ using namespace kda355;
 
 extern "C" int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArgs* a) {
     if (const int rc = check_decode_sizes(a)) return rc;
-    return 0;
+    if (a->B == 0) return 0;
+    const Plan p = plan_of(a);
+    const int64_t own = p.grid + (int64_t)a->B * p.own.groups;
+    return (p.pre_slots * (p.pre.rows / 32) + own * (p.own.rows / 32)) * SLOT_TILE;
 }
 
 extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
@@ -126,7 +575,8 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     if (a->B == 0) return 0;
     KDA_CHECK_ARG(a->q_latent && a->q_pe && a->cache && a->block_table && a->seq_lens && a->out && a->table_width >= 1,
                   "latent_decode: a required pointer is null");
-    KDA_CHECK_ARG(!a->prefix_table || (a->prefix_len && a->prefix_width >= 1), "latent_decode: prefix_table needs prefix_len");
+    KDA_CHECK_ARG(a->prefix_table ? a->prefix_len && a->prefix_width >= 1 : a->prefix_width == 0,
+                  "latent_decode: prefix_table needs prefix_len and prefix_width");
     KDA_CHECK_ARG(a->pages >= 1 && a->table_stride >= a->table_width, "latent_decode: pages=%lld table_stride=%lld",
                   (long long)a->pages, (long long)a->table_stride);
     KDA_CHECK_ARG(rows16(a->q_latent, a->ql_row, a->ql_head) && rows16(a->q_pe, a->qp_row, a->qp_head) &&
@@ -134,14 +584,24 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
                   "latent_decode: q and out rows must be 16-byte aligned");
     KDA_CHECK_ARG(rows16(a->cache, a->page_stride) && a->page_stride >= (int64_t)a->page_size * ROW,
                   "latent_decode: cache pages must be dense and 16-byte aligned");
+    KDA_CHECK_ARG(a->scale > 0.f, "latent_decode: scale must be positive");
     const int64_t need = kda355_latent_decode_workspace_bytes(a);
-    KDA_CHECK_ARG(need == 0 || (a->workspace && aligned(a->workspace, 256) && a->workspace_bytes >= need),
+    KDA_CHECK_ARG(a->workspace && aligned(a->workspace, 256) && a->workspace_bytes >= need,
                   "latent_decode: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((uint32_t)(a->B * a->S), a->H);
-    if (a->dtype == KDA355_DTYPE_BF16)
-        hipLaunchKernelGGL(decode_kernel<__bf16>, grid, dim3(256), 0, s, *a);
-    else
-        hipLaunchKernelGGL(decode_kernel<_Float16>, grid, dim3(256), 0, s, *a);
-    return launched("latent_decode");
+    const Plan p = plan_of(a);
+    const dim3 join((uint32_t)a->B * p.own.groups, p.own.rows / 32 * 16);
+    if (a->dtype == KDA355_DTYPE_BF16) {
+        hipLaunchKernelGGL(decode_kernel<Bf16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+        hipLaunchKernelGGL(join_kernel<Bf16>, join, dim3(THREADS), 0, s, *a, p);
+    } else {
+        hipLaunchKernelGGL(decode_kernel<Fp16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+        hipLaunchKernelGGL(join_kernel<Fp16>, join, dim3(THREADS), 0, s, *a, p);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) {
+        set_error("latent_decode: launch failed: %s", hipGetErrorString(e));
+        return KDA355_ELAUNCH;
+    }
+    return 0;
 }

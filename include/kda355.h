@@ -334,7 +334,8 @@ int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* args, kda355_stream
  * seq_lens[n] cached tokens, the S new ones among them: token s sees j < seq_lens[n] - (S - 1 - s).  seq_lens is clamped
  * to [0, table_width * page_size].
  * With prefix_table, every sequence first sees the prefix_len[0] tokens of those pages (all S tokens see all of them),
- * then its own; the prefix is read once for all rows.  A row that sees nothing gets zeros and an lse of -inf.
+ * then its own; the prefix is read once for all rows.  A row that sees nothing gets zeros and an lse of -inf.  scale must be
+ * positive, B * S * H below 2^29.
  */
 typedef struct KdaLatentDecodeArgs {
     const void* q_latent;        /* [B * S, H, 512], strides in elements */

@@ -88,7 +88,10 @@ BAD += [("latent_decode", _decode_args, kw, msg) for kw, msg in [
     (dict(table_width=0), b"null"), (dict(prefix_table=FAKE), b"prefix_len"),
     (dict(prefix_table=FAKE, prefix_len=FAKE, prefix_width=0), b"prefix_len"), (dict(pages=0), b"pages"),
     (dict(table_stride=3), b"table_stride"), (dict(q_latent=FAKE + 8), b"aligned"), (dict(qp_row=4), b"aligned"),
-    (dict(out=FAKE + 2), b"aligned"), (dict(page_stride=64 * 576 - 8), b"dense"), (dict(cache=FAKE + 8), b"aligned")]]
+    (dict(out=FAKE + 2), b"aligned"), (dict(page_stride=64 * 576 - 8), b"dense"), (dict(cache=FAKE + 8), b"aligned"),
+    (dict(scale=0.0), b"positive"), (dict(scale=float("nan")), b"positive"), (dict(num_cus=-1), b"num_cus"),
+    (dict(table_width=1 << 28, page_size=1), b"2^28"), (dict(prefix_width=8), b"prefix_table"),
+    (dict(B=1 << 22), b"too large"), (dict(workspace=0), b"workspace"), (dict(workspace_bytes=0), b"workspace")]]
 BAD += [(op, _tokens_args, kw, msg) for op in ("latent_append", "latent_gather") for kw, msg in [
     (dict(T=-1), b"T=-1"), (dict(pages=0), b"pages=0"), (dict(page_size=0), b"page_size=0"), (dict(cache=0), b"null"),
     (dict(T=1 << 25), b"2^25"), (dict(page_stride=100), b"dense"), (dict(cache=FAKE + 4), b"aligned")]]
