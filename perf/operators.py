@@ -387,9 +387,8 @@ def _plain_compact(st):
 
 # --------------------------------------------------------------------------------------------------------- own kernels
 def _kda355():
-    pkg = str(Path(__file__).resolve().parent.parent / "eat-kernels_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
+    if "kda355" not in sys.modules:  # a program finds its package once, not at every call
+        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "eat-kernels_amd"))
     import kda355
     return kda355
 
