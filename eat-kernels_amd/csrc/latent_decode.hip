@@ -36,7 +36,10 @@ struct Plan {
     Groups own, pre;       // of a sequence's rows; of all rows of the batch, for the prefix (no groups: no prefix)
     int grid;
     int64_t pre_slots;     // workspace: prefix parts, then the sequences'
+    uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift, x < 2^31
 };
+__device__ __forceinline__ uint32_t page_of(const Plan& p, uint32_t tok) { return (uint32_t)((uint64_t)tok * p.page_mul >> p.page_shift); }
+__device__ const uint4 zero_row[ROW_BYTES / 16] = {};  // what a token that is not there reads
 
 // ------------------------------------------------------------------------------------------------ who does what
 struct Cut {
@@ -131,6 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
     const float sc = a.scale * 1.44269504088896f;
     const int64_t page_bytes = a.page_stride * 2;
     const char* const cache = static_cast<const char*>(a.cache);
+    const uint32_t turned = (lane + 16 * w) & 63;  // the token of a tile whose address this lane computes
     const int rt = w & 1, kh = w >> 1;  // the wave's scores: row tile, keys 32 kh ..
     // LDS read addresses within a tile: key 32 kh + c (scores), values as in the second product (attend.h)
     const uint32_t ka = (32 * kh + c) * LAT_BYTES + ((half ^ swz16(c)) << 4);
@@ -198,57 +202,60 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
             return r;
         }();
         const uint32_t pages_at = lds + LDS_PAGES + w * 512;
-        auto load_pages = [&](uint32_t tile) {  // the page numbers of a tile's tokens
-            const uint32_t tok = tile * BN + lane;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
+        auto load_pages = [&](uint32_t tile) {  // the page numbers of a tile's tokens, the wave's own 16 first
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane(pages_at + (tile & 1) * 256)),
-                         "v"(tok / (uint32_t)a.page_size * 4), "s"(table_rsrc)
+                         "v"(page_of(p, tile * BN + turned) * 4), "s"(table_rsrc)
                          : "memory");
         };
         // tile -> buffer; returns which of its tokens are there (in the tokens that the group sees, not in a hole)
         auto load_tile = [&](uint32_t tile, uint32_t buf) {
-            const uint32_t tok = tile * BN + lane;
+            const uint32_t tok = tile * BN + turned;
             const int page = *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 1) * 256 + lane * 4);
             const bool in = tok < (uint32_t)last && page >= 0 && page < a.pages;
             const uint64_t there = __builtin_amdgcn_ballot_w64(in);
-            const int64_t at_byte = in ? page * page_bytes + (int64_t)(tok % (uint32_t)a.page_size) * ROW_BYTES : 0;
+            const uint64_t at_byte = (uint64_t)(in ? cache + (page * page_bytes + (int64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES)
+                                                   : reinterpret_cast<const char*>(zero_row));
             const uint32_t lo = (uint32_t)at_byte, hi = (uint32_t)(at_byte >> 32);
-            const uint32_t base = lds + buf * TILE_BYTES;
+            uint32_t lane16 = lane << 4;
+            asm("" : "+v"(lane16));  // the 16 offsets below are made anew for every tile, not kept in registers
+            const uint32_t base = lds + buf * TILE_BYTES + 16 * w * LAT_BYTES, pe = lds + buf * TILE_BYTES + TILE_PE + 16 * w * PE_BYTES;
             // wave w brings tokens 16 w .. 16 w + 15, a token's 64 latent pieces at a time (swz16)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int t = 16 * w + i;
-                const uint64_t b = (uint64_t)__builtin_amdgcn_readlane(hi, t) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, t);
-                u32x4 rs = tile_rsrc(cache + b);
-                rs[2] = there >> t & 1 ? LAT_BYTES : 0;  // a token that is not there reads as zeros
-                load_to_lds(base + t * LAT_BYTES, rs, (uint32_t)(lane ^ swz16(i)) << 4, 0);
+            for (int i = 0; i < 16; i += 4) {
+                uint64_t b[4];
+                uint32_t v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    b[x] = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i + x) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i + x);
+                    v[x] = lane16 ^ swz16(i + x) << 4;
+                }
+                load_rows4(base + i * LAT_BYTES, b, v);
             }
-            // positional parts, 8 lanes a token; one that is not there reads the cache's first row (its scores are replaced)
+            // positional parts, 8 lanes a token
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int t = 16 * w + 8 * i + (lane >> 3);
+                const int t = 8 * i + (lane >> 3);
                 const uint64_t b = (uint64_t)(uint32_t)__shfl((int)hi, t) << 32 | (uint32_t)__shfl((int)lo, t);
-                const char* src = cache + b + LAT_BYTES + (((lane & 7) ^ swz8(t)) << 4);
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
-                                 __builtin_amdgcn_readfirstlane(base + TILE_PE + (16 * w + 8 * i) * PE_BYTES)),
-                             "v"(src)
+                                 __builtin_amdgcn_readfirstlane(pe + 8 * i * PE_BYTES)),
+                             "v"(b + LAT_BYTES + (((lane & 7) ^ swz8(t)) << 4))
                              : "memory");
             }
-            return there;
+            return w ? there << (16 * w) | there >> (64 - 16 * w) : there;
         };
 
         f32x16 acc[RT][4] = {};  // [row tile][32 values]
         float mo[RT] = {M_START, M_START}, l = 0.f;
         bool special = false;
         uint64_t there = 0;
-        if (t0 < stop) {
-            load_pages(t0);
-            load_pages(t0 + 1);
-            wait_loads<0>();
+        load_pages(t0);
+        load_pages(t0 + 1);
+        wait_loads<0>();
 #pragma unroll
-            for (int i = 0; i < 36; ++i) asm volatile("" : "+v"(q[i]));  // the queries are there too: no later wait for them
-            there = load_tile(t0, t0 & 1);
-        }
+        // the queries are there too (the compiler waits for them here and not in the loop), in accumulation registers
+        for (int i = 0; i < 36; ++i) asm volatile("" : "+a"(q[i]));
+        if (t0 < stop) there = load_tile(t0, t0 & 1);
         for (uint32_t tile = t0; tile < stop; ++tile) {
             wait_loads<0>();
             lds_barrier();  // the tile is whole, and every wave is done with the one before it
@@ -285,6 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
                                   : lds_read16((tb + pa) ^ ((i - 32) << 5));
                 };
                 u32x4 kf[2][4];
+                f32x16 s2 = {};  // two chains of products
 #pragma unroll
                 for (int x = 0; x < 4; ++x) kf[0][x] = key(x);
 #pragma unroll
@@ -294,9 +302,10 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                         for (int x = 0; x < 4; ++x) kf[(i + 1) & 1][x] = key(4 * i + 4 + x);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) s = T::mfma(kf[i & 1][x], q[4 * i + x], s);
+                    for (int x = 0; x < 4; ++x) (x & 1 ? s2 : s) = T::mfma(kf[i & 1][x], q[4 * i + x], x & 1 ? s2 : s);
                 }
                 __builtin_amdgcn_sched_barrier(0);
+                s += s2;
                 if (mixed || now != ~0ull) {
                     const int left = mine - k0 - 32 * kh;
                     const uint32_t vis = ((uint32_t)(now >> (32 * kh)) & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u)) >> (4 * half);
@@ -552,6 +561,10 @@ Plan plan_of(const KdaLatentDecodeArgs* a) {
     const int cus = a->num_cus ? a->num_cus : 256;
     p.grid = cus > p.own.groups + p.pre.groups ? cus : p.own.groups + p.pre.groups;
     p.pre_slots = p.pre.groups ? p.grid : 0;
+    int bits = 0;  // 2^bits >= page_size: page_mul page_size = 2^(31 + bits) + e, e < 2^bits, so the quotient is exact
+    while ((1ll << bits) < a->page_size) ++bits;
+    p.page_shift = 31 + bits;
+    p.page_mul = (uint32_t)(((1ull << p.page_shift) + a->page_size - 1) / a->page_size);
     return p;
 }
 

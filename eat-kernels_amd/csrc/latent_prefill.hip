@@ -96,15 +96,18 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
                     pr = tile_rsrc(ph + (int64_t)t0 * a.pe_row);
         const uint32_t base = lds + buf * TILE_BYTES + 16 * w * (HD * 2), pbase = lds + buf * TILE_BYTES + TILE_PE + 16 * w * (PE * 2);
         auto issue = [&](auto whole) {
+            uint32_t ko[4], vo[4], ks[4], vs[4], po[2], ps[2];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = whole || lt + 4 * i < left;
-                load_to_lds(base + 4 * i * (HD * 2), kr, in ? koff[i] : LDS_ZERO, i * kstep);
-                load_to_lds(base + TILE_V + 4 * i * (HD * 2), vr, in ? voff[i] : LDS_ZERO, i * vstep);
+                ko[i] = in ? koff[i] : LDS_ZERO, ks[i] = i * kstep;
+                vo[i] = in ? voff[i] : LDS_ZERO, vs[i] = i * vstep;
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                load_to_lds(pbase + 8 * i * (PE * 2), pr, whole || pt + 8 * i < left ? poff[i] : LDS_ZERO, i * pstep);
+            for (int i = 0; i < 2; ++i) po[i] = whole || pt + 8 * i < left ? poff[i] : LDS_ZERO, ps[i] = i * pstep;
+            load_to_lds4(base, kr, ko, ks);
+            load_to_lds4(base + TILE_V, vr, vo, vs);
+            load_to_lds2(pbase, pr, po, ps);
         };
         if (left >= BN) issue(std::true_type{}); else issue(std::false_type{});
     };
