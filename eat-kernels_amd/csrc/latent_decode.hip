@@ -1,16 +1,21 @@
 // Latent attention, absorbed form over a paged cache (gfx950): all heads of a sequence read the same 576-wide token rows, whose
 // first 512 values are keys and values at once.
 //
-// The query rows (token, head) of a sequence are taken in groups of up to 64 (two row tiles of 32) and the keys in tiles of 64.
+// The query rows (token, head) of a sequence are taken in groups of up to 64 (two row tiles of 32) and the keys in tiles of 32.
 // The work is cut along the keys: a launch of about one workgroup a CU, each with an equal run of key tiles through the packed
 // sequences (all groups of a sequence side by side, so that their reads of the same keys meet in one L2), and with a shared
 // prefix some of the workgroups walk its tiles for groups of all rows of the batch.  Every workgroup finds its run from the
 // lengths on the device.  A run that holds a sequence whole writes its output; parts are left in the workspace in fp32 and
 // joined by a second kernel:  o = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s.
 //
-// Token rows come straight into LDS (72 KiB a tile, the next one under way while one is computed).  Of the 4 waves, wave w
-// computes the scores of row tile w % 2 with keys 32 (w / 2) .. + 31 of the tile (its queries in 144 registers), and then
-// values 128 w .. 128 w + 127 of all rows and keys, with the other waves' weights read from LDS.
+// 8 waves, two a SIMD, of two kinds.  In the step of tile j the score waves 0 .. 3 (row tile w % 2, keys 16 (w / 2) .. + 15; their
+// queries in 144 registers) compute its scores and leave its weights in LDS, while the value waves 4 .. 7 add tile j - 1 to values
+// 128 (w - 4) .. + 127 of all rows (128 accumulators) and bring tile j + 2 straight into LDS (36 KiB a tile, four tiles): matrix
+// instructions of one kind run beside the softmax, the waits and the address arithmetic of the other.  One barrier a tile.
+// Scores come from 16x16x32 instructions (keys as rows), so that every key fragment read serves two of them; values from
+// 32x32x16 with one fragment for both row tiles.
+#include <type_traits>
+
 #include "attend.h"
 
 namespace kda355 {
@@ -18,8 +23,10 @@ namespace {
 
 constexpr int LAT = KDA355_LATENT_DIM, ROW = KDA355_LATENT_ROW, PE = KDA355_LATENT_PE;
 constexpr int ROW_BYTES = ROW * 2, LAT_BYTES = LAT * 2, PE_BYTES = PE * 2;
-constexpr int WAVES = 4, THREADS = WAVES * 64;
-constexpr int BN = 64;                                  // keys of a tile
+constexpr int SCORE_WAVES = 4, VALUE_WAVES = 4, THREADS = (SCORE_WAVES + VALUE_WAVES) * 64;
+constexpr int JOIN_WAVES = 4;
+constexpr int BN = 32, BUFS = 4;                        // keys of a tile, tiles in LDS
+constexpr int LOADS = 10;                               // of a value wave a tile: 8 of latent rows, positional parts, page numbers
 constexpr int RT = 2, MAX_ROWS = 32 * RT;               // row tiles, query rows of a group
 constexpr uint32_t MIN_TILES = 1;                       // least run of a workgroup
 constexpr int SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;  // workspace of 32 rows: accumulators, (m, l) of each row
@@ -100,16 +107,41 @@ __device__ __forceinline__ At sequence_of(const KdaLatentDecodeArgs& a, uint32_t
 }
 
 // ------------------------------------------------------------------------------------------------ LDS
-constexpr int TILE_PE = BN * LAT_BYTES, TILE_BYTES = TILE_PE + BN * PE_BYTES;  // latent rows | positional parts
-constexpr int LDS_P = 2 * TILE_BYTES;                // weights: [row tile][16-key step][lane] 16 bytes
-constexpr int LDS_MAX = LDS_P + RT * 4 * 1024;       // a tile's maxima [wave][32], at the end the sums of rows
-constexpr int LDS_FLAG = LDS_MAX + WAVES * 128;      // does wave w's tile raise the maximum
-constexpr int LDS_PAGES = LDS_FLAG + 256;            // page numbers of a tile's tokens: [wave][tile % 2][64]
-constexpr int LDS_BYTES = LDS_PAGES + WAVES * 2 * 256;
+// A tile: latent rows in blocks of 4 tokens x 16 pieces of 16 bytes, piece p of token t at block 4 (t / 4) + p / 16, row t % 4,
+// place (p % 16) ^ turn(t) (a block is one load of a wave); then the positional parts, piece p of token t at p ^ swz8(t).
+// 16-byte reads go 16 lanes at a time, lanes 0 .. 3, 12 .. 15, 20 .. 23, 24 .. 27 of 32 and the others, transposed reads 16 lanes
+// in order: with this turn the former touch all 16 places of 256 bytes (4 cycles each; 8 with other turns that were measured) and the
+// latter all 8 of 128.
+__device__ __forceinline__ int turn(int t) { return (t & 3) << 1 | (t >> 3 & 1) | ((t >> 2 ^ t >> 3) & 1) << 3; }
+constexpr int BLOCK = 1024, TILE_PE = BN * LAT_BYTES, TILE_BYTES = TILE_PE + BN * PE_BYTES;
+constexpr int LDS_P = BUFS * TILE_BYTES;             // weights: [tile % 2][row tile][16-key step][row][key] 16 bits
+constexpr int LDS_MAX = LDS_P + 2 * 4096;            // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
+constexpr int LDS_FLAG = LDS_MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
+constexpr int LDS_THERE = LDS_FLAG + 64;             // is the token there [tile % 4][32] bytes
+constexpr int LDS_PAGES = LDS_THERE + 4 * BN;        // page numbers [value wave][tile % 4][64]
+constexpr int LDS_BYTES = LDS_PAGES + VALUE_WAVES * 4 * 256;
 static_assert(LDS_BYTES <= 160 * 1024, "");
 
+// 64 lanes x 16 bytes from src (a lane's) + OFFSET into a block of LDS (the instruction adds its offset to both addresses)
+template <int OFFSET>
+__device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(__builtin_amdgcn_readfirstlane(lds - OFFSET)),
+                 "v"(src), "n"(OFFSET)
+                 : "memory");
+}
+template <int I>
+using Int = std::integral_constant<int, I>;
+// the four lane groups of 16 joined
+template <typename F>
+__device__ __forceinline__ float join_groups(float x, F f) {
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = f(__uint_as_float(a.x), __uint_as_float(a.y));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return f(__uint_as_float(b.x), __uint_as_float(b.y));
+}
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
+__global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
     __shared__ __align__(1024) unsigned char sm[LDS_BYTES];
     const uint32_t lds = lds_offset(sm);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -134,17 +166,21 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
     const float sc = a.scale * 1.44269504088896f;
     const int64_t page_bytes = a.page_stride * 2;
     const char* const cache = static_cast<const char*>(a.cache);
-    const uint32_t turned = (lane + 16 * w) & 63;  // the token of a tile whose address this lane computes
-    const int rt = w & 1, kh = w >> 1;  // the wave's scores: row tile, keys 32 kh ..
-    // LDS read addresses within a tile: key 32 kh + c (scores), values as in the second product (attend.h)
-    const uint32_t ka = (32 * kh + c) * LAT_BYTES + ((half ^ swz16(c)) << 4);
-    const uint32_t pa = TILE_PE + (32 * kh + c) * PE_BYTES + ((half ^ swz8(c)) << 4);
+    const bool scores = w < SCORE_WAVES;
+    const int rt = w & 1, kh = w >> 1 & 1;  // a score wave's row tile and keys 16 kh ..
+    const int vw = w & 3;                   // a value wave's 128 values
+    const int c16 = lane & 15, quad = lane >> 4;
+    // LDS read addresses within a tile: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step; values as operand rows
+    // (key 8 half + e of a 16-key step is element e)
+    const int kt = 16 * kh + c16;
+    const uint32_t ka = (kt >> 2) * (4 * BLOCK) + (kt & 3) * 256 + ((quad ^ turn(kt)) << 4);
+    const uint32_t pa = TILE_PE + kt * PE_BYTES + ((quad ^ swz8(kt)) << 4);
     uint32_t va[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        const int i16 = lane & 15, t = 4 * half + 8 * x + (i16 >> 2);
-        const int e = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-        va[x] = t * LAT_BYTES + w * 256 + ((e ^ swz16(t)) << 4) + (i16 & 1) * 8;
+        const int t = 8 * half + 4 * x + (c16 >> 2);
+        const int e = 2 * (quad & 1) + ((c16 & 3) >> 1);
+        va[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
     }
 
     while (u < end) {
@@ -173,213 +209,288 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
         }
         tokens = __builtin_amdgcn_readfirstlane(tokens);
         if (t0 >= t1) continue;  // a sequence without tokens
-        const int tiles = (r1 - r0 + 31) / 32;              // row tiles
-        const int row = r0 + 32 * rt + c;                   // this lane's row in the wave's scores
-        const bool active = rt < tiles;
         // tokens that a row sees: all for the prefix, all but the draft tokens after its own for a sequence
         const int hidden = prefix ? 0 : a.S - 1 + n * a.S;  // (minus the row's token)
         auto sees = [&](int r) { return prefix ? tokens : tokens - (hidden - r / a.H); };
         const int first = __builtin_amdgcn_readfirstlane(sees(r0)), last = __builtin_amdgcn_readfirstlane(sees(r1 - 1));
-        const int mine = sees(min(row, r1 - 1));
-        const uint32_t stop = min(t1, last > 0 ? ((uint32_t)last + BN - 1) / BN : 0u);
+        const uint32_t stop = max(t0, min(t1, last > 0 ? ((uint32_t)last + BN - 1) / BN : 0u));
 
-        // ---- queries: operand registers, straight from memory (rows past the end repeat the last one)
-        u32x4 q[36];
-        if (active) {
-            const int r = min(row, r1 - 1), t = r / a.H, h = r - t * a.H;
-            const uint16_t* ql = static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head + 8 * half;
-            const uint16_t* qp = static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head + 8 * half;
+        const uint32_t n_tiles = stop - t0;
+        // A tile's weights are relative to a past maximum of their rows, which is raised only when some row of a wave exceeds it
+        // by SLACK (the result is the same for any reference): after the fact, at the start of the next step.
+        auto flags = [&](uint32_t tile) { return *reinterpret_cast<const u32x4*>(sm + LDS_FLAG + (tile & 1) * 16); };
+        auto any = [](u32x4 fl) { return __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0; };
+        // the new reference of the group's row r after `tile`; returns the factor of what is there
+        auto raise = [&](uint32_t tile, int r, float& m) {
+            const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + r * 4);
+            const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + (RT * 32 + r) * 4);
+            const float mn = fmaxf(m, fmaxf(m0, m1) - T::B), f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            return f;
+        };
+        if (scores) {
+            // ================================================================ score waves
+            const int row0 = r0 + 32 * rt + c16;  // this lane's rows: row0, row0 + 16
+            u32x4 q[2][18];  // operand registers, straight from memory (rows past the end repeat the last one)
+            int mine[2];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) q[i] = *reinterpret_cast<const u32x4*>(ql + 16 * i);
+            for (int x = 0; x < 2; ++x) {
+                const int r = min(row0 + 16 * x, r1 - 1), t = r / a.H, h = r - t * a.H;
+                mine[x] = sees(r);
+                const uint16_t* ql = static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head + 8 * quad;
+                const uint16_t* qp = static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head + 8 * quad;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[32 + i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
+                for (int i = 0; i < 16; ++i) q[x][i] = *reinterpret_cast<const u32x4*>(ql + 32 * i);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) q[x][16 + i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+            }
+            float mo[2] = {M_START, M_START}, l[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+            f32x4 s[2] = {};
+            auto weights = [&](uint32_t tile, int x) {  // of rows row0 + 16 x, relative to mo[x]; leaves their sum
+                float p0[4];
+                sum[x] = 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p0[r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], sc, -mo[x]));
+                    sum[x] += p0[r];
+                }
+                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * rt + kh) * 1024 + x * 512 + c16 * 32 + quad * 8) =
+                    u32x2{T::pack(p0[0], p0[1]), T::pack(p0[2], p0[3])};
+            };
+            auto settle = [&](uint32_t tile, u32x4 fl) {  // what the step of `tile` left open
+                if (any(fl)) {
+                    if (__builtin_amdgcn_readfirstlane(rt ? fl[1] | fl[3] : fl[0] | fl[2]))
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            l[x] *= raise(tile, 32 * rt + 16 * x + c16, mo[x]);
+                            weights(tile, x);
+                        }
+                    lds_barrier();  // the weights anew
+                }
+                l[0] += sum[0];
+                l[1] += sum[1];
+            };
+            u32x4 fl = {};
+            lds_barrier();  // the first tile
+            for (uint32_t tile = t0; tile < stop; ++tile) {
+                const uint32_t tb = lds + (tile % BUFS) * TILE_BYTES;
+                const int k0 = (int)(tile * BN);
+                if (tile > t0) fl = flags(tile - 1);
+                const int there8 = *(sm + LDS_THERE + (tile % BUFS) * BN + c);
+                // ---- 18 steps for both halves of the rows, in two chains each, the operands read five steps ahead
+                auto key = [&](int i) {
+                    return i < 16 ? lds_read16(((tb + ka) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tb + pa) ^ ((i - 16) << 6));
+                };
+                f32x4 z[2][2] = {};
+                u32x4 kf[6];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) kf[i] = key(i);
+                __builtin_amdgcn_sched_barrier(0);
+                settle(tile - 1, fl);
+#pragma unroll
+                for (int i = 0; i < 18; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i + 5 < 18) kf[(i + 5) % 6] = key(i + 5);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) z[y][i & 1] = T::mfma16(kf[i % 6], q[y][i], z[y][i & 1]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) s[x] = z[x][0] + z[x][1];
+                const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(there8 != 0);
+                if (k0 + BN > first || there != ~0u) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int left = mine[x] - k0;
+                        const uint32_t vis = (there & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u)) >> (16 * kh + 4 * quad);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!(vis >> r & 1)) s[x][r] = -INFINITY;
+                    }
+                }
+                float mx[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    mx[x] = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
+                    mx[x] = join_groups(mx[x], [](float p, float q) { return fmaxf(p, q); }) * sc;
+                    *reinterpret_cast<float*>(sm + LDS_MAX + (tile & 1) * 512 + (w * 32 + 16 * x + c16) * 4) = mx[x];  // (the groups' values agree)
+                    weights(tile, x);
+                }
+                const bool up = __builtin_amdgcn_ballot_w64(fmaxf(mx[0] - mo[0], mx[1] - mo[1]) > T::B + T::SLACK) != 0;
+                *reinterpret_cast<int*>(sm + LDS_FLAG + (tile & 1) * 16 + w * 4) = up;
+                lds_barrier();  // the tile's weights; the next tile is whole
+            }
+            if (n_tiles) settle(stop - 1, flags(stop - 1));
+            lds_barrier();  // the last maxima are read
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                l[x] = join_groups(l[x], [](float p, float q) { return p + q; });
+                if (quad == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + 16 * x + c16) * 4) = l[x];
+            }
+            lds_barrier();
+            lds_barrier();  // the value waves have read it
+            continue;
         }
 
+        // ==================================================================== value waves
         // ---- loads
         const u32x4 table_rsrc = [&] {
             u32x4 r = tile_rsrc(table);
             r[2] = __builtin_amdgcn_readfirstlane(width) * 4;  // entries past the table read as zeros (and are past `last`)
             return r;
         }();
-        const uint32_t pages_at = lds + LDS_PAGES + w * 512;
-        auto load_pages = [&](uint32_t tile) {  // the page numbers of a tile's tokens, the wave's own 16 first
+        const uint32_t pages_at = lds + LDS_PAGES + vw * 1024;
+        const int own8 = 8 * vw + (lane & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
+        auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
-                             __builtin_amdgcn_readfirstlane(pages_at + (tile & 1) * 256)),
-                         "v"(page_of(p, tile * BN + turned) * 4), "s"(table_rsrc)
+                             __builtin_amdgcn_readfirstlane(pages_at + (tile & 3) * 256)),
+                         "v"(page_of(p, tile * BN + own8) * 4), "s"(table_rsrc)
                          : "memory");
         };
-        // tile -> buffer; returns which of its tokens are there (in the tokens that the group sees, not in a hole)
-        auto load_tile = [&](uint32_t tile, uint32_t buf) {
-            const uint32_t tok = tile * BN + turned;
-            const int page = *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 1) * 256 + lane * 4);
-            const bool in = tok < (uint32_t)last && page >= 0 && page < a.pages;
-            const uint64_t there = __builtin_amdgcn_ballot_w64(in);
-            const uint64_t at_byte = (uint64_t)(in ? cache + (page * page_bytes + (int64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES)
-                                                   : reinterpret_cast<const char*>(zero_row));
-            const uint32_t lo = (uint32_t)at_byte, hi = (uint32_t)(at_byte >> 32);
-            uint32_t lane16 = lane << 4;
-            asm("" : "+v"(lane16));  // the 16 offsets below are made anew for every tile, not kept in registers
-            const uint32_t base = lds + buf * TILE_BYTES + 16 * w * LAT_BYTES, pe = lds + buf * TILE_BYTES + TILE_PE + 16 * w * PE_BYTES;
-            // wave w brings tokens 16 w .. 16 w + 15, a token's 64 latent pieces at a time (swz16)
+        // where the next tile to be brought stands: this lane's pieces of 4 + 4 tokens and of the positional parts, found in
+        // steps that can be spread: the page, the address of the lane's token, the addresses for the lane's pieces
+        uint64_t at_latent[2], at_pe;
+        auto find_page = [&](uint32_t tile) {
+            return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 3) * 256 + lane * 4);
+        };
+        auto find_token = [&](uint32_t tile, int page) {
+            const uint32_t tok = tile * BN + own8;
+            const bool in = tok < (uint32_t)last && page >= 0 && page < a.pages;  // in the tokens that the group sees, no hole
+            *(sm + LDS_THERE + (tile % BUFS) * BN + own8) = in;
+            return (uint64_t)(in ? cache + (page * page_bytes + (int64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES)
+                                 : reinterpret_cast<const char*>(zero_row));
+        };
+        auto find_pieces = [&](uint64_t at) {
+            const int lo = (int)(uint32_t)at, hi = (int)(uint32_t)(at >> 32);
+            auto of = [&](int t) { return (uint64_t)(uint32_t)__shfl(hi, t) << 32 | (uint32_t)__shfl(lo, t); };
+            at_latent[0] = of(quad), at_latent[1] = of(4 + quad), at_pe = of(lane >> 3);
+        };
+        auto find_places = [&] {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                uint64_t b[4];
-                uint32_t v[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    b[x] = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i + x) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, i + x);
-                    v[x] = lane16 ^ swz16(i + x) << 4;
-                }
-                load_rows4(base + i * LAT_BYTES, b, v);
-            }
-            // positional parts, 8 lanes a token
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = 8 * i + (lane >> 3);
-                const uint64_t b = (uint64_t)(uint32_t)__shfl((int)hi, t) << 32 | (uint32_t)__shfl((int)lo, t);
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
-                                 __builtin_amdgcn_readfirstlane(pe + 8 * i * PE_BYTES)),
-                             "v"(b + LAT_BYTES + (((lane & 7) ^ swz8(t)) << 4))
-                             : "memory");
-            }
-            return w ? there << (16 * w) | there >> (64 - 16 * w) : there;
+            for (int x = 0; x < 2; ++x) at_latent[x] += (c16 ^ turn(8 * vw + 4 * x + quad)) << 4;
+            at_pe += LAT_BYTES + (((lane & 7) ^ swz8(8 * vw + (lane >> 3))) << 4);
+        };
+        auto bring = [&](uint32_t tile, auto i) {  // load i of 9: four of 4 tokens, four of 4 more, the positional parts
+            constexpr int I = decltype(i)::value;
+            const uint32_t base = lds + (tile % BUFS) * TILE_BYTES;
+            if constexpr (I < 8)
+                load_block<(I & 3) * 256>(base + (2 * vw + (I >> 2)) * (4 * BLOCK) + (I & 3) * BLOCK, at_latent[I >> 2]);
+            else
+                load_block<0>(base + TILE_PE + 8 * vw * PE_BYTES, at_pe);
         };
 
         f32x16 acc[RT][4] = {};  // [row tile][32 values]
-        float mo[RT] = {M_START, M_START}, l = 0.f;
+        float mo[RT] = {M_START, M_START};
         bool special = false;
-        uint64_t there = 0;
-        load_pages(t0);
-        load_pages(t0 + 1);
-        wait_loads<0>();
-#pragma unroll
-        // the queries are there too (the compiler waits for them here and not in the loop), in accumulation registers
-        for (int i = 0; i < 36; ++i) asm volatile("" : "+a"(q[i]));
-        if (t0 < stop) there = load_tile(t0, t0 & 1);
-        for (uint32_t tile = t0; tile < stop; ++tile) {
-            wait_loads<0>();
-            lds_barrier();  // the tile is whole, and every wave is done with the one before it
-            const uint64_t now = there;
-            if (tile + 1 < stop) {
-                there = load_tile(tile + 1, (tile + 1) & 1);
-                load_pages(tile + 2);
-            }
-            const uint32_t tb = lds + (tile & 1) * TILE_BYTES;
-            const int k0 = (int)(tile * BN);
-            const bool mixed = k0 + BN > first;  // some row does not see some token of the tile
-            f32x16 s = {};
-            auto weights = [&](float m) {  // of this tile, relative to m; returns their sum
-                float sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    u32x4 pk;
-#pragma unroll
-                    for (int r = 0; r < 8; r += 2) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[8 * k + r], sc, -m));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[8 * k + r + 1], sc, -m));
-                        sum += x + y;
-                        pk[r >> 1] = T::pack(x, y);
-                    }
-                    *reinterpret_cast<u32x4*>(sm + LDS_P + (rt * 4 + 2 * kh + k) * 1024 + lane * 16) = pk;
-                }
-                return sum;
+        // One step: `tile` added, the value waves' loads of tile + 3 (past the end: zeros) and the addresses of tile + 4 between
+        // the products.  LAST: nothing is brought.
+        auto step = [&](uint32_t tile, auto last_) {
+            constexpr bool LAST = decltype(last_)::value;
+            const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
+            const uint32_t vb = lds + (tile % BUFS) * TILE_BYTES, pb = lds + LDS_P + (tile & 1) * 4096 + c * 32 + half * 16;
+            auto value = [&](int k, int d) {
+                const u32x2 v0 = lds_read_tr(((vb + va[0]) ^ (d << 6)) + k * 16 * BLOCK);
+                const u32x2 v1 = lds_read_tr(((vb + va[1]) ^ (d << 6)) + k * 16 * BLOCK);
+                return u32x4{v0.x, v0.y, v1.x, v1.y};
             };
-            float sum = 0.f;
-            if (active) {
-                // ---- scores: 36 steps, the operands of the next four read while four run
-                auto key = [&](int i) {
-                    return i < 32 ? lds_read16(((tb + ka) ^ ((i & 7) << 5)) + (i >> 3) * 256)
-                                  : lds_read16((tb + pa) ^ ((i - 32) << 5));
-                };
-                u32x4 kf[2][4];
-                f32x16 s2 = {};  // two chains of products
+            auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
+            const u32x4 fl = flags(tile);
+            u32x4 vf[4], pf[RT];
+            int page = 0;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) kf[0][x] = key(x);
-#pragma unroll
-                for (int i = 0; i < 9; ++i) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (i < 8)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) kf[(i + 1) & 1][x] = key(4 * i + 4 + x);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) (x & 1 ? s2 : s) = T::mfma(kf[i & 1][x], q[4 * i + x], x & 1 ? s2 : s);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                s += s2;
-                if (mixed || now != ~0ull) {
-                    const int left = mine - k0 - 32 * kh;
-                    const uint32_t vis = ((uint32_t)(now >> (32 * kh)) & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u)) >> (4 * half);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!(vis >> ((r & 3) + 8 * (r >> 2)) & 1)) s[r] = -INFINITY;
-                }
-                // ---- running softmax: weights relative to a past maximum, which is raised below only when some row of
-                // the wave exceeds it by SLACK (the result is the same for any reference)
-                float mx = s[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-                mx = max_halves(mx) * sc;
-                const float m = rt ? mo[1] : mo[0];
-                const bool raise = __builtin_amdgcn_ballot_w64(mx - m > T::B + T::SLACK) != 0;
-                if (half == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + c) * 4) = mx;
-                if (lane == 0) *reinterpret_cast<int*>(sm + LDS_FLAG + w * 4) = raise;
-                sum = weights(m);
-            } else if (lane == 0) {
-                *reinterpret_cast<int*>(sm + LDS_FLAG + w * 4) = 0;
-            }
-            lds_barrier();  // weights, maxima and flags of all waves
-            const u32x4 fl = *reinterpret_cast<const u32x4*>(sm + LDS_FLAG);
-            if (__builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3])) {
+            for (int d = 0; d < 4; ++d) vf[d] = value(0, d);
+            if constexpr (!LAST) page = find_page(tile + 4);
+            __builtin_amdgcn_sched_barrier(0);
+            if (any(fl)) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     if (!__builtin_amdgcn_readfirstlane(fl[r] | fl[r + RT])) continue;
-                    const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (r * 32 + c) * 4);
-                    const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + ((r + RT) * 32 + c) * 4);
-                    const float mn = fmaxf(mo[r], fmaxf(m0, m1) - T::B);
-                    const float f = __builtin_amdgcn_exp2f(mo[r] - mn);
-                    mo[r] = mn;
+                    const float f = raise(tile, 32 * r + c, mo[r]);
 #pragma unroll
                     for (int d = 0; d < 4; ++d) acc[r][d] *= f;
-                    if (r == rt) {
-                        l *= f;
-                        sum = weights(mn);
-                    }
                 }
                 lds_barrier();  // the weights anew
             }
-            l += sum;
-            // ---- values: the wave's 128 of every row, 16 keys a step, the next step's operands read while one runs
-            auto value = [&](int k, int d) {
-                const u32x2 v0 = lds_read_tr(((tb + va[0]) ^ (d << 6)) + k * 16 * LAT_BYTES);
-                const u32x2 v1 = lds_read_tr(((tb + va[1]) ^ (d << 6)) + k * 16 * LAT_BYTES);
-                return u32x4{v0.x, v0.y, v1.x, v1.y};
-            };
-            auto weight = [&](int r, int k) { return lds_read16(lds + LDS_P + (r * 4 + k) * 1024 + lane * 16); };
-            u32x4 vf[2][4], pf[2][RT];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) vf[0][d] = value(0, d);
+            for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
+            uint64_t at = 0;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) pf[0][r] = weight(r, 0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (k < 3) {
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) vf[(k + 1) & 1][d] = value(k + 1, d);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) pf[(k + 1) & 1][r] = weight(r, k + 1);
-                }
+            for (int k = 0; k < 2; ++k) {
+                u32x4 pn[RT];
                 if (mixed)
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        special |= nonfinite<T>(vf[k & 1][d]);
-                        vf[k & 1][d] = finite_part<T>(vf[k & 1][d]);
+                        special |= nonfinite<T>(vf[d]);
+                        vf[d] = finite_part<T>(vf[d]);
                     }
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int d = 0; d < 4; ++d) {
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) acc[r][d] = T::mfma(vf[k & 1][d], pf[k & 1][r], acc[r][d]);
+                    for (int r = 0; r < RT; ++r) acc[r][d] = T::mfma(vf[d], pf[r], acc[r][d]);
+                    if (k == 0) {  // the second half's operands
+                        vf[d] = value(1, d);
+                        if (d == 2)
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) pn[r] = weight(1, r);
+                    }
+                    if constexpr (!LAST) {
+                        if (k == 0) {
+                            if (d == 0) bring(tile + 3, Int<0>{});
+                            if (d == 1) bring(tile + 3, Int<1>{});
+                            if (d == 2) bring(tile + 3, Int<2>{});
+                            if (d == 3) bring(tile + 3, Int<3>{});
+                        } else {
+                            if (d == 0) bring(tile + 3, Int<4>{}), at = find_token(tile + 4, page);
+                            if (d == 1) bring(tile + 3, Int<5>{});
+                            if (d == 2) bring(tile + 3, Int<6>{});
+                            if (d == 3) bring(tile + 3, Int<7>{});
+                        }
+                    }
+                }
+                if (k == 0)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) pf[r] = pn[r];
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!LAST) {
+                bring(tile + 3, Int<8>{});
+                find_pieces(at);
+                load_pages(tile + 6);
+                find_places();
+                wait_loads<LOADS>();
+                lds_barrier();  // the next tile's weights; the tile after it is whole
+            }
+        };
+        if (n_tiles) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_pages(t0 + i);
+            wait_loads<0>();
+            auto find_tile = [&](uint32_t tile) {
+                find_pieces(find_token(tile, find_page(tile)));
+                find_places();
+            };
+            auto whole_tile = [&](uint32_t tile) {
+                find_tile(tile);
+                bring(tile, Int<0>{}), bring(tile, Int<1>{}), bring(tile, Int<2>{}), bring(tile, Int<3>{}), bring(tile, Int<4>{});
+                bring(tile, Int<5>{}), bring(tile, Int<6>{}), bring(tile, Int<7>{}), bring(tile, Int<8>{});
+            };
+            whole_tile(t0);
+            whole_tile(t0 + 1);
+            load_pages(t0 + 4);
+            wait_loads<LOADS>();
+            lds_barrier();  // the first tile
+            // while the first tile's scores are computed: tile t0 + 2, and where t0 + 3 stands
+            whole_tile(t0 + 2);
+            find_tile(t0 + 3);
+            load_pages(t0 + 5);
+            wait_loads<LOADS>();
+            lds_barrier();  // the first tile's weights; the second tile is whole
+            for (uint32_t tile = t0; tile + 1 < stop; ++tile) step(tile, std::false_type{});
+            step(stop - 1, std::true_type{});
+            wait_loads<0>();  // what was brought past the end
+        } else {
+            lds_barrier();
         }
 
         if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the tokens that not every row sees
@@ -388,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
                 const int page = table[j / a.page_size];
                 if (page < 0 || page >= a.pages) continue;
                 const uint16_t* vr = reinterpret_cast<const uint16_t*>(cache + page * page_bytes) + (int64_t)(j % a.page_size) * ROW +
-                                     128 * w + 4 * half;
+                                     128 * vw + 4 * half;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int i = r0 + 32 * r + c;
@@ -404,9 +515,8 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
             }
         }
 
-        // ---- results: the two waves of a row tile have summed half of its keys each
-        l = sum_halves(l);
-        if (half == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + c) * 4) = l;
+        // ---- results: the two score waves of a row tile have summed half of its keys each
+        lds_barrier();  // the last maxima are read
         lds_barrier();
         float ls[RT];
 #pragma unroll
@@ -421,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
                 if (i >= r1) break;
                 const float inv = ls[r] > 0.f ? 1.f / ls[r] : 0.f;
                 const int t = i / a.H, h = i - t * a.H;
-                uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 128 * w + 4 * half;
+                uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 128 * vw + 4 * half;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -430,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
                             ls[r] == 0.f ? u32x2{0u, 0u}
                                          : u32x2{T::pack(acc[r][d][e] * inv, acc[r][d][e + 1] * inv),
                                                  T::pack(acc[r][d][e + 2] * inv, acc[r][d][e + 3] * inv)};
-                if (a.lse && w == 0 && half == 0)
+                if (a.lse && vw == 0 && half == 0)
                     a.lse[i] = ls[r] == 0.f ? -INFINITY : (mo[r] + __builtin_amdgcn_logf(ls[r])) * 0.69314718055995f;
             }
         } else {
@@ -441,14 +551,14 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 if (r0 + 32 * r + c >= r1) break;
-                char* o = out + r * SLOT_TILE + w * 16384 + lane * 16;
+                char* o = out + r * SLOT_TILE + vw * 16384 + lane * 16;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<f32x4*>(o + (d * 4 + e) * 1024) =
                             f32x4{acc[r][d][4 * e], acc[r][d][4 * e + 1], acc[r][d][4 * e + 2], acc[r][d][4 * e + 3]};
-                if (w == 0 && half == 0) *reinterpret_cast<f32x2*>(out + r * SLOT_TILE + SLOT_ACC + c * 8) = f32x2{mo[r], ls[r]};
+                if (vw == 0 && half == 0) *reinterpret_cast<f32x2*>(out + r * SLOT_TILE + SLOT_ACC + c * 8) = f32x2{mo[r], ls[r]};
             }
         }
     }
@@ -458,9 +568,9 @@ __global__ void __launch_bounds__(THREADS, 1) decode_kernel(KdaLatentDecodeArgs 
 // One workgroup for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
 // v, v + 4, ... and the waves' sums meet in LDS.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) join_kernel(KdaLatentDecodeArgs a, Plan p) {
-    __shared__ float sm_m[WAVES][32], sm_l[WAVES][32];
-    __shared__ f32x4 sm_a[WAVES][4][64];
+__global__ void __launch_bounds__(JOIN_WAVES * 64) join_kernel(KdaLatentDecodeArgs a, Plan p) {
+    __shared__ float sm_m[JOIN_WAVES][32], sm_l[JOIN_WAVES][32];
+    __shared__ f32x4 sm_a[JOIN_WAVES][4][64];
     const int tid = threadIdx.x, v = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
     const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
@@ -502,11 +612,11 @@ __global__ void __launch_bounds__(THREADS) join_kernel(KdaLatentDecodeArgs a, Pl
         const char* ws = static_cast<const char*>(a.workspace);
         const int64_t own_bytes = (int64_t)(p.own.rows / 32) * SLOT_TILE, pre_bytes = (int64_t)(p.pre.rows / 32) * SLOT_TILE;
         const char* own_ws = ws + p.pre_slots * pre_bytes + g * own_bytes + rt * SLOT_TILE;
-        for (uint32_t i = v; i < parts; i += WAVES) add(own_ws + ((int64_t)p0 + i + n) * p.own.groups * own_bytes, c);
+        for (uint32_t i = v; i < parts; i += JOIN_WAVES) add(own_ws + ((int64_t)p0 + i + n) * p.own.groups * own_bytes, c);
         if (pre_parts) {
             const int gp = r / p.pre.rows, rp = r - gp * p.pre.rows;
             const char* pre_ws = ws + gp * pre_bytes + (rp >> 5) * SLOT_TILE;
-            for (uint32_t i = v; i < pre_parts; i += WAVES) add(pre_ws + (int64_t)i * p.pre.groups * pre_bytes, rp & 31);
+            for (uint32_t i = v; i < pre_parts; i += JOIN_WAVES) add(pre_ws + (int64_t)i * p.pre.groups * pre_bytes, rp & 31);
         }
     }
     if (half == 0) {
@@ -517,12 +627,12 @@ __global__ void __launch_bounds__(THREADS) join_kernel(KdaLatentDecodeArgs a, Pl
     for (int e = 0; e < 4; ++e) sm_a[v][e][lane] = acc[e];
     __syncthreads();
     if (!valid) return;
-    float M = M_START, L = 0.f, f[WAVES];
+    float M = M_START, L = 0.f, f[JOIN_WAVES];
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) M = fmaxf(M, sm_m[i][c]);
+    for (int i = 0; i < JOIN_WAVES; ++i) M = fmaxf(M, sm_m[i][c]);
     f32x4 o = {};
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
+    for (int i = 0; i < JOIN_WAVES; ++i) {
         f[i] = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
         L += sm_l[i][c] * f[i];
         o += sm_a[i][v][lane] * f[i];  // wave v finishes values 8 v .. 8 v + 7 of the block
@@ -606,10 +716,10 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     const dim3 join((uint32_t)a->B * p.own.groups, p.own.rows / 32 * 16);
     if (a->dtype == KDA355_DTYPE_BF16) {
         hipLaunchKernelGGL(decode_kernel<Bf16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
-        hipLaunchKernelGGL(join_kernel<Bf16>, join, dim3(THREADS), 0, s, *a, p);
+        hipLaunchKernelGGL(join_kernel<Bf16>, join, dim3(JOIN_WAVES * 64), 0, s, *a, p);
     } else {
         hipLaunchKernelGGL(decode_kernel<Fp16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
-        hipLaunchKernelGGL(join_kernel<Fp16>, join, dim3(THREADS), 0, s, *a, p);
+        hipLaunchKernelGGL(join_kernel<Fp16>, join, dim3(JOIN_WAVES * 64), 0, s, *a, p);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
