@@ -24,11 +24,14 @@ namespace {
 constexpr int LAT = KDA355_LATENT_DIM, ROW = KDA355_LATENT_ROW, PE = KDA355_LATENT_PE;
 constexpr int ROW_BYTES = ROW * 2, LAT_BYTES = LAT * 2, PE_BYTES = PE * 2;
 constexpr int SCORE_WAVES = 4, VALUE_WAVES = 4, THREADS = (SCORE_WAVES + VALUE_WAVES) * 64;
-constexpr int JOIN_WAVES = 4;
 constexpr int BN = 32, BUFS = 4;                        // keys of a tile, tiles in LDS
 constexpr int LOADS = 10;                               // of a value wave a tile: 8 of latent rows, positional parts, page numbers
 constexpr int RT = 2, MAX_ROWS = 32 * RT;               // row tiles, query rows of a group
-constexpr uint32_t MIN_TILES = 1;                       // least run of a workgroup
+// The cut is by cost: beginning a sequence (lengths, queries, page numbers and first tile one after the other) takes about as
+// long as LEAD tiles, which stand in front of every sequence's own; a run is MIN_RUN of these units at least.  Measured: 64
+// ragged sequences 146 us without LEAD, 142 with 3, 136 with 8 and with 16; 64 short ones behind 32768 tokens 230, 202, 190 and
+// 190; one sequence of 4097 tokens 20.3 us with runs of 1, 17.9 of 3, 18.5 of 4.
+constexpr uint32_t LEAD = 8, MIN_RUN = 3;
 constexpr int SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;  // workspace of 32 rows: accumulators, (m, l) of each row
 
 struct Groups {
@@ -50,12 +53,16 @@ __device__ const uint4 zero_row[ROW_BYTES / 16] = {};  // what a token that is n
 
 // ------------------------------------------------------------------------------------------------ who does what
 struct Cut {
-    uint32_t own, pre, run;  // key tiles of all sequences, of the prefix; tiles of a workgroup
+    uint32_t own, pre, run;  // units of all sequences, tiles of the prefix; units of a workgroup
     uint32_t pre_wgs, own_wgs;
 };
 __device__ __forceinline__ int tokens_of(int len, int width, int page_size) { return min(max(len, 0), width * page_size); }
 __device__ __forceinline__ uint32_t tiles_of(const KdaLatentDecodeArgs& a, int n) {
     return ((uint32_t)tokens_of(a.seq_lens[n], a.table_width, a.page_size) + BN - 1) / BN;
+}
+__device__ __forceinline__ uint32_t units_of(const KdaLatentDecodeArgs& a, int n) {
+    const uint32_t t = tiles_of(a, n);
+    return t ? t + LEAD : 0;
 }
 __device__ __forceinline__ uint32_t cdiv(uint32_t x, uint32_t y) { return x / y + (x % y != 0); }
 
@@ -65,9 +72,9 @@ __device__ __forceinline__ Cut cut(const KdaLatentDecodeArgs& a, const Plan& p, 
     c.own = own;
     c.pre = p.pre.groups ? ((uint32_t)tokens_of(a.prefix_len[0], a.prefix_width, a.page_size) + BN - 1) / BN : 0;
     c.pre = __builtin_amdgcn_readfirstlane(c.pre);
-    const uint32_t most = max(max(c.own, c.pre), MIN_TILES);  // one run a group: always fits
+    const uint32_t most = max(max(c.own, c.pre), MIN_RUN);  // one run a group: always fits
     const double all = (double)p.pre.groups * c.pre + (double)p.own.groups * c.own;
-    const uint32_t lo = min(max((uint32_t)__builtin_ceil(all / p.grid), MIN_TILES), most);
+    const uint32_t lo = min(max((uint32_t)__builtin_ceil(all / p.grid), MIN_RUN), most);
     const int lane = threadIdx.x & 63;
     const double f = lane < 32 ? 1.0 + lane / 64.0 : 1.5 * (double)exp2f((lane - 31) * 0.25f);
     const uint32_t r = lane == 63 ? most : (uint32_t)fmin(__builtin_ceil(lo * f), (double)most);
@@ -84,12 +91,12 @@ __device__ __forceinline__ uint32_t sum_wave(uint32_t x) {
     return __builtin_amdgcn_readfirstlane(x);
 }
 struct At { int n; uint32_t before; };
-// the sequence that holds tile u of all (u < their sum), and the tiles before it
+// the sequence that holds unit u of all (u < their sum), and the units before it
 __device__ __forceinline__ At sequence_of(const KdaLatentDecodeArgs& a, uint32_t u) {
     const int lane = threadIdx.x & 63;
     uint32_t before = 0;
     for (int n0 = 0; n0 < a.B; n0 += 64) {
-        const uint32_t t = n0 + lane < a.B ? tiles_of(a, n0 + lane) : 0;
+        const uint32_t t = n0 + lane < a.B ? units_of(a, n0 + lane) : 0;
         uint32_t s = t;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -148,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const int c = lane & 31, half = lane >> 5;
 
     uint32_t own = 0;
-    for (int n = lane; n < a.B; n += 64) own += tiles_of(a, n);
+    for (int n = lane; n < a.B; n += 64) own += units_of(a, n);
     const Cut cu = cut(a, p, sum_wave(own));
     const uint32_t wgs = cu.pre_wgs + cu.own_wgs;
     if (blockIdx.x >= wgs) return;
@@ -201,14 +208,15 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             table = a.block_table + n * a.table_stride, width = a.table_width;
             const int rows = a.S * a.H;
             r0 = n * rows + g * gr.rows, r1 = min(r0 + gr.rows, (n + 1) * rows);
-            const uint32_t tiles = ((uint32_t)tokens + BN - 1) / BN;
-            t0 = u - at.before, t1 = min(tiles, end - at.before);
+            const uint32_t tiles = ((uint32_t)tokens + BN - 1) / BN, units = tiles ? tiles + LEAD : 0;
+            const uint32_t from = u - at.before, to = min(units, end - at.before);
+            t0 = from > LEAD ? from - LEAD : 0, t1 = to > LEAD ? to - LEAD : 0;
             whole = t0 == 0 && t1 == tiles && cu.pre == 0;
-            u = at.before + t1;
-            if (t1 == tiles) at = {n + 1, at.before + tiles};
+            u = at.before + to;
+            if (to == units) at = {n + 1, at.before + units};
         }
         tokens = __builtin_amdgcn_readfirstlane(tokens);
-        if (t0 >= t1) continue;  // a sequence without tokens
+        if (t0 >= t1) continue;  // no tokens, or not the first
         // tokens that a row sees: all for the prefix, all but the draft tokens after its own for a sequence
         const int hidden = prefix ? 0 : a.S - 1 + n * a.S;  // (minus the row's token)
         auto sees = [&](int r) { return prefix ? tokens : tokens - (hidden - r / a.H); };
@@ -220,11 +228,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // by SLACK (the result is the same for any reference): after the fact, at the start of the next step.
         auto flags = [&](uint32_t tile) { return *reinterpret_cast<const u32x4*>(sm + LDS_FLAG + (tile & 1) * 16); };
         auto any = [](u32x4 fl) { return __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0; };
-        // the new reference of the group's row r after `tile`; returns the factor of what is there
+        // the new reference of the group's row r after `tile`, by its own scores alone; returns the factor of what is there
         auto raise = [&](uint32_t tile, int r, float& m) {
             const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + r * 4);
             const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + (RT * 32 + r) * 4);
-            const float mn = fmaxf(m, fmaxf(m0, m1) - T::B), f = __builtin_amdgcn_exp2f(m - mn);
+            const float mx = fmaxf(m0, m1), mn = mx - m > T::B + T::SLACK ? mx - T::B : m, f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             return f;
         };
@@ -565,26 +573,27 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 }
 
 // ------------------------------------------------------------------------------------------------ joining the parts
-// One workgroup for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
-// v, v + 4, ... and the waves' sums meet in LDS.
-template <typename T>
-__global__ void __launch_bounds__(JOIN_WAVES * 64) join_kernel(KdaLatentDecodeArgs a, Plan p) {
-    __shared__ float sm_m[JOIN_WAVES][32], sm_l[JOIN_WAVES][32];
-    __shared__ f32x4 sm_a[JOIN_WAVES][4][64];
+// One workgroup of W waves for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
+// v, v + W, ..., two at a time, and the waves' sums meet in LDS.  Bound by the latency of its reads: a few calls with many parts
+// take 16 waves (one sequence in 44 parts: 5.4 us, with 4 waves XXX), many with few parts 4 (4096 rows: 12.5 us).
+template <typename T, int W>
+__global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Plan p) {
+    __shared__ float sm_m[W][32], sm_l[W][32];
+    __shared__ f32x4 sm_a[W][4][64];
     const int tid = threadIdx.x, v = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
     const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
     const int rt = blockIdx.y >> 4, block = blockIdx.y & 15;  // value block: values 32 block ..
     uint32_t own = 0, before = 0;
     for (int i = lane; i < a.B; i += 64) {
-        const uint32_t t = tiles_of(a, i);
+        const uint32_t t = units_of(a, i);
         own += t;
         if (i < n) before += t;
     }
     const Cut cu = cut(a, p, sum_wave(own));
     before = sum_wave(before);
     const uint32_t tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, n));
-    const uint32_t p0 = before / cu.run, p1 = tiles ? (before + tiles - 1) / cu.run + 1 : p0;
+    const uint32_t p0 = (before + LEAD) / cu.run, p1 = tiles ? (before + LEAD + tiles - 1) / cu.run + 1 : p0;
     const uint32_t parts = p1 - p0, pre_parts = cu.pre ? cdiv(cu.pre, cu.run) : 0;
     if (pre_parts == 0 && parts == 1) return;  // written by the workgroup that had it whole
     const int rows = a.S * a.H;
@@ -595,28 +604,43 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) join_kernel(KdaLatentDecodeAr
 
     float m = M_START, l = 0.f;
     f32x4 acc[4] = {};
-    auto add = [&](const char* slot_tile, int cc) {
-        const f32x2 ml = *reinterpret_cast<const f32x2*>(slot_tile + SLOT_ACC + cc * 8);
+    struct Part {
+        f32x2 ml;
         f32x4 x[4];
+    };
+    auto load = [&](const char* slot_tile, int cc) {
+        Part y;
+        y.ml = *reinterpret_cast<const f32x2*>(slot_tile + SLOT_ACC + cc * 8);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            x[e] = *reinterpret_cast<const f32x4*>(slot_tile + (block * 4 + e) * 1024 + (32 * half + cc) * 16);
-        const float mn = fmaxf(m, ml.x);
-        const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml.x - mn);
+            y.x[e] = *reinterpret_cast<const f32x4*>(slot_tile + (block * 4 + e) * 1024 + (32 * half + cc) * 16);
+        return y;
+    };
+    auto add = [&](const Part& y) {
+        const float mn = fmaxf(m, y.ml.x);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(y.ml.x - mn);
         m = mn;
-        l = l * f0 + ml.y * f1;
+        l = l * f0 + y.ml.y * f1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f0 + x[e] * f1;
+        for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f0 + y.x[e] * f1;
+    };
+    auto walk = [&](const char* at, int64_t step, uint32_t n, int cc) {
+        uint32_t i = v;
+        for (; W > 4 && i + W < n; i += 2 * W) {
+            const Part y0 = load(at + i * step, cc), y1 = load(at + (i + W) * step, cc);
+            add(y0);
+            add(y1);
+        }
+        for (; i < n; i += W) add(load(at + i * step, cc));
     };
     if (valid) {
         const char* ws = static_cast<const char*>(a.workspace);
         const int64_t own_bytes = (int64_t)(p.own.rows / 32) * SLOT_TILE, pre_bytes = (int64_t)(p.pre.rows / 32) * SLOT_TILE;
-        const char* own_ws = ws + p.pre_slots * pre_bytes + g * own_bytes + rt * SLOT_TILE;
-        for (uint32_t i = v; i < parts; i += JOIN_WAVES) add(own_ws + ((int64_t)p0 + i + n) * p.own.groups * own_bytes, c);
+        walk(ws + p.pre_slots * pre_bytes + rt * SLOT_TILE + (((int64_t)p0 + n) * p.own.groups + g) * own_bytes, p.own.groups * own_bytes,
+             parts, c);
         if (pre_parts) {
             const int gp = r / p.pre.rows, rp = r - gp * p.pre.rows;
-            const char* pre_ws = ws + gp * pre_bytes + (rp >> 5) * SLOT_TILE;
-            for (uint32_t i = v; i < pre_parts; i += JOIN_WAVES) add(pre_ws + (int64_t)i * p.pre.groups * pre_bytes, rp & 31);
+            walk(ws + gp * pre_bytes + (rp >> 5) * SLOT_TILE, p.pre.groups * pre_bytes, pre_parts, rp & 31);
         }
     }
     if (half == 0) {
@@ -626,16 +650,16 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) join_kernel(KdaLatentDecodeAr
 #pragma unroll
     for (int e = 0; e < 4; ++e) sm_a[v][e][lane] = acc[e];
     __syncthreads();
-    if (!valid) return;
-    float M = M_START, L = 0.f, f[JOIN_WAVES];
+    if (!valid || v >= 4) return;
+    float M = M_START, L = 0.f, f;
 #pragma unroll
-    for (int i = 0; i < JOIN_WAVES; ++i) M = fmaxf(M, sm_m[i][c]);
+    for (int i = 0; i < W; ++i) M = fmaxf(M, sm_m[i][c]);
     f32x4 o = {};
 #pragma unroll
-    for (int i = 0; i < JOIN_WAVES; ++i) {
-        f[i] = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
-        L += sm_l[i][c] * f[i];
-        o += sm_a[i][v][lane] * f[i];  // wave v finishes values 8 v .. 8 v + 7 of the block
+    for (int i = 0; i < W; ++i) {
+        f = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
+        L += sm_l[i][c] * f;
+        o += sm_a[i][v][lane] * f;  // wave v finishes values 8 v .. 8 v + 7 of the block
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     const int t = r / a.H, h = r - t * a.H;
@@ -660,7 +684,7 @@ int check_decode_sizes(const KdaLatentDecodeArgs* a) {
     KDA_CHECK_ARG(span < (1ll << 31) && (int64_t)a->prefix_width * a->page_size < (1ll << 31),
                   "latent_decode: a table spans 2^31 tokens or more");
     KDA_CHECK_ARG(a->table_width < (1 << 28) && a->prefix_width < (1 << 28), "latent_decode: a table of 2^28 pages or more");
-    KDA_CHECK_ARG(a->B * (span / BN + 1) < (1ll << 31), "latent_decode: the tables span 2^36 tokens or more");
+    KDA_CHECK_ARG(a->B * (span / BN + 1 + LEAD) < (1ll << 31), "latent_decode: the tables span 2^36 tokens or more");
     return 0;
 }
 
@@ -714,13 +738,16 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const Plan p = plan_of(a);
     const dim3 join((uint32_t)a->B * p.own.groups, p.own.rows / 32 * 16);
-    if (a->dtype == KDA355_DTYPE_BF16) {
-        hipLaunchKernelGGL(decode_kernel<Bf16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
-        hipLaunchKernelGGL(join_kernel<Bf16>, join, dim3(JOIN_WAVES * 64), 0, s, *a, p);
-    } else {
-        hipLaunchKernelGGL(decode_kernel<Fp16>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
-        hipLaunchKernelGGL(join_kernel<Fp16>, join, dim3(JOIN_WAVES * 64), 0, s, *a, p);
-    }
+    const bool few = (int64_t)join.x * join.y <= p.grid;  // at most a workgroup a CU: likely many parts each
+    auto launch = [&](auto type) {
+        typedef decltype(type) T;
+        hipLaunchKernelGGL(decode_kernel<T>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+        if (few)
+            hipLaunchKernelGGL((join_kernel<T, 16>), join, dim3(16 * 64), 0, s, *a, p);
+        else
+            hipLaunchKernelGGL((join_kernel<T, 4>), join, dim3(4 * 64), 0, s, *a, p);
+    };
+    if (a->dtype == KDA355_DTYPE_BF16) launch(Bf16{}); else launch(Fp16{});
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         set_error("latent_decode: launch failed: %s", hipGetErrorString(e));

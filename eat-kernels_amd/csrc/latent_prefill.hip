@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
         mx = max_halves(mx) * sc;
         if (__builtin_amdgcn_ballot_w64(mx - mo > T::B + T::SLACK)) {
-            const float mn = fmaxf(mo, mx - T::B);
+            const float mn = mx - mo > T::B + T::SLACK ? mx - T::B : mo;  // by the row's own scores alone
             const float f = __builtin_amdgcn_exp2f(mo - mn);
             mo = mn;
             l *= f;
