@@ -34,8 +34,13 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _cus = {}
 
 
+# A decode step makes dozens of these calls, each of a few microseconds on the GPU, so the checks below first ask for what is
+# right in as few steps as possible, and look closer only to name what is wrong.
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object (2 us)
+
+
 def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(device.index)
 
 
 def _num_cus(device):
@@ -58,39 +63,47 @@ def _first(name, t):
 
 def _rows(name, t, shape, dtype, device):
     """The tensor has this shape and a dense last dimension; returns its other strides."""
-    _need(name, t, dtype, device)
-    if tuple(t.shape) != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device:
+        _need(name, t, dtype, device)
+    if t.shape != shape:
         raise ValueError(f"kda355: {name} must be {list(shape)}, got {list(t.shape)}")
     st = t.stride()
-    if shape[-1] > 1 and st[-1] != 1:
+    if st[-1] != 1:
         raise ValueError(f"kda355: the last dimension of {name} must be dense")
     # the stride of a dimension of one is never used: any value is valid there, odd ones too
-    return [s if n > 1 else 0 for s, n in zip(st[:-1], shape)]
+    if len(st) == 3:
+        return st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0
+    return (st[0] if shape[0] > 1 else 0,)
 
 
 def _index(name, t, shape, device, dtype=torch.int32):
-    _need(name, t, dtype, device)
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device:
+        _need(name, t, dtype, device)
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"kda355: {name} must be a contiguous {dtype} {list(shape)} tensor, got {list(t.shape)}")
 
 
 def _table(name, t, device):
     """Row stride of a [rows, width] int32 page table with dense rows."""
-    _need(name, t, torch.int32, device)
-    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"kda355: {name} must be [rows, width >= 1] with dense rows, got {list(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != device:
+        _need(name, t, torch.int32, device)
+    sh, st = t.shape, t.stride()
+    if len(sh) != 2 or sh[1] < 1 or (sh[1] > 1 and st[1] != 1):
+        raise ValueError(f"kda355: {name} must be [rows, width >= 1] with dense rows, got {list(sh)}")
+    return st[0] if sh[0] > 1 else sh[1]
 
 
 def _cache(cache, dtype, device):
     """(pages, page_size, page stride) of a cache."""
-    _need("cache", cache, dtype, device)
-    if cache.dim() != 3 or cache.shape[2] != ROW or cache.shape[0] < 1 or cache.shape[1] < 1:
-        raise ValueError(f"kda355: cache must be [pages, page_size, {ROW}], got {list(cache.shape)}")
-    pages, size, _ = cache.shape
-    if cache.stride(2) != 1 or (size > 1 and cache.stride(1) != ROW):
+    if not isinstance(cache, torch.Tensor) or cache.dtype is not dtype or cache.device != device:
+        _need("cache", cache, dtype, device)
+    sh, st = cache.shape, cache.stride()
+    if len(sh) != 3 or sh[2] != ROW or sh[0] < 1 or sh[1] < 1:
+        raise ValueError(f"kda355: cache must be [pages, page_size, {ROW}], got {list(sh)}")
+    pages, size, _ = sh
+    if st[2] != 1 or (size > 1 and st[1] != ROW):
         raise ValueError("kda355: cache must be dense within a page")
-    return pages, size, cache.stride(0) if pages > 1 else size * ROW
+    return pages, size, st[0] if pages > 1 else size * ROW
 
 
 def _lse_ptr(lse, shape, device):

@@ -17,6 +17,7 @@ Errors: TypeError for a wrong dtype or device, ValueError for a wrong shape or s
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -26,7 +27,7 @@ from .recurrent import _need
 
 
 def _pools(pools, slots=None):
-    """(device, [KdaPool]) of a list of [slots, ...] tensors with dense rows."""
+    """(device, [(address, row bytes, slot stride, slots)]) of a list of [slots, ...] tensors with dense rows."""
     if isinstance(pools, torch.Tensor):
         pools = (pools,)
     out, dev = [], None
@@ -37,38 +38,63 @@ def _pools(pools, slots=None):
             dev = t.device
         if t.device != dev or dev.type != "cuda":
             raise TypeError("kda355: pools must be on one GPU")
-        if t.dim() < 1 or (slots is not None and t.shape[0] != slots):
+        sh = t.shape
+        if len(sh) < 1 or (slots is not None and sh[0] != slots):
             raise ValueError(f"kda355: pool {i} must be [{slots if slots is not None else 'slots'}, ...], "
-                             f"got {list(t.shape)}")
-        if t.shape[0] == 0:
+                             f"got {list(sh)}")
+        n = sh[0]
+        if n == 0:
             continue
-        exp = 1
-        for d in range(t.dim() - 1, 0, -1):
-            if t.shape[d] != 1 and t.stride(d) != exp:
-                raise ValueError(f"kda355: the rows of pool {i} must be dense")
-            exp *= t.shape[d]
         size = t.element_size()
-        row = exp * size
-        stride = t.stride(0) * size if t.shape[0] > 1 else row
+        if t.is_contiguous():
+            row = t.numel() // n * size
+            stride = row
+        else:
+            st, exp = t.stride(), 1
+            for d in range(len(sh) - 1, 0, -1):
+                if sh[d] != 1 and st[d] != exp:
+                    raise ValueError(f"kda355: the rows of pool {i} must be dense")
+                exp *= sh[d]
+            row = exp * size
+            stride = st[0] * size if n > 1 else row
         if row == 0:
             continue
-        out.append(_lib.KdaPool(t.data_ptr(), row, stride, t.shape[0]))
+        out.append((t.data_ptr(), row, stride, n))
     return dev, out
 
 
-def _launch(name, dev, pools, n, src, dst, ws, table=None, lens=None, refs=None, free=None, num=None, stride=0, rows=0,
-            width=0, pages=0, size=1):
-    a = _lib.KdaPagesArgs(num_pools=len(pools), n=n, src=src, dst=dst, block_table=table, seq_lens=lens, ref_counts=refs,
-                          free_pages=free, num_free=num, workspace=ws, table_stride=stride, rows=rows, table_width=width,
-                          pages=pages, page_size=size)
-    for i, p in enumerate(pools):
-        a.pool[i] = p
-    _lib.check(getattr(_lib.lib(), f"kda355_{name}_launch")(ctypes.byref(a), _stream(dev)), name)
+# KdaPagesArgs in one go: its 24 pools would be as many objects
+_PACK = struct.Struct(f"={4 * _lib.MAX_POOLS}q2i8Qq4i")
+assert _PACK.size == ctypes.sizeof(_lib.KdaPagesArgs)
+_NO_POOLS = (0,) * (4 * _lib.MAX_POOLS)
+
+
+def _launch(name, dev, pools, n, src, dst, ws, table=0, lens=0, refs=0, free=0, num=0, stride=0, rows=0, width=0, pages=0,
+            size=1):
+    flat = _NO_POOLS
+    if pools:
+        flat = [v for p in pools for v in p]
+        flat += _NO_POOLS[len(flat):]
+    try:
+        a = _lib.KdaPagesArgs.from_buffer_copy(
+            _PACK.pack(*flat, len(pools), n, src, dst, table, lens, refs, free, num, ws, stride, rows, width, pages, size))
+    except struct.error as e:
+        raise ValueError(f"kda355: {name}: a size is out of range ({e})") from None
+    _lib.check(_LAUNCH[name](ctypes.byref(a), _stream(dev)), name)
+
+
+class _Entries(dict):
+    def __missing__(self, name):
+        f = self[name] = getattr(_lib.lib(), f"kda355_{name}_launch")
+        return f
+
+
+_LAUNCH = _Entries()
 
 
 def _copy(dev, pools, n, src, dst):
     for i in range(0, len(pools), _lib.MAX_POOLS):
-        _launch("copy_rows", dev, pools[i:i + _lib.MAX_POOLS], n, src, dst, None)
+        _launch("copy_rows", dev, pools[i:i + _lib.MAX_POOLS], n, src, dst, 0)
 
 
 def _book(block_table, ref_counts, free_pages, num_free):
@@ -127,7 +153,7 @@ def free_pages(block_table, seq_lens, ref_counts, free_pages, num_free, rows, pa
     _index("seq_lens", seq_lens, (block_table.shape[0],), dev)
     n = rows.numel() if isinstance(rows, torch.Tensor) else 0
     _index("rows", rows, (n,), dev)
-    _launch("free_pages", dev, [], n, rows.data_ptr(), None, None, lens=seq_lens.data_ptr(), size=int(page_size), **book)
+    _launch("free_pages", dev, [], n, rows.data_ptr(), 0, 0, lens=seq_lens.data_ptr(), size=int(page_size), **book)
 
 
 def compact_pages(pools, block_table, ref_counts, free_pages, num_free):
@@ -140,7 +166,7 @@ def compact_pages(pools, block_table, ref_counts, free_pages, num_free):
         raise TypeError(f"kda355: pools must be on {dev}, got {pool_dev}")
     ws = torch.empty(2 * pages + 2, dtype=torch.int32, device=dev)
     at = ws.data_ptr()
-    _launch("compact_pages", dev, ps[:_lib.MAX_POOLS], 0, None, None, at, **book)
+    _launch("compact_pages", dev, ps[:_lib.MAX_POOLS], 0, 0, 0, at, **book)
     half = pages // 2
     if half:
         _copy(dev, ps[_lib.MAX_POOLS:], half, at + 4 * pages, at + 4 * (pages + half))
