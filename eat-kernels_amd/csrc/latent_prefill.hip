@@ -18,50 +18,146 @@ namespace {
 constexpr int BM = 128, BN = 64, WAVES = 4;
 constexpr int HD = 128, PE = 64;
 constexpr int TILE_V = BN * HD * 2, TILE_PE = 2 * TILE_V, TILE_BYTES = TILE_PE + BN * PE * 2;  // k | v | shared part
+constexpr int SLOT_ACC = BM * HD * 4, SLOT = SLOT_ACC + BM * 8;  // workspace of a part: accumulators, (m, l) of each row
+// Where rows are few and keys many, the keys are cut: a sequence whose last row tile sees more key tiles than a workgroup's fair
+// share of all (and than MIN_RUN) has every row tile walked in that many pieces, whose parts a second kernel joins.
+constexpr int MIN_RUN = 3;
 constexpr int64_t MAX_ROW = 1 << 23;  // row strides up to this many elements: a tile's byte offsets stay below 2^31
 
-struct Where { int n, tile; };
-// row tile `i` of all sequences -> (sequence, its tile); n < 0 past the last one.  Every lane of a wave takes a sequence.
-__device__ __forceinline__ Where locate(const int32_t* cu, int N, int64_t T, int i) {
+struct Plan { int grid, share, slots; };  // workgroups; those that share the work; parts in the workspace
+struct Seq {
+    int tiles, most, pieces;  // row tiles; key tiles of the last one; pieces of each
+};
+struct Span {
+    int64_t q0, k0;
+    int Lq, Lk, shift;  // row i sees keys j <= i + shift, j < Lk
+};
+__device__ __forceinline__ Span span_of(const KdaLatentPrefillArgs& a, int n) {
+    Span s;
+    s.q0 = min(max((int64_t)a.cu_q[n], (int64_t)0), a.Tq), s.k0 = min(max((int64_t)a.cu_k[n], (int64_t)0), a.Tk);
+    s.Lq = (int)max(min((int64_t)a.cu_q[n + 1], a.Tq) - s.q0, (int64_t)0);
+    s.Lk = (int)max(min((int64_t)a.cu_k[n + 1], a.Tk) - s.k0, (int64_t)0);
+    s.shift = a.flags & KDA355_LATENT_CAUSAL ? s.Lk - s.Lq : s.Lk;
+    return s;
+}
+// key tiles that row tile `i` sees
+__device__ __forceinline__ int key_tiles(const Span& s, int i) {
+    const int seen = min(s.Lk, min(i * BM + BM, s.Lq) + s.shift);
+    return seen > 0 ? (seen + BN - 1) / BN : 0;
+}
+// key tiles of a piece of a row tile that sees `n` of them
+__device__ __forceinline__ int run_of(int n, int pieces) { return max((n + pieces - 1) / pieces, MIN_RUN); }
+__device__ __forceinline__ int scan_wave(int x) {  // inclusive
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int n0 = 0; n0 < N; n0 += 64) {
-        const int n = n0 + lane;
-        int tiles = 0;
-        if (n < N) {
-            const int64_t a = min(max((int64_t)cu[n], (int64_t)0), T), b = min((int64_t)cu[n + 1], T);
-            tiles = b > a ? (int)((b - a + BM - 1) / BM) : 0;
-        }
-        int s = tiles;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(s, d);
-            if (lane >= d) s += y;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+// every lane takes a sequence; the first 64 are loaded once
+struct Spans {
+    const KdaLatentPrefillArgs& a;
+    Span mine;
+    __device__ __forceinline__ explicit Spans(const KdaLatentPrefillArgs& args) : a(args), mine(span_of(args, min((int)(threadIdx.x & 63), args.N - 1))) {}
+    __device__ __forceinline__ Span operator[](int n) const { return n < 64 ? mine : span_of(a, n); }  // n % 64: the lane
+};
+// The longest run of a piece: a fair share of the key tiles of all row tiles (about).
+__device__ __forceinline__ int longest_run(const KdaLatentPrefillArgs& a, const Spans& spans, int slots) {
+    const int lane = threadIdx.x & 63;
+    float all = 0.f;
+    for (int n = lane; n < a.N; n += 64) {
+        const Span s = spans[n];
+        const int tiles = (s.Lq + BM - 1) / BM;
+        if (tiles) all += (float)tiles * (0.5f * (key_tiles(s, 0) + key_tiles(s, tiles - 1)));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    return __builtin_amdgcn_readfirstlane(max((int)fminf(__builtin_ceilf(all * a.H / slots), 1e9f), MIN_RUN));
+}
+__device__ __forceinline__ Seq seq_of(const Span& s, int run) {
+    Seq q;
+    q.tiles = (s.Lq + BM - 1) / BM;
+    q.most = q.tiles ? key_tiles(s, q.tiles - 1) : 0;
+    q.pieces = max((q.most + run - 1) / run, 1);
+    return q;
+}
+// What all workgroups find alike: the longest run, and of a head all pieces, the pieces of split row tiles, and those row tiles.
+struct Cut { int run, pieces, parts, split; };
+__device__ __forceinline__ Cut cut(const KdaLatentPrefillArgs& a, const Spans& spans, const Plan& p) {
+    Cut c = {longest_run(a, spans, p.share), 0, 0, 0};
+    for (int again = 0; again < 2; ++again) {
+        int pieces = 0, parts = 0, split = 0;
+        for (int n = threadIdx.x & 63; n < a.N; n += 64) {
+            const Seq q = seq_of(spans[n], c.run);
+            pieces += q.tiles * q.pieces;
+            if (q.pieces > 1) parts += q.tiles * q.pieces, split += q.tiles;
         }
+        c.pieces = __builtin_amdgcn_readlane(scan_wave(pieces), 63);
+        c.parts = __builtin_amdgcn_readlane(scan_wave(parts), 63);
+        c.split = __builtin_amdgcn_readlane(scan_wave(split), 63);
+        // (always so, but for the rounding of the sum: pieces <= row tiles + 2 share / H, parts <= 4 share / H)
+        if ((int64_t)c.pieces * a.H <= p.grid && (int64_t)c.parts * a.H <= p.slots) break;
+        c.run = 1 << 30;
+    }
+    return c;
+}
+struct Where {
+    int n, tile, piece, pieces;  // sequence, row tile, piece of it, pieces of the row tile
+    int slot;                    // of the row tile's first piece among the split ones of the head
+};
+// Piece `i` of a head (SPLIT: split row tile i); n < 0 past the last one.
+template <bool SPLIT>
+__device__ __forceinline__ Where locate(const KdaLatentPrefillArgs& a, const Spans& spans, int run, int i) {
+    const int lane = threadIdx.x & 63;
+    int before = 0, parts_before = 0;
+    for (int n0 = 0; n0 < a.N; n0 += 64) {
+        const int n = n0 + lane;
+        const Seq q = n < a.N ? seq_of(spans[n], run) : Seq{0, 0, 1};
+        const int parts = q.pieces > 1 ? q.tiles * q.pieces : 0;
+        const int mine = SPLIT ? (parts ? q.tiles : 0) : q.tiles * q.pieces;
+        const int s = scan_wave(mine), ps = scan_wave(parts);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(before + s > i);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            return {n0 + l, i - before - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(tiles, l))};
+            const int at = i - before - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(mine, l));
+            Where w;
+            w.n = n0 + l;
+            w.pieces = __builtin_amdgcn_readlane(q.pieces, l);
+            w.tile = SPLIT ? at : at / w.pieces;
+            w.piece = SPLIT ? 0 : at - w.tile * w.pieces;
+            w.slot = parts_before + __builtin_amdgcn_readlane(ps, l) - __builtin_amdgcn_readlane(parts, l) + w.tile * w.pieces;
+            return w;
         }
         before += __builtin_amdgcn_readlane(s, 63);
+        parts_before += __builtin_amdgcn_readlane(ps, 63);
     }
-    return {-1, 0};
+    return {-1, 0, 0, 1, 0};
 }
 
 template <typename T>
-__global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefillArgs a, int tiles) {
+__global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefillArgs a, Plan p) {
     __shared__ __align__(1024) unsigned char sm[2 * TILE_BYTES];
-    const int task = xcd_task(blockIdx.x, gridDim.x);  // an XCD works on few heads at a time: their keys stay in its L2
-    const int h = __builtin_amdgcn_readfirstlane(task / tiles);
-    const Where at = locate(a.cu_q, a.N, a.Tq, tiles - 1 - (task - h * tiles));  // long walks first
+    const Spans spans(a);
+    const Cut cu = cut(a, spans, p);
+    if ((int64_t)blockIdx.x >= (int64_t)cu.pieces * a.H) return;
+    // A piece of all heads side by side, long walks first (the last of a causal sequence), so that what starts last is short.
+    // With 8 heads or a multiple, a head stays on one XCD, whose L2 its keys pass.  (A head's pieces side by side and few heads
+    // at a time: 8192 causal tokens, 32 heads 700 us instead of 659.)
+    const int i = __builtin_amdgcn_readfirstlane(blockIdx.x / a.H), h = __builtin_amdgcn_readfirstlane(blockIdx.x - i * a.H);
+    const Where at = locate<false>(a, spans, cu.run, cu.pieces - 1 - i);
     const int n = __builtin_amdgcn_readfirstlane(at.n);
     if (n < 0) return;
     const int m0 = __builtin_amdgcn_readfirstlane(at.tile) * BM;
-    const int64_t q0 = min(max((int64_t)a.cu_q[n], (int64_t)0), a.Tq), k0 = min(max((int64_t)a.cu_k[n], (int64_t)0), a.Tk);
-    const int Lq = (int)(min((int64_t)a.cu_q[n + 1], a.Tq) - q0);
-    const int Lk = (int)max(min((int64_t)a.cu_k[n + 1], a.Tk) - k0, (int64_t)0);
-    const bool causal = a.flags & KDA355_LATENT_CAUSAL;
-    const int shift = causal ? Lk - Lq : Lk;  // row i sees keys j <= i + shift, j < Lk
+    const Span sp = span_of(a, n);
+    const int64_t q0 = sp.q0, k0 = sp.k0;
+    const int Lq = __builtin_amdgcn_readfirstlane(sp.Lq), Lk = __builtin_amdgcn_readfirstlane(sp.Lk), shift = __builtin_amdgcn_readfirstlane(sp.shift);
+    const int ntiles = __builtin_amdgcn_readfirstlane(key_tiles(sp, at.tile));
+    const int length = run_of(ntiles, at.pieces), first = __builtin_amdgcn_readfirstlane(at.piece * length);
+    const int last = __builtin_amdgcn_readfirstlane(min(first + length, ntiles));  // this piece's key tiles
+    if (at.piece > 0 && first >= ntiles) return;  // (a short row tile of a split sequence; the join counts its pieces alike)
+    const bool part = ntiles > length;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
     const int row = m0 + 32 * w + c;
@@ -128,16 +224,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     f32x16 acc[4] = {};
     float mo = M_START, l = 0.f;
     bool special = false;
-    const int seen = min(Lk, min(m0 + BM, Lq) + shift);        // keys that any row of the workgroup sees
     const int mine = min(Lk, min(m0 + 32 * w + 32, Lq) + shift);  // ... of this wave
     const int full = min(Lk, m0 + 32 * w + 1 + shift);         // keys that every row of this wave sees
-    const int ntiles = seen > 0 ? (seen + BN - 1) / BN : 0;
-
-    if (ntiles > 0) load_tile(0, 0);
-    for (int j = 0; j < ntiles; ++j) {
+    if (first < last) load_tile(first, first & 1);
+    for (int j = first; j < last; ++j) {
         wait_loads<0>();
         lds_barrier();  // tile j is whole, and every wave has read tile j - 1
-        if (j + 1 < ntiles) load_tile(j + 1, (j + 1) & 1);
+        if (j + 1 < last) load_tile(j + 1, (j + 1) & 1);
         const int t0 = j * BN;
         if (t0 >= mine) continue;  // wave-uniform; the barrier is at the top
         const uint32_t tb = lds + (j & 1) * TILE_BYTES;
@@ -162,12 +255,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = t0 + BN > full;  // some row of the wave does not see some key of the tile
         if (masked) {
-            const int last = min(row + shift, Lk - 1) - t0 - 4 * half;
+            const int seen = min(row + shift, Lk - 1) - t0 - 4 * half;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (32 * b + (r & 3) + 8 * (r >> 2) > last) s[b][r] = -INFINITY;
+                    if (32 * b + (r & 3) + 8 * (r >> 2) > seen) s[b][r] = -INFINITY;
         }
         // ---- running softmax: the maximum is raised, and the accumulator rescaled, only when some row of the wave
         // exceeds it by SLACK (the result is the same for any reference; weights stay within the type's range)
@@ -221,9 +314,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     }
 
     if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the keys that not every row sees
-        const int last = min(row + shift, Lk - 1);
+        const int seen = min(row + shift, Lk - 1);
 #pragma unroll 1
-        for (int j = max(full, 0) & ~(BN - 1); j < mine; ++j) {
+        for (int j = max(max(full, 0) & ~(BN - 1), first * BN); j < min(mine, last * BN); ++j) {
             const uint16_t* vr = vh + (int64_t)j * a.v_row + 4 * half;
 #pragma unroll
             for (int d = 0; d < 4; ++d)
@@ -232,14 +325,25 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = T::up(vr[32 * d + 8 * g + e]);
-                        if (j <= last && !(fabsf(x) < INFINITY)) acc[d][4 * g + e] += x;
+                        if (j <= seen && !(fabsf(x) < INFINITY)) acc[d][4 * g + e] += x;
                     }
         }
     }
 
-    // ---- o = acc / l
     l = sum_halves(l);
     if (row >= Lq) return;
+    if (part) {
+        char* slot = static_cast<char*>(a.workspace) + ((int64_t)h * cu.parts + at.slot + at.piece) * SLOT;
+        if (half == 0) *reinterpret_cast<f32x2*>(slot + SLOT_ACC + (32 * w + c) * 8) = f32x2{mo, l};
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(slot + ((w * 4 + d) * 4 + g) * 1024 + lane * 16) =
+                    f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        return;
+    }
+    // ---- o = acc / l
     const float inv = l > 0.f ? 1.f / l : 0.f;
     uint16_t* o = static_cast<uint16_t*>(a.out) + (q0 + row) * a.out_row + h * a.out_head + 4 * half;
 #pragma unroll
@@ -254,6 +358,62 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         a.lse[(q0 + row) * a.H + h] = l == 0.f ? -INFINITY : (mo + __builtin_amdgcn_logf(l)) * 0.69314718055995f;
 }
 
+// ------------------------------------------------------------------------------------------------ joining the parts
+// One workgroup for 32 rows (blockIdx.y) of a split row tile; wave d takes values 32 d .., parts two at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(KdaLatentPrefillArgs a, Plan p) {
+    const Spans spans(a);
+    const Cut cu = cut(a, spans, p);
+    for (int64_t task = blockIdx.x; task < (int64_t)cu.split * a.H; task += gridDim.x) {
+        const int h = __builtin_amdgcn_readfirstlane((int)(task / cu.split));
+        const Where at = locate<true>(a, spans, cu.run, (int)(task - (int64_t)h * cu.split));
+        const Span sp = span_of(a, __builtin_amdgcn_readfirstlane(at.n));
+        const int ntiles = key_tiles(sp, at.tile), length = run_of(ntiles, at.pieces);
+        if (ntiles <= length) continue;  // one piece: written by its workgroup
+        const int parts = __builtin_amdgcn_readfirstlane((ntiles + length - 1) / length);
+        const int d = threadIdx.x >> 6, lane = threadIdx.x & 63, w = blockIdx.y, c = lane & 31, half = lane >> 5;
+        const int row = at.tile * BM + 32 * w + c;
+        if (row >= sp.Lq) continue;
+        const char* slot = static_cast<const char*>(a.workspace) + ((int64_t)h * cu.parts + at.slot) * SLOT;
+        struct Part {
+            f32x2 ml;
+            f32x4 x[4];
+        };
+        auto load = [&](int i) {
+            Part y;
+            y.ml = *reinterpret_cast<const f32x2*>(slot + (int64_t)i * SLOT + SLOT_ACC + (32 * w + c) * 8);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) y.x[g] = *reinterpret_cast<const f32x4*>(slot + (int64_t)i * SLOT + ((w * 4 + d) * 4 + g) * 1024 + lane * 16);
+            return y;
+        };
+        float m = M_START, l = 0.f;
+        f32x4 acc[4] = {};
+        auto add = [&](const Part& y) {
+            const float mn = fmaxf(m, y.ml.x);
+            const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(y.ml.x - mn);
+            m = mn;
+            l = l * f0 + y.ml.y * f1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) acc[g] = acc[g] * f0 + y.x[g] * f1;
+        };
+        int i = 0;
+        for (; i + 1 < parts; i += 2) {
+            const Part y0 = load(i), y1 = load(i + 1);
+            add(y0);
+            add(y1);
+        }
+        if (i < parts) add(load(i));
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint16_t* o = static_cast<uint16_t*>(a.out) + (sp.q0 + row) * a.out_row + h * a.out_head + 32 * d + 4 * half;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<u32x2*>(o + 8 * g) =
+                l == 0.f ? u32x2{0u, 0u} : u32x2{T::pack(acc[g][0] * inv, acc[g][1] * inv), T::pack(acc[g][2] * inv, acc[g][3] * inv)};
+        if (a.lse && d == 0 && half == 0)
+            a.lse[(sp.q0 + row) * a.H + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055995f;
+    }
+}
+
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 // rows of 16-byte pieces: aligned base, strides in multiples of 8 elements
 bool rows16(const void* p, int64_t s0, int64_t s1 = 0) { return aligned(p, 16) && s0 % 8 == 0 && s1 % 8 == 0; }
@@ -264,14 +424,35 @@ bool near(int64_t row) { return row >= 0 && row <= MAX_ROW; }
 
 using namespace kda355;
 
-extern "C" int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* a, kda355_stream_t stream) {
+static int check_prefill_sizes(const KdaLatentPrefillArgs* a) {
     KDA_CHECK_ARG(a != nullptr, "latent_prefill: null args");
-    KDA_CHECK_ARG(a->N >= 0 && a->H >= 1 && a->Tq >= 0 && a->Tk >= 0, "latent_prefill: N=%d H=%d Tq=%lld Tk=%lld", a->N, a->H,
-                  (long long)a->Tq, (long long)a->Tk);
+    KDA_CHECK_ARG(a->N >= 0 && a->H >= 1 && a->Tq >= 0 && a->Tk >= 0 && a->num_cus >= 0 && a->num_cus <= 65536,
+                  "latent_prefill: N=%d H=%d Tq=%lld Tk=%lld num_cus=%d", a->N, a->H, (long long)a->Tq, (long long)a->Tk, a->num_cus);
+    KDA_CHECK_ARG(a->Tq < (1ll << 30) && a->Tk < (1ll << 30), "latent_prefill: 2^30 tokens or more");
+    KDA_CHECK_ARG((a->Tq / BM + a->N) * a->H < (1ll << 22), "latent_prefill: grid too large");
+    return 0;
+}
+static Plan plan_of(const KdaLatentPrefillArgs* a) {
+    const int64_t rows = (a->Tq / BM + a->N) * a->H;  // at least the row tiles of all sequences and heads
+    Plan p;
+    p.share = 2 * (a->num_cus ? a->num_cus : 256);  // two workgroups a CU
+    p.grid = (int)(rows + 2 * p.share);
+    const int64_t most = rows * ((a->Tk / BN + 1 + MIN_RUN - 1) / MIN_RUN);
+    p.slots = (int)(most < 4 * p.share ? most : 4 * p.share);
+    return p;
+}
+
+extern "C" int64_t kda355_latent_prefill_workspace_bytes(const KdaLatentPrefillArgs* a) {
+    if (const int rc = check_prefill_sizes(a)) return rc;
+    if (a->N == 0 || a->Tq == 0) return 0;
+    return (int64_t)plan_of(a).slots * SLOT;
+}
+
+extern "C" int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* a, kda355_stream_t stream) {
+    if (const int rc = check_prefill_sizes(a)) return rc;
     KDA_CHECK_ARG(a->dtype == KDA355_DTYPE_BF16 || a->dtype == KDA355_DTYPE_FP16, "latent_prefill: dtype %d", a->dtype);
     KDA_CHECK_ARG((a->flags & ~KDA355_LATENT_CAUSAL) == 0, "latent_prefill: unknown flags 0x%x", a->flags);
     if (a->N == 0 || a->Tq == 0) return 0;
-    KDA_CHECK_ARG(a->Tq < (1ll << 30) && a->Tk < (1ll << 30), "latent_prefill: 2^30 tokens or more");
     KDA_CHECK_ARG(a->q && a->out && a->cu_q && a->cu_k && (a->Tk == 0 || (a->k && a->v && a->k_pe)),
                   "latent_prefill: a required pointer is null");
     KDA_CHECK_ARG(rows16(a->q, a->q_row, a->q_head) && rows16(a->k, a->k_row, a->k_head) && rows16(a->v, a->v_row, a->v_head) &&
@@ -279,14 +460,18 @@ extern "C" int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* a, kda35
                   "latent_prefill: rows must be 16-byte aligned");
     KDA_CHECK_ARG(near(a->k_row) && near(a->v_row) && near(a->pe_row), "latent_prefill: token strides of k, v and k_pe must be at most 2^23");
     KDA_CHECK_ARG(a->scale > 0.f, "latent_prefill: scale must be positive");
-    const int64_t tiles = a->Tq / BM + a->N;  // at least the sum of every sequence's row tiles
-    KDA_CHECK_ARG(tiles * a->H < (1ll << 23), "latent_prefill: grid too large");
+    const int64_t need = kda355_latent_prefill_workspace_bytes(a);
+    KDA_CHECK_ARG(a->workspace && aligned(a->workspace, 256) && a->workspace_bytes >= need,
+                  "latent_prefill: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((uint32_t)(tiles * a->H));
-    if (a->dtype == KDA355_DTYPE_BF16)
-        hipLaunchKernelGGL(prefill_kernel<Bf16>, grid, dim3(WAVES * 64), 0, s, *a, (int)tiles);
-    else
-        hipLaunchKernelGGL(prefill_kernel<Fp16>, grid, dim3(WAVES * 64), 0, s, *a, (int)tiles);
+    const Plan p = plan_of(a);
+    const dim3 join(p.slots / 2 < 1 ? 1 : min(p.slots / 2, p.share), WAVES);  // a split row tile has two parts at least
+    auto launch = [&](auto type) {
+        typedef decltype(type) T;
+        hipLaunchKernelGGL(prefill_kernel<T>, dim3(p.grid), dim3(WAVES * 64), 0, s, *a, p);
+        hipLaunchKernelGGL(join_kernel<T>, join, dim3(256), 0, s, *a, p);
+    };
+    if (a->dtype == KDA355_DTYPE_BF16) launch(Bf16{}); else launch(Fp16{});
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         set_error("latent_prefill: launch failed: %s", hipGetErrorString(e));

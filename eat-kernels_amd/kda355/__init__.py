@@ -20,14 +20,14 @@ from .prefill import chunk_kda, kda_prefill, plan, prefill, prefill_prepare  # n
 from .recurrent import fused_recurrent_kda, spec_commit  # noqa: F401
 from .decode import decode  # noqa: F401
 from .latent import (latent_append, latent_decode, latent_decode_workspace_bytes, latent_gather,  # noqa: F401
-                     latent_prefill)
+                     latent_prefill, latent_prefill_workspace_bytes)
 from .pages import compact_pages, copy_rows, fork_pages, free_pages  # noqa: F401
 from .health import (decode_cotenant_mode, decode_health, decode_warmup, prefill_health,  # noqa: F401
                      prefill_range_guard)
 from . import ops  # noqa: F401  (registers torch.ops.kda355.*)
 
 __all__ = ["chunk_kda", "kda_prefill", "plan", "prefill", "prefill_prepare", "fused_recurrent_kda", "spec_commit", "decode",
-           "latent_prefill", "latent_decode", "latent_decode_workspace_bytes", "latent_append", "latent_gather",
+           "latent_prefill", "latent_prefill_workspace_bytes", "latent_decode", "latent_decode_workspace_bytes", "latent_append", "latent_gather",
            "copy_rows", "fork_pages", "free_pages", "compact_pages",
            "decode_warmup", "decode_cotenant_mode", "decode_health", "prefill_health", "prefill_range_guard",
            "lib", "LIB_PATH"]

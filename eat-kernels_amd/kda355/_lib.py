@@ -97,8 +97,9 @@ class KdaLatentPrefillArgs(ctypes.Structure):
     _fields_ = [
         ("q", P), ("k", P), ("v", P), ("k_pe", P), ("out", P), ("lse", P), ("cu_q", P), ("cu_k", P),
         ("q_row", I64), ("q_head", I64), ("k_row", I64), ("k_head", I64), ("v_row", I64), ("v_head", I64),
-        ("pe_row", I64), ("out_row", I64), ("out_head", I64), ("Tq", I64), ("Tk", I64),
-        ("N", I32), ("H", I32), ("dtype", I32), ("flags", U32), ("scale", F32), ("reserved", I32),
+        ("pe_row", I64), ("out_row", I64), ("out_head", I64), ("Tq", I64), ("Tk", I64), ("workspace", P),
+        ("workspace_bytes", I64),
+        ("N", I32), ("H", I32), ("dtype", I32), ("flags", U32), ("scale", F32), ("num_cus", I32),
     ]
 
 
@@ -169,8 +170,10 @@ def lib():
             f = getattr(L, f"kda355_{name}_launch")
             f.argtypes = [ctypes.POINTER(args), P]
             f.restype = ctypes.c_int
-        L.kda355_latent_decode_workspace_bytes.argtypes = [ctypes.POINTER(KdaLatentDecodeArgs)]
-        L.kda355_latent_decode_workspace_bytes.restype = I64
+        for name, args in (("latent_prefill", KdaLatentPrefillArgs), ("latent_decode", KdaLatentDecodeArgs)):
+            f = getattr(L, f"kda355_{name}_workspace_bytes")
+            f.argtypes = [ctypes.POINTER(args)]
+            f.restype = I64
         L.kda355_last_error.restype = ctypes.c_char_p
         L.kda355_version.restype = ctypes.c_int
         _lib = L
@@ -206,7 +209,7 @@ def exported_symbols():
     """Names declared in include/kda355.h that the library must export."""
     return ["kda355_recurrent_launch", "kda355_spec_commit_launch", "kda355_decode_launch", "kda355_prefill_plan",
             "kda355_prefill_workspace_bytes", "kda355_prefill_launch", "kda355_prefill_launch_noalloc",
-            "kda355_latent_prefill_launch", "kda355_latent_decode_workspace_bytes", "kda355_latent_decode_launch",
+            "kda355_latent_prefill_workspace_bytes", "kda355_latent_prefill_launch", "kda355_latent_decode_workspace_bytes", "kda355_latent_decode_launch",
             "kda355_latent_append_launch", "kda355_latent_gather_launch", "kda355_copy_rows_launch",
             "kda355_fork_pages_launch", "kda355_free_pages_launch", "kda355_compact_pages_launch",
             "kda355_last_error", "kda355_version"]

@@ -113,12 +113,30 @@ def _lse_ptr(lse, shape, device):
     return lse.data_ptr()
 
 
-def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal=True, *, out=None, lse=None):
+def _workspace(a, need, workspace, device, name):
+    """The caller's workspace, or one from torch's allocator, into the arguments; returned so that it lives as long as the call."""
+    if need < 0:
+        _lib.check(int(need), name)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        _need("workspace", workspace, torch.uint8, device)
+        if not workspace.is_contiguous() or workspace.numel() < need:
+            raise ValueError(f"kda355: workspace must be contiguous with >= {need} bytes")
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    return workspace
+
+
+def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal=True, *, out=None, lse=None,
+                   workspace=None):
     """The expanded form over packed sequences: q [Tq, H, 192] (128 | 64), k and v [Tk, H, 128], k_pe [Tk, 64] shared by the
     heads.  cu_seqlens_q / cu_seqlens_k int32 [N + 1] on the device; the queries are the last tokens of their sequences, so
     with `causal` query i of Lq sees keys j <= i + Lk - Lq.  Returns out [Tq, H, 128]; `lse` (fp32 [Tq, H]) receives the
     logarithms of the softmax sums, for joining with the attention over other keys.  A query that sees no key gets zeros and
-    -inf, and keys it does not see never reach it, whatever they hold."""
+    -inf, and keys it does not see never reach it, whatever they hold.
+
+    workspace: uint8 tensor of latent_prefill_workspace_bytes(...); by default one is taken from torch's allocator for the
+    call.  Calls that may overlap need workspaces of their own."""
     dev, dt = _first("q", q)
     if q.dim() != 3 or q.shape[2] != HEAD + PE:
         raise ValueError(f"kda355: q must be [Tq, H, {HEAD + PE}], got {list(q.shape)}")
@@ -138,10 +156,23 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
     o_st = _rows("out", out, (Tq, H, HEAD), dt, dev)
     a = _lib.KdaLatentPrefillArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(), _lse_ptr(lse, (Tq, H), dev),
-        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *q_st, *k_st, *v_st, *pe_st, *o_st, Tq, Tk, N, H, _DTYPES[dt],
-        1 if causal else 0, SCALE if scale is None else float(scale), 0)
-    _lib.check(_lib.lib().kda355_latent_prefill_launch(ctypes.byref(a), _stream(dev)), "latent_prefill")
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *q_st, *k_st, *v_st, *pe_st, *o_st, Tq, Tk, None, 0, N, H, _DTYPES[dt],
+        1 if causal else 0, SCALE if scale is None else float(scale), _num_cus(dev))
+    L, p = _lib.lib(), ctypes.byref(a)
+    need = L.kda355_latent_prefill_workspace_bytes(p)
+    if need:
+        workspace = _workspace(a, need, workspace, dev, "latent_prefill")
+    _lib.check(L.kda355_latent_prefill_launch(p, _stream(dev)), "latent_prefill")
     return out
+
+
+def latent_prefill_workspace_bytes(N, H, Tq, Tk, *, num_cus=256):
+    """Bytes of device workspace that latent_prefill() needs for these sizes (host only)."""
+    a = _lib.KdaLatentPrefillArgs(N=N, H=H, Tq=Tq, Tk=Tk, num_cus=num_cus)
+    need = _lib.lib().kda355_latent_prefill_workspace_bytes(ctypes.byref(a))
+    if need < 0:
+        _lib.check(int(need), "latent_prefill_workspace_bytes")
+    return int(need)
 
 
 def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, out=None, lse=None, prefix_table=None,
@@ -186,19 +217,11 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
         prefix_table.data_ptr() if width else None, prefix_len.data_ptr() if width else None, out.data_ptr(),
         _lse_ptr(lse, (T, H), dev), None, *ql_st, *qp_st, *o_st, page_stride, pages, table_stride, 0, B, S, H, size,
         block_table.shape[1], width, _DTYPES[dt], _num_cus(dev), SCALE if scale is None else float(scale), 0)
-    L = _lib.lib()
-    need = L.kda355_latent_decode_workspace_bytes(ctypes.byref(a))
-    if need < 0:
-        _lib.check(int(need), "latent_decode")
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    else:
-        _need("workspace", workspace, torch.uint8, dev)
-        if not workspace.is_contiguous() or workspace.numel() < need:
-            raise ValueError(f"kda355: workspace must be contiguous with >= {need} bytes")
-    if workspace is not None:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    _lib.check(L.kda355_latent_decode_launch(ctypes.byref(a), _stream(dev)), "latent_decode")
+    L, p = _lib.lib(), ctypes.byref(a)
+    need = L.kda355_latent_decode_workspace_bytes(p)
+    if need:
+        workspace = _workspace(a, need, workspace, dev, "latent_decode")
+    _lib.check(L.kda355_latent_decode_launch(p, _stream(dev)), "latent_decode")
     return out
 
 

@@ -73,7 +73,7 @@ SCHEMAS = {
         "Tensor num_accepted_tokens, bool slot0_reserved=True) -> ()",
     "latent_prefill":
         "latent_prefill(Tensor q, Tensor k, Tensor v, Tensor k_pe, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
-        "Tensor(a!) out, float? scale=None, bool causal=True, Tensor(b!)? lse=None) -> ()",
+        "Tensor(a!) out, float? scale=None, bool causal=True, Tensor(b!)? lse=None, Tensor(c!)? workspace=None) -> ()",
     "latent_decode":
         "latent_decode(Tensor q_latent, Tensor q_pe, Tensor cache, Tensor block_table, Tensor seq_lens, "
         "Tensor(a!) out, float? scale=None, Tensor(b!)? lse=None, Tensor? prefix_table=None, "
@@ -230,8 +230,9 @@ def _spec_commit_op(scratch, scratch_indices, pool, pool_indices, num_accepted_t
     _recurrent.spec_commit(scratch, scratch_indices, pool, pool_indices, num_accepted_tokens, slot0_reserved)
 
 
-def _latent_prefill_op(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, out, scale=None, causal=True, lse=None):
-    _latent.latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale, causal, out=out, lse=lse)
+def _latent_prefill_op(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, out, scale=None, causal=True, lse=None,
+                       workspace=None):
+    _latent.latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale, causal, out=out, lse=lse, workspace=workspace)
 
 
 def _latent_decode_op(q_latent, q_pe, cache, block_table, seq_lens, out, scale=None, lse=None, prefix_table=None,

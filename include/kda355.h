@@ -320,12 +320,17 @@ typedef struct KdaLatentPrefillArgs {
     const int32_t* cu_k; /* [N + 1], the same for Tk */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, pe_row, out_row, out_head;
     int64_t Tq, Tk;
+    void* workspace;     /* kda355_latent_prefill_workspace_bytes(args), 256-byte aligned; nothing in it has to start at
+                            zero, launches that may overlap need their own */
+    int64_t workspace_bytes;
     int32_t N, H, dtype;
     uint32_t flags;      /* KDA355_LATENT_CAUSAL or 0 */
-    float scale;
-    int32_t reserved;
+    float scale;         /* positive */
+    int32_t num_cus;     /* CUs to fill (0: 256) */
 } KdaLatentPrefillArgs;
 
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL. */
+int64_t kda355_latent_prefill_workspace_bytes(const KdaLatentPrefillArgs* args);
 int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* args, kda355_stream_t stream);
 
 /*

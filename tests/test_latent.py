@@ -44,7 +44,8 @@ FAKE = 1 << 20  # a 16-byte aligned address that is never read: every call below
 
 def _prefill_args(**kw):
     a = dict(q=FAKE, k=FAKE, v=FAKE, k_pe=FAKE, out=FAKE, cu_q=FAKE, cu_k=FAKE, q_row=384, q_head=192, k_row=256, k_head=128,
-             v_row=256, v_head=128, pe_row=64, out_row=256, out_head=128, Tq=8, Tk=8, N=1, H=2, scale=1.0)
+             v_row=256, v_head=128, pe_row=64, out_row=256, out_head=128, Tq=8, Tk=8, N=1, H=2, scale=1.0,
+             workspace=FAKE, workspace_bytes=1 << 40)
     a.update(kw)
     return _lib().KdaLatentPrefillArgs(**a)
 
@@ -80,7 +81,8 @@ BAD = [("latent_prefill", _prefill_args, kw, msg) for kw, msg in [
     (dict(q=0), b"null"), (dict(k=0), b"null"), (dict(cu_k=0), b"null"), (dict(q=FAKE + 8), b"aligned"),
     (dict(k_row=260), b"aligned"), (dict(v_head=4), b"aligned"), (dict(pe_row=65), b"aligned"), (dict(out_head=4), b"aligned"),
     (dict(Tk=1 << 30), b"2^30"), (dict(Tq=1 << 30), b"2^30"), (dict(scale=0.0), b"positive"), (dict(scale=-1.0), b"positive"),
-    (dict(scale=float("nan")), b"positive"), (dict(k_row=(1 << 23) + 8), b"2^23"), (dict(H=1 << 23), b"grid")]]
+    (dict(scale=float("nan")), b"positive"), (dict(k_row=(1 << 23) + 8), b"2^23"), (dict(H=1 << 23), b"grid"), (dict(workspace=0), b"workspace"),
+    (dict(workspace=FAKE + 16), b"workspace"), (dict(workspace_bytes=100), b"workspace"), (dict(num_cus=-1), b"num_cus")]]
 BAD += [("latent_decode", _decode_args, kw, msg) for kw, msg in [
     (dict(B=-1), b"B=-1"), (dict(S=0), b"S=0"), (dict(H=0), b"H=0"), (dict(page_size=0), b"page_size"),
     (dict(table_width=1 << 30), b"2^31"), (dict(prefix_width=1 << 30), b"2^31"), (dict(B=1 << 20, S=1 << 10, H=2), b"too large"),
@@ -152,6 +154,11 @@ def test_workspace_is_checked():
             assert m.lib().kda355_latent_decode_launch(ctypes.byref(a), None) == m.EINVAL
     with pytest.raises(ValueError):
         kda355.latent_decode_workspace_bytes(1, 0, 1, 1, 1)
+    for N, H, Tq, Tk in ((1, 16, 77, 1277), (1, 32, 8192, 8192), (64, 96, 64, 1 << 20)):
+        assert 0 < kda355.latent_prefill_workspace_bytes(N, H, Tq, Tk) < 1 << 30
+    assert kda355.latent_prefill_workspace_bytes(0, 1, 0, 0) == 0
+    with pytest.raises(ValueError):
+        kda355.latent_prefill_workspace_bytes(1, 0, 1, 1)
 
 
 def test_cpu_tensors_raise():
