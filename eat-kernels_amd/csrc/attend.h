@@ -51,41 +51,21 @@ struct Fp16 {
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
 
-// N x (64 lanes x 16 bytes) from global memory into N KiB of LDS from byte `lds` (wave-uniform), lane l's piece i at
-// lds + 1024 i + 16 l, from byte voff[i] (a lane's) + soff[i] (the wave's).  Lane offsets at or past the descriptor's size read
-// as zeros.  In asm, because the compiler would wait for every such load before any read of LDS; whoever reads the data waits
-// with wait_loads() and a barrier.  A vector memory instruction may read an SGPR that a vector instruction wrote (readlane:
-// spilled descriptors too) five wait states later at the earliest, and the compiler does not look into asm: s_nop 4.
-constexpr uint32_t LDS_ZERO = 0x80000000u;  // a lane offset that is out of range for every descriptor below
-#define KDA_NEXT_M0 "\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t"
-__device__ __forceinline__ void load_to_lds4(uint32_t lds, u32x4 rsrc, const uint32_t (&voff)[4], const uint32_t (&soff)[4]) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, %6 offen lds" KDA_NEXT_M0
-                 "buffer_load_dwordx4 %3, %1, %7 offen lds" KDA_NEXT_M0 "buffer_load_dwordx4 %4, %1, %8 offen lds" KDA_NEXT_M0
-                 "buffer_load_dwordx4 %5, %1, %9 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-                 "s"(rsrc), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(__builtin_amdgcn_readfirstlane(soff[0])),
-                 "s"(__builtin_amdgcn_readfirstlane(soff[1])), "s"(__builtin_amdgcn_readfirstlane(soff[2])),
-                 "s"(__builtin_amdgcn_readfirstlane(soff[3]))
-                 : "memory", "scc");
+// 64 lanes x 16 bytes from global memory into 1 KiB of LDS at byte `lds` (wave-uniform), lane l's piece at lds + 16 l, from byte
+// voff (a lane's) of the descriptor; pieces past its size read as zeros.  In asm, because the compiler would wait for every
+// such load before any read of LDS; whoever reads the data waits with wait_loads() and a barrier.  A vector memory instruction
+// may read an SGPR that a vector instruction wrote (readlane: spilled descriptors too) five wait states later at the earliest,
+// and the compiler does not look into asm: s_nop 4.  A CU takes about 16 cycles a load, and a wave that asks for more than a few
+// at once stalls: the kernels spread them between matrix instructions.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, u32x4 rsrc, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+                 "v"(voff), "s"(rsrc)
+                 : "memory");
 }
-__device__ __forceinline__ void load_to_lds2(uint32_t lds, u32x4 rsrc, const uint32_t (&voff)[2], const uint32_t (&soff)[2]) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %1, %4 offen lds" KDA_NEXT_M0
-                 "buffer_load_dwordx4 %3, %1, %5 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-                 "s"(rsrc), "v"(voff[0]), "v"(voff[1]), "s"(__builtin_amdgcn_readfirstlane(soff[0])),
-                 "s"(__builtin_amdgcn_readfirstlane(soff[1]))
-                 : "memory", "scc");
-}
-// the same from four rows of their own, base[i] (the wave's) + voff[i]
-__device__ __forceinline__ void load_rows4(uint32_t lds, const uint64_t (&base)[4], const uint32_t (&voff)[4]) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %5" KDA_NEXT_M0
-                 "global_load_lds_dwordx4 %2, %6" KDA_NEXT_M0 "global_load_lds_dwordx4 %3, %7" KDA_NEXT_M0
-                 "global_load_lds_dwordx4 %4, %8" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
-                 "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(base[0]), "s"(base[1]), "s"(base[2]), "s"(base[3])
-                 : "memory", "scc");
-}
-__device__ __forceinline__ u32x4 tile_rsrc(const void* base) {
+__device__ __forceinline__ u32x4 tile_rsrc(const void* base, uint32_t size) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);
     return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
-                 0x7fffffffu, 0x00020000u};
+                 (uint32_t)__builtin_amdgcn_readfirstlane(size), 0x00020000u};
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // all but the N youngest loads of this wave have arrived

@@ -342,11 +342,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 
         // ==================================================================== value waves
         // ---- loads
-        const u32x4 table_rsrc = [&] {
-            u32x4 r = tile_rsrc(table);
-            r[2] = __builtin_amdgcn_readfirstlane(width) * 4;  // entries past the table read as zeros (and are past `last`)
-            return r;
-        }();
+        const u32x4 table_rsrc = tile_rsrc(table, (uint32_t)width * 4);  // entries past the table read as zeros (and are past `last`)
         const uint32_t pages_at = lds + LDS_PAGES + vw * 1024;
         const int own8 = 8 * vw + (lane & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
         auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens

@@ -180,32 +180,31 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t piece = ((lane & 15) ^ ((lane >> 4) << 2) ^ i) * 16;
-        koff[i] = (uint32_t)lt * (uint32_t)(2 * a.k_row) + piece;
-        voff[i] = (uint32_t)lt * (uint32_t)(2 * a.v_row) + piece;
+        koff[i] = (uint32_t)(lt + 4 * i) * (uint32_t)(2 * a.k_row) + piece;
+        voff[i] = (uint32_t)(lt + 4 * i) * (uint32_t)(2 * a.v_row) + piece;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) poff[i] = (uint32_t)pt * (uint32_t)(2 * a.pe_row) + ((lane & 7) ^ swz8(pt + 8 * i)) * 16;
-    const uint32_t kstep = 8 * (uint32_t)a.k_row, vstep = 8 * (uint32_t)a.v_row, pstep = 16 * (uint32_t)a.pe_row;
-    auto load_tile = [&](int j, int buf) {
-        const int t0 = j * BN, left = Lk - t0;
-        const u32x4 kr = tile_rsrc(kh + (int64_t)t0 * a.k_row), vr = tile_rsrc(vh + (int64_t)t0 * a.v_row),
-                    pr = tile_rsrc(ph + (int64_t)t0 * a.pe_row);
-        const uint32_t base = lds + buf * TILE_BYTES + 16 * w * (HD * 2), pbase = lds + buf * TILE_BYTES + TILE_PE + 16 * w * (PE * 2);
-        auto issue = [&](auto whole) {
-            uint32_t ko[4], vo[4], ks[4], vs[4], po[2], ps[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = whole || lt + 4 * i < left;
-                ko[i] = in ? koff[i] : LDS_ZERO, ks[i] = i * kstep;
-                vo[i] = in ? voff[i] : LDS_ZERO, vs[i] = i * vstep;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) po[i] = whole || pt + 8 * i < left ? poff[i] : LDS_ZERO, ps[i] = i * pstep;
-            load_to_lds4(base, kr, ko, ks);
-            load_to_lds4(base + TILE_V, vr, vo, vs);
-            load_to_lds2(pbase, pr, po, ps);
-        };
-        if (left >= BN) issue(std::true_type{}); else issue(std::false_type{});
+    for (int i = 0; i < 2; ++i) poff[i] = (uint32_t)(pt + 8 * i) * (uint32_t)(2 * a.pe_row) + ((lane & 7) ^ swz8(pt + 8 * i)) * 16;
+    // A tile's descriptors end with the row of its last token, so that tokens past it read as zeros (where rows overlap or are
+    // one and the same: as its values, and like the zeros they are hidden).
+    struct Tile { u32x4 k, v, pe; uint32_t at; };
+    auto tile_at = [&](int j) {
+        const int t0 = j * BN;
+        const uint32_t n = min(Lk - t0, BN) - 1, some = j < last ? ~0u : 0u;  // past the piece: nothing is read
+        Tile t;
+        t.k = tile_rsrc(kh + (int64_t)t0 * a.k_row, (n * (uint32_t)(2 * a.k_row) + HD * 2) & some);
+        t.v = tile_rsrc(vh + (int64_t)t0 * a.v_row, (n * (uint32_t)(2 * a.v_row) + HD * 2) & some);
+        t.pe = tile_rsrc(ph + (int64_t)t0 * a.pe_row, (n * (uint32_t)(2 * a.pe_row) + PE * 2) & some);
+        t.at = lds + (j & 1) * TILE_BYTES + 16 * w * (HD * 2);
+        return t;
+    };
+    auto bring = [&](const Tile& t, int i) {  // load i of 10
+        if (i < 4)
+            load_to_lds(t.at + 4 * i * (HD * 2), t.k, koff[i]);
+        else if (i < 8)
+            load_to_lds(t.at + TILE_V + 4 * (i - 4) * (HD * 2), t.v, voff[i - 4]);
+        else
+            load_to_lds(t.at - 16 * w * (HD * 2) + TILE_PE + (16 * w + 8 * (i - 8)) * (PE * 2), t.pe, poff[i - 8]);
     };
 
     // ---- LDS read addresses (byte offsets within a tile; key step, value tile and key block are xors and constants)
@@ -224,17 +223,29 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     f32x16 acc[4] = {};
     float mo = M_START, l = 0.f;
     bool special = false;
-    const int mine = min(Lk, min(m0 + 32 * w + 32, Lq) + shift);  // ... of this wave
+    const int mine = m0 + 32 * w < Lq ? min(Lk, min(m0 + 32 * w + 32, Lq) + shift) : 0;  // keys that any row of this wave sees
     const int full = min(Lk, m0 + 32 * w + 1 + shift);         // keys that every row of this wave sees
-    if (first < last) load_tile(first, first & 1);
+    if (first < last) {
+        const Tile t = tile_at(first);
+#pragma unroll
+        for (int i = 0; i < 10; ++i) bring(t, i);
+    }
+    // the queries are there before the loop: the compiler would wait for them, and so for the next tile, in it
+#pragma unroll
+    for (int i = 0; i < 12; ++i) asm volatile("" : "+v"(q[i]));
     for (int j = first; j < last; ++j) {
         wait_loads<0>();
         lds_barrier();  // tile j is whole, and every wave has read tile j - 1
-        if (j + 1 < last) load_tile(j + 1, (j + 1) & 1);
         const int t0 = j * BN;
-        if (t0 >= mine) continue;  // wave-uniform; the barrier is at the top
+        const Tile next = tile_at(j + 1);
+        if (t0 >= mine) {  // wave-uniform; the barrier is at the top
+#pragma unroll
+            for (int i = 0; i < 10; ++i) bring(next, i);
+            continue;
+        }
         const uint32_t tb = lds + (j & 1) * TILE_BYTES;
-        // ---- scores: 24 steps (key step i of 12, key block b of 2), the operands of the next four read while four run
+        // ---- scores: 24 steps (key step i of 12, key block b of 2), the operands of the next four read while four run, the next
+        // tile's loads between them
         f32x16 s[2] = {};
         auto key = [&](int x) {
             const int i = x >> 1, b = x & 1;
@@ -250,7 +261,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
 #pragma unroll
                 for (int x = 0; x < 4; ++x) kf[(g + 1) & 1][x] = key(4 * g + 4 + x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[x & 1] = T::mfma(kf[g & 1][x], q[2 * g + (x >> 1)], s[x & 1]);
+            for (int x = 0; x < 4; ++x) {
+                s[x & 1] = T::mfma(kf[g & 1][x], q[2 * g + (x >> 1)], s[x & 1]);
+                if (g < 5 && (x & 1)) bring(next, 2 * g + (x >> 1));
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
         const bool masked = t0 + BN > full;  // some row of the wave does not see some key of the tile
@@ -313,6 +327,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         }
     }
 
+    wait_loads<0>();  // (nothing is left in flight towards LDS)
     if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the keys that not every row sees
         const int seen = min(row + shift, Lk - 1);
 #pragma unroll 1
