@@ -188,14 +188,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     // A tile's descriptors end with the row of its last token, so that tokens past it read as zeros (where rows overlap or are
     // one and the same: as its values, and like the zeros they are hidden).
     struct Tile { u32x4 k, v, pe; uint32_t at; };
-    auto tile_at = [&](int j) {
-        const int t0 = j * BN;
-        const uint32_t n = min(Lk - t0, BN) - 1, some = j < last ? ~0u : 0u;  // past the piece: nothing is read
+    const uint32_t krow = 2 * (uint32_t)a.k_row, vrow = 2 * (uint32_t)a.v_row, prow = 2 * (uint32_t)a.pe_row;
+    const char* kn = reinterpret_cast<const char*>(kh) + (int64_t)first * BN * krow;  // the next tile to be brought
+    const char* vn = reinterpret_cast<const char*>(vh) + (int64_t)first * BN * vrow;
+    const char* pn = reinterpret_cast<const char*>(ph) + (int64_t)first * BN * prow;
+    auto tile_at = [&](int j) {  // called for one after the other
+        const bool whole = j * BN + BN <= Lk, some = j < last;  // past the piece: nothing is read
+        const uint32_t n = whole ? BN - 1 : Lk - j * BN - 1;
         Tile t;
-        t.k = tile_rsrc(kh + (int64_t)t0 * a.k_row, (n * (uint32_t)(2 * a.k_row) + HD * 2) & some);
-        t.v = tile_rsrc(vh + (int64_t)t0 * a.v_row, (n * (uint32_t)(2 * a.v_row) + HD * 2) & some);
-        t.pe = tile_rsrc(ph + (int64_t)t0 * a.pe_row, (n * (uint32_t)(2 * a.pe_row) + PE * 2) & some);
+        t.k = tile_rsrc(kn, some ? n * krow + HD * 2 : 0);
+        t.v = tile_rsrc(vn, some ? n * vrow + HD * 2 : 0);
+        t.pe = tile_rsrc(pn, some ? n * prow + PE * 2 : 0);
         t.at = lds + (j & 1) * TILE_BYTES + 16 * w * (HD * 2);
+        kn += BN * (int64_t)krow, vn += BN * (int64_t)vrow, pn += BN * (int64_t)prow;
         return t;
     };
     auto bring = [&](const Tile& t, int i) {  // load i of 10
@@ -233,16 +238,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     // the queries are there before the loop: the compiler would wait for them, and so for the next tile, in it
 #pragma unroll
     for (int i = 0; i < 12; ++i) asm volatile("" : "+v"(q[i]));
-    for (int j = first; j < last; ++j) {
+    auto tile = [&](int j, auto masked_) {  // MASKED: some row of the wave does not see some key of the tile
+        constexpr bool MASKED = decltype(masked_)::value;
         wait_loads<0>();
         lds_barrier();  // tile j is whole, and every wave has read tile j - 1
         const int t0 = j * BN;
         const Tile next = tile_at(j + 1);
-        if (t0 >= mine) {  // wave-uniform; the barrier is at the top
-#pragma unroll
-            for (int i = 0; i < 10; ++i) bring(next, i);
-            continue;
-        }
         const uint32_t tb = lds + (j & 1) * TILE_BYTES;
         // ---- scores: 24 steps (key step i of 12, key block b of 2), the operands of the next four read while four run, the next
         // tile's loads between them
@@ -267,8 +268,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        const bool masked = t0 + BN > full;  // some row of the wave does not see some key of the tile
-        if (masked) {
+        if constexpr (MASKED) {
             const int seen = min(row + shift, Lk - 1) - t0 - 4 * half;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
             if (k < 3)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) vf[(k + 1) & 1][d] = value(k + 1, d);
-            if (masked)
+            if constexpr (MASKED)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     special |= nonfinite<T>(vf[k & 1][d]);
@@ -325,8 +325,18 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
 #pragma unroll
             for (int d = 0; d < 4; ++d) acc[d] = T::mfma(vf[k & 1][d], p[k], acc[d]);
         }
+    };
+    const int clean = min(last, max(full, 0) / BN), mixed = min(last, (mine + BN - 1) / BN);
+    int j = first;
+    for (; j < clean; ++j) tile(j, std::false_type{});
+    for (; j < mixed; ++j) tile(j, std::true_type{});
+    for (; j < last; ++j) {  // tiles that only later rows see
+        wait_loads<0>();
+        lds_barrier();
+        const Tile next = tile_at(j + 1);
+#pragma unroll
+        for (int i = 0; i < 10; ++i) bring(next, i);
     }
-
     wait_loads<0>();  // (nothing is left in flight towards LDS)
     if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the keys that not every row sees
         const int seen = min(row + shift, Lk - 1);
