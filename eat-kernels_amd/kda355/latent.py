@@ -21,6 +21,7 @@ Errors: TypeError for a wrong dtype or device, ValueError for a wrong shape or s
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -34,8 +35,19 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _cus = {}
 
 
-# A decode step makes dozens of these calls, each of a few microseconds on the GPU, so the checks below first ask for what is
-# right in as few steps as possible, and look closer only to name what is wrong.
+# A decode step makes dozens of these calls, each of a few microseconds on the GPU.  What the checks look at (types, devices,
+# shapes, strides) comes back call after call, so every entry keeps what it found for it: the checked sizes and strides, packed as
+# the C struct's bytes.  The addresses are the call's own.
+_MOST = 4096  # kept at a time, per entry
+
+
+def _keep(seen, key, plan):
+    if len(seen) >= _MOST:
+        seen.clear()
+    seen[key] = plan
+    return plan
+
+
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object (2 us)
 
 
@@ -106,25 +118,53 @@ def _cache(cache, dtype, device):
     return pages, size, st[0] if pages > 1 else size * ROW
 
 
-def _lse_ptr(lse, shape, device):
-    if lse is None:
-        return None
-    _index("lse", lse, shape, device, torch.float32)
-    return lse.data_ptr()
+def _workspace(need, workspace, device):
+    """The caller's workspace or one from torch's allocator, kept by the call until its launch (None for none)."""
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _need("workspace", workspace, torch.uint8, device)
+    if not workspace.is_contiguous() or workspace.numel() < need:
+        raise ValueError(f"kda355: workspace must be contiguous with >= {need} bytes")
+    return workspace
 
 
-def _workspace(a, need, workspace, device, name):
-    """The caller's workspace, or one from torch's allocator, into the arguments; returned so that it lives as long as the call."""
+def _bytes_needed(name, a):
+    need = getattr(_lib.lib(), f"kda355_{name}_workspace_bytes")(ctypes.byref(a))
     if need < 0:
         _lib.check(int(need), name)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    else:
-        _need("workspace", workspace, torch.uint8, device)
-        if not workspace.is_contiguous() or workspace.numel() < need:
-            raise ValueError(f"kda355: workspace must be contiguous with >= {need} bytes")
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    return workspace
+    return int(need)
+
+
+def _sig(t):
+    """What the checks look at of an optional argument."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+_prefill_seen, _decode_seen, _append_seen, _gather_seen = {}, {}, {}, {}
+_PTR2, _PTR7, _PTR8, _PTR10 = (struct.Struct(f"{n}Q") for n in (2, 7, 8, 10))
+
+
+def _plan_prefill(q, k, v, k_pe, cu_q, cu_k, scale, causal, out, lse):
+    """(device, dtype, out shape, bytes of workspace, struct bytes behind the pointers, those behind the workspace)."""
+    dev, dt = _first("q", q)
+    if q.dim() != 3 or q.shape[2] != HEAD + PE:
+        raise ValueError(f"kda355: q must be [Tq, H, {HEAD + PE}], got {list(q.shape)}")
+    Tq, H = q.shape[0], q.shape[1]
+    Tk = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else 0
+    strides = (_rows("q", q, (Tq, H, HEAD + PE), dt, dev) + _rows("k", k, (Tk, H, HEAD), dt, dev) +
+               _rows("v", v, (Tk, H, HEAD), dt, dev) + _rows("k_pe", k_pe, (Tk, PE), dt, dev))
+    N = cu_q.numel() - 1 if isinstance(cu_q, torch.Tensor) else 0
+    if isinstance(cu_q, torch.Tensor) and N < 0:
+        raise ValueError("kda355: cu_seqlens_q must have at least one entry")
+    _index("cu_seqlens_q", cu_q, (N + 1,), dev)
+    _index("cu_seqlens_k", cu_k, (N + 1,), dev)
+    strides += (H * HEAD, HEAD) if out is None else _rows("out", out, (Tq, H, HEAD), dt, dev)
+    if lse is not None:
+        _index("lse", lse, (Tq, H), dev, torch.float32)
+    a = _lib.KdaLatentPrefillArgs(*[None] * 8, *strides, Tq, Tk, None, 0, N, H, _DTYPES[dt], 1 if causal else 0,
+                                  SCALE if scale is None else float(scale), _num_cus(dev))
+    b, at = bytes(a), _lib.KdaLatentPrefillArgs.workspace.offset
+    return dev, dt, (Tq, H, HEAD), _bytes_needed("latent_prefill", a), b[_PTR8.size:at], b[at + 16:]
 
 
 def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal=True, *, out=None, lse=None,
@@ -137,62 +177,40 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
 
     workspace: uint8 tensor of latent_prefill_workspace_bytes(...); by default one is taken from torch's allocator for the
     call.  Calls that may overlap need workspaces of their own."""
-    dev, dt = _first("q", q)
-    if q.dim() != 3 or q.shape[2] != HEAD + PE:
-        raise ValueError(f"kda355: q must be [Tq, H, {HEAD + PE}], got {list(q.shape)}")
-    Tq, H = q.shape[0], q.shape[1]
-    Tk = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() else 0
-    q_st = _rows("q", q, (Tq, H, HEAD + PE), dt, dev)
-    k_st = _rows("k", k, (Tk, H, HEAD), dt, dev)
-    v_st = _rows("v", v, (Tk, H, HEAD), dt, dev)
-    pe_st = _rows("k_pe", k_pe, (Tk, PE), dt, dev)
-    N = cu_seqlens_q.numel() - 1 if isinstance(cu_seqlens_q, torch.Tensor) else 0
-    if isinstance(cu_seqlens_q, torch.Tensor) and N < 0:
-        raise ValueError("kda355: cu_seqlens_q must have at least one entry")
-    _index("cu_seqlens_q", cu_seqlens_q, (N + 1,), dev)
-    _index("cu_seqlens_k", cu_seqlens_k, (N + 1,), dev)
+    try:
+        key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype,
+               v.device, k_pe.shape, k_pe.stride(), k_pe.dtype, k_pe.device, cu_seqlens_q.shape, cu_seqlens_q.stride(),
+               cu_seqlens_q.dtype, cu_seqlens_q.device, cu_seqlens_k.shape, cu_seqlens_k.stride(), cu_seqlens_k.dtype,
+               cu_seqlens_k.device, scale, causal, _sig(out), _sig(lse))
+        plan = _prefill_seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        plan = _keep(_prefill_seen, key, _plan_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse))
+    dev, dt, shape, need, mid, tail = plan
     if out is None:
-        out = torch.empty(Tq, H, HEAD, dtype=dt, device=dev)
-    o_st = _rows("out", out, (Tq, H, HEAD), dt, dev)
-    a = _lib.KdaLatentPrefillArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(), _lse_ptr(lse, (Tq, H), dev),
-        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *q_st, *k_st, *v_st, *pe_st, *o_st, Tq, Tk, None, 0, N, H, _DTYPES[dt],
-        1 if causal else 0, SCALE if scale is None else float(scale), _num_cus(dev))
-    L, p = _lib.lib(), ctypes.byref(a)
-    need = L.kda355_latent_prefill_workspace_bytes(p)
-    if need:
-        workspace = _workspace(a, need, workspace, dev, "latent_prefill")
-    _lib.check(L.kda355_latent_prefill_launch(p, _stream(dev)), "latent_prefill")
+        out = torch.empty(shape, dtype=dt, device=dev)
+    ws = _workspace(need, workspace, dev)
+    a = _lib.KdaLatentPrefillArgs.from_buffer_copy(
+        _PTR8.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                   cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()) + mid +
+        _PTR2.pack(0 if ws is None else ws.data_ptr(), need) + tail)
+    _lib.check(_lib.lib().kda355_latent_prefill_launch(ctypes.byref(a), _stream(dev)), "latent_prefill")
     return out
 
 
 def latent_prefill_workspace_bytes(N, H, Tq, Tk, *, num_cus=256):
     """Bytes of device workspace that latent_prefill() needs for these sizes (host only)."""
-    a = _lib.KdaLatentPrefillArgs(N=N, H=H, Tq=Tq, Tk=Tk, num_cus=num_cus)
-    need = _lib.lib().kda355_latent_prefill_workspace_bytes(ctypes.byref(a))
-    if need < 0:
-        _lib.check(int(need), "latent_prefill_workspace_bytes")
-    return int(need)
+    return _bytes_needed("latent_prefill", _lib.KdaLatentPrefillArgs(N=N, H=H, Tq=Tq, Tk=Tk, num_cus=num_cus))
 
 
-def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, out=None, lse=None, prefix_table=None,
-                  prefix_len=None, workspace=None):
-    """The absorbed form over the paged cache: q_latent [B * S, H, 512] and q_pe [B * S, H, 64], S tokens a sequence (row
-    n * S + s), block_table int32 [B, width], seq_lens int32 [B] the cached tokens of each sequence, its S new ones among
-    them (token s sees j < seq_lens[n] - (S - 1 - s)).  Returns out [B * S, H, 512] in the latent space; `lse` (fp32
-    [B * S, H]) as in latent_prefill.
-
-    prefix_table (int32 [width]) and prefix_len (int32 [1]) name the pages of a prefix that all B sequences share and see in
-    front of their own tokens; it is read once for the whole batch.  block_table and seq_lens then hold what follows it.
-
-    workspace: uint8 tensor of latent_decode_workspace_bytes(...); by default one is taken from torch's allocator for the
-    call.  Calls that may overlap need workspaces of their own."""
+def _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, prefix_table, prefix_len):
+    """(device, dtype, out shape, bytes of workspace, struct bytes behind the pointers)."""
     dev, dt = _first("q_latent", q_latent)
     if q_latent.dim() != 3 or q_latent.shape[2] != LATENT:
         raise ValueError(f"kda355: q_latent must be [B * S, H, {LATENT}], got {list(q_latent.shape)}")
     T, H = q_latent.shape[0], q_latent.shape[1]
-    ql_st = _rows("q_latent", q_latent, (T, H, LATENT), dt, dev)
-    qp_st = _rows("q_pe", q_pe, (T, H, PE), dt, dev)
+    strides = _rows("q_latent", q_latent, (T, H, LATENT), dt, dev) + _rows("q_pe", q_pe, (T, H, PE), dt, dev)
     pages, size, page_stride = _cache(cache, dt, dev)
     table_stride = _table("block_table", block_table, dev)
     B = block_table.shape[0]
@@ -209,43 +227,76 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
         width = prefix_table.numel() if isinstance(prefix_table, torch.Tensor) else 0
         _index("prefix_table", prefix_table, (max(1, width),), dev)
         _index("prefix_len", prefix_len, (1,), dev)
+    strides += (H * LATENT, LATENT) if out is None else _rows("out", out, (T, H, LATENT), dt, dev)
+    if lse is not None:
+        _index("lse", lse, (T, H), dev, torch.float32)
+    a = _lib.KdaLatentDecodeArgs(*[None] * 10, *strides, page_stride, pages, table_stride, 0, B, S, H, size, block_table.shape[1],
+                                 width, _DTYPES[dt], _num_cus(dev), SCALE if scale is None else float(scale), 0)
+    a.workspace_bytes = need = _bytes_needed("latent_decode", a)
+    return dev, dt, (T, H, LATENT), need, bytes(a)[_PTR10.size:]
+
+
+def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, out=None, lse=None, prefix_table=None,
+                  prefix_len=None, workspace=None):
+    """The absorbed form over the paged cache: q_latent [B * S, H, 512] and q_pe [B * S, H, 64], S tokens a sequence (row
+    n * S + s), block_table int32 [B, width], seq_lens int32 [B] the cached tokens of each sequence, its S new ones among
+    them (token s sees j < seq_lens[n] - (S - 1 - s)).  Returns out [B * S, H, 512] in the latent space; `lse` (fp32
+    [B * S, H]) as in latent_prefill.
+
+    prefix_table (int32 [width]) and prefix_len (int32 [1]) name the pages of a prefix that all B sequences share and see in
+    front of their own tokens; it is read once for the whole batch.  block_table and seq_lens then hold what follows it.
+
+    workspace: uint8 tensor of latent_decode_workspace_bytes(...); by default one is taken from torch's allocator for the
+    call.  Calls that may overlap need workspaces of their own."""
+    try:
+        key = (q_latent.shape, q_latent.stride(), q_latent.dtype, q_latent.device, q_pe.shape, q_pe.stride(), q_pe.dtype,
+               q_pe.device, cache.shape, cache.stride(), cache.dtype, cache.device, block_table.shape, block_table.stride(),
+               block_table.dtype, block_table.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, scale,
+               _sig(out), _sig(lse), _sig(prefix_table), _sig(prefix_len))
+        plan = _decode_seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        plan = _keep(_decode_seen, key, _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, prefix_table,
+                                                     prefix_len))
+    dev, dt, shape, need, tail = plan
     if out is None:
-        out = torch.empty(T, H, LATENT, dtype=dt, device=dev)
-    o_st = _rows("out", out, (T, H, LATENT), dt, dev)
-    a = _lib.KdaLatentDecodeArgs(
-        q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        prefix_table.data_ptr() if width else None, prefix_len.data_ptr() if width else None, out.data_ptr(),
-        _lse_ptr(lse, (T, H), dev), None, *ql_st, *qp_st, *o_st, page_stride, pages, table_stride, 0, B, S, H, size,
-        block_table.shape[1], width, _DTYPES[dt], _num_cus(dev), SCALE if scale is None else float(scale), 0)
-    L, p = _lib.lib(), ctypes.byref(a)
-    need = L.kda355_latent_decode_workspace_bytes(p)
-    if need:
-        workspace = _workspace(a, need, workspace, dev, "latent_decode")
-    _lib.check(L.kda355_latent_decode_launch(p, _stream(dev)), "latent_decode")
+        out = torch.empty(shape, dtype=dt, device=dev)
+    ws = _workspace(need, workspace, dev)
+    a = _lib.KdaLatentDecodeArgs.from_buffer_copy(
+        _PTR10.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                    0 if prefix_table is None else prefix_table.data_ptr(), 0 if prefix_len is None else prefix_len.data_ptr(),
+                    out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr()) + tail)
+    _lib.check(_lib.lib().kda355_latent_decode_launch(ctypes.byref(a), _stream(dev)), "latent_decode")
     return out
 
 
 def latent_decode_workspace_bytes(B, S, H, page_size, table_width, prefix_width=0, *, num_cus=256):
     """Bytes of device workspace that latent_decode() needs for these sizes (host only)."""
-    a = _lib.KdaLatentDecodeArgs(B=B, S=S, H=H, page_size=page_size, table_width=table_width, prefix_width=prefix_width,
-                                 num_cus=num_cus)
-    need = _lib.lib().kda355_latent_decode_workspace_bytes(ctypes.byref(a))
-    if need < 0:
-        _lib.check(int(need), "latent_decode_workspace_bytes")
-    return int(need)
+    return _bytes_needed("latent_decode", _lib.KdaLatentDecodeArgs(B=B, S=S, H=H, page_size=page_size, table_width=table_width,
+                                                                   prefix_width=prefix_width, num_cus=num_cus))
 
 
 def latent_append(latent, k_pe, cache, slots):
     """cache row slots[t] (= page * page_size + offset, int64 [T]) <- latent [T, 512] | k_pe [T, 64]; slots outside the cache
     (padding: -1) are skipped.  The cache is written in place and returned."""
-    dev, dt = _first("latent", latent)
-    T = latent.shape[0] if latent.dim() else 0
-    l_st = _rows("latent", latent, (T, LATENT), dt, dev)
-    p_st = _rows("k_pe", k_pe, (T, PE), dt, dev)
-    pages, size, page_stride = _cache(cache, dt, dev)
-    _index("slots", slots, (T,), dev, torch.int64)
-    a = _lib.KdaLatentTokensArgs(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), None, None, None,
-                                 *l_st, *p_st, 0, page_stride, pages, 0, T, size, 0, 0, 0)
+    try:
+        key = (latent.shape, latent.stride(), latent.dtype, latent.device, k_pe.shape, k_pe.stride(), k_pe.dtype, k_pe.device,
+               cache.shape, cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
+        plan = _append_seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        dev, dt = _first("latent", latent)
+        T = latent.shape[0] if latent.dim() else 0
+        strides = _rows("latent", latent, (T, LATENT), dt, dev) + _rows("k_pe", k_pe, (T, PE), dt, dev)
+        pages, size, page_stride = _cache(cache, dt, dev)
+        _index("slots", slots, (T,), dev, torch.int64)
+        a = _lib.KdaLatentTokensArgs(*[None] * 7, *strides, 0, page_stride, pages, 0, T, size, 0, 0, 0)
+        plan = _keep(_append_seen, key, (dev, bytes(a)[_PTR7.size:]))
+    dev, tail = plan
+    a = _lib.KdaLatentTokensArgs.from_buffer_copy(
+        _PTR7.pack(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), 0, 0, 0) + tail)
     _lib.check(_lib.lib().kda355_latent_append_launch(ctypes.byref(a), _stream(dev)), "latent_append")
     return cache
 
@@ -253,15 +304,26 @@ def latent_append(latent, k_pe, cache, slots):
 def latent_gather(cache, block_table, cu_seqlens, out):
     """out [T, 576] row cu_seqlens[n] + j <- token j of sequence n (block_table int32 [N, width], cu_seqlens int32 [N + 1] on
     the device); tokens in holes or past the table give zero rows, rows of `out` past the last sequence stay as they are."""
-    dev, dt = _first("cache", cache)
-    pages, size, page_stride = _cache(cache, dt, dev)
-    table_stride = _table("block_table", block_table, dev)
-    N = block_table.shape[0]
-    _index("cu_seqlens", cu_seqlens, (N + 1,), dev)
-    T = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() else 0
-    o_st = _rows("out", out, (T, ROW), dt, dev)
-    a = _lib.KdaLatentTokensArgs(None, None, cache.data_ptr(), None, block_table.data_ptr(), cu_seqlens.data_ptr(),
-                                 out.data_ptr(), 0, 0, *o_st, page_stride, pages, table_stride, T, size,
-                                 block_table.shape[1], N, 0)
+    try:
+        key = (cache.shape, cache.stride(), cache.dtype, cache.device, block_table.shape, block_table.stride(), block_table.dtype,
+               block_table.device, cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device, out.shape,
+               out.stride(), out.dtype, out.device)
+        plan = _gather_seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        dev, dt = _first("cache", cache)
+        pages, size, page_stride = _cache(cache, dt, dev)
+        table_stride = _table("block_table", block_table, dev)
+        N = block_table.shape[0]
+        _index("cu_seqlens", cu_seqlens, (N + 1,), dev)
+        T = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() else 0
+        o_st = _rows("out", out, (T, ROW), dt, dev)
+        a = _lib.KdaLatentTokensArgs(*[None] * 7, 0, 0, *o_st, page_stride, pages, table_stride, T, size, block_table.shape[1], N,
+                                     0)
+        plan = _keep(_gather_seen, key, (dev, bytes(a)[_PTR7.size:]))
+    dev, tail = plan
+    a = _lib.KdaLatentTokensArgs.from_buffer_copy(
+        _PTR7.pack(0, 0, cache.data_ptr(), 0, block_table.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr()) + tail)
     _lib.check(_lib.lib().kda355_latent_gather_launch(ctypes.byref(a), _stream(dev)), "latent_gather")
     return out

@@ -22,14 +22,15 @@ import struct
 import torch
 
 from . import _lib
-from .latent import _index, _stream, _table
-from .recurrent import _need
+from .latent import _index, _keep, _stream, _table
+
+
+def _sequence(pools):
+    return pools if isinstance(pools, (list, tuple)) else (pools,) if isinstance(pools, torch.Tensor) else tuple(pools)
 
 
 def _pools(pools, slots=None):
-    """(device, [(address, row bytes, slot stride, slots)]) of a list of [slots, ...] tensors with dense rows."""
-    if isinstance(pools, torch.Tensor):
-        pools = (pools,)
+    """(device, [(row bytes, slot stride, slots)]) of a list of [slots, ...] tensors with dense rows; None for an empty one."""
     out, dev = [], None
     for i, t in enumerate(pools):
         if not isinstance(t, torch.Tensor):
@@ -43,7 +44,8 @@ def _pools(pools, slots=None):
             raise ValueError(f"kda355: pool {i} must be [{slots if slots is not None else 'slots'}, ...], "
                              f"got {list(sh)}")
         n = sh[0]
-        if n == 0:
+        if t.numel() == 0:
+            out.append(None)
             continue
         size = t.element_size()
         if t.is_contiguous():
@@ -57,9 +59,7 @@ def _pools(pools, slots=None):
                 exp *= sh[d]
             row = exp * size
             stride = st[0] * size if n > 1 else row
-        if row == 0:
-            continue
-        out.append((t.data_ptr(), row, stride, n))
+        out.append((row, stride, n))
     return dev, out
 
 
@@ -69,20 +69,6 @@ assert _PACK.size == ctypes.sizeof(_lib.KdaPagesArgs)
 _NO_POOLS = (0,) * (4 * _lib.MAX_POOLS)
 
 
-def _launch(name, dev, pools, n, src, dst, ws, table=0, lens=0, refs=0, free=0, num=0, stride=0, rows=0, width=0, pages=0,
-            size=1):
-    flat = _NO_POOLS
-    if pools:
-        flat = [v for p in pools for v in p]
-        flat += _NO_POOLS[len(flat):]
-    try:
-        a = _lib.KdaPagesArgs.from_buffer_copy(
-            _PACK.pack(*flat, len(pools), n, src, dst, table, lens, refs, free, num, ws, stride, rows, width, pages, size))
-    except struct.error as e:
-        raise ValueError(f"kda355: {name}: a size is out of range ({e})") from None
-    _lib.check(_LAUNCH[name](ctypes.byref(a), _stream(dev)), name)
-
-
 class _Entries(dict):
     def __missing__(self, name):
         f = self[name] = getattr(_lib.lib(), f"kda355_{name}_launch")
@@ -90,14 +76,42 @@ class _Entries(dict):
 
 
 _LAUNCH = _Entries()
+# What was found right is kept by what the checks look at (latent.py): (device, pages, table stride, rows, width, page size,
+# [(row bytes, slot stride, slots) of each pool])
+_seen = {}
 
 
-def _copy(dev, pools, n, src, dst):
-    for i in range(0, len(pools), _lib.MAX_POOLS):
-        _launch("copy_rows", dev, pools[i:i + _lib.MAX_POOLS], n, src, dst, 0)
+def _key(name, page_size, pools, tensors):
+    return (name, page_size, tuple([(t.shape, t.stride(), t.dtype, t.device) for t in pools]),
+            tuple([(t.shape, t.stride(), t.dtype, t.device) for t in tensors]))
+
+
+def _launch(name, dev, pools, n, src, dst, ws, book=(0, 0, 0, 0, 0), stride=0, rows=0, width=0, pages=0, size=1):
+    """`pools`: address, row bytes, slot stride and slots of one after the other; `book`: the addresses of the bookkeeping."""
+    try:
+        a = _lib.KdaPagesArgs.from_buffer_copy(
+            _PACK.pack(*pools, *_NO_POOLS[len(pools):], len(pools) // 4, n, src, dst, *book, ws, stride, rows, width, pages, size))
+    except struct.error as e:
+        raise ValueError(f"kda355: {name}: a size is out of range ({e})") from None
+    _lib.check(_LAUNCH[name](ctypes.byref(a), _stream(dev)), name)
+
+
+def _addresses(pools, found):
+    """The flat list of _launch() for pools that were found right (empty ones have no entry)."""
+    out = []
+    for t, p in zip(pools, found):
+        if p is not None:
+            out += (t.data_ptr(), *p)
+    return out
+
+
+def _copy(dev, flat, n, src, dst):
+    for i in range(0, len(flat), 4 * _lib.MAX_POOLS):
+        _launch("copy_rows", dev, flat[i:i + 4 * _lib.MAX_POOLS], n, src, dst, 0)
 
 
 def _book(block_table, ref_counts, free_pages, num_free):
+    """(device, pages, table stride, rows, width)"""
     dev = block_table.device if isinstance(block_table, torch.Tensor) else None
     if dev is None or dev.type != "cuda":
         raise TypeError("kda355: block_table must be a tensor on a GPU")
@@ -106,21 +120,44 @@ def _book(block_table, ref_counts, free_pages, num_free):
     _index("ref_counts", ref_counts, (max(1, pages),), dev)
     _index("free_pages", free_pages, (pages,), dev)
     _index("num_free", num_free, (1,), dev)
-    return dev, pages, dict(table=block_table.data_ptr(), refs=ref_counts.data_ptr(), free=free_pages.data_ptr(),
-                            num=num_free.data_ptr(), stride=stride, rows=block_table.shape[0], width=block_table.shape[1],
-                            pages=pages)
+    return dev, pages, stride, block_table.shape[0], block_table.shape[1]
+
+
+def _check(name, page_size, pools, block_table, ref_counts, free_pages, num_free, seq_lens=None, **rows):
+    """The checks of a bookkeeping call, or what they found for the like of it before."""
+    try:
+        key = _key(name, page_size, pools, (block_table, ref_counts, free_pages, num_free, *rows.values()) +
+                   (() if seq_lens is None else (seq_lens,)))
+        plan = _seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        found = _book(block_table, ref_counts, free_pages, num_free)
+        dev, pages = found[:2]
+        if name != "compact_pages":
+            _index("seq_lens", seq_lens, (found[3],), dev)
+        pool_dev, ps = _pools(pools, pages)
+        if pool_dev is not None and pool_dev != dev:
+            raise TypeError(f"kda355: pools must be on {dev}, got {pool_dev}")
+        n = None
+        for what, t in rows.items():
+            n = t.numel() if n is None and isinstance(t, torch.Tensor) else n or 0
+            _index(what, t, (n,), dev)
+        plan = _keep(_seen, key, found + (int(page_size), ps))
+    return plan
 
 
 def copy_rows(pools, src, dst):
     """pool[dst[i]] <- pool[src[i]] in every pool of the list (int32 [n] rows; pairs with a row outside a pool are skipped
     there).  No dst may be another pair's src or dst."""
+    pools = _sequence(pools)
     dev, ps = _pools(pools)
     if dev is None:
         return
     n = src.numel() if isinstance(src, torch.Tensor) else 0
     _index("src", src, (n,), dev)
     _index("dst", dst, (n,), dev)
-    _copy(dev, ps, n, src.data_ptr(), dst.data_ptr())
+    _copy(dev, _addresses(pools, ps), n, src.data_ptr(), dst.data_ptr())
 
 
 def fork_pages(pools, block_table, seq_lens, ref_counts, free_pages, num_free, parents, children, page_size):
@@ -128,45 +165,44 @@ def fork_pages(pools, block_table, seq_lens, ref_counts, free_pages, num_free, p
     last page is copied in every pool to a page from the stack.  Where the stack is empty the child gets length 0 and no
     pages.  What a child row held before is overwritten, not released (free_pages() first).  Pairs outside the table are
     skipped; children must differ from one another and from every parent."""
-    dev, pages, book = _book(block_table, ref_counts, free_pages, num_free)
-    _index("seq_lens", seq_lens, (block_table.shape[0],), dev)
-    pool_dev, ps = _pools(pools, pages)
-    if pool_dev is not None and pool_dev != dev:
-        raise TypeError(f"kda355: pools must be on {dev}, got {pool_dev}")
-    n = parents.numel() if isinstance(parents, torch.Tensor) else 0
-    _index("parents", parents, (n,), dev)
-    _index("children", children, (n,), dev)
+    pools = _sequence(pools)
+    dev, pages, stride, rows, width, size, ps = _check(
+        "fork_pages", page_size, pools, block_table, ref_counts, free_pages, num_free, seq_lens, parents=parents, children=children)
+    n = parents.numel()
     if n == 0:
         return
     ws = torch.empty(2 * n, dtype=torch.int32, device=dev)
-    at = ws.data_ptr()
-    first, rest = ps[:_lib.MAX_POOLS], ps[_lib.MAX_POOLS:]
-    _launch("fork_pages", dev, first, n, parents.data_ptr(), children.data_ptr(), at, lens=seq_lens.data_ptr(),
-            size=int(page_size), **book)
-    _copy(dev, rest, n, at, at + 4 * n)
+    at, flat = ws.data_ptr(), _addresses(pools, ps)
+    most = 4 * _lib.MAX_POOLS
+    _launch("fork_pages", dev, flat[:most], n, parents.data_ptr(), children.data_ptr(), at,
+            (block_table.data_ptr(), seq_lens.data_ptr(), ref_counts.data_ptr(), free_pages.data_ptr(), num_free.data_ptr()),
+            stride, rows, width, pages, size)
+    if len(flat) > most:
+        _copy(dev, flat[most:], n, at, at + 4 * n)
 
 
 def free_pages(block_table, seq_lens, ref_counts, free_pages, num_free, rows, page_size):
     """The sequences rows[i] (int32 [n], all different) give up the pages of their tokens: their table rows become holes and
     their lengths 0; pages that nobody holds any more go onto the stack, the highest first (the lowest is taken next)."""
-    dev, _, book = _book(block_table, ref_counts, free_pages, num_free)
-    _index("seq_lens", seq_lens, (block_table.shape[0],), dev)
-    n = rows.numel() if isinstance(rows, torch.Tensor) else 0
-    _index("rows", rows, (n,), dev)
-    _launch("free_pages", dev, [], n, rows.data_ptr(), 0, 0, lens=seq_lens.data_ptr(), size=int(page_size), **book)
+    dev, pages, stride, count, width, size, _ = _check("free_pages", page_size, (), block_table, ref_counts, free_pages, num_free,
+                                                       seq_lens, rows=rows)
+    _launch("free_pages", dev, [], rows.numel(), rows.data_ptr(), 0, 0,
+            (block_table.data_ptr(), seq_lens.data_ptr(), ref_counts.data_ptr(), free_pages.data_ptr(), num_free.data_ptr()),
+            stride, count, width, pages, size)
 
 
 def compact_pages(pools, block_table, ref_counts, free_pages, num_free):
     """Moves the held pages to the start of every pool: with L pages held, the i-th held page at or above L goes into the
     i-th free one below L.  block_table, ref_counts and the stack (L is taken next) follow.  Afterwards pages L and up hold
     nothing: the pools can be cut there."""
-    dev, pages, book = _book(block_table, ref_counts, free_pages, num_free)
-    pool_dev, ps = _pools(pools, pages)
-    if pool_dev is not None and pool_dev != dev:
-        raise TypeError(f"kda355: pools must be on {dev}, got {pool_dev}")
+    pools = _sequence(pools)
+    dev, pages, stride, rows, width, _, ps = _check("compact_pages", 1, pools, block_table, ref_counts, free_pages, num_free)
     ws = torch.empty(2 * pages + 2, dtype=torch.int32, device=dev)
-    at = ws.data_ptr()
-    _launch("compact_pages", dev, ps[:_lib.MAX_POOLS], 0, 0, 0, at, **book)
+    at, flat = ws.data_ptr(), _addresses(pools, ps)
+    most = 4 * _lib.MAX_POOLS
+    _launch("compact_pages", dev, flat[:most], 0, 0, 0, at,
+            (block_table.data_ptr(), 0, ref_counts.data_ptr(), free_pages.data_ptr(), num_free.data_ptr()),
+            stride, rows, width, pages)
     half = pages // 2
-    if half:
-        _copy(dev, ps[_lib.MAX_POOLS:], half, at + 4 * pages, at + 4 * (pages + half))
+    if half and len(flat) > most:
+        _copy(dev, flat[most:], half, at + 4 * pages, at + 4 * (pages + half))
