@@ -12,51 +12,91 @@ namespace {
 
 constexpr int ROW = KDA355_LATENT_ROW, LAT = KDA355_LATENT_DIM;
 constexpr int ROW_Q = ROW / 8, LAT_Q = LAT / 8;  // 16-byte pieces of a cache row, of its latent part
-constexpr int TOK_THREADS = 256;
+constexpr int TOK_THREADS = 192, TOKENS = 8, PIECES = TOKENS * ROW_Q / TOK_THREADS;  // 3 pieces a thread
+static_assert(PIECES * TOK_THREADS == TOKENS * ROW_Q, "");
 constexpr int SCAN_THREADS = 1024;
 constexpr int COPY_THREADS = 256, COPY_PER = 4;   // 16 KiB a workgroup
 constexpr int MAX_PAIRS = 1 << 23;                // rows of a launch: 256 threads each, below 2^32 in all
 constexpr int FREED = INT32_MIN;                  // count of a page freed in this call, until the stack has it
 
 // ------------------------------------------------------------------------------------------------ token rows
+// A workgroup moves TOKENS rows: as many lanes find where they stand, then every thread has PIECES reads under way at once.  64 k
+// tokens read back and 6 k written: 33.7 us with 8 rows (4.9 TB/s); data in the caches, 30.2 with 8, 31.7 with 32, and a small
+// call 6.2 us with 8, 9.4 with 32.
 __global__ void __launch_bounds__(TOK_THREADS) append_kernel(KdaLatentTokensArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * TOK_THREADS + threadIdx.x;
-    const int64_t t = i / ROW_Q;
-    const int c = (int)(i - t * ROW_Q);
-    if (t >= a.T) return;
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.pages * a.page_size) return;
-    const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
-    const uint16_t* src = c < LAT_Q ? static_cast<const uint16_t*>(a.latent) + t * a.latent_row + c * 8
-                                    : static_cast<const uint16_t*>(a.k_pe) + t * a.pe_row + (c - LAT_Q) * 8;
-    uint16_t* dst = static_cast<uint16_t*>(a.cache) + page * a.page_stride + off * ROW + c * 8;
-    *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
+    __shared__ char* to[TOKENS];
+    const int64_t first = (int64_t)blockIdx.x * TOKENS;
+    if (threadIdx.x < TOKENS) {
+        const int64_t t = first + threadIdx.x, slot = t < a.T ? a.slots[t] : -1;
+        char* row = nullptr;
+        if (slot >= 0 && slot < a.pages * a.page_size) {
+            const int64_t page = slot / a.page_size;
+            row = static_cast<char*>(a.cache) + 2 * (page * a.page_stride + (slot - page * a.page_size) * ROW);
+        }
+        to[threadIdx.x] = row;
+    }
+    __syncthreads();
+    u32x4 x[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = i * TOK_THREADS + threadIdx.x, t = p / ROW_Q, c = p - t * ROW_Q;
+        if (!to[t]) continue;
+        const uint16_t* src = c < LAT_Q ? static_cast<const uint16_t*>(a.latent) + (first + t) * a.latent_row + c * 8
+                                        : static_cast<const uint16_t*>(a.k_pe) + (first + t) * a.pe_row + (c - LAT_Q) * 8;
+        x[i] = *reinterpret_cast<const u32x4*>(src);
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = i * TOK_THREADS + threadIdx.x, t = p / ROW_Q, c = p - t * ROW_Q;
+        if (to[t]) *reinterpret_cast<u32x4*>(to[t] + c * 16) = x[i];
+    }
 }
 
 __global__ void __launch_bounds__(TOK_THREADS) gather_kernel(KdaLatentTokensArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * TOK_THREADS + threadIdx.x;
-    const int64_t t = i / ROW_Q;
-    const int c = (int)(i - t * ROW_Q);
-    if (t >= a.T) return;
-    int lo = 0, hi = a.N;  // the sequence of row t: the last n with cu[n] <= t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid; else hi = mid;
+    __shared__ const char* from[TOKENS];
+    __shared__ char* to[TOKENS];
+    const int64_t first = (int64_t)blockIdx.x * TOKENS;
+    if (threadIdx.x < TOKENS) {
+        const int64_t t = first + threadIdx.x;
+        const char* row = nullptr;
+        char* out = nullptr;
+        if (t < a.T) {
+            int lo = 0, hi = a.N;  // the sequence of row t: the last n with cu[n] <= t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.cu[mid] <= t) lo = mid; else hi = mid;
+            }
+            const int64_t j = t - a.cu[lo];
+            if (j >= 0 && t < a.cu[lo + 1]) {
+                out = static_cast<char*>(a.out) + 2 * t * a.out_row;
+                const int64_t p = j / a.page_size;
+                if (p < a.table_width) {
+                    const int64_t page = a.block_table[lo * a.table_stride + p];
+                    if (page >= 0 && page < a.pages)
+                        row = static_cast<const char*>(a.cache) + 2 * (page * a.page_stride + (j - p * a.page_size) * ROW);
+                }
+            }
+        }
+        from[threadIdx.x] = row;
+        to[threadIdx.x] = out;
     }
-    if (t < a.cu[lo] || t >= a.cu[lo + 1]) return;
-    const int64_t j = t - a.cu[lo], p = j / a.page_size;
-    u32x4 x = {0, 0, 0, 0};
-    if (p < a.table_width) {
-        const int64_t page = a.block_table[lo * a.table_stride + p];
-        if (page >= 0 && page < a.pages)
-            x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.cache) + page * a.page_stride +
-                                                (j - p * a.page_size) * ROW + c * 8);
+    __syncthreads();
+    u32x4 x[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = i * TOK_THREADS + threadIdx.x, t = p / ROW_Q, c = p - t * ROW_Q;
+        x[i] = from[t] ? *reinterpret_cast<const u32x4*>(from[t] + c * 16) : u32x4{0, 0, 0, 0};
     }
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + t * a.out_row + c * 8) = x;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int p = i * TOK_THREADS + threadIdx.x, t = p / ROW_Q, c = p - t * ROW_Q;
+        if (to[t]) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(to[t] + c * 16));  // (39.5 -> 33.7 us)
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ row copies
-// one 16 KiB segment of row src -> row dst of one pool
+// One 16 KiB segment of row src -> row dst of one pool.  The stores pass the caches: 600 MB moved in 134 us instead of 137, 64
+// part-filled pages copied in 4 pools and their bookkeeping in 16.3 instead of 17.3; 8 pieces a thread instead of 4: 210 us.
 __device__ __forceinline__ void copy_segment(const KdaPool& p, int64_t src, int64_t dst, int seg) {
     if (src < 0 || src >= p.slots || dst < 0 || dst >= p.slots || src == dst) return;
     const char* s = static_cast<const char*>(p.base) + src * p.slot_stride;
@@ -71,7 +111,7 @@ __device__ __forceinline__ void copy_segment(const KdaPool& p, int64_t src, int6
 #pragma unroll
     for (int i = 0; i < COPY_PER; ++i) {
         const int64_t b = b0 + i * COPY_THREADS * 16;
-        if (b < p.row_bytes) *reinterpret_cast<u32x4*>(d + b) = x[i];
+        if (b < p.row_bytes) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(d + b));
     }
 }
 
@@ -184,6 +224,9 @@ __global__ void __launch_bounds__(COPY_THREADS) fork_rows_kernel(KdaPagesArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------ free
+// A reference is taken back by a plain difference, and the last holder marks the page.  Counts may change in any order: one at
+// or below zero (which a caller's mistake leaves) is put back, and a mark, added too, stays whatever comes between.  (Compare and
+// swap on a page that 1000 sequences share: 3.1 ms instead of 93 us.)
 __global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a) {
     const int r = a.src[blockIdx.x];
     if (r < 0 || r >= a.rows) return;
@@ -192,13 +235,8 @@ __global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a)
     for (int j = threadIdx.x; j < a.table_width; j += COPY_THREADS) {
         const int page = row[j];
         if (j < used && page >= 0 && page < a.pages) {
-            int32_t* ref = a.ref_counts + page;
-            int cur = load_fresh(ref);
-            while (cur > 0) {  // the last holder marks the page; a count already at zero stays
-                const int seen = atomicCAS(ref, cur, cur == 1 ? FREED : cur - 1);
-                if (seen == cur) break;
-                cur = seen;
-            }
+            const int before = atomicSub(a.ref_counts + page, 1);
+            if (before <= 1) atomicAdd(a.ref_counts + page, before == 1 ? FREED : 1);
         }
         row[j] = -1;
     }
@@ -228,6 +266,56 @@ __global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a)
                 if (at < a.pages) a.free_pages[at] = p;
                 ++at;
             }
+        top += total;
+    }
+    if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
+}
+
+// The same in one workgroup and one launch, where there is little to give up: the marks are bits in LDS.  Its differences come
+// from one CU: 128 table entries 4.3 us (two launches 4.5), 4160 8.2 (5.5), 8192 15.6 (7.6).  A launch takes 2.7 us of the
+// caller's time, so it is taken up to where it costs the GPU no more than that.
+constexpr int FREE_SMALL = 5 * SCAN_THREADS;        // table entries
+constexpr int FREE_WORDS = 8192;                    // 32 pages each
+__global__ void __launch_bounds__(SCAN_THREADS) free_small_kernel(KdaPagesArgs a) {
+    __shared__ uint32_t marks[FREE_WORDS];
+    __shared__ int sw[SCAN_THREADS / 64];
+    const int words = (a.pages + 31) / 32;
+    for (int i = threadIdx.x; i < words; i += SCAN_THREADS) marks[i] = 0;
+    __syncthreads();
+    const int all = a.n * a.table_width;
+    for (int e = threadIdx.x; e < all; e += SCAN_THREADS) {
+        const int i = e / a.table_width, j = e - i * a.table_width, r = a.src[i];
+        if (r < 0 || r >= a.rows) continue;
+        const int used = (row_len(a, r) + a.page_size - 1) / a.page_size;
+        int32_t* at = a.block_table + r * a.table_stride + j;
+        const int page = *at;
+        if (j < used && page >= 0 && page < a.pages) {
+            const int before = atomicSub(a.ref_counts + page, 1);
+            if (before == 1)
+                atomicOr(&marks[page >> 5], 1u << (page & 31));
+            else if (before <= 0)
+                atomicAdd(a.ref_counts + page, 1);
+        }
+        *at = -1;
+    }
+    __syncthreads();  // every thread has read the lengths
+    for (int i = threadIdx.x; i < a.n; i += SCAN_THREADS) {
+        const int r = a.src[i];
+        if (r >= 0 && r < a.rows) a.seq_lens[r] = 0;
+    }
+    int top = a.num_free[0];
+    top = top < 0 ? 0 : top > a.pages ? a.pages : top;
+    for (int hi = words; hi > 0; hi -= SCAN_THREADS) {  // the highest pages first
+        const int at = hi - 1 - (int)threadIdx.x;
+        uint32_t m = at >= 0 ? marks[at] : 0;
+        int total;
+        int slot = top + block_scan(__popc(m), sw, total);
+        while (m) {
+            const int b = 31 - __clz((int)m);
+            m ^= 1u << b;
+            if (slot < a.pages) a.free_pages[slot] = at * 32 + b;
+            ++slot;
+        }
         top += total;
     }
     if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
@@ -349,7 +437,7 @@ extern "C" int kda355_latent_append_launch(const KdaLatentTokensArgs* a, kda355_
     KDA_CHECK_ARG(a->latent && a->k_pe && a->slots, "latent_append: a required pointer is null");
     KDA_CHECK_ARG(aligned(a->latent, 16) && aligned(a->k_pe, 16) && a->latent_row % 8 == 0 && a->pe_row % 8 == 0,
                   "latent_append: latent and k_pe rows must be 16-byte aligned");
-    const int64_t wgs = (a->T * ROW_Q + TOK_THREADS - 1) / TOK_THREADS;
+    const int64_t wgs = (a->T + TOKENS - 1) / TOKENS;
     hipLaunchKernelGGL(append_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
     return launched("latent_append");
 }
@@ -361,7 +449,7 @@ extern "C" int kda355_latent_gather_launch(const KdaLatentTokensArgs* a, kda355_
                   a->N, a->table_width);
     KDA_CHECK_ARG(a->block_table && a->cu && a->out, "latent_gather: a required pointer is null");
     KDA_CHECK_ARG(aligned(a->out, 16) && a->out_row % 8 == 0, "latent_gather: out rows must be 16-byte aligned");
-    const int64_t wgs = (a->T * ROW_Q + TOK_THREADS - 1) / TOK_THREADS;
+    const int64_t wgs = (a->T + TOKENS - 1) / TOKENS;
     hipLaunchKernelGGL(gather_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
     return launched("latent_gather");
 }
@@ -399,6 +487,10 @@ extern "C" int kda355_free_pages_launch(const KdaPagesArgs* a, kda355_stream_t s
     if (a->n == 0) return 0;
     KDA_CHECK_ARG(a->src, "free_pages: a required pointer is null");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if ((int64_t)a->n * a->table_width <= FREE_SMALL && a->pages <= 32 * FREE_WORDS) {
+        hipLaunchKernelGGL(free_small_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+        return launched("free_pages");
+    }
     hipLaunchKernelGGL(free_rows_kernel, dim3(a->n), dim3(COPY_THREADS), 0, s, *a);
     hipLaunchKernelGGL(free_push_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
     return launched("free_pages");
