@@ -18,6 +18,7 @@ constexpr int SCAN_THREADS = 1024;
 constexpr int COPY_THREADS = 256, COPY_PER = 4;   // 16 KiB a workgroup
 constexpr int MAX_PAIRS = 1 << 23;                // rows of a launch: 256 threads each, below 2^32 in all
 constexpr int FREED = INT32_MIN;                  // count of a page freed in this call, until the stack has it
+constexpr int MOST_HOLDERS = 1 << 30;             // no count reaches it
 
 // ------------------------------------------------------------------------------------------------ token rows
 // A workgroup moves TOKENS rows: as many lanes find where they stand, then every thread has PIECES reads under way at once.  64 k
@@ -224,9 +225,9 @@ __global__ void __launch_bounds__(COPY_THREADS) fork_rows_kernel(KdaPagesArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------ free
-// A reference is taken back by a plain difference, and the last holder marks the page.  Counts may change in any order: one at
-// or below zero (which a caller's mistake leaves) is put back, and a mark, added too, stays whatever comes between.  (Compare and
-// swap on a page that 1000 sequences share: 3.1 ms instead of 93 us.)
+// A reference is taken back by a plain difference, and the last holder marks the page.  Counts may change in any order: a holder
+// too many (a caller's mistake) finds zero or less, or the mark, or what wraps around below it, and puts its difference back.
+// (Compare and swap on a page that 1000 sequences share: 3.1 ms instead of 93 us.)
 __global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a) {
     const int r = a.src[blockIdx.x];
     if (r < 0 || r >= a.rows) return;
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a)
         const int page = row[j];
         if (j < used && page >= 0 && page < a.pages) {
             const int before = atomicSub(a.ref_counts + page, 1);
-            if (before <= 1) atomicAdd(a.ref_counts + page, before == 1 ? FREED : 1);
+            if (before <= 1 || before >= MOST_HOLDERS) atomicAdd(a.ref_counts + page, before == 1 ? FREED : 1);
         }
         row[j] = -1;
     }

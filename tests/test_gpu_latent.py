@@ -185,6 +185,69 @@ def test_prefill_bad_offsets_stay_inside():
     assert (out == 0).all() or torch.equal(out, o)
 
 
+def test_prefill_cut_along_the_keys():
+    """Few queries over many keys: pieces of a sequence that come together again, empty ones and rows that see nothing among
+    them; a workspace full of NaN leaves no trace, on another stream too."""
+    x = Expanded([40, 3, 0, 300, 9], [20, 6000, 100, 900, 0], 3, BF)
+    o, lse = x.check()
+    assert (o[:20] == 0).all() and torch.isinf(lse[:20]).all() and (o[343:] == 0).all()
+    need = kda355.latent_prefill_workspace_bytes(5, 3, 352, 7020, num_cus=torch.cuda.get_device_properties(0).multi_processor_count)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+    q, k, v, pe = (t.to(DEV) for t in (x.q, x.k, x.v, x.pe))
+    cu_q, cu_k = _i32(x.cu_q), _i32(x.cu_k)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        l2 = torch.empty_like(lse, device=DEV)
+        o2 = kda355.latent_prefill(q, k, v, pe, cu_q, cu_k, lse=l2, workspace=ws)
+    side.synchronize()
+    assert torch.equal(o2.cpu(), o) and torch.equal(l2.cpu(), lse)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_prefill_any(seed):
+    g = torch.Generator().manual_seed(100 + seed)
+    pick = lambda top, n: torch.randint(0, top, (n,), generator=g).tolist()  # noqa: E731
+    n = 1 + pick(6, 1)[0]
+    lq = pick(200, n)
+    lk = [a + b if c else b for a, b, c in zip(lq, pick(700, n), pick(4, n))]
+    Expanded(lq, lk, 1 + pick(5, 1)[0], (BF, HF)[seed % 2], ("dense", "joint", "wide")[seed % 3], seed=seed).check(seed != 4)
+
+
+def test_prefill_captured_with_other_lengths():
+    """One graph replayed with other boundaries, every replay against the eager result and the plain form."""
+    xs = [Expanded(lq, lk, 2, BF, "dense", seed=i) for i, (lq, lk) in enumerate(
+        [([100, 7, 43], [300, 50, 150]), ([1, 148, 1], [400, 90, 10]), ([0, 150, 0], [0, 200, 300]), ([5, 5, 140], [1, 498, 1])])]
+    q, k, v, pe = (torch.empty_like(t, device=DEV) for t in (xs[0].q, xs[0].k, xs[0].v, xs[0].pe))
+    cu_q, cu_k = _i32([0] * 4), _i32([0] * 4)
+    out, lse = torch.empty(150, 2, HEAD, dtype=BF, device=DEV), torch.empty(150, 2, device=DEV)
+
+    def step():
+        kda355.latent_prefill(q, k, v, pe, cu_q, cu_k, out=out, lse=lse)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for x in xs + xs[:1]:
+        for t, y in ((q, x.q), (k, x.k), (v, x.v), (pe, x.pe)):
+            t.copy_(y)
+        cu_q.copy_(_i32(x.cu_q))
+        cu_k.copy_(_i32(x.cu_k))
+        graph.replay()
+        torch.cuda.synchronize()
+        got, got_lse = out.clone(), lse.clone()
+        step()
+        assert torch.equal(got, out) and torch.equal(got_lse, lse)
+        for n, h, ref in R.prefill(x.q, x.k, x.v, x.pe, x.cu_q, x.cu_k, True, SCALE):
+            a, b = x.cu_q[n], x.cu_q[n + 1]
+            R.check(got[a:b, h].cpu(), got_lse[a:b, h].cpu(), ref, BF, HEAD + PE, f"replay seq {n} head {h}")
+
+
 # ================================================================================================ absorbed form
 class Absorbed:
     def __init__(self, lens, S, H, size, dtype, prefix=None, seed=0, std=1.0, spare=2):
@@ -377,6 +440,16 @@ def test_decode_prefix_equals_copies():
     assert (lse - lse2).abs().max() < 1e-4
 
 
+@pytest.mark.parametrize("seed", range(10))
+def test_decode_any(seed):
+    g = torch.Generator().manual_seed(200 + seed)
+    pick = lambda top, n: torch.randint(0, top, (n,), generator=g).tolist()  # noqa: E731
+    B, S, H = 1 + pick(9, 1)[0], 1 + pick(8, 1)[0], 1 + pick(130, 1)[0]
+    top = (40, 600, 2500)[seed % 3]
+    Absorbed(pick(top, B), S, H, 1 + pick(150, 1)[0], (BF, HF)[seed % 2], prefix=pick(900, 1)[0] if seed % 4 == 1 else None,
+             seed=seed).check()
+
+
 def test_decode_far_offsets():
     """Pages further apart than 32 bits can address."""
     x = Absorbed([900], 1, 12, 64, BF)
@@ -503,3 +576,34 @@ def test_ops_run_the_same_kernels():
     out = torch.empty_like(o)
     torch.ops.kda355.latent_decode(a.ql.to(DEV), a.qp.to(DEV), a.cache.to(DEV), a.table.to(DEV), _i32(a.lens), out)
     assert torch.equal(out, o)
+
+
+def test_refused_after_a_like_call_was_taken():
+    """What a call of the same shapes had found right does not let another one through."""
+    x = Expanded([8], [8], 2, BF, "dense")
+    q, k, v, pe = (t.to(DEV) for t in (x.q, x.k, x.v, x.pe))
+    cu = _i32([0, 8])
+    for _ in range(2):
+        kda355.latent_prefill(q, k, v, pe, cu, cu)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    few = torch.empty(kda355.latent_prefill_workspace_bytes(1, 2, 8, 8, num_cus=cus) - 1, dtype=torch.uint8, device=DEV)
+    odd = torch.empty(8 * 2 * 192 + 1, device=DEV, dtype=BF)[1:].view(8, 2, 192)  # the same shape and strides, 2 bytes off
+    for bad in (dict(q=odd), dict(k=k[:7]), dict(cu_seqlens_k=_i32([0, 4, 8])), dict(workspace=few)):
+        with pytest.raises(ValueError):
+            kda355.latent_prefill(**{**dict(q=q, k=k, v=v, k_pe=pe, cu_seqlens_q=cu, cu_seqlens_k=cu), **bad})
+    for bad in (dict(q=q.half()), dict(cu_seqlens_q=cu.cpu()), dict(v=v.cpu())):
+        with pytest.raises(TypeError):
+            kda355.latent_prefill(**{**dict(q=q, k=k, v=v, k_pe=pe, cu_seqlens_q=cu, cu_seqlens_k=cu), **bad})
+    a = Absorbed([20, 5], 1, 4, 16, BF)
+    args = dict(q_latent=a.ql.to(DEV), q_pe=a.qp.to(DEV), cache=a.cache.to(DEV), block_table=a.table.to(DEV), seq_lens=_i32([20, 5]))
+    few = torch.empty(kda355.latent_decode_workspace_bytes(2, 1, 4, 16, a.table.shape[1], num_cus=cus) - 1, dtype=torch.uint8,
+                      device=DEV)
+    for _ in range(2):
+        kda355.latent_decode(**args)
+    for bad in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(seq_lens=_i32([1])),
+                dict(workspace=few)):
+        with pytest.raises(ValueError):
+            kda355.latent_decode(**{**args, **bad})
+    for bad in (dict(cache=args["cache"].half()), dict(seq_lens=_i32([20, 5]).float()), dict(q_pe=a.qp)):
+        with pytest.raises(TypeError):
+            kda355.latent_decode(**{**args, **bad})

@@ -206,6 +206,28 @@ def test_free(rows, width, pages, live, seed):
     assert d.lens.tolist() == book.lens
 
 
+@pytest.mark.parametrize("rows,size", [(20, 4), (300, 4)])
+@pytest.mark.parametrize("extra", [0, 1, 200])
+def test_free_shared_by_many(rows, size, extra):
+    """Pages that all sequences share, given up by all of them or by all but `extra`; a page whose count is too low by two and
+    by all but one is freed once."""
+    width, pages = 20, 64
+    extra = min(extra, rows - 1)
+    table = [[5, 9, 40, 41] + [-1] * 16 for _ in range(rows)]
+    refs = [0] * pages
+    for p in (5, 9):
+        refs[p] = rows
+    refs[40], refs[41] = rows - 2, 1
+    free = [p for p in range(pages) if refs[p] == 0]
+    book = Book(table, [4 * size - 1] * rows, refs, free + [-1] * (pages - len(free)), len(free), size)
+    d = _Device(book)
+    which = list(range(extra, rows))
+    kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, _i32(which), size)
+    book.release(which)
+    d.same(book)
+    assert d.lens.tolist() == book.lens
+
+
 @pytest.mark.parametrize("rows,width,pages,live,layers,seed", [(1, 1, 1, 1, 1, 0), (1, 1, 1, 0, 1, 0), (8, 5, 61, 30, 2, 1),
                                                                (20, 9, 300, 170, 27, 2), (300, 40, 9000, 6000, 0, 3),
                                                                (4, 3, 2, 1, 1, 4)])
@@ -300,3 +322,28 @@ def test_page_refusals():
         kda355.latent_gather(pools[0], d.table.long(), _i32([0] * 5), torch.zeros(1, ROW, device=DEV).bfloat16())
     with pytest.raises(ValueError):
         kda355.latent_gather(pools[0], d.table, _i32([0] * 4), torch.zeros(1, ROW, device=DEV).bfloat16())
+
+
+def test_refused_after_a_like_call_was_taken():
+    """What a call of the same shapes had found right does not let another one through."""
+    book, pools = _make(random.Random(1), 4, 3, 4, 20, 5)
+    d = _Device(book, pad=0)
+    one, cache = _i32([0]), pools[0]
+    lat, pe, slots = _random((2, 512), torch.bfloat16, 1), _random((2, 64), torch.bfloat16, 2), torch.tensor([0, 1], device=DEV)
+    out = torch.empty(4, ROW, dtype=torch.bfloat16, device=DEV)
+    for _ in range(2):
+        kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, one, 4)
+        kda355.latent_append(lat, pe, cache, slots)
+        kda355.latent_gather(cache, d.table, _i32([0, 1, 2, 3, 4]), out)
+    for size in (0, -1, 1 << 31):
+        with pytest.raises(ValueError):
+            kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, one, size)
+    for bad in (dict(latent=lat.half()), dict(k_pe=pe.float()), dict(slots=slots.int()), dict(cache=cache.cpu())):
+        with pytest.raises(TypeError):
+            kda355.latent_append(**{**dict(latent=lat, k_pe=pe, cache=cache, slots=slots), **bad})
+    with pytest.raises(ValueError):
+        kda355.latent_append(lat, pe, cache, slots[:1])
+    with pytest.raises(ValueError):  # the same shape, 2 bytes off
+        kda355.latent_append(_random((1026,), torch.bfloat16, 1)[1:1025].view(2, 512), pe, cache, slots)
+    with pytest.raises(TypeError):
+        kda355.latent_gather(cache, d.table, torch.zeros(5, dtype=torch.int64, device=DEV), out)
