@@ -104,6 +104,17 @@ __device__ __forceinline__ float sum_halves(float x) {
     return __uint_as_float(r.x) + __uint_as_float(r.y);
 }
 
+// inclusive prefix sum over the lanes (all of them active)
+__device__ __forceinline__ int scan_wave(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // within 16 lanes: 1, 2, 4, 8 below
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lanes 15 and 47 to the 16 after them
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+    return x;
+}
+
 // ------------------------------------------------------------------------------------------------ running softmax
 // State of a lane's row: mo = m - B in log2 units, l = this half's sum of the weights.  Starts far below any score but
 // finite, so that hidden scores (-inf) give weights of 0 and never a NaN.

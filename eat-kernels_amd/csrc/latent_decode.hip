@@ -45,6 +45,7 @@ struct Groups {
 struct Plan {
     Groups own, pre;       // of a sequence's rows; of all rows of the batch, for the prefix (no groups: no prefix)
     int grid;
+    float per_wg;          // 1 / grid
     int64_t pre_slots;     // workspace: prefix parts, then the sequences'
     uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift, x < 2^31
 };
@@ -54,55 +55,53 @@ __device__ const uint4 zero_row[ROW_BYTES / 16] = {};  // what a token that is n
 // ------------------------------------------------------------------------------------------------ who does what
 struct Cut {
     uint32_t own, pre, run;  // units of all sequences, tiles of the prefix; units of a workgroup
-    uint32_t pre_wgs, own_wgs;
+    uint32_t pre_runs, pre_wgs, own_wgs;
 };
 __device__ __forceinline__ int tokens_of(int len, int width, int page_size) { return min(max(len, 0), width * page_size); }
-__device__ __forceinline__ uint32_t tiles_of(const KdaLatentDecodeArgs& a, int n) {
-    return ((uint32_t)tokens_of(a.seq_lens[n], a.table_width, a.page_size) + BN - 1) / BN;
-}
-__device__ __forceinline__ uint32_t units_of(const KdaLatentDecodeArgs& a, int n) {
-    const uint32_t t = tiles_of(a, n);
-    return t ? t + LEAD : 0;
-}
+__device__ __forceinline__ uint32_t tiles_of(int tokens) { return ((uint32_t)tokens + BN - 1) / BN; }
+__device__ __forceinline__ uint32_t units_of(int tokens) { return tokens ? tiles_of(tokens) + LEAD : 0; }
 __device__ __forceinline__ uint32_t cdiv(uint32_t x, uint32_t y) { return x / y + (x % y != 0); }
+// The sequences' tokens: every lane has one of the first 64, loaded once.
+struct Lengths {
+    const KdaLatentDecodeArgs& a;
+    int mine;
+    __device__ __forceinline__ int load(int n) const { return tokens_of(a.seq_lens[n], a.table_width, a.page_size); }
+    __device__ __forceinline__ explicit Lengths(const KdaLatentDecodeArgs& args) : a(args), mine(load(min((int)(threadIdx.x & 63), args.B - 1))) {}
+    __device__ __forceinline__ int of_lane(int n) const { return n >= a.B ? 0 : n < 64 ? mine : load(n); }  // n % 64: the lane
+    __device__ __forceinline__ int of(int n) const {  // n: the same in all lanes
+        return n < 64 ? __builtin_amdgcn_readlane(mine, n) : __builtin_amdgcn_readfirstlane(load(n));
+    }
+};
 
 // The shortest run (to 1.6 %) with which the grid covers everything, the same in every wave: the lanes try 64 candidates.
 __device__ __forceinline__ Cut cut(const KdaLatentDecodeArgs& a, const Plan& p, uint32_t own) {
     Cut c;
     c.own = own;
-    c.pre = p.pre.groups ? ((uint32_t)tokens_of(a.prefix_len[0], a.prefix_width, a.page_size) + BN - 1) / BN : 0;
+    c.pre = p.pre.groups ? tiles_of(tokens_of(a.prefix_len[0], a.prefix_width, a.page_size)) : 0;
     c.pre = __builtin_amdgcn_readfirstlane(c.pre);
     const uint32_t most = max(max(c.own, c.pre), MIN_RUN);  // one run a group: always fits
-    const double all = (double)p.pre.groups * c.pre + (double)p.own.groups * c.own;
-    const uint32_t lo = min(max((uint32_t)__builtin_ceil(all / p.grid), MIN_RUN), most);
+    const float all = (float)p.pre.groups * (float)c.pre + (float)p.own.groups * (float)c.own, top = (float)most;
+    const float lo = fmaxf(fminf(__builtin_ceilf(all * p.per_wg), top), (float)MIN_RUN);
     const int lane = threadIdx.x & 63;
-    const double f = lane < 32 ? 1.0 + lane / 64.0 : 1.5 * (double)exp2f((lane - 31) * 0.25f);
-    const uint32_t r = lane == 63 ? most : (uint32_t)fmin(__builtin_ceil(lo * f), (double)most);
-    const uint64_t wgs = (uint64_t)p.pre.groups * cdiv(c.pre, r) + (uint64_t)p.own.groups * cdiv(c.own, r);
+    const float f = lane < 32 ? 1.f + lane * (1.f / 64) : 1.5f * __builtin_amdgcn_exp2f((lane - 31) * 0.25f);
+    const uint32_t r = lane == 63 ? most : min((uint32_t)fminf(__builtin_ceilf(lo * f), top), most);
+    const uint32_t pre = p.pre.groups ? cdiv(c.pre, r) : 0, mine = cdiv(c.own, r);
+    const uint64_t wgs = (uint64_t)p.pre.groups * pre + (uint64_t)p.own.groups * mine;
     const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(wgs <= (uint32_t)p.grid) | 1ull << 63);
     c.run = __builtin_amdgcn_readlane(r, l);
-    c.pre_wgs = __builtin_amdgcn_readfirstlane(p.pre.groups * cdiv(c.pre, c.run));
-    c.own_wgs = __builtin_amdgcn_readfirstlane(p.own.groups * cdiv(c.own, c.run));
+    c.pre_runs = __builtin_amdgcn_readlane(pre, l);
+    c.pre_wgs = p.pre.groups * c.pre_runs;
+    c.own_wgs = p.own.groups * __builtin_amdgcn_readlane(mine, l);
     return c;
 }
-__device__ __forceinline__ uint32_t sum_wave(uint32_t x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ uint32_t sum_wave(uint32_t x) { return __builtin_amdgcn_readlane(scan_wave(x), 63); }
 struct At { int n; uint32_t before; };
 // the sequence that holds unit u of all (u < their sum), and the units before it
-__device__ __forceinline__ At sequence_of(const KdaLatentDecodeArgs& a, uint32_t u) {
+__device__ __forceinline__ At sequence_of(const Lengths& lens, uint32_t u) {
     const int lane = threadIdx.x & 63;
     uint32_t before = 0;
-    for (int n0 = 0; n0 < a.B; n0 += 64) {
-        const uint32_t t = n0 + lane < a.B ? units_of(a, n0 + lane) : 0;
-        uint32_t s = t;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t y = __shfl_up(s, d);
-            if (lane >= d) s += y;
-        }
+    for (int n0 = 0; n0 < lens.a.B; n0 += 64) {
+        const uint32_t t = units_of(lens.of_lane(n0 + lane)), s = scan_wave(t);
         const uint64_t hit = __builtin_amdgcn_ballot_w64(before + s > u);
         if (hit) {
             const int l = __builtin_ctzll(hit);
@@ -110,7 +109,7 @@ __device__ __forceinline__ At sequence_of(const KdaLatentDecodeArgs& a, uint32_t
         }
         before += __builtin_amdgcn_readlane(s, 63);
     }
-    return {a.B, before};
+    return {lens.a.B, before};
 }
 
 // ------------------------------------------------------------------------------------------------ LDS
@@ -136,6 +135,9 @@ __device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
                  "v"(src), "n"(OFFSET)
                  : "memory");
 }
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int l) {
+    return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), l) << 32 | (uint32_t)__shfl((int)(uint32_t)x, l);
+}
 template <int I>
 using Int = std::integral_constant<int, I>;
 // the four lane groups of 16 joined
@@ -154,8 +156,34 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
 
+    asm volatile("" ::"s"(a.q_latent), "s"(a.ql_row), "s"(a.page_stride), "s"(a.B), "s"(p.grid));  // all arguments at once
+    const Lengths lens(a);
+    // ---- what does not depend on the lengths, while they come
+    const float sc = a.scale * 1.44269504088896f;
+    const int64_t page_bytes = a.page_stride * 2;
+    const char* const cache = static_cast<const char*>(a.cache);
+    const bool scores = w < SCORE_WAVES;
+    const int rt = w & 1, kh = w >> 1 & 1;  // a score wave's row tile and keys 16 kh ..
+    const int vw = w & 3;                   // a value wave's 128 values
+    const int c16 = lane & 15, quad = lane >> 4;
+    // LDS read addresses within a tile.  Of a score wave: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step, latent and
+    // positional; of a value wave: values as operand rows (key 8 half + e of a 16-key step is element e), e < 4 and from 4 on.
+    uint32_t ra[2];
+    if (scores) {
+        const int t = 16 * kh + c16;
+        ra[0] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
+        ra[1] = TILE_PE + t * PE_BYTES + ((quad ^ swz8(t)) << 4);
+    } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int t = 8 * half + 4 * x + (c16 >> 2);
+            const int e = 2 * (quad & 1) + ((c16 & 3) >> 1);
+            ra[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
+        }
+    }
+
     uint32_t own = 0;
-    for (int n = lane; n < a.B; n += 64) own += units_of(a, n);
+    for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
     const Cut cu = cut(a, p, sum_wave(own));
     const uint32_t wgs = cu.pre_wgs + cu.own_wgs;
     if (blockIdx.x >= wgs) return;
@@ -168,27 +196,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const uint32_t end = min((piece + 1) * cu.run, prefix ? cu.pre : cu.own);
     uint32_t u = piece * cu.run;
     At at = {0, 0};
-    if (!prefix) at = sequence_of(a, u);
-
-    const float sc = a.scale * 1.44269504088896f;
-    const int64_t page_bytes = a.page_stride * 2;
-    const char* const cache = static_cast<const char*>(a.cache);
-    const bool scores = w < SCORE_WAVES;
-    const int rt = w & 1, kh = w >> 1 & 1;  // a score wave's row tile and keys 16 kh ..
-    const int vw = w & 3;                   // a value wave's 128 values
-    const int c16 = lane & 15, quad = lane >> 4;
-    // LDS read addresses within a tile: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step; values as operand rows
-    // (key 8 half + e of a 16-key step is element e)
-    const int kt = 16 * kh + c16;
-    const uint32_t ka = (kt >> 2) * (4 * BLOCK) + (kt & 3) * 256 + ((quad ^ turn(kt)) << 4);
-    const uint32_t pa = TILE_PE + kt * PE_BYTES + ((quad ^ swz8(kt)) << 4);
-    uint32_t va[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int t = 8 * half + 4 * x + (c16 >> 2);
-        const int e = 2 * (quad & 1) + ((c16 & 3) >> 1);
-        va[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
-    }
+    if (!prefix) at = sequence_of(lens, u);
 
     while (u < end) {
         // ---- the segment: key tiles [t0, t1) of one key sequence, for rows [r0, r1) of the batch
@@ -204,11 +212,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             u = end;
         } else {
             n = at.n;
-            tokens = tokens_of(a.seq_lens[n], a.table_width, a.page_size);
+            tokens = lens.of(n);
             table = a.block_table + n * a.table_stride, width = a.table_width;
             const int rows = a.S * a.H;
             r0 = n * rows + g * gr.rows, r1 = min(r0 + gr.rows, (n + 1) * rows);
-            const uint32_t tiles = ((uint32_t)tokens + BN - 1) / BN, units = tiles ? tiles + LEAD : 0;
+            const uint32_t tiles = tiles_of(tokens), units = units_of(tokens);
             const uint32_t from = u - at.before, to = min(units, end - at.before);
             t0 = from > LEAD ? from - LEAD : 0, t1 = to > LEAD ? to - LEAD : 0;
             whole = t0 == 0 && t1 == tiles && cu.pre == 0;
@@ -239,19 +247,53 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         if (scores) {
             // ================================================================ score waves
             const int row0 = r0 + 32 * rt + c16;  // this lane's rows: row0, row0 + 16
-            u32x4 q[2][18];  // operand registers, straight from memory (rows past the end repeat the last one)
+            // The queries come through the LDS of tiles t0 + 2 and t0 + 3, a row tile in each, laid out like keys, half of it by
+            // either of its two waves (rows past the end repeat the last one).  (Straight into registers, 64 bytes of 16 rows at a
+            // time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of 64 heads; 1900 and
+            // 4800 so.)
             int mine[2];
+            const uint32_t qb = lds + (t0 + 2 + rt) % BUFS * TILE_BYTES;
+            const bool some = n_tiles && row0 - c16 < r1;
+            {
+                uint64_t latent = 0, pe = 0;  // of row 16 kh + c16 of the tile
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int r = min(row0 + 16 * x, r1 - 1), t = r / a.H, h = r - t * a.H;
-                mine[x] = sees(r);
-                const uint16_t* ql = static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head + 8 * quad;
-                const uint16_t* qp = static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head + 8 * quad;
+                for (int x = 0; x < 2; ++x) {
+                    const int r = min(row0 + 16 * x, r1 - 1), t = r / a.H, h = r - t * a.H;
+                    mine[x] = sees(r);
+                    if (x == kh) {
+                        latent = (uint64_t)(static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head);
+                        pe = (uint64_t)(static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head);
+                    }
+                }
+                if (some) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) q[x][i] = *reinterpret_cast<const u32x4*>(ql + 32 * i);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint64_t from = of_lane(latent, 4 * i + quad) + ((c16 ^ turn(4 * i + quad)) << 4);
+                        const uint32_t to = qb + (4 * kh + i) * (4 * BLOCK);
+                        load_block<0>(to, from);
+                        load_block<256>(to + BLOCK, from);
+                        load_block<512>(to + 2 * BLOCK, from);
+                        load_block<768>(to + 3 * BLOCK, from);
+                    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) q[x][16 + i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+                    for (int i = 0; i < 2; ++i)
+                        load_block<0>(qb + TILE_PE + (16 * kh + 8 * i) * PE_BYTES,
+                                      of_lane(pe, 8 * i + (lane >> 3)) + (((lane & 7) ^ swz8(8 * i + (lane >> 3))) << 4));
+                }
             }
+            wait_loads<0>();
+            lds_barrier();  // the first tile, the queries
+            u32x4 q[2][18] = {};
+            if (some)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t at = qb + ra[0] + (x - kh) * (16 * LAT_BYTES), pat = qb + ra[1] + (x - kh) * (16 * PE_BYTES);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) q[x][16 + i] = lds_read16(pat ^ (i << 6));
+                }
+            lds_barrier();  // the queries are in registers
             float mo[2] = {M_START, M_START}, l[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
             f32x4 s[2] = {};
             auto weights = [&](uint32_t tile, int x) {  // of rows row0 + 16 x, relative to mo[x]; leaves their sum
@@ -279,7 +321,6 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 l[1] += sum[1];
             };
             u32x4 fl = {};
-            lds_barrier();  // the first tile
             for (uint32_t tile = t0; tile < stop; ++tile) {
                 const uint32_t tb = lds + (tile % BUFS) * TILE_BYTES;
                 const int k0 = (int)(tile * BN);
@@ -287,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 const int there8 = *(sm + LDS_THERE + (tile % BUFS) * BN + c);
                 // ---- 18 steps for both halves of the rows, in two chains each, the operands read five steps ahead
                 auto key = [&](int i) {
-                    return i < 16 ? lds_read16(((tb + ka) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tb + pa) ^ ((i - 16) << 6));
+                    return i < 16 ? lds_read16(((tb + ra[0]) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tb + ra[1]) ^ ((i - 16) << 6));
                 };
                 f32x4 z[2][2] = {};
                 u32x4 kf[6];
@@ -342,9 +383,12 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 
         // ==================================================================== value waves
         // ---- loads
+        const uint32_t pages = (uint32_t)min(a.pages, (int64_t)1 << 31);
         const u32x4 table_rsrc = tile_rsrc(table, (uint32_t)width * 4);  // entries past the table read as zeros (and are past `last`)
         const uint32_t pages_at = lds + LDS_PAGES + vw * 1024;
-        const int own8 = 8 * vw + (lane & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
+        int me = lane;  // (computed anew for every segment: the score waves have no registers for what follows from it)
+        asm volatile("" : "+v"(me));
+        const int own8 = 8 * vw + (me & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
         auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane(pages_at + (tile & 3) * 256)),
@@ -359,21 +403,18 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         };
         auto find_token = [&](uint32_t tile, int page) {
             const uint32_t tok = tile * BN + own8;
-            const bool in = tok < (uint32_t)last && page >= 0 && page < a.pages;  // in the tokens that the group sees, no hole
+            const bool in = tok < (uint32_t)last && (uint32_t)page < pages;  // in the tokens that the group sees, no hole
             *(sm + LDS_THERE + (tile % BUFS) * BN + own8) = in;
-            return (uint64_t)(in ? cache + (page * page_bytes + (int64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES)
-                                 : reinterpret_cast<const char*>(zero_row));
+            uint64_t at = (uint64_t)cache + (uint32_t)page * (uint64_t)page_bytes +
+                          (uint64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES;
+            asm volatile("" : "+v"(at));  // (a choice of two, not a branch)
+            return in ? at : (uint64_t)zero_row;
         };
-        auto find_pieces = [&](uint64_t at) {
-            const int lo = (int)(uint32_t)at, hi = (int)(uint32_t)(at >> 32);
-            auto of = [&](int t) { return (uint64_t)(uint32_t)__shfl(hi, t) << 32 | (uint32_t)__shfl(lo, t); };
-            at_latent[0] = of(quad), at_latent[1] = of(4 + quad), at_pe = of(lane >> 3);
-        };
-        auto find_places = [&] {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) at_latent[x] += (c16 ^ turn(8 * vw + 4 * x + quad)) << 4;
-            at_pe += LAT_BYTES + (((lane & 7) ^ swz8(8 * vw + (lane >> 3))) << 4);
-        };
+        const uint32_t piece4[2] = {(uint32_t)((me & 15) ^ turn(8 * vw + (me >> 4))) << 4,
+                                    (uint32_t)((me & 15) ^ turn(8 * vw + 4 + (me >> 4))) << 4};
+        const uint32_t piece8 = LAT_BYTES + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
+        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + piece4[x]; };
+        auto find_pe = [&](uint64_t at) { at_pe = of_lane(at, me >> 3) + piece8; };
         auto bring = [&](uint32_t tile, auto i) {  // load i of 9: four of 4 tokens, four of 4 more, the positional parts
             constexpr int I = decltype(i)::value;
             const uint32_t base = lds + (tile % BUFS) * TILE_BYTES;
@@ -393,14 +434,16 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
             const uint32_t vb = lds + (tile % BUFS) * TILE_BYTES, pb = lds + LDS_P + (tile & 1) * 4096 + c * 32 + half * 16;
             auto value = [&](int k, int d) {
-                const u32x2 v0 = lds_read_tr(((vb + va[0]) ^ (d << 6)) + k * 16 * BLOCK);
-                const u32x2 v1 = lds_read_tr(((vb + va[1]) ^ (d << 6)) + k * 16 * BLOCK);
+                const u32x2 v0 = lds_read_tr(((vb + ra[0]) ^ (d << 6)) + k * 16 * BLOCK);
+                const u32x2 v1 = lds_read_tr(((vb + ra[1]) ^ (d << 6)) + k * 16 * BLOCK);
                 return u32x4{v0.x, v0.y, v1.x, v1.y};
             };
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
             u32x4 vf[4], pf[RT];
             int page = 0;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
 #pragma unroll
             for (int d = 0; d < 4; ++d) vf[d] = value(0, d);
             if constexpr (!LAST) page = find_page(tile + 4);
@@ -410,13 +453,14 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 for (int r = 0; r < RT; ++r) {
                     if (!__builtin_amdgcn_readfirstlane(fl[r] | fl[r + RT])) continue;
                     const float f = raise(tile, 32 * r + c, mo[r]);
+                    if (tile != t0)  // (nothing is there yet)
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                        for (int d = 0; d < 4; ++d) acc[r][d] *= f;
                 }
                 lds_barrier();  // the weights anew
-            }
 #pragma unroll
-            for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
+                for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
+            }
             uint64_t at = 0;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -438,17 +482,17 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                             for (int r = 0; r < RT; ++r) pn[r] = weight(1, r);
                     }
-                    if constexpr (!LAST) {
+                    if constexpr (!LAST) {  // (what an address is taken from is needed no more)
                         if (k == 0) {
                             if (d == 0) bring(tile + 3, Int<0>{});
-                            if (d == 1) bring(tile + 3, Int<1>{});
+                            if (d == 1) bring(tile + 3, Int<1>{}), at = find_token(tile + 4, page);
                             if (d == 2) bring(tile + 3, Int<2>{});
-                            if (d == 3) bring(tile + 3, Int<3>{});
+                            if (d == 3) bring(tile + 3, Int<3>{}), bring(tile + 3, Int<8>{});
                         } else {
-                            if (d == 0) bring(tile + 3, Int<4>{}), at = find_token(tile + 4, page);
-                            if (d == 1) bring(tile + 3, Int<5>{});
-                            if (d == 2) bring(tile + 3, Int<6>{});
-                            if (d == 3) bring(tile + 3, Int<7>{});
+                            if (d == 0) bring(tile + 3, Int<4>{}), find_latent(at, 0);
+                            if (d == 1) bring(tile + 3, Int<5>{}), find_pe(at);
+                            if (d == 2) bring(tile + 3, Int<6>{}), load_pages(tile + 6);
+                            if (d == 3) bring(tile + 3, Int<7>{}), find_latent(at, 1);
                         }
                     }
                 }
@@ -458,10 +502,6 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
-                bring(tile + 3, Int<8>{});
-                find_pieces(at);
-                load_pages(tile + 6);
-                find_places();
                 wait_loads<LOADS>();
                 lds_barrier();  // the next tile's weights; the tile after it is whole
             }
@@ -471,8 +511,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             for (int i = 0; i < 4; ++i) load_pages(t0 + i);
             wait_loads<0>();
             auto find_tile = [&](uint32_t tile) {
-                find_pieces(find_token(tile, find_page(tile)));
-                find_places();
+                const uint64_t at = find_token(tile, find_page(tile));
+                find_latent(at, 0), find_latent(at, 1), find_pe(at);
             };
             auto whole_tile = [&](uint32_t tile) {
                 find_tile(tile);
@@ -483,7 +523,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             whole_tile(t0 + 1);
             load_pages(t0 + 4);
             wait_loads<LOADS>();
-            lds_barrier();  // the first tile
+            lds_barrier();  // the first tile, the queries
+            lds_barrier();  // the queries are in registers
             // while the first tile's scores are computed: tile t0 + 2, and where t0 + 3 stands
             whole_tile(t0 + 2);
             find_tile(t0 + 3);
@@ -494,6 +535,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             step(stop - 1, std::true_type{});
             wait_loads<0>();  // what was brought past the end
         } else {
+            lds_barrier();
             lds_barrier();
         }
 
@@ -571,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 // ------------------------------------------------------------------------------------------------ joining the parts
 // One workgroup of W waves for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
 // v, v + W, ..., two at a time, and the waves' sums meet in LDS.  Bound by the latency of its reads: a few calls with many parts
-// take 16 waves (one sequence in 44 parts: 5.4 us, with 4 waves XXX), many with few parts 4 (4096 rows: 12.5 us).
+// take 16 waves (one sequence in 44 parts: 5.4 us, with 4 waves 7.4), many with few parts 4 (4096 rows: 12.5 us).
 template <typename T, int W>
 __global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Plan p) {
     __shared__ float sm_m[W][32], sm_l[W][32];
@@ -580,17 +622,18 @@ __global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Pla
     const int c = lane & 31, half = lane >> 5;
     const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
     const int rt = blockIdx.y >> 4, block = blockIdx.y & 15;  // value block: values 32 block ..
+    const Lengths lens(a);
     uint32_t own = 0, before = 0;
     for (int i = lane; i < a.B; i += 64) {
-        const uint32_t t = units_of(a, i);
+        const uint32_t t = units_of(lens.of_lane(i));
         own += t;
         if (i < n) before += t;
     }
     const Cut cu = cut(a, p, sum_wave(own));
     before = sum_wave(before);
-    const uint32_t tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, n));
+    const uint32_t tiles = tiles_of(lens.of(n));
     const uint32_t p0 = (before + LEAD) / cu.run, p1 = tiles ? (before + LEAD + tiles - 1) / cu.run + 1 : p0;
-    const uint32_t parts = p1 - p0, pre_parts = cu.pre ? cdiv(cu.pre, cu.run) : 0;
+    const uint32_t parts = p1 - p0, pre_parts = cu.pre_runs;
     if (pre_parts == 0 && parts == 1) return;  // written by the workgroup that had it whole
     const int rows = a.S * a.H;
     const int rq = g * p.own.rows + 32 * rt;  // within the sequence
@@ -690,6 +733,7 @@ Plan plan_of(const KdaLatentDecodeArgs* a) {
     p.pre = a->prefix_width ? Groups::of((int64_t)a->B * a->S * a->H) : Groups{32, 0};
     const int cus = a->num_cus ? a->num_cus : 256;
     p.grid = cus > p.own.groups + p.pre.groups ? cus : p.own.groups + p.pre.groups;
+    p.per_wg = 1.f / p.grid;
     p.pre_slots = p.pre.groups ? p.grid : 0;
     int bits = 0;  // 2^bits >= page_size: page_mul page_size = 2^(31 + bits) + e, e < 2^bits, so the quotient is exact
     while ((1ll << bits) < a->page_size) ++bits;

@@ -47,15 +47,6 @@ __device__ __forceinline__ int key_tiles(const Span& s, int i) {
 }
 // key tiles of a piece of a row tile that sees `n` of them
 __device__ __forceinline__ int run_of(int n, int pieces) { return max((n + pieces - 1) / pieces, MIN_RUN); }
-__device__ __forceinline__ int scan_wave(int x) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
 // every lane takes a sequence; the first 64 are loaded once
 struct Spans {
     const KdaLatentPrefillArgs& a;
