@@ -62,6 +62,13 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, u32x4 rsrc, uint32_t v
                  "v"(voff), "s"(rsrc)
                  : "memory");
 }
+// 64 lanes x 16 bytes from src (a lane's) + OFFSET into a block of LDS (the instruction adds its offset to both addresses)
+template <int OFFSET>
+__device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(__builtin_amdgcn_readfirstlane(lds - OFFSET)),
+                 "v"(src), "n"(OFFSET)
+                 : "memory");
+}
 __device__ __forceinline__ u32x4 tile_rsrc(const void* base, uint32_t size) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);
     return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)),
@@ -113,6 +120,19 @@ __device__ __forceinline__ int scan_wave(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lanes 15 and 47 to the 16 after them
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
     return x;
+}
+
+// the sum over the lanes, in every lane
+__device__ __forceinline__ float sum_wave(float x) {
+    auto add = [&](int y) { x += __uint_as_float((uint32_t)y); };
+    auto bits = [&] { return (int)__float_as_uint(x); };
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x111, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x112, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x114, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x118, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x142, 0xa, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, bits(), 0x143, 0xc, 0xf, false));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(bits(), 63));
 }
 
 // ------------------------------------------------------------------------------------------------ running softmax

@@ -128,13 +128,6 @@ constexpr int LDS_PAGES = LDS_THERE + 4 * BN;        // page numbers [value wave
 constexpr int LDS_BYTES = LDS_PAGES + VALUE_WAVES * 4 * 256;
 static_assert(LDS_BYTES <= 160 * 1024, "");
 
-// 64 lanes x 16 bytes from src (a lane's) + OFFSET into a block of LDS (the instruction adds its offset to both addresses)
-template <int OFFSET>
-__device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(__builtin_amdgcn_readfirstlane(lds - OFFSET)),
-                 "v"(src), "n"(OFFSET)
-                 : "memory");
-}
 __device__ __forceinline__ uint64_t of_lane(uint64_t x, int l) {
     return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), l) << 32 | (uint32_t)__shfl((int)(uint32_t)x, l);
 }

@@ -20,7 +20,8 @@ constexpr int HD = 128, PE = 64;
 constexpr int TILE_V = BN * HD * 2, TILE_PE = 2 * TILE_V, TILE_BYTES = TILE_PE + BN * PE * 2;  // k | v | shared part
 constexpr int SLOT_ACC = BM * HD * 4, SLOT = SLOT_ACC + BM * 8;  // workspace of a part: accumulators, (m, l) of each row
 // Where rows are few and keys many, the keys are cut: a sequence whose last row tile sees more key tiles than a workgroup's fair
-// share of all (and than MIN_RUN) has every row tile walked in that many pieces, whose parts a second kernel joins.
+// share of all (and than MIN_RUN) has every row tile walked in that many pieces, whose parts a second kernel joins.  (77 rows over
+// 1277 keys, 16 heads: 16.0 us in pieces of 2 tiles, 15.3 of 3, 17.3 of 4.)
 constexpr int MIN_RUN = 3;
 constexpr int64_t MAX_ROW = 1 << 23;  // row strides up to this many elements: a tile's byte offsets stay below 2^31
 
@@ -29,14 +30,14 @@ struct Seq {
     int tiles, most, pieces;  // row tiles; key tiles of the last one; pieces of each
 };
 struct Span {
-    int64_t q0, k0;
+    int q0, k0;         // (below 2^30)
     int Lq, Lk, shift;  // row i sees keys j <= i + shift, j < Lk
 };
 __device__ __forceinline__ Span span_of(const KdaLatentPrefillArgs& a, int n) {
+    const int Tq = (int)a.Tq, Tk = (int)a.Tk;
     Span s;
-    s.q0 = min(max((int64_t)a.cu_q[n], (int64_t)0), a.Tq), s.k0 = min(max((int64_t)a.cu_k[n], (int64_t)0), a.Tk);
-    s.Lq = (int)max(min((int64_t)a.cu_q[n + 1], a.Tq) - s.q0, (int64_t)0);
-    s.Lk = (int)max(min((int64_t)a.cu_k[n + 1], a.Tk) - s.k0, (int64_t)0);
+    s.q0 = min(max(a.cu_q[n], 0), Tq), s.k0 = min(max(a.cu_k[n], 0), Tk);
+    s.Lq = max(min(a.cu_q[n + 1], Tq) - s.q0, 0), s.Lk = max(min(a.cu_k[n + 1], Tk) - s.k0, 0);
     s.shift = a.flags & KDA355_LATENT_CAUSAL ? s.Lk - s.Lq : s.Lk;
     return s;
 }
@@ -53,6 +54,12 @@ struct Spans {
     Span mine;
     __device__ __forceinline__ explicit Spans(const KdaLatentPrefillArgs& args) : a(args), mine(span_of(args, min((int)(threadIdx.x & 63), args.N - 1))) {}
     __device__ __forceinline__ Span operator[](int n) const { return n < 64 ? mine : span_of(a, n); }  // n % 64: the lane
+    __device__ __forceinline__ Span of(int n) const {                                                  // n: the same in all lanes
+        const Span s = n < 64 ? mine : span_of(a, n);
+        const int l = n < 64 ? n : 0;
+        return {__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.k0, l), __builtin_amdgcn_readlane(s.Lq, l),
+                __builtin_amdgcn_readlane(s.Lk, l), __builtin_amdgcn_readlane(s.shift, l)};
+    }
 };
 // The longest run of a piece: a fair share of the key tiles of all row tiles (about).
 __device__ __forceinline__ int longest_run(const KdaLatentPrefillArgs& a, const Spans& spans, int slots) {
@@ -63,9 +70,7 @@ __device__ __forceinline__ int longest_run(const KdaLatentPrefillArgs& a, const 
         const int tiles = (s.Lq + BM - 1) / BM;
         if (tiles) all += (float)tiles * (0.5f * (key_tiles(s, 0) + key_tiles(s, tiles - 1)));
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
-    return __builtin_amdgcn_readfirstlane(max((int)fminf(__builtin_ceilf(all * a.H / slots), 1e9f), MIN_RUN));
+    return __builtin_amdgcn_readfirstlane(max((int)fminf(__builtin_ceilf(sum_wave(all) * a.H / slots), 1e9f), MIN_RUN));
 }
 __device__ __forceinline__ Seq seq_of(const Span& s, int run) {
     Seq q;
@@ -74,20 +79,38 @@ __device__ __forceinline__ Seq seq_of(const Span& s, int run) {
     q.pieces = max((q.most + run - 1) / run, 1);
     return q;
 }
+// The pieces of 64 sequences, one a lane, with what the lanes before it and itself have together.
+struct Pieces {
+    Seq q;
+    int pieces, parts, split;
+};
+__device__ __forceinline__ Pieces pieces_of(const KdaLatentPrefillArgs& a, const Spans& spans, int run, int n) {
+    Pieces p;
+    p.q = n < a.N ? seq_of(spans[n], run) : Seq{0, 0, 1};
+    const bool cut = p.q.pieces > 1;
+    p.pieces = scan_wave(p.q.tiles * p.q.pieces);
+    p.parts = scan_wave(cut ? p.q.tiles * p.q.pieces : 0);
+    p.split = scan_wave(cut ? p.q.tiles : 0);
+    return p;
+}
 // What all workgroups find alike: the longest run, and of a head all pieces, the pieces of split row tiles, and those row tiles.
-struct Cut { int run, pieces, parts, split; };
+struct Cut {
+    int run, pieces, parts, split;
+    Pieces first;  // the first 64 sequences
+};
 __device__ __forceinline__ Cut cut(const KdaLatentPrefillArgs& a, const Spans& spans, const Plan& p) {
-    Cut c = {longest_run(a, spans, p.share), 0, 0, 0};
+    const int lane = threadIdx.x & 63;
+    Cut c;
+    c.run = longest_run(a, spans, p.share);
     for (int again = 0; again < 2; ++again) {
-        int pieces = 0, parts = 0, split = 0;
-        for (int n = threadIdx.x & 63; n < a.N; n += 64) {
-            const Seq q = seq_of(spans[n], c.run);
-            pieces += q.tiles * q.pieces;
-            if (q.pieces > 1) parts += q.tiles * q.pieces, split += q.tiles;
+        c.pieces = c.parts = c.split = 0;
+        for (int n0 = 0; n0 < a.N; n0 += 64) {
+            const Pieces x = pieces_of(a, spans, c.run, n0 + lane);
+            if (n0 == 0) c.first = x;
+            c.pieces += __builtin_amdgcn_readlane(x.pieces, 63);
+            c.parts += __builtin_amdgcn_readlane(x.parts, 63);
+            c.split += __builtin_amdgcn_readlane(x.split, 63);
         }
-        c.pieces = __builtin_amdgcn_readlane(scan_wave(pieces), 63);
-        c.parts = __builtin_amdgcn_readlane(scan_wave(parts), 63);
-        c.split = __builtin_amdgcn_readlane(scan_wave(split), 63);
         // (always so, but for the rounding of the sum: pieces <= row tiles + 2 share / H, parts <= 4 share / H)
         if ((int64_t)c.pieces * a.H <= p.grid && (int64_t)c.parts * a.H <= p.slots) break;
         c.run = 1 << 30;
@@ -100,29 +123,28 @@ struct Where {
 };
 // Piece `i` of a head (SPLIT: split row tile i); n < 0 past the last one.
 template <bool SPLIT>
-__device__ __forceinline__ Where locate(const KdaLatentPrefillArgs& a, const Spans& spans, int run, int i) {
+__device__ __forceinline__ Where locate(const KdaLatentPrefillArgs& a, const Spans& spans, const Cut& c, int i) {
     const int lane = threadIdx.x & 63;
     int before = 0, parts_before = 0;
     for (int n0 = 0; n0 < a.N; n0 += 64) {
-        const int n = n0 + lane;
-        const Seq q = n < a.N ? seq_of(spans[n], run) : Seq{0, 0, 1};
-        const int parts = q.pieces > 1 ? q.tiles * q.pieces : 0;
-        const int mine = SPLIT ? (parts ? q.tiles : 0) : q.tiles * q.pieces;
-        const int s = scan_wave(mine), ps = scan_wave(parts);
+        const Pieces x = n0 == 0 ? c.first : pieces_of(a, spans, c.run, n0 + lane);
+        const int s = SPLIT ? x.split : x.pieces, all = x.q.tiles * x.q.pieces;
         const uint64_t hit = __builtin_amdgcn_ballot_w64(before + s > i);
         if (hit) {
-            const int l = __builtin_ctzll(hit);
-            const int at = i - before - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(mine, l));
+            const int l = __builtin_ctzll(hit), pieces = __builtin_amdgcn_readlane(x.q.pieces, l);
+            const int parts = pieces > 1 ? __builtin_amdgcn_readlane(all, l) : 0;
+            const int mine = SPLIT ? __builtin_amdgcn_readlane(x.q.tiles, l) : __builtin_amdgcn_readlane(all, l);
+            const int at = i - before - (__builtin_amdgcn_readlane(s, l) - mine);
             Where w;
             w.n = n0 + l;
-            w.pieces = __builtin_amdgcn_readlane(q.pieces, l);
-            w.tile = SPLIT ? at : at / w.pieces;
-            w.piece = SPLIT ? 0 : at - w.tile * w.pieces;
-            w.slot = parts_before + __builtin_amdgcn_readlane(ps, l) - __builtin_amdgcn_readlane(parts, l) + w.tile * w.pieces;
+            w.pieces = pieces;
+            w.tile = SPLIT ? at : at / pieces;
+            w.piece = SPLIT ? 0 : at - w.tile * pieces;
+            w.slot = parts_before + __builtin_amdgcn_readlane(x.parts, l) - parts + w.tile * pieces;
             return w;
         }
         before += __builtin_amdgcn_readlane(s, 63);
-        parts_before += __builtin_amdgcn_readlane(ps, 63);
+        parts_before += __builtin_amdgcn_readlane(x.parts, 63);
     }
     return {-1, 0, 0, 1, 0};
 }
@@ -130,6 +152,7 @@ __device__ __forceinline__ Where locate(const KdaLatentPrefillArgs& a, const Spa
 template <typename T>
 __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefillArgs a, Plan p) {
     __shared__ __align__(1024) unsigned char sm[2 * TILE_BYTES];
+    asm volatile("" ::"s"(a.q), "s"(a.q_row), "s"(a.Tq), "s"(a.num_cus), "s"(p.grid));  // all arguments at once
     const Spans spans(a);
     const Cut cu = cut(a, spans, p);
     if ((int64_t)blockIdx.x >= (int64_t)cu.pieces * a.H) return;
@@ -137,13 +160,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     // With 8 heads or a multiple, a head stays on one XCD, whose L2 its keys pass.  (A head's pieces side by side and few heads
     // at a time: 8192 causal tokens, 32 heads 700 us instead of 659.)
     const int i = __builtin_amdgcn_readfirstlane(blockIdx.x / a.H), h = __builtin_amdgcn_readfirstlane(blockIdx.x - i * a.H);
-    const Where at = locate<false>(a, spans, cu.run, cu.pieces - 1 - i);
+    const Where at = locate<false>(a, spans, cu, cu.pieces - 1 - i);
     const int n = __builtin_amdgcn_readfirstlane(at.n);
     if (n < 0) return;
     const int m0 = __builtin_amdgcn_readfirstlane(at.tile) * BM;
-    const Span sp = span_of(a, n);
+    const Span sp = spans.of(n);
     const int64_t q0 = sp.q0, k0 = sp.k0;
-    const int Lq = __builtin_amdgcn_readfirstlane(sp.Lq), Lk = __builtin_amdgcn_readfirstlane(sp.Lk), shift = __builtin_amdgcn_readfirstlane(sp.shift);
+    const int Lq = sp.Lq, Lk = sp.Lk, shift = sp.shift;
     const int ntiles = __builtin_amdgcn_readfirstlane(key_tiles(sp, at.tile));
     const int length = run_of(ntiles, at.pieces), first = __builtin_amdgcn_readfirstlane(at.piece * length);
     const int last = __builtin_amdgcn_readfirstlane(min(first + length, ntiles));  // this piece's key tiles
@@ -152,14 +175,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
     const int row = m0 + 32 * w + c;
-
-    // ---- queries: operand registers, straight from memory (rows past the end repeat the last one)
-    u32x4 q[12];
-    {
-        const uint16_t* qr = static_cast<const uint16_t*>(a.q) + (q0 + min(row, Lq - 1)) * a.q_row + h * a.q_head + 8 * half;
-#pragma unroll
-        for (int i = 0; i < 12; ++i) q[i] = *reinterpret_cast<const u32x4*>(qr + 16 * i);
-    }
 
     // ---- tile loads: wave w brings tokens 16 w .. 16 w + 15
     const uint16_t* kh = static_cast<const uint16_t*>(a.k) + k0 * a.k_row + h * a.k_head;
@@ -225,6 +240,25 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         const Tile t = tile_at(first);
 #pragma unroll
         for (int i = 0; i < 10; ++i) bring(t, i);
+    }
+    // ---- queries: a wave's 32 rows (past the end the last one again).  Their first 128 come through the LDS of the second tile,
+    // 256 bytes a row, laid out like keys, the last 64 straight, 32 bytes of every row at a time (all of them so: 15.6 us instead of 15.3
+    // for 77 rows and 1277 keys).
+    u32x4 q[12] = {};
+    if (m0 + 32 * w < Lq) {
+        const uint16_t* qh = static_cast<const uint16_t*>(a.q) + q0 * a.q_row + h * a.q_head;
+        const uint32_t at = lds + ((first + 1) & 1) * TILE_BYTES + 32 * w * (HD * 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 4);
+            load_block<0>(at + i * 1024, (uint64_t)(qh + min(m0 + 32 * w + r, Lq - 1) * a.q_row) + (((lane & 15) ^ swz16(r)) << 4));
+        }
+        const uint16_t* qr = qh + min(row, Lq - 1) * a.q_row + 8 * half;
+#pragma unroll
+        for (int i = 8; i < 12; ++i) q[i] = *reinterpret_cast<const u32x4*>(qr + 16 * i);
+        wait_loads<0>();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = lds_read16((at + ka) ^ (i << 5));
     }
     // the queries are there before the loop: the compiler would wait for them, and so for the next tile, in it
 #pragma unroll
@@ -382,8 +416,8 @@ __global__ void __launch_bounds__(256) join_kernel(KdaLatentPrefillArgs a, Plan 
     const Cut cu = cut(a, spans, p);
     for (int64_t task = blockIdx.x; task < (int64_t)cu.split * a.H; task += gridDim.x) {
         const int h = __builtin_amdgcn_readfirstlane((int)(task / cu.split));
-        const Where at = locate<true>(a, spans, cu.run, (int)(task - (int64_t)h * cu.split));
-        const Span sp = span_of(a, __builtin_amdgcn_readfirstlane(at.n));
+        const Where at = locate<true>(a, spans, cu, (int)(task - (int64_t)h * cu.split));
+        const Span sp = spans.of(__builtin_amdgcn_readfirstlane(at.n));
         const int ntiles = key_tiles(sp, at.tile), length = run_of(ntiles, at.pieces);
         if (ntiles <= length) continue;  // one piece: written by its workgroup
         const int parts = __builtin_amdgcn_readfirstlane((ntiles + length - 1) / length);
@@ -420,13 +454,13 @@ __global__ void __launch_bounds__(256) join_kernel(KdaLatentPrefillArgs a, Plan 
         }
         if (i < parts) add(load(i));
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint16_t* o = static_cast<uint16_t*>(a.out) + (sp.q0 + row) * a.out_row + h * a.out_head + 32 * d + 4 * half;
+        uint16_t* o = static_cast<uint16_t*>(a.out) + ((int64_t)sp.q0 + row) * a.out_row + h * a.out_head + 32 * d + 4 * half;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
             *reinterpret_cast<u32x2*>(o + 8 * g) =
                 l == 0.f ? u32x2{0u, 0u} : u32x2{T::pack(acc[g][0] * inv, acc[g][1] * inv), T::pack(acc[g][2] * inv, acc[g][3] * inv)};
         if (a.lse && d == 0 && half == 0)
-            a.lse[(sp.q0 + row) * a.H + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055995f;
+            a.lse[((int64_t)sp.q0 + row) * a.H + h] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055995f;
     }
 }
 
