@@ -272,32 +272,35 @@ __global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a)
     if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
 }
 
-// The same in one workgroup and one launch, where there is little to give up: the marks are bits in LDS.  Its differences come
-// from one CU: 128 table entries 4.3 us (two launches 4.5), 4160 8.2 (5.5), 8192 15.6 (7.6).  A launch takes 2.7 us of the
-// caller's time, so it is taken up to where it costs the GPU no more than that.
-constexpr int FREE_SMALL = 5 * SCAN_THREADS;        // table entries
-constexpr int FREE_WORDS = 8192;                    // 32 pages each
+// The same in one workgroup and one launch, where there is little to give up: what each page loses is counted in LDS, so that no
+// two threads meet in memory.  128 table entries 3.7 us (two launches 5.0), 2048 4.8 (5.7), 4160 5.9 (5.6; with differences in
+// memory 9.2), 8192 9.8 (7.6).  A launch takes 2.7 us of the caller's time, so it is taken up to where the GPU is about as fast.
+constexpr int FREE_SMALL = 5 * SCAN_THREADS, FREE_STEPS = 4;  // table entries, those of a thread at a time
+constexpr int FREE_PAGES = 16 * 1024;
 __global__ void __launch_bounds__(SCAN_THREADS) free_small_kernel(KdaPagesArgs a) {
-    __shared__ uint32_t marks[FREE_WORDS];
+    __shared__ int lost[FREE_PAGES];
     __shared__ int sw[SCAN_THREADS / 64];
-    const int words = (a.pages + 31) / 32;
-    for (int i = threadIdx.x; i < words; i += SCAN_THREADS) marks[i] = 0;
+    for (int i = threadIdx.x; i < a.pages; i += SCAN_THREADS) lost[i] = 0;
     __syncthreads();
     const int all = a.n * a.table_width;
-    for (int e = threadIdx.x; e < all; e += SCAN_THREADS) {
-        const int i = e / a.table_width, j = e - i * a.table_width, r = a.src[i];
-        if (r < 0 || r >= a.rows) continue;
-        const int used = (row_len(a, r) + a.page_size - 1) / a.page_size;
-        int32_t* at = a.block_table + r * a.table_stride + j;
-        const int page = *at;
-        if (j < used && page >= 0 && page < a.pages) {
-            const int before = atomicSub(a.ref_counts + page, 1);
-            if (before == 1)
-                atomicOr(&marks[page >> 5], 1u << (page & 31));
-            else if (before <= 0)
-                atomicAdd(a.ref_counts + page, 1);
+    for (int e0 = threadIdx.x; e0 < all; e0 += FREE_STEPS * SCAN_THREADS) {
+        int32_t* at[FREE_STEPS];
+        int page[FREE_STEPS];
+#pragma unroll
+        for (int k = 0; k < FREE_STEPS; ++k) {  // rows, lengths and pages of all of them under way at once
+            const int e = min(e0 + k * SCAN_THREADS, all - 1), i = e / a.table_width, j = e - i * a.table_width;
+            const int r = a.src[i], row = min(max(r, 0), a.rows - 1);
+            at[k] = a.block_table + row * a.table_stride + j;
+            page[k] = *at[k];
+            const bool mine = e0 + k * SCAN_THREADS < all && r == row;
+            if (!mine) at[k] = nullptr;
+            if (!mine || (int64_t)j * a.page_size >= row_len(a, row)) page[k] = -1;
         }
-        *at = -1;
+#pragma unroll
+        for (int k = 0; k < FREE_STEPS; ++k) {
+            if (page[k] >= 0 && page[k] < a.pages) atomicAdd(&lost[page[k]], 1);
+            if (at[k]) *at[k] = -1;
+        }
     }
     __syncthreads();  // every thread has read the lengths
     for (int i = threadIdx.x; i < a.n; i += SCAN_THREADS) {
@@ -306,17 +309,27 @@ __global__ void __launch_bounds__(SCAN_THREADS) free_small_kernel(KdaPagesArgs a
     }
     int top = a.num_free[0];
     top = top < 0 ? 0 : top > a.pages ? a.pages : top;
-    for (int hi = words; hi > 0; hi -= SCAN_THREADS) {  // the highest pages first
-        const int at = hi - 1 - (int)threadIdx.x;
-        uint32_t m = at >= 0 ? marks[at] : 0;
-        int total;
-        int slot = top + block_scan(__popc(m), sw, total);
-        while (m) {
-            const int b = 31 - __clz((int)m);
-            m ^= 1u << b;
-            if (slot < a.pages) a.free_pages[slot] = at * 32 + b;
-            ++slot;
+    for (int hi = a.pages; hi > 0; hi -= FREE_STEPS * SCAN_THREADS) {  // the highest pages first
+        int mine[FREE_STEPS], count = 0;
+#pragma unroll
+        for (int k = 0; k < FREE_STEPS; ++k) {
+            const int p = hi - 1 - FREE_STEPS * (int)threadIdx.x - k;
+            mine[k] = 0;
+            if (p < 0 || lost[p] == 0) continue;
+            const int held = a.ref_counts[p];
+            if (held <= 0) continue;  // (a caller's mistake)
+            mine[k] = lost[p] >= held;
+            a.ref_counts[p] = mine[k] ? 0 : held - lost[p];
+            count += mine[k];
         }
+        int total;
+        int slot = top + block_scan(count, sw, total);
+#pragma unroll
+        for (int k = 0; k < FREE_STEPS; ++k)
+            if (mine[k]) {
+                if (slot < a.pages) a.free_pages[slot] = hi - 1 - FREE_STEPS * (int)threadIdx.x - k;
+                ++slot;
+            }
         top += total;
     }
     if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
@@ -488,7 +501,7 @@ extern "C" int kda355_free_pages_launch(const KdaPagesArgs* a, kda355_stream_t s
     if (a->n == 0) return 0;
     KDA_CHECK_ARG(a->src, "free_pages: a required pointer is null");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if ((int64_t)a->n * a->table_width <= FREE_SMALL && a->pages <= 32 * FREE_WORDS) {
+    if ((int64_t)a->n * a->table_width <= FREE_SMALL && a->pages <= FREE_PAGES) {
         hipLaunchKernelGGL(free_small_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
         return launched("free_pages");
     }
