@@ -180,6 +180,20 @@ def lib():
     return _lib
 
 
+class _Launches(dict):
+    """kda355_<name>_launch, called with its arguments' bytes: 0.4 us less than with a Structure and a pointer to it."""
+
+    def __missing__(self, name):
+        f = lib()[f"kda355_{name}_launch"]  # (an object of its own: the attribute's takes the Structure)
+        f.argtypes = [ctypes.c_char_p, P]
+        f.restype = ctypes.c_int
+        self[name] = f
+        return f
+
+
+LAUNCH = _Launches()
+
+
 def noalloc_lib():
     """libkda355_noalloc.so (kda355_prefill_launch_noalloc and its static device scratch), loaded on first use only: a
     process that never calls the no-allocation entry point never holds the scratch."""

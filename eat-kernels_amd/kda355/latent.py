@@ -191,11 +191,12 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
     if out is None:
         out = torch.empty(shape, dtype=dt, device=dev)
     ws = _workspace(need, workspace, dev)
-    a = _lib.KdaLatentPrefillArgs.from_buffer_copy(
-        _PTR8.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                   cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()) + mid +
-        _PTR2.pack(0 if ws is None else ws.data_ptr(), need) + tail)
-    _lib.check(_lib.lib().kda355_latent_prefill_launch(ctypes.byref(a), _stream(dev)), "latent_prefill")
+    args = (_PTR8.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(),
+                       0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()) + mid +
+            _PTR2.pack(0 if ws is None else ws.data_ptr(), need) + tail)
+    rc = _lib.LAUNCH["latent_prefill"](args, _stream(dev))
+    if rc:
+        _lib.check(rc, "latent_prefill")
     return out
 
 
@@ -263,11 +264,13 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
     if out is None:
         out = torch.empty(shape, dtype=dt, device=dev)
     ws = _workspace(need, workspace, dev)
-    a = _lib.KdaLatentDecodeArgs.from_buffer_copy(
-        _PTR10.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                    0 if prefix_table is None else prefix_table.data_ptr(), 0 if prefix_len is None else prefix_len.data_ptr(),
-                    out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr()) + tail)
-    _lib.check(_lib.lib().kda355_latent_decode_launch(ctypes.byref(a), _stream(dev)), "latent_decode")
+    args = (_PTR10.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                        0 if prefix_table is None else prefix_table.data_ptr(),
+                        0 if prefix_len is None else prefix_len.data_ptr(),
+                        out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr()) + tail)
+    rc = _lib.LAUNCH["latent_decode"](args, _stream(dev))
+    if rc:
+        _lib.check(rc, "latent_decode")
     return out
 
 
@@ -295,9 +298,10 @@ def latent_append(latent, k_pe, cache, slots):
         a = _lib.KdaLatentTokensArgs(*[None] * 7, *strides, 0, page_stride, pages, 0, T, size, 0, 0, 0)
         plan = _keep(_append_seen, key, (dev, bytes(a)[_PTR7.size:]))
     dev, tail = plan
-    a = _lib.KdaLatentTokensArgs.from_buffer_copy(
-        _PTR7.pack(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), 0, 0, 0) + tail)
-    _lib.check(_lib.lib().kda355_latent_append_launch(ctypes.byref(a), _stream(dev)), "latent_append")
+    args = _PTR7.pack(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), 0, 0, 0) + tail
+    rc = _lib.LAUNCH["latent_append"](args, _stream(dev))
+    if rc:
+        _lib.check(rc, "latent_append")
     return cache
 
 
@@ -323,7 +327,8 @@ def latent_gather(cache, block_table, cu_seqlens, out):
                                      0)
         plan = _keep(_gather_seen, key, (dev, bytes(a)[_PTR7.size:]))
     dev, tail = plan
-    a = _lib.KdaLatentTokensArgs.from_buffer_copy(
-        _PTR7.pack(0, 0, cache.data_ptr(), 0, block_table.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr()) + tail)
-    _lib.check(_lib.lib().kda355_latent_gather_launch(ctypes.byref(a), _stream(dev)), "latent_gather")
+    args = _PTR7.pack(0, 0, cache.data_ptr(), 0, block_table.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr()) + tail
+    rc = _lib.LAUNCH["latent_gather"](args, _stream(dev))
+    if rc:
+        _lib.check(rc, "latent_gather")
     return out

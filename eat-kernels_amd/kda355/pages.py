@@ -63,19 +63,13 @@ def _pools(pools, slots=None):
     return dev, out
 
 
-# KdaPagesArgs in one go: its 24 pools would be as many objects
-_PACK = struct.Struct(f"={4 * _lib.MAX_POOLS}q2i8Qq4i")
-assert _PACK.size == ctypes.sizeof(_lib.KdaPagesArgs)
-_NO_POOLS = (0,) * (4 * _lib.MAX_POOLS)
+# KdaPagesArgs in three pieces (its 24 pools would be as many objects): the pools that there are, zeros, what follows the pools
+_POOLS = [struct.Struct(f"={4 * n}q") for n in range(_lib.MAX_POOLS + 1)]
+_REST = [bytes(32 * (_lib.MAX_POOLS - n)) for n in range(_lib.MAX_POOLS + 1)]
+_PACK = struct.Struct("=2i8Qq4i")
+assert 32 * _lib.MAX_POOLS + _PACK.size == ctypes.sizeof(_lib.KdaPagesArgs)
 
 
-class _Entries(dict):
-    def __missing__(self, name):
-        f = self[name] = getattr(_lib.lib(), f"kda355_{name}_launch")
-        return f
-
-
-_LAUNCH = _Entries()
 # What was found right is kept by what the checks look at (latent.py): (device, pages, table stride, rows, width, page size,
 # [(row bytes, slot stride, slots) of each pool])
 _seen = {}
@@ -88,12 +82,15 @@ def _key(name, page_size, pools, tensors):
 
 def _launch(name, dev, pools, n, src, dst, ws, book=(0, 0, 0, 0, 0), stride=0, rows=0, width=0, pages=0, size=1):
     """`pools`: address, row bytes, slot stride and slots of one after the other; `book`: the addresses of the bookkeeping."""
+    count = len(pools) // 4
     try:
-        a = _lib.KdaPagesArgs.from_buffer_copy(
-            _PACK.pack(*pools, *_NO_POOLS[len(pools):], len(pools) // 4, n, src, dst, *book, ws, stride, rows, width, pages, size))
+        args = (_POOLS[count].pack(*pools) + _REST[count] +
+                _PACK.pack(count, n, src, dst, *book, ws, stride, rows, width, pages, size))
     except struct.error as e:
         raise ValueError(f"kda355: {name}: a size is out of range ({e})") from None
-    _lib.check(_LAUNCH[name](ctypes.byref(a), _stream(dev)), name)
+    rc = _lib.LAUNCH[name](args, _stream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _addresses(pools, found):
