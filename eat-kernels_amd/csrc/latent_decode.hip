@@ -604,17 +604,17 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 }
 
 // ------------------------------------------------------------------------------------------------ joining the parts
-// One workgroup of W waves for 32 rows and 32 values (blockIdx.y: row tile, then the 16 blocks of values); wave v takes the parts
-// v, v + W, ..., two at a time, and the waves' sums meet in LDS.  Bound by the latency of its reads: a few calls with many parts
-// take 16 waves (one sequence in 44 parts: 5.4 us, with 4 waves 7.4), many with few parts 4 (4096 rows: 12.5 us).
-template <typename T, int W>
-__global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Plan p) {
-    __shared__ float sm_m[W][32], sm_l[W][32];
-    __shared__ f32x4 sm_a[W][4][64];
-    const int tid = threadIdx.x, v = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+// For 32 rows and 32 values of a sequence, two parts at a time.  SPLIT: a workgroup of 16 waves, wave v takes the parts v, v + 16,
+// ..., and their sums meet in LDS (few rows with many parts: one sequence in 44 parts 5.4 us, in 4 waves 7.4).  Otherwise every one
+// of 4 waves has a block of 32 values of its own and all parts (4096 rows: 11.2 us; with four waves to a block as above 12.4, much of it
+// for finding out what there is to do).
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 1024 : 256) join_kernel(KdaLatentDecodeArgs a, Plan p) {
+    constexpr int W = SPLIT ? 16 : 1;  // waves to a block
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), v = SPLIT ? w : 0, lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
     const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
-    const int rt = blockIdx.y >> 4, block = blockIdx.y & 15;  // value block: values 32 block ..
+    const int rt = blockIdx.y / (SPLIT ? 16 : 4), block = SPLIT ? blockIdx.y & 15 : (blockIdx.y & 3) * 4 + w;  // values 32 block ..
     const Lengths lens(a);
     uint32_t own = 0, before = 0;
     for (int i = lane; i < a.B; i += 64) {
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Pla
     };
     auto walk = [&](const char* at, int64_t step, uint32_t n, int cc) {
         uint32_t i = v;
-        for (; W > 4 && i + W < n; i += 2 * W) {
+        for (; i + W < n; i += 2 * W) {
             const Part y0 = load(at + i * step, cc), y1 = load(at + (i + W) * step, cc);
             add(y0);
             add(y1);
@@ -675,29 +675,39 @@ __global__ void __launch_bounds__(W * 64) join_kernel(KdaLatentDecodeArgs a, Pla
             walk(ws + gp * pre_bytes + (rp >> 5) * SLOT_TILE, p.pre.groups * pre_bytes, pre_parts, rp & 31);
         }
     }
-    if (half == 0) {
-        sm_m[v][c] = m;
-        sm_l[v][c] = l;
+    auto write = [&](int at, f32x4 o, float M, float L) {  // values 32 block + at ..
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const int t = r / a.H, h = r - t * a.H;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 32 * block + at;
+        *reinterpret_cast<u32x2*>(out) = L == 0.f ? u32x2{0u, 0u} : u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+        if (a.lse && block == 0 && at == 0) a.lse[r] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.69314718055995f;
+    };
+    if constexpr (SPLIT) {
+        __shared__ float sm_m[W][32], sm_l[W][32];
+        __shared__ f32x4 sm_a[W][4][64];
+        if (half == 0) {
+            sm_m[v][c] = m;
+            sm_l[v][c] = l;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm_a[v][e][lane] = acc[e];
+        __syncthreads();
+        if (!valid || v >= 4) return;
+        float M = M_START, L = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) M = fmaxf(M, sm_m[i][c]);
+        f32x4 o = {};
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float f = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
+            L += sm_l[i][c] * f;
+            o += sm_a[i][v][lane] * f;
+        }
+        write(8 * v + 4 * half, o, M, L);  // wave v finishes values 8 v .. 8 v + 7 of the block
+    } else if (valid) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) write(8 * e + 4 * half, acc[e], m, l);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sm_a[v][e][lane] = acc[e];
-    __syncthreads();
-    if (!valid || v >= 4) return;
-    float M = M_START, L = 0.f, f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) M = fmaxf(M, sm_m[i][c]);
-    f32x4 o = {};
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        f = __builtin_amdgcn_exp2f(sm_m[i][c] - M);
-        L += sm_l[i][c] * f;
-        o += sm_a[i][v][lane] * f;  // wave v finishes values 8 v .. 8 v + 7 of the block
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    const int t = r / a.H, h = r - t * a.H;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 32 * block + 8 * v + 4 * half;
-    *reinterpret_cast<u32x2*>(out) = L == 0.f ? u32x2{0u, 0u} : u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
-    if (a.lse && block == 0 && v == 0 && half == 0) a.lse[r] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.69314718055995f;
 }
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -770,15 +780,15 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
                   "latent_decode: needs %lld bytes of 256-byte aligned workspace", (long long)need);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const Plan p = plan_of(a);
-    const dim3 join((uint32_t)a->B * p.own.groups, p.own.rows / 32 * 16);
-    const bool few = (int64_t)join.x * join.y <= p.grid;  // at most a workgroup a CU: likely many parts each
+    const uint32_t join = (uint32_t)a->B * p.own.groups, tiles = p.own.rows / 32;
+    const bool few = (int64_t)join * tiles * 16 <= p.grid;  // blocks of rows and values: likely many parts each
     auto launch = [&](auto type) {
         typedef decltype(type) T;
         hipLaunchKernelGGL(decode_kernel<T>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
         if (few)
-            hipLaunchKernelGGL((join_kernel<T, 16>), join, dim3(16 * 64), 0, s, *a, p);
+            hipLaunchKernelGGL((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), 0, s, *a, p);
         else
-            hipLaunchKernelGGL((join_kernel<T, 4>), join, dim3(4 * 64), 0, s, *a, p);
+            hipLaunchKernelGGL((join_kernel<T, false>), dim3(join, tiles * 4), dim3(256), 0, s, *a, p);
     };
     if (a->dtype == KDA355_DTYPE_BF16) launch(Bf16{}); else launch(Fp16{});
     const hipError_t e = hipGetLastError();
