@@ -22,7 +22,7 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 // down to 2^-23 of the maximum.
 struct Bf16 {
     static constexpr float B = 0.f, SLACK = 8.f;
-    static constexpr uint32_t EXP = 0x7f807f80u, EXP_ONE = 0x00800080u, ONE = 0x3f80u;
+    static constexpr uint32_t EXP = 0x7f807f80u, EXP_ONE = 0x00800080u;
     static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -34,7 +34,7 @@ struct Bf16 {
 };
 struct Fp16 {
     static constexpr float B = 9.f, SLACK = 6.f;
-    static constexpr uint32_t EXP = 0x7c007c00u, EXP_ONE = 0x04000400u, ONE = 0x3c00u;
+    static constexpr uint32_t EXP = 0x7c007c00u, EXP_ONE = 0x04000400u;
     static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
@@ -97,11 +97,6 @@ __device__ __forceinline__ int swz16(int t) { return ((t & 3) << 2) | ((t >> 2) 
 __device__ __forceinline__ int swz8(int t) { return (t >> 1) & 7; }
 
 // ------------------------------------------------------------------------------------------------ lanes
-// the other half wave's value of the same row
-__device__ __forceinline__ float other_half(float x) {
-    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
-    return __uint_as_float((threadIdx.x & 32) ? r.x : r.y);
-}
 __device__ __forceinline__ float max_halves(float x) {
     const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
     return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));

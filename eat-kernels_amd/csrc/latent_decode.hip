@@ -14,6 +14,14 @@
 // instructions of one kind run beside the softmax, the waits and the address arithmetic of the other.  One barrier a tile.
 // Scores come from 16x16x32 instructions (keys as rows), so that every key fragment read serves two of them; values from
 // 32x32x16 with one fragment for both row tiles.
+//
+// Bound: with many rows of few sequences the two products, 576 and 512 cycles of a SIMD's matrix core a tile; a step takes about 1900,
+// with LDS (160 KiB read and written a step) and the instructions of the longer kind of wave behind them.  16 sequences of 6000 to
+// 9900 tokens, 8 draft tokens, 96 heads: 248 us, 0.86 PFLOP/s; 64 sequences of 32 heads behind 32768 shared tokens: 163 us, 0.91
+// PFLOP/s.  With a row tile or two a sequence HBM: 64 ragged sequences, 64 heads, 129 us, 4.25 TB/s.  One sequence of 4097 tokens, 12
+// heads: 15.5 us, 10.5 of it this kernel (lengths and cut 2.2, queries and first tile 2.3, three tiles and the end 4.5) and 5 the join.
+// Eight waves of one kind with the value dimensions split: 141 / 296 / 234 us instead of 142 / 260 / 227; four of one kind, one a SIMD,
+// pipelined: 142 / 276 / 264 (64 ragged, drafts, shared prefix).
 #include <type_traits>
 
 #include "attend.h"
