@@ -40,7 +40,8 @@ constexpr int RT = 2, MAX_ROWS = 32 * RT;               // row tiles, query rows
 // ragged sequences 146 us without LEAD, 142 with 3, 136 with 8 and with 16; 64 short ones behind 32768 tokens 230, 202, 190 and
 // 190; one sequence of 4097 tokens 20.3 us with runs of 1, 17.9 of 3, 18.5 of 4.
 constexpr uint32_t LEAD = 8, MIN_RUN = 3;
-constexpr int SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;  // workspace of 32 rows: accumulators, (m, l) of each row
+// workspace: the cut for the second kernel (run, runs of the prefix), then slots, of 32 rows: accumulators, (m, l) of each row
+constexpr int SLOTS = 256, SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;
 
 struct Groups {
     int rows, groups;  // rows of a group, groups
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
     const Cut cu = cut(a, p, sum_wave(own));
     const uint32_t wgs = cu.pre_wgs + cu.own_wgs;
+    if (blockIdx.x == 0 && tid == 0) *static_cast<u32x2*>(a.workspace) = u32x2{cu.run, cu.pre_runs};
     if (blockIdx.x >= wgs) return;
     const uint32_t task = xcd_task(blockIdx.x, wgs);  // neighbours read the same keys: on one XCD
     const bool prefix = task < cu.pre_wgs;
@@ -594,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             // the part's slot; piece + n names a sequence's parts uniquely, since both only grow along the tiles
             const int64_t slot_bytes = (int64_t)(gr.rows / 32) * SLOT_TILE;
             const int64_t slot = prefix ? (int64_t)id : ((int64_t)piece + n) * gr.groups + g;
-            char* out = static_cast<char*>(a.workspace) + (prefix ? 0 : p.pre_slots * (p.pre.rows / 32) * SLOT_TILE) + slot * slot_bytes;
+            char* out = static_cast<char*>(a.workspace) + SLOTS + (prefix ? 0 : p.pre_slots * (p.pre.rows / 32) * SLOT_TILE) + slot * slot_bytes;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 if (r0 + 32 * r + c >= r1) break;
@@ -621,20 +623,17 @@ __global__ void __launch_bounds__(SPLIT ? 1024 : 256) join_kernel(KdaLatentDecod
     constexpr int W = SPLIT ? 16 : 1;  // waves to a block
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), v = SPLIT ? w : 0, lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
-    const int n = blockIdx.x / p.own.groups, g = blockIdx.x - n * p.own.groups;
+    const int n = __builtin_amdgcn_readfirstlane(blockIdx.x / p.own.groups), g = blockIdx.x - n * p.own.groups;
+    asm volatile("" ::"s"(a.q_latent), "s"(a.ql_row), "s"(a.page_stride), "s"(a.B), "s"(p.grid));  // all arguments at once
     const int rt = blockIdx.y / (SPLIT ? 16 : 4), block = SPLIT ? blockIdx.y & 15 : (blockIdx.y & 3) * 4 + w;  // values 32 block ..
     const Lengths lens(a);
-    uint32_t own = 0, before = 0;
-    for (int i = lane; i < a.B; i += 64) {
-        const uint32_t t = units_of(lens.of_lane(i));
-        own += t;
-        if (i < n) before += t;
-    }
-    const Cut cu = cut(a, p, sum_wave(own));
+    const u32x2 cu = *static_cast<const u32x2*>(a.workspace);
+    uint32_t before = 0;
+    for (int i = lane; i < n; i += 64) before += units_of(lens.of_lane(i));
     before = sum_wave(before);
-    const uint32_t tiles = tiles_of(lens.of(n));
-    const uint32_t p0 = (before + LEAD) / cu.run, p1 = tiles ? (before + LEAD + tiles - 1) / cu.run + 1 : p0;
-    const uint32_t parts = p1 - p0, pre_parts = cu.pre_runs;
+    const uint32_t tiles = tiles_of(lens.of(n)), run = __builtin_amdgcn_readfirstlane(cu.x);
+    const uint32_t p0 = (before + LEAD) / run, p1 = tiles ? (before + LEAD + tiles - 1) / run + 1 : p0;
+    const uint32_t parts = p1 - p0, pre_parts = __builtin_amdgcn_readfirstlane(cu.y);
     if (pre_parts == 0 && parts == 1) return;  // written by the workgroup that had it whole
     const int rows = a.S * a.H;
     const int rq = g * p.own.rows + 32 * rt;  // within the sequence
@@ -674,7 +673,7 @@ __global__ void __launch_bounds__(SPLIT ? 1024 : 256) join_kernel(KdaLatentDecod
         for (; i < n; i += W) add(load(at + i * step, cc));
     };
     if (valid) {
-        const char* ws = static_cast<const char*>(a.workspace);
+        const char* ws = static_cast<const char*>(a.workspace) + SLOTS;
         const int64_t own_bytes = (int64_t)(p.own.rows / 32) * SLOT_TILE, pre_bytes = (int64_t)(p.pre.rows / 32) * SLOT_TILE;
         walk(ws + p.pre_slots * pre_bytes + rt * SLOT_TILE + (((int64_t)p0 + n) * p.own.groups + g) * own_bytes, p.own.groups * own_bytes,
              parts, c);
@@ -763,7 +762,7 @@ extern "C" int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArg
     if (a->B == 0) return 0;
     const Plan p = plan_of(a);
     const int64_t own = p.grid + (int64_t)a->B * p.own.groups;
-    return (p.pre_slots * (p.pre.rows / 32) + own * (p.own.rows / 32)) * SLOT_TILE;
+    return SLOTS + (p.pre_slots * (p.pre.rows / 32) + own * (p.own.rows / 32)) * SLOT_TILE;
 }
 
 extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
