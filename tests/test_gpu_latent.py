@@ -214,6 +214,17 @@ def test_prefill_any(seed):
     Expanded(lq, lk, 1 + pick(5, 1)[0], (BF, HF)[seed % 2], ("dense", "joint", "wide")[seed % 3], seed=seed).check(seed != 4)
 
 
+@pytest.mark.parametrize("N", [64, 65, 150])
+def test_prefill_many_sequences(N):
+    """More sequences than a wave has lanes, empty ones and one that is cut among them."""
+    g = torch.Generator().manual_seed(N)
+    lq = torch.randint(0, 30, (N,), generator=g).tolist()
+    lk = [a + b for a, b in zip(lq, torch.randint(0, 60, (N,), generator=g).tolist())]
+    lq[N - 1], lk[N - 1], lq[3], lk[3] = 5, 6000, 200, 3
+    lk[N // 2] = 0
+    Expanded(lq, lk, 2, BF).check()
+
+
 def test_prefill_captured_with_other_lengths():
     """One graph replayed with other boundaries, every replay against the eager result and the plain form."""
     xs = [Expanded(lq, lk, 2, BF, "dense", seed=i) for i, (lq, lk) in enumerate(
@@ -420,6 +431,14 @@ def test_decode_later_draft_tokens_do_not_matter(value, H, S):
     ([0, 0], 1, 8, 16, 70), ([0, 2], 3, 8, 16, 0)])
 def test_decode_prefix(lens, S, H, size, prefix, dtype):
     Absorbed(lens, S, H, size, dtype, prefix=prefix).check()
+
+
+@pytest.mark.parametrize("B,S,H", [(64, 1, 3), (65, 2, 16), (150, 1, 40)])
+def test_decode_many_sequences_behind_a_prefix(B, S, H):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 90, (B,), generator=g).tolist()
+    lens[B - 1] = 1500
+    Absorbed(lens, S, H, 16, BF, prefix=333).check()
 
 
 def test_decode_prefix_long():
