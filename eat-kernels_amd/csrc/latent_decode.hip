@@ -34,7 +34,7 @@ constexpr int ROW_BYTES = ROW * 2, LAT_BYTES = LAT * 2, PE_BYTES = PE * 2;
 constexpr int SCORE_WAVES = 4, VALUE_WAVES = 4, THREADS = (SCORE_WAVES + VALUE_WAVES) * 64;
 constexpr int BN = 32, BUFS = 4;                        // keys of a tile, tiles in LDS
 constexpr int LOADS = 10;                               // of a value wave a tile: 8 of latent rows, positional parts, page numbers
-constexpr int RT = 2, MAX_ROWS = 32 * RT;               // row tiles, query rows of a group
+constexpr int MAX_ROWS = 64;                            // query rows of a group
 // The cut is by cost: beginning a sequence (lengths, queries, page numbers and first tile one after the other) takes about as
 // long as LEAD tiles, which stand in front of every sequence's own; a run is MIN_RUN of these units at least.  Measured: 64
 // ragged sequences 146 us without LEAD, 142 with 3, 136 with 8 and with 16; 64 short ones behind 32768 tokens 230, 202, 190 and
@@ -45,8 +45,8 @@ constexpr int SLOTS = 256, SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;
 
 struct Groups {
     int rows, groups;  // rows of a group, groups
-    static Groups of(int64_t n) {
-        const int64_t g = (n + MAX_ROWS - 1) / MAX_ROWS;
+    static Groups of(int64_t n, int most) {
+        const int64_t g = (n + most - 1) / most;
         const int64_t r = g ? (n + 32 * g - 1) / (32 * g) * 32 : 32;  // in tiles of 32, about equal
         return {(int)r, (int)((n + r - 1) / r)};
     }
@@ -151,7 +151,7 @@ __device__ __forceinline__ float join_groups(float x, F f) {
     return f(__uint_as_float(b.x), __uint_as_float(b.y));
 }
 
-template <typename T>
+template <typename T, int RT>
 __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
     __shared__ __align__(1024) unsigned char sm[LDS_BYTES];
     const uint32_t lds = lds_offset(sm);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const int64_t page_bytes = a.page_stride * 2;
     const char* const cache = static_cast<const char*>(a.cache);
     const bool scores = w < SCORE_WAVES;
-    const int rt = w & 1, kh = w >> 1 & 1;  // a score wave's row tile and keys 16 kh ..
+    const int rw = w & 1, kh = w >> 1 & 1;  // a score wave's rows 16 RT rw .. (16 RT of them) and keys 16 kh ..
     const int vw = w & 3;                   // a value wave's 128 values
     const int c16 = lane & 15, quad = lane >> 4;
     // LDS read addresses within a tile.  Of a score wave: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step, latent and
@@ -242,63 +242,73 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // the new reference of the group's row r after `tile`, by its own scores alone; returns the factor of what is there
         auto raise = [&](uint32_t tile, int r, float& m) {
             const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + r * 4);
-            const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + (RT * 32 + r) * 4);
+            const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + (MAX_ROWS + r) * 4);
             const float mx = fmaxf(m0, m1), mn = mx - m > T::B + T::SLACK ? mx - T::B : m, f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             return f;
         };
         if (scores) {
             // ================================================================ score waves
-            const int row0 = r0 + 32 * rt + c16;  // this lane's rows: row0, row0 + 16
-            // The queries come through the LDS of tiles t0 + 2 and t0 + 3, a row tile in each, laid out like keys, half of it by
-            // either of its two waves (rows past the end repeat the last one).  (Straight into registers, 64 bytes of 16 rows at a
-            // time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of 64 heads; 1900 and
-            // 4800 so.)
-            int mine[2];
-            const uint32_t qb = lds + (t0 + 2 + rt) % BUFS * TILE_BYTES;
+            const int row0 = r0 + 16 * RT * rw + c16;  // this lane's rows: row0, and with two row tiles row0 + 16
+            // The queries come through the LDS of tiles t0 + 2 and t0 + 3, a row tile in each, laid out like keys, half of a wave's
+            // rows by it and half by the other wave that has them (rows past the end repeat the last one).  (Straight into registers,
+            // 64 bytes of 16 rows at a time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of
+            // 64 heads; 1900 and 4800 so.)
+            int mine[RT];
+            const uint32_t qb = lds + (t0 + 2 + (RT > 1 ? rw : 0)) % BUFS * TILE_BYTES;
             const bool some = n_tiles && row0 - c16 < r1;
+            auto half_of = [&](int x) { return RT > 1 ? x : rw; };  // of the row tile: where rows row0 + 16 x stand
             {
-                uint64_t latent = 0, pe = 0;  // of row 16 kh + c16 of the tile
+                int me = lane;  // (not kept from one segment to the next: there are no registers for it)
+                asm volatile("" : "+v"(me));
+                const int x0 = RT > 1 ? kh : 0, at0 = RT > 1 ? 0 : 8 * kh;  // this wave loads rows row0 - c16 + 16 x0 + at0 ..
+                uint64_t latent = 0, pe = 0;                                // of row row0 + 16 x0
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < RT; ++x) {
                     const int r = min(row0 + 16 * x, r1 - 1), t = r / a.H, h = r - t * a.H;
                     mine[x] = sees(r);
-                    if (x == kh) {
+                    if (x == x0) {
                         latent = (uint64_t)(static_cast<const uint16_t*>(a.q_latent) + t * a.ql_row + h * a.ql_head);
                         pe = (uint64_t)(static_cast<const uint16_t*>(a.q_pe) + t * a.qp_row + h * a.qp_head);
                     }
                 }
                 if (some) {
+                    const uint32_t block = qb + (4 * half_of(x0) + at0 / 4) * (4 * BLOCK);
+                    const uint32_t pe_block = qb + TILE_PE + (16 * half_of(x0) + at0) * PE_BYTES;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint64_t from = of_lane(latent, 4 * i + quad) + ((c16 ^ turn(4 * i + quad)) << 4);
-                        const uint32_t to = qb + (4 * kh + i) * (4 * BLOCK);
+                    for (int i = 0; i < 2 * RT; ++i) {
+                        const int t = at0 + 4 * i + (me >> 4);
+                        const uint64_t from = of_lane(latent, t) + (((me & 15) ^ turn(t)) << 4);
+                        const uint32_t to = block + i * (4 * BLOCK);
                         load_block<0>(to, from);
                         load_block<256>(to + BLOCK, from);
                         load_block<512>(to + 2 * BLOCK, from);
                         load_block<768>(to + 3 * BLOCK, from);
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        load_block<0>(qb + TILE_PE + (16 * kh + 8 * i) * PE_BYTES,
-                                      of_lane(pe, 8 * i + (lane >> 3)) + (((lane & 7) ^ swz8(8 * i + (lane >> 3))) << 4));
+                    for (int i = 0; i < RT; ++i) {
+                        const int t = at0 + 8 * i + (me >> 3);
+                        load_block<0>(pe_block + 8 * i * PE_BYTES, of_lane(pe, t) + (((me & 7) ^ swz8(t)) << 4));
+                    }
                 }
             }
             wait_loads<0>();
             lds_barrier();  // the first tile, the queries
-            u32x4 q[2][18] = {};
+            u32x4 q[RT][18] = {};
             if (some)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t at = qb + ra[0] + (x - kh) * (16 * LAT_BYTES), pat = qb + ra[1] + (x - kh) * (16 * PE_BYTES);
+                for (int x = 0; x < RT; ++x) {
+                    const uint32_t at = qb + ra[0] + (half_of(x) - kh) * (16 * LAT_BYTES), pat = qb + ra[1] + (half_of(x) - kh) * (16 * PE_BYTES);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) q[x][16 + i] = lds_read16(pat ^ (i << 6));
                 }
             lds_barrier();  // the queries are in registers
-            float mo[2] = {M_START, M_START}, l[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-            f32x4 s[2] = {};
+            float mo[RT], l[RT] = {}, sum[RT] = {};
+#pragma unroll
+            for (int x = 0; x < RT; ++x) mo[x] = M_START;
+            f32x4 s[RT] = {};
             auto weights = [&](uint32_t tile, int x) {  // of rows row0 + 16 x, relative to mo[x]; leaves their sum
                 float p0[4];
                 sum[x] = 0.f;
@@ -307,21 +317,21 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     p0[r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], sc, -mo[x]));
                     sum[x] += p0[r];
                 }
-                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * rt + kh) * 1024 + x * 512 + c16 * 32 + quad * 8) =
+                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * (RT > 1 ? rw : 0) + kh) * 1024 + half_of(x) * 512 + c16 * 32 + quad * 8) =
                     u32x2{T::pack(p0[0], p0[1]), T::pack(p0[2], p0[3])};
             };
             auto settle = [&](uint32_t tile, u32x4 fl) {  // what the step of `tile` left open
                 if (any(fl)) {
-                    if (__builtin_amdgcn_readfirstlane(rt ? fl[1] | fl[3] : fl[0] | fl[2]))
+                    if (RT == 1 || __builtin_amdgcn_readfirstlane(rw ? fl[1] | fl[3] : fl[0] | fl[2]))
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            l[x] *= raise(tile, 32 * rt + 16 * x + c16, mo[x]);
+                        for (int x = 0; x < RT; ++x) {
+                            l[x] *= raise(tile, 16 * RT * rw + 16 * x + c16, mo[x]);
                             weights(tile, x);
                         }
                     lds_barrier();  // the weights anew
                 }
-                l[0] += sum[0];
-                l[1] += sum[1];
+#pragma unroll
+                for (int x = 0; x < RT; ++x) l[x] += sum[x];
             };
             u32x4 fl = {};
             for (uint32_t tile = t0; tile < stop; ++tile) {
@@ -333,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 auto key = [&](int i) {
                     return i < 16 ? lds_read16(((tb + ra[0]) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tb + ra[1]) ^ ((i - 16) << 6));
                 };
-                f32x4 z[2][2] = {};
+                f32x4 z[RT][2] = {};
                 u32x4 kf[6];
 #pragma unroll
                 for (int i = 0; i < 5; ++i) kf[i] = key(i);
@@ -344,15 +354,15 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     __builtin_amdgcn_sched_barrier(0);
                     if (i + 5 < 18) kf[(i + 5) % 6] = key(i + 5);
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) z[y][i & 1] = T::mfma16(kf[i % 6], q[y][i], z[y][i & 1]);
+                    for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf[i % 6], q[y][i], z[y][i & 1]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) s[x] = z[x][0] + z[x][1];
+                for (int x = 0; x < RT; ++x) s[x] = z[x][0] + z[x][1];
                 const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(there8 != 0);
                 if (k0 + BN > first || there != ~0u) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
+                    for (int x = 0; x < RT; ++x) {
                         const int left = mine[x] - k0;
                         const uint32_t vis = (there & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u)) >> (16 * kh + 4 * quad);
 #pragma unroll
@@ -360,24 +370,24 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                             if (!(vis >> r & 1)) s[x][r] = -INFINITY;
                     }
                 }
-                float mx[2];
+                float mx[RT];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < RT; ++x) {
                     mx[x] = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
                     mx[x] = join_groups(mx[x], [](float p, float q) { return fmaxf(p, q); }) * sc;
-                    *reinterpret_cast<float*>(sm + LDS_MAX + (tile & 1) * 512 + (w * 32 + 16 * x + c16) * 4) = mx[x];  // (the groups' values agree)
+                    *reinterpret_cast<float*>(sm + LDS_MAX + (tile & 1) * 512 + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = mx[x];  // (the groups' values agree)
                     weights(tile, x);
                 }
-                const bool up = __builtin_amdgcn_ballot_w64(fmaxf(mx[0] - mo[0], mx[1] - mo[1]) > T::B + T::SLACK) != 0;
+                const bool up = __builtin_amdgcn_ballot_w64(fmaxf(mx[0] - mo[0], mx[RT - 1] - mo[RT - 1]) > T::B + T::SLACK) != 0;
                 *reinterpret_cast<int*>(sm + LDS_FLAG + (tile & 1) * 16 + w * 4) = up;
                 lds_barrier();  // the tile's weights; the next tile is whole
             }
             if (n_tiles) settle(stop - 1, flags(stop - 1));
             lds_barrier();  // the last maxima are read
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < RT; ++x) {
                 l[x] = join_groups(l[x], [](float p, float q) { return p + q; });
-                if (quad == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (w * 32 + 16 * x + c16) * 4) = l[x];
+                if (quad == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = l[x];
             }
             lds_barrier();
             lds_barrier();  // the value waves have read it
@@ -428,7 +438,9 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         };
 
         f32x16 acc[RT][4] = {};  // [row tile][32 values]
-        float mo[RT] = {M_START, M_START};
+        float mo[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) mo[r] = M_START;
         bool special = false;
         // One step: `tile` added, the value waves' loads of tile + 3 (past the end: zeros) and the addresses of tile + 4 between
         // the products.  LAST: nothing is brought.
@@ -454,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             if (any(fl)) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    if (!__builtin_amdgcn_readfirstlane(fl[r] | fl[r + RT])) continue;
+                    if (RT > 1 && !__builtin_amdgcn_readfirstlane(fl[r] | fl[r + 2])) continue;
                     const float f = raise(tile, 32 * r + c, mo[r]);
                     if (tile != t0)  // (nothing is there yet)
 #pragma unroll
@@ -571,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
         for (int r = 0; r < RT; ++r)
             ls[r] = *reinterpret_cast<const float*>(sm + LDS_MAX + (r * 32 + c) * 4) +
-                    *reinterpret_cast<const float*>(sm + LDS_MAX + ((r + RT) * 32 + c) * 4);
+                    *reinterpret_cast<const float*>(sm + LDS_MAX + (MAX_ROWS + r * 32 + c) * 4);
         lds_barrier();  // free for the next segment
         if (whole) {
 #pragma unroll
@@ -739,9 +751,18 @@ int check_decode_sizes(const KdaLatentDecodeArgs* a) {
 
 Plan plan_of(const KdaLatentDecodeArgs* a) {
     Plan p;
-    p.own = Groups::of((int64_t)a->S * a->H);
-    p.pre = a->prefix_width ? Groups::of((int64_t)a->B * a->S * a->H) : Groups{32, 0};
     const int cus = a->num_cus ? a->num_cus : 256;
+    // Groups of 64 rows read the keys least often.  Of 32 rows, and with a kernel for one row tile, whose steps are shorter (about 1400
+    // cycles instead of 2000), where even tables full of tokens leave workgroups over: 8 sequences of 12 heads behind 2000 shared
+    // tokens 15.2 us instead of 17.1.
+    const int64_t rows = (int64_t)a->S * a->H, own = a->B * (((int64_t)a->table_width * a->page_size + BN - 1) / BN + LEAD);
+    const int64_t pre = ((int64_t)a->prefix_width * a->page_size + BN - 1) / BN;
+    auto plan = [&](int most) {
+        p.own = Groups::of(rows, most);
+        p.pre = a->prefix_width ? Groups::of(a->B * rows, most) : Groups{32, 0};
+        return p.own.groups * ((own + MIN_RUN - 1) / MIN_RUN) + p.pre.groups * ((pre + MIN_RUN - 1) / MIN_RUN);
+    };
+    if (plan(32) > cus) plan(MAX_ROWS);
     p.grid = cus > p.own.groups + p.pre.groups ? cus : p.own.groups + p.pre.groups;
     p.per_wg = 1.f / p.grid;
     p.pre_slots = p.pre.groups ? p.grid : 0;
@@ -791,7 +812,10 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     const bool few = (int64_t)join * tiles * 16 <= p.grid;  // blocks of rows and values: likely many parts each
     auto launch = [&](auto type) {
         typedef decltype(type) T;
-        hipLaunchKernelGGL(decode_kernel<T>, dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+        if (p.own.rows > 32 || p.pre.rows > 32)  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
+            hipLaunchKernelGGL((decode_kernel<T, 2>), dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+        else
+            hipLaunchKernelGGL((decode_kernel<T, 1>), dim3(p.grid), dim3(THREADS), 0, s, *a, p);
         if (few)
             hipLaunchKernelGGL((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), 0, s, *a, p);
         else

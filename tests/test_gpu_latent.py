@@ -323,6 +323,15 @@ class Absorbed:
         return o, lse
 
 
+    def widen(self, entries=1 << 20):
+        """Tables with room for many more tokens: the work is grouped for long lists of pages."""
+        pad = torch.full((len(self.lens), entries // self.size // len(self.lens)), -1, dtype=torch.int32)
+        self.table = torch.cat([self.table, pad], dim=1)
+        if self.prefix_table is not None:
+            self.prefix_table = torch.cat([self.prefix_table, torch.full((entries // self.size,), -1, dtype=torch.int32)])
+        return self
+
+
 DECODE = [
     ([1], 1, 1, 1), ([1], 1, 12, 16), ([2, 31, 32, 33], 1, 4, 16), ([63, 64, 65, 127, 128, 129], 1, 16, 64),
     ([0, 5, 0, 300], 1, 12, 64), ([1000], 1, 32, 272), ([500, 3], 1, 33, 100), ([700, 40], 1, 64, 64), ([290], 1, 96, 16),
@@ -336,6 +345,12 @@ DECODE = [
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_decode_lengths(lens, S, H, size, dtype):
     Absorbed(lens, S, H, size, dtype).check()
+
+
+@pytest.mark.parametrize("lens,S,H,size", DECODE, ids=[f"{len(c[0])}seq-{max(c[0])}-S{c[1]}-H{c[2]}-p{c[3]}" for c in DECODE])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_lengths_in_wide_tables(lens, S, H, size, dtype):
+    Absorbed(lens, S, H, size, dtype).widen().check()
 
 
 @pytest.mark.parametrize("lens,S,H,size", [([400, 90], 1, 12, 64), ([130, 77, 1], 4, 16, 16), ([513], 1, 128, 100)])
@@ -370,6 +385,21 @@ def test_decode_score_ranges(kind, H, dtype):
     flat[1500:] = float("nan")
     x.cache[rows] = flat.view(24, 64, ROW)
     x.check()
+
+
+@pytest.mark.parametrize("kind", ["rising", "spike_first", "spike_last"])
+@pytest.mark.parametrize("H,dtype", [(2, BF), (40, HF), (100, BF)])
+def test_decode_score_ranges_in_wide_tables(kind, H, dtype):
+    x = Absorbed([1500], 1, H, 64, dtype)
+    rows = x.table[0, :24].long()
+    flat = x.cache[rows].reshape(-1, ROW)
+    x.qp[..., 0] = 8.0 if kind == "rising" else 16.0
+    flat[:, LAT] = (torch.arange(24 * 64) / 16).to(dtype) if kind == "rising" else 0.0
+    if kind != "rising":
+        flat[0 if kind == "spike_first" else 1400, LAT] = 24.0
+    flat[1500:] = float("nan")
+    x.cache[rows] = flat.view(24, 64, ROW)
+    x.widen().check()
 
 
 def test_decode_fp16_many_small_weights():
@@ -422,6 +452,27 @@ def test_decode_later_draft_tokens_do_not_matter(value, H, S):
     for n in range(3):
         a, b = n * S, (n + 1) * S - 1
         assert torch.equal(o[a:b], o2[a:b]) and torch.equal(lse[a:b], lse2[a:b])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("H,S", [(4, 3), (40, 2), (96, 4)])
+def test_decode_later_draft_tokens_do_not_matter_in_wide_tables(value, H, S):
+    x = Absorbed([130, 64, 33], S, H, 16, BF).widen()
+    o, lse = x.check()
+    for n in range(3):
+        j = x.lens[n] - 1
+        x.cache[int(x.table[n, j // 16]), j % 16, 7] = value
+    o2, lse2 = x.run()
+    for n in range(3):
+        a, b = n * S, (n + 1) * S - 1
+        assert torch.equal(o[a:b], o2[a:b].cpu()) and torch.equal(lse[a:b], lse2[a:b].cpu())
+
+
+@pytest.mark.parametrize("lens,S,H,size,prefix", [
+    ([1, 33, 64], 1, 12, 16, 100), ([5, 0, 300], 1, 12, 64, 1000), ([40, 7], 2, 96, 64, 129), ([10, 20, 30], 1, 128, 272, 500),
+    ([12] * 40, 1, 4, 16, 257), ([50, 60], 1, 8, 16, 0), ([0, 2], 3, 8, 16, 0)])
+def test_decode_prefix_in_wide_tables(lens, S, H, size, prefix):
+    Absorbed(lens, S, H, size, BF, prefix=prefix).widen().check()
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])

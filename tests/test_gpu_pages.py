@@ -206,6 +206,15 @@ def test_free(rows, width, pages, live, seed):
     assert d.lens.tolist() == book.lens
 
 
+def test_free_few_of_many_pages():
+    rng = random.Random(7)
+    book, _ = _make(rng, 8, 5, 16, 40000, 30, layers=0)
+    d = _Device(book)
+    kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, _i32([1, 6, 3]), 16)
+    book.release([1, 6, 3])
+    d.same(book)
+
+
 @pytest.mark.parametrize("rows,size", [(20, 4), (300, 4)])
 @pytest.mark.parametrize("extra", [0, 1, 200])
 def test_free_shared_by_many(rows, size, extra):
