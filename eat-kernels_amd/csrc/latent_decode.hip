@@ -813,13 +813,13 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     auto launch = [&](auto type) {
         typedef decltype(type) T;
         if (p.own.rows > 32 || p.pre.rows > 32)  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
-            hipLaunchKernelGGL((decode_kernel<T, 2>), dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+            launch_kernel((decode_kernel<T, 2>), dim3(p.grid), dim3(THREADS), s, *a, p);
         else
-            hipLaunchKernelGGL((decode_kernel<T, 1>), dim3(p.grid), dim3(THREADS), 0, s, *a, p);
+            launch_kernel((decode_kernel<T, 1>), dim3(p.grid), dim3(THREADS), s, *a, p);
         if (few)
-            hipLaunchKernelGGL((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), 0, s, *a, p);
+            launch_kernel((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), s, *a, p);
         else
-            hipLaunchKernelGGL((join_kernel<T, false>), dim3(join, tiles * 4), dim3(256), 0, s, *a, p);
+            launch_kernel((join_kernel<T, false>), dim3(join, tiles * 4), dim3(256), s, *a, p);
     };
     if (a->dtype == KDA355_DTYPE_BF16) launch(Bf16{}); else launch(Fp16{});
     const hipError_t e = hipGetLastError();

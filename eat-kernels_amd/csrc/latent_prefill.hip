@@ -523,8 +523,8 @@ extern "C" int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* a, kda35
     const dim3 join(p.slots / 2 < 1 ? 1 : min(p.slots / 2, p.share), WAVES);  // a split row tile has two parts at least
     auto launch = [&](auto type) {
         typedef decltype(type) T;
-        hipLaunchKernelGGL(prefill_kernel<T>, dim3(p.grid), dim3(WAVES * 64), 0, s, *a, p);
-        hipLaunchKernelGGL(join_kernel<T>, join, dim3(256), 0, s, *a, p);
+        launch_kernel(prefill_kernel<T>, dim3(p.grid), dim3(WAVES * 64), s, *a, p);
+        launch_kernel(join_kernel<T>, join, dim3(256), s, *a, p);
     };
     if (a->dtype == KDA355_DTYPE_BF16) launch(Bf16{}); else launch(Fp16{});
     const hipError_t e = hipGetLastError();

@@ -452,7 +452,7 @@ extern "C" int kda355_latent_append_launch(const KdaLatentTokensArgs* a, kda355_
     KDA_CHECK_ARG(aligned(a->latent, 16) && aligned(a->k_pe, 16) && a->latent_row % 8 == 0 && a->pe_row % 8 == 0,
                   "latent_append: latent and k_pe rows must be 16-byte aligned");
     const int64_t wgs = (a->T + TOKENS - 1) / TOKENS;
-    hipLaunchKernelGGL(append_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
+    launch_kernel(append_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), reinterpret_cast<hipStream_t>(stream), *a);
     return launched("latent_append");
 }
 
@@ -464,7 +464,7 @@ extern "C" int kda355_latent_gather_launch(const KdaLatentTokensArgs* a, kda355_
     KDA_CHECK_ARG(a->block_table && a->cu && a->out, "latent_gather: a required pointer is null");
     KDA_CHECK_ARG(aligned(a->out, 16) && a->out_row % 8 == 0, "latent_gather: out rows must be 16-byte aligned");
     const int64_t wgs = (a->T + TOKENS - 1) / TOKENS;
-    hipLaunchKernelGGL(gather_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), 0, reinterpret_cast<hipStream_t>(stream), *a);
+    launch_kernel(gather_kernel, dim3((uint32_t)wgs), dim3(TOK_THREADS), reinterpret_cast<hipStream_t>(stream), *a);
     return launched("latent_gather");
 }
 
@@ -475,8 +475,8 @@ extern "C" int kda355_copy_rows_launch(const KdaPagesArgs* a, kda355_stream_t st
     KDA_CHECK_ARG(a->n >= 0 && a->n < MAX_PAIRS, "copy_rows: n=%d", a->n);
     if (a->n == 0 || a->num_pools == 0) return 0;
     KDA_CHECK_ARG(a->src && a->dst, "copy_rows: a required pointer is null");
-    hipLaunchKernelGGL(copy_rows_kernel, dim3(a->n, segs, a->num_pools), dim3(COPY_THREADS), 0,
-                       reinterpret_cast<hipStream_t>(stream), *a);
+    launch_kernel(copy_rows_kernel, dim3(a->n, segs, a->num_pools), dim3(COPY_THREADS),
+                  reinterpret_cast<hipStream_t>(stream), *a);
     return launched("copy_rows");
 }
 
@@ -489,8 +489,8 @@ extern "C" int kda355_fork_pages_launch(const KdaPagesArgs* a, kda355_stream_t s
     if (a->n == 0) return 0;
     KDA_CHECK_ARG(a->src && a->dst && a->workspace, "fork_pages: a required pointer is null");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(fork_take_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
-    hipLaunchKernelGGL(fork_rows_kernel, dim3(a->n, segs, a->num_pools + 1), dim3(COPY_THREADS), 0, s, *a);
+    launch_kernel(fork_take_kernel, dim3(1), dim3(SCAN_THREADS), s, *a);
+    launch_kernel(fork_rows_kernel, dim3(a->n, segs, a->num_pools + 1), dim3(COPY_THREADS), s, *a);
     return launched("fork_pages");
 }
 
@@ -502,11 +502,11 @@ extern "C" int kda355_free_pages_launch(const KdaPagesArgs* a, kda355_stream_t s
     KDA_CHECK_ARG(a->src, "free_pages: a required pointer is null");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if ((int64_t)a->n * a->table_width <= FREE_SMALL && a->pages <= FREE_PAGES) {
-        hipLaunchKernelGGL(free_small_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+        launch_kernel(free_small_kernel, dim3(1), dim3(SCAN_THREADS), s, *a);
         return launched("free_pages");
     }
-    hipLaunchKernelGGL(free_rows_kernel, dim3(a->n), dim3(COPY_THREADS), 0, s, *a);
-    hipLaunchKernelGGL(free_push_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+    launch_kernel(free_rows_kernel, dim3(a->n), dim3(COPY_THREADS), s, *a);
+    launch_kernel(free_push_kernel, dim3(1), dim3(SCAN_THREADS), s, *a);
     return launched("free_pages");
 }
 
@@ -517,8 +517,8 @@ extern "C" int kda355_compact_pages_launch(const KdaPagesArgs* a, kda355_stream_
     if (const int rc = check_table(a, "compact_pages", false)) return rc;
     KDA_CHECK_ARG(a->workspace, "compact_pages: a required pointer is null");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(SCAN_THREADS), 0, s, *a);
+    launch_kernel(compact_plan_kernel, dim3(1), dim3(SCAN_THREADS), s, *a);
     const int half = a->pages / 2;
-    hipLaunchKernelGGL(compact_move_kernel, dim3(half < 1 ? 1 : half, segs, a->num_pools + 1), dim3(COPY_THREADS), 0, s, *a);
+    launch_kernel(compact_move_kernel, dim3(half < 1 ? 1 : half, segs, a->num_pools + 1), dim3(COPY_THREADS), s, *a);
     return launched("compact_pages");
 }

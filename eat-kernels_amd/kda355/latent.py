@@ -189,7 +189,7 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
         plan = _keep(_prefill_seen, key, _plan_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale, causal, out, lse))
     dev, dt, shape, need, mid, tail = plan
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=dt, device=dev)  # (0.4 us less than empty)
     ws = _workspace(need, workspace, dev)
     args = (_PTR8.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(),
                        0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()) + mid +
@@ -262,7 +262,7 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
                                                      prefix_len))
     dev, dt, shape, need, tail = plan
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=dt, device=dev)  # (0.4 us less than empty)
     ws = _workspace(need, workspace, dev)
     args = (_PTR10.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
                         0 if prefix_table is None else prefix_table.data_ptr(),
