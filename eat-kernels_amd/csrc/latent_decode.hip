@@ -14,12 +14,14 @@
 // instructions of one kind run beside the softmax, the waits and the address arithmetic of the other.  One barrier a tile.
 // Scores come from 16x16x32 instructions (keys as rows), so that every key fragment read serves two of them; values from
 // 32x32x16 with one fragment for both row tiles.
+// With one row tile a group (RT = 1) a score wave has rows 16 (w % 2) .. + 15 of it and everything of a row is there once.
 //
 // Bound: with many rows of few sequences the two products, 576 and 512 cycles of a SIMD's matrix core a tile; a step takes about 1900,
 // with LDS (160 KiB read and written a step) and the instructions of the longer kind of wave behind them.  16 sequences of 6000 to
 // 9900 tokens, 8 draft tokens, 96 heads: 248 us, 0.86 PFLOP/s; 64 sequences of 32 heads behind 32768 shared tokens: 163 us, 0.91
-// PFLOP/s.  With a row tile or two a sequence HBM: 64 ragged sequences, 64 heads, 129 us, 4.25 TB/s.  One sequence of 4097 tokens, 12
-// heads: 15.5 us, 10.5 of it this kernel (lengths and cut 2.2, queries and first tile 2.3, three tiles and the end 4.5) and 5 the join.
+// PFLOP/s.  With a row tile or two a sequence HBM: 64 ragged sequences, 64 heads, 128 us, 4.3 TB/s.  One sequence of 4097 tokens, 12
+// heads: 13.9 us from a graph, 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5
+// the join.
 // Eight waves of one kind with the value dimensions split: 141 / 296 / 234 us instead of 142 / 260 / 227; four of one kind, one a SIMD,
 // pipelined: 142 / 276 / 264 (64 ragged, drafts, shared prefix).
 #include <type_traits>
@@ -37,8 +39,7 @@ constexpr int LOADS = 10;                               // of a value wave a til
 constexpr int MAX_ROWS = 64;                            // query rows of a group
 // The cut is by cost: beginning a sequence (lengths, queries, page numbers and first tile one after the other) takes about as
 // long as LEAD tiles, which stand in front of every sequence's own; a run is MIN_RUN of these units at least.  Measured: 64
-// ragged sequences 146 us without LEAD, 142 with 3, 136 with 8 and with 16; 64 short ones behind 32768 tokens 230, 202, 190 and
-// 190; one sequence of 4097 tokens 20.3 us with runs of 1, 17.9 of 3, 18.5 of 4.
+// ragged sequences 138 us with LEAD 4, 134 with 6 and with 8; one sequence of 4097 tokens 14.4 us with runs of 2, 13.9 of 3, 14.3 of 4.
 constexpr uint32_t LEAD = 8, MIN_RUN = 3;
 // workspace: the cut for the second kernel (run, runs of the prefix), then slots, of 32 rows: accumulators, (m, l) of each row
 constexpr int SLOTS = 256, SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;
@@ -627,7 +628,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 
 // ------------------------------------------------------------------------------------------------ joining the parts
 // For 32 rows and 32 values of a sequence, two parts at a time.  SPLIT: a workgroup of 16 waves, wave v takes the parts v, v + 16,
-// ..., and their sums meet in LDS (few rows with many parts: one sequence in 44 parts 5.4 us, in 4 waves 7.4).  Otherwise every one
+// ..., and their sums meet in LDS (few rows with many parts: one sequence in 44 parts 5.4 us, in 4 waves 7.4; 4.5 where the
+// cut is read and not found again).  Otherwise every one
 // of 4 waves has a block of 32 values of its own and all parts (4096 rows: 11.2 us; with four waves to a block as above 12.4, much of it
 // for finding out what there is to do).
 template <typename T, bool SPLIT>
