@@ -125,12 +125,12 @@ __device__ __forceinline__ At sequence_of(const Lengths& lens, uint32_t u) {
 // ------------------------------------------------------------------------------------------------ LDS
 // A tile: latent rows in blocks of 4 tokens x 16 pieces of 16 bytes, piece p of token t at block 4 (t / 4) + p / 16, row t % 4,
 // place (p % 16) ^ turn(t) (a block is one load of a wave); then the positional parts, piece p of token t at p ^ swz8(t).
-// 16-byte reads go 16 lanes at a time, lanes 0 .. 3, 12 .. 15, 20 .. 23, 24 .. 27 of 32 and the others, transposed reads 16 lanes
-// in order: with this turn the former touch all 16 places of 256 bytes (4 cycles each; 8 with other turns that were measured) and the
-// latter all 8 of 128.
-__device__ __forceinline__ int turn(int t) { return (t & 3) << 1 | (t >> 3 & 1) | ((t >> 2 ^ t >> 3) & 1) << 3; }
+// 16-byte reads go 16 lanes at a time, lanes 0 .. 3, 12 .. 15, 20 .. 23, 24 .. 27 of 32 and the others, transposed reads 32 lanes in
+// order: with this turn the former touch all 16 places of 256 bytes, and so do the latter.  (A turn that serves the former alone
+// and weights without their turn: 35 % more LDS cycles, 1 % more time.)
+__device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) << 1; }
 constexpr int BLOCK = 1024, TILE_PE = BN * LAT_BYTES, TILE_BYTES = TILE_PE + BN * PE_BYTES;
-constexpr int LDS_P = BUFS * TILE_BYTES;             // weights: [tile % 2][row tile][16-key step][row][key] 16 bits
+constexpr int LDS_P = BUFS * TILE_BYTES;             // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
 constexpr int LDS_MAX = LDS_P + 2 * 4096;            // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
 constexpr int LDS_FLAG = LDS_MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
 constexpr int LDS_THERE = LDS_FLAG + 64;             // is the token there [tile % 4][32] bytes
@@ -318,7 +318,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     p0[r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], sc, -mo[x]));
                     sum[x] += p0[r];
                 }
-                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * (RT > 1 ? rw : 0) + kh) * 1024 + half_of(x) * 512 + c16 * 32 + quad * 8) =
+                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * (RT > 1 ? rw : 0) + kh) * 1024 + half_of(x) * 512 + c16 * 32 +
+                                          (quad ^ (c16 >> 3) << 1) * 8) =
                     u32x2{T::pack(p0[0], p0[1]), T::pack(p0[2], p0[3])};
             };
             auto settle = [&](uint32_t tile, u32x4 fl) {  // what the step of `tile` left open
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         auto step = [&](uint32_t tile, auto last_) {
             constexpr bool LAST = decltype(last_)::value;
             const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
-            const uint32_t vb = lds + (tile % BUFS) * TILE_BYTES, pb = lds + LDS_P + (tile & 1) * 4096 + c * 32 + half * 16;
+            const uint32_t vb = lds + (tile % BUFS) * TILE_BYTES, pb = lds + LDS_P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
             auto value = [&](int k, int d) {
                 const u32x2 v0 = lds_read_tr(((vb + ra[0]) ^ (d << 6)) + k * 16 * BLOCK);
                 const u32x2 v1 = lds_read_tr(((vb + ra[1]) ^ (d << 6)) + k * 16 * BLOCK);
