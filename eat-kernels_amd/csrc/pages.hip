@@ -157,7 +157,8 @@ __device__ __forceinline__ int row_len(const KdaPagesArgs& a, int row) {
 }
 
 // pair i -> workspace[i] = page to copy from (-1: none), workspace[n + i] = page taken (-1: none needed, -2: no page
-// left, -3: pair skipped).  The stack and its height follow.
+// left, -3: pair skipped).  A part-filled last page that is a hole needs none: a page taken for it would hold what its last
+// owner left, and the child would see it.  The stack and its height follow.
 __global__ void __launch_bounds__(SCAN_THREADS) fork_take_kernel(KdaPagesArgs a) {
     __shared__ int sw[SCAN_THREADS / 64];
     int top = a.num_free[0];
@@ -165,13 +166,13 @@ __global__ void __launch_bounds__(SCAN_THREADS) fork_take_kernel(KdaPagesArgs a)
     int taken = 0;
     for (int i0 = 0; i0 < a.n; i0 += SCAN_THREADS) {
         const int i = i0 + threadIdx.x;
-        int par = -1, len = 0, ok = 0, tail = 0;
+        int ok = 0, tail = 0, last = -1;  // is the parent's last page part-filled and there; that page
         if (i < a.n) {
-            par = a.src[i];
-            const int child = a.dst[i];
+            const int par = a.src[i], child = a.dst[i];
             ok = par >= 0 && par < a.rows && child >= 0 && child < a.rows && par != child;
-            if (ok) len = row_len(a, par);
-            tail = ok && len % a.page_size != 0;
+            const int len = ok ? row_len(a, par) : 0;
+            if (len % a.page_size != 0) last = a.block_table[par * a.table_stride + len / a.page_size];
+            tail = last >= 0 && last < a.pages;
         }
         int total;
         const int rank = taken + block_scan(tail, sw, total);
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) fork_take_kernel(KdaPagesArgs a)
                     a.free_pages[top - 1 - rank] = -1;
                     if (page >= 0 && page < a.pages) {
                         to = page;
-                        from = a.block_table[par * a.table_stride + len / a.page_size];
+                        from = last;
                     }
                 }
             }

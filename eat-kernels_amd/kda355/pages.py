@@ -159,9 +159,10 @@ def copy_rows(pools, src, dst):
 
 def fork_pages(pools, block_table, seq_lens, ref_counts, free_pages, num_free, parents, children, page_size):
     """Sequence children[i] becomes a copy of parents[i] (int32 [n] rows of block_table): full pages are shared, a part-filled
-    last page is copied in every pool to a page from the stack.  Where the stack is empty the child gets length 0 and no
-    pages.  What a child row held before is overwritten, not released (free_pages() first).  Pairs outside the table are
-    skipped; children must differ from one another and from every parent."""
+    last page is copied in every pool to a page from the stack.  Holes stay holes: a part-filled last page that is one takes no
+    page.  Where the stack is empty the child gets length 0 and no pages.  What a child row held before is overwritten, not
+    released (free_pages() first).  Pairs outside the table are skipped; children must differ from one another and from every
+    parent."""
     pools = _sequence(pools)
     dev, pages, stride, rows, width, size, ps = _check(
         "fork_pages", page_size, pools, block_table, ref_counts, free_pages, num_free, seq_lens, parents=parents, children=children)

@@ -422,9 +422,9 @@ typedef struct KdaPagesArgs {
    pair's src or dst. */
 int kda355_copy_rows_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 /* Sequence dst[i] becomes a copy of src[i], in the order of i: its full pages are shared, a part-filled last page is copied
-   in every pool to a page taken from the stack.  Where the stack is empty, the child gets length 0 and no pages.  What the
-   child row held before is overwritten, not released.  Pairs outside [0, rows) are skipped; children must differ from one
-   another and from every parent. */
+   in every pool to a page taken from the stack.  Holes stay holes: a part-filled last page that is one takes no page.  Where
+   the stack is empty, the child gets length 0 and no pages.  What the child row held before is overwritten, not released.
+   Pairs outside [0, rows) are skipped; children must differ from one another and from every parent. */
 int kda355_fork_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 /* Sequences src[i] (all different) give up the pages of their seq_lens tokens; rows become holes, lengths 0.  Pages that
    nobody holds any more go onto the stack, the highest first. */

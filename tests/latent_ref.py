@@ -129,7 +129,7 @@ class Book:
                 continue
             n = self._length(p)
             full, new = n // self.size, None
-            if n % self.size:
+            if n % self.size and 0 <= self.table[p][full] < pages:  # (a hole stays one: there is nothing to copy)
                 new = -2
                 if self.num > 0:
                     self.num -= 1
@@ -147,8 +147,7 @@ class Book:
                 if 0 <= g < pages:
                     self.refs[g] += 1
             if new is not None:
-                if 0 <= self.table[p][full] < pages:
-                    self.moves.append((self.table[p][full], new))
+                self.moves.append((self.table[p][full], new))
                 self.refs[new] = 1
                 row = row + [new]
             self.table[c], self.lens[c] = row + [-1] * (width - len(row)), n

@@ -356,3 +356,41 @@ def test_refused_after_a_like_call_was_taken():
         kda355.latent_append(_random((1026,), torch.bfloat16, 1)[1:1025].view(2, 512), pe, cache, slots)
     with pytest.raises(TypeError):
         kda355.latent_gather(cache, d.table, torch.zeros(5, dtype=torch.int64, device=DEV), out)
+
+
+@pytest.mark.parametrize("hole", [-1, -7, 6, 10 ** 6])
+def test_fork_with_a_hole_as_last_page(hole):
+    """A part-filled last page outside the pool: the child has a hole there too and no page is taken for it, so that the
+    child sees what its parent sees, and not what some page's last owner left."""
+    size, pages = 16, 6
+    d = _Device(Book([[0, hole, -1], [2, 3, -1], [9, 9, 9], [9, 9, 9], [9, 9, 9]], [20, 24, 5, 5, 5], [1, 0, 1, 1, 0, 0],
+                     [5, 4, 1, -1, -1, -1], 3, size))
+    pools = [_random((pages, size, ROW), torch.bfloat16, 60 + i) for i in range(2)]
+    pools[0][:] = torch.randn(pages, size, ROW, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    before = [_bits(t).cpu().clone() for t in pools]
+    kda355.fork_pages(pools, d.table, d.lens, d.refs, d.free, d.num, _i32([0, 1, 0]), _i32([2, 3, 4]), size)
+    assert d.table.tolist() == [[0, hole, -1], [2, 3, -1], [0, -1, -1], [2, 1, -1], [0, -1, -1]]
+    assert d.lens.tolist() == [20, 24, 20, 24, 20]
+    assert d.refs.tolist() == [3, 1, 2, 1, 0, 0]
+    assert d.free.tolist() == [5, 4, -1, -1, -1, -1] and d.num.tolist() == [2]
+    _contents(pools, before, [(3, 1)])
+    g = torch.Generator().manual_seed(6)
+    ql, qp = (torch.randn(1, 4, n, generator=g).to(torch.bfloat16).to(DEV) for n in (512, 64))
+    seen = [kda355.latent_decode(ql, qp, pools[0], d.table[r:r + 1].contiguous(), d.lens[r:r + 1].contiguous()) for r in range(5)]
+    assert torch.isfinite(seen[0]).all()
+    for parent, child in ((0, 2), (1, 3), (0, 4)):
+        assert torch.equal(seen[parent], seen[child])
+
+
+def test_fork_holes_do_not_use_up_the_stack():
+    """Two pages left, three forks that need one among four whose last page is a hole: the pages go to the first two."""
+    size = 8
+    book = Book([[0, 1], [2, -1]] + [[-1, -1]] * 7, [12, 12] + [0] * 7, [1, 1, 1, 0, 0], [4, 3, -1, -1, -1], 2, size)
+    d = _Device(book)
+    pools = [_random((5, size, ROW), torch.float16, 70)]
+    before = [_bits(t).cpu().clone() for t in pools]
+    kda355.fork_pages(pools, d.table, d.lens, d.refs, d.free, d.num, _i32([1, 0, 1, 1, 0, 0, 1]), _i32([2, 3, 4, 5, 6, 7, 8]), size)
+    assert d.table.tolist()[2:] == [[2, -1], [0, 3], [2, -1], [2, -1], [0, 4], [-1, -1], [2, -1]]
+    assert d.lens.tolist()[2:] == [12, 12, 12, 12, 12, 0, 12]
+    assert d.refs.tolist() == [3, 1, 5, 1, 1] and d.free.tolist() == [-1] * 5 and d.num.tolist() == [0]
+    _contents(pools, before, [(1, 3), (1, 4)])
