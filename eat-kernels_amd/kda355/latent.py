@@ -162,7 +162,7 @@ def _plan_prefill(q, k, v, k_pe, cu_q, cu_k, scale, causal, out, lse):
     if lse is not None:
         _index("lse", lse, (Tq, H), dev, torch.float32)
     a = _lib.KdaLatentPrefillArgs(*[None] * 8, *strides, Tq, Tk, None, 0, N, H, _DTYPES[dt], 1 if causal else 0,
-                                  SCALE if scale is None else float(scale), _num_cus(dev))
+                                  scale, _num_cus(dev))
     b, at = bytes(a), _lib.KdaLatentPrefillArgs.workspace.offset
     return dev, dt, (Tq, H, HEAD), _bytes_needed("latent_prefill", a), b[_PTR8.size:at], b[at + 16:]
 
@@ -177,6 +177,7 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
 
     workspace: uint8 tensor of latent_prefill_workspace_bytes(...); by default one is taken from torch's allocator for the
     call.  Calls that may overlap need workspaces of their own."""
+    scale, causal = SCALE if scale is None else float(scale), bool(causal)  # (what is kept is keyed by their values)
     try:
         key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype,
                v.device, k_pe.shape, k_pe.stride(), k_pe.dtype, k_pe.device, cu_seqlens_q.shape, cu_seqlens_q.stride(),
@@ -232,7 +233,7 @@ def _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, 
     if lse is not None:
         _index("lse", lse, (T, H), dev, torch.float32)
     a = _lib.KdaLatentDecodeArgs(*[None] * 10, *strides, page_stride, pages, table_stride, 0, B, S, H, size, block_table.shape[1],
-                                 width, _DTYPES[dt], _num_cus(dev), SCALE if scale is None else float(scale), 0)
+                                 width, _DTYPES[dt], _num_cus(dev), scale, 0)
     a.workspace_bytes = need = _bytes_needed("latent_decode", a)
     return dev, dt, (T, H, LATENT), need, bytes(a)[_PTR10.size:]
 
@@ -249,6 +250,7 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
 
     workspace: uint8 tensor of latent_decode_workspace_bytes(...); by default one is taken from torch's allocator for the
     call.  Calls that may overlap need workspaces of their own."""
+    scale = SCALE if scale is None else float(scale)  # (what is kept is keyed by its value)
     try:
         key = (q_latent.shape, q_latent.stride(), q_latent.dtype, q_latent.device, q_pe.shape, q_pe.stride(), q_pe.dtype,
                q_pe.device, cache.shape, cache.stride(), cache.dtype, cache.device, block_table.shape, block_table.stride(),

@@ -677,3 +677,24 @@ def test_refused_after_a_like_call_was_taken():
     for bad in (dict(cache=args["cache"].half()), dict(seq_lens=_i32([20, 5]).float()), dict(q_pe=a.qp)):
         with pytest.raises(TypeError):
             kda355.latent_decode(**{**args, **bad})
+
+
+def test_a_scale_that_is_written_again_counts_anew():
+    """A scale may be given as anything that float() takes: its value at the call is the one that counts, and nothing that
+    is kept from one call for the next holds on to it."""
+    x, a = Expanded([9], [20], 2, BF), Absorbed([20, 5], 1, 4, 16, BF, prefix=30)
+    s, flag = torch.tensor(0.25), torch.tensor(True)
+    for value in (0.25, 0.03125, 0.25):
+        s.fill_(value)
+        for run in (lambda z: x.run(scale=z), lambda z: a.run(scale=z)):
+            (o, lse), (o2, lse2) = run(s), run(value)
+            assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    for value in (True, False, True):
+        flag.fill_(value)
+        (o, lse), (o2, lse2) = x.run(flag), x.run(value)
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    for seen in (kda355.latent._prefill_seen, kda355.latent._decode_seen):
+        assert not any(isinstance(part, torch.Tensor) for key in seen for part in key)
+    for bad in ("much", [1.0]):
+        with pytest.raises((TypeError, ValueError)):
+            x.run(scale=bad)
