@@ -122,6 +122,7 @@ def _book(block_table, ref_counts, free_pages, num_free):
 
 def _check(name, page_size, pools, block_table, ref_counts, free_pages, num_free, seq_lens=None, **rows):
     """The checks of a bookkeeping call, or what they found for the like of it before."""
+    page_size = int(page_size)  # (what is kept is keyed by its value)
     try:
         key = _key(name, page_size, pools, (block_table, ref_counts, free_pages, num_free, *rows.values()) +
                    (() if seq_lens is None else (seq_lens,)))
@@ -140,7 +141,7 @@ def _check(name, page_size, pools, block_table, ref_counts, free_pages, num_free
         for what, t in rows.items():
             n = t.numel() if n is None and isinstance(t, torch.Tensor) else n or 0
             _index(what, t, (n,), dev)
-        plan = _keep(_seen, key, found + (int(page_size), ps))
+        plan = _keep(_seen, key, found + (page_size, ps))
     return plan
 
 

@@ -394,3 +394,25 @@ def test_fork_holes_do_not_use_up_the_stack():
     assert d.lens.tolist()[2:] == [12, 12, 12, 12, 12, 0, 12]
     assert d.refs.tolist() == [3, 1, 5, 1, 1] and d.free.tolist() == [-1] * 5 and d.num.tolist() == [0]
     _contents(pools, before, [(1, 3), (1, 4)])
+
+
+def test_a_page_size_that_is_written_again_counts_anew():
+    """A page size may be given as anything that int() takes: its value at the call is the one that counts, and nothing that
+    is kept from one call for the next holds on to it."""
+    size = torch.tensor(4)
+    for value in (4, 8, 4):
+        size.fill_(value)
+        book, pools = _make(random.Random(12), 6, 5, value, 30, 12)
+        book.table[4], book.lens[4], book.table[5], book.lens[5] = [-1] * 5, 0, [-1] * 5, 0
+        pools = [_random((30, 8, ROW), torch.bfloat16, 80)]  # (the same shape for either size)
+        before = [_bits(t).cpu().clone() for t in pools]
+        d = _Device(book)
+        kda355.fork_pages(pools, d.table, d.lens, d.refs, d.free, d.num, _i32([0, 1]), _i32([4, 5]), size)
+        book.fork([0, 1], [4, 5])
+        d.same(book)
+        _contents(pools, before, book.moves)
+        kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, _i32([1, 2]), size)
+        book.release([1, 2])
+        d.same(book)
+        assert d.lens.tolist() == book.lens
+    assert not any(isinstance(part, torch.Tensor) for key in kda355.pages._seen for part in key)
