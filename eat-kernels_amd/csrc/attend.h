@@ -137,8 +137,8 @@ constexpr float M_START = -1e30f;
 
 // ------------------------------------------------------------------------------------------------ values nobody sees
 // A product with weight 0 is not 0 where the value is infinite or NaN.  In tiles where some rows see a key and others do
-// not, values that are not finite are taken out of the matrix product; a kernel that met one adds it to the rows that see
-// it once its key loop is done (a positive weight leaves such a value as it is).
+// not, values that are not finite are taken out of the matrix product; a kernel that met one gives it to the rows that see
+// it once its key loop is done.
 template <typename T>
 __device__ __forceinline__ bool nonfinite(u32x4 a) {
     uint32_t f = 0;

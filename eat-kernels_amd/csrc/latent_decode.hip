@@ -556,9 +556,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             lds_barrier();
         }
 
-        if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the tokens that not every row sees
+        // Infinite or NaN values in tiles that not every row sees whole (from the tile of `first` on).  A row that sees such a token has a
+        // score of +inf or NaN, and NaN throughout, or one of -inf, and with it a weight of 0 and a NaN in place of this value.
+        if (__builtin_amdgcn_ballot_w64(special)) {
 #pragma unroll 1
-            for (int j = max(first, (int)(t0 * BN)); j < min(last, (int)(stop * BN)); ++j) {
+            for (int j = max(first & ~(BN - 1), (int)(t0 * BN)); j < min(last, (int)(stop * BN)); ++j) {
                 const int page = table[j / a.page_size];
                 if (page < 0 || page >= a.pages) continue;
                 const uint16_t* vr = reinterpret_cast<const uint16_t*>(cache + page * page_bytes) + (int64_t)(j % a.page_size) * ROW +
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float x = T::up(vr[32 * d + 8 * (e >> 2) + (e & 3)]);
-                            if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] += x;
+                            if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] = NAN;
                         }
                 }
             }

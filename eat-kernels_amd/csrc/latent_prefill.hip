@@ -368,7 +368,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) prefill_kernel(KdaLatentPrefill
         for (int i = 0; i < 10; ++i) bring(next, i);
     }
     wait_loads<0>();  // (nothing is left in flight towards LDS)
-    if (__builtin_amdgcn_ballot_w64(special)) {  // infinite or NaN values among the keys that not every row sees
+    // Infinite or NaN values in tiles that not every row sees whole.  A positive weight leaves such a value as it is, however small: it is
+    // added even where the weight has become 0 in fp32 (a tile that every row sees gives 0 inf = NaN there).
+    if (__builtin_amdgcn_ballot_w64(special)) {
         const int seen = min(row + shift, Lk - 1);
 #pragma unroll 1
         for (int j = max(max(full, 0) & ~(BN - 1), first * BN); j < min(mine, last * BN); ++j) {

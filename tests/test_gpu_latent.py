@@ -698,3 +698,44 @@ def test_a_scale_that_is_written_again_counts_anew():
     for bad in ("much", [1.0]):
         with pytest.raises((TypeError, ValueError)):
             x.run(scale=bad)
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("H,S,prefix", [(4, 1, None), (12, 3, None), (40, 2, None), (96, 1, None), (12, 1, 75), (96, 2, 75)])
+def test_decode_infinite_values_that_are_seen(value, wide, H, S, prefix):
+    """A token whose score is -inf because one of its values is infinite has a weight of 0, and 0 times that value is NaN: in
+    that channel of every row that sees it, wherever the token stands (a tile that all rows see whole or not), and nowhere
+    else."""
+    lens, size = [105, 64, 40], 16
+    for at in (3, 33, 60, 66, 97, 100, 103):  # within sequence 0, or within the prefix; tiles end at 64 and 96
+        x = Absorbed(lens, S, H, size, BF, prefix=prefix)
+        if prefix is not None and at >= prefix:
+            continue
+        x.ql[..., 7] = -1.0 if value > 0 else 1.0
+        pages = x.prefix_table if prefix is not None else x.table[0]
+        x.cache[int(pages[at // size]), at % size, 7] = value
+        if wide:
+            x.widen()
+        o, lse = x.run()
+        o, lse = o.cpu(), lse.cpu()
+        head, head_there = R.cache_rows(x.cache, x.prefix_table, prefix) if prefix is not None else R.cache_rows(x.cache, [], 0)
+        for n, length in enumerate(lens):
+            rows, there = R.cache_rows(x.cache, x.table[n], length)
+            rows, there = torch.cat([head, rows]), torch.cat([head_there, there])
+            P, j = len(head), torch.arange(len(head) + length)
+            s = torch.arange(S).repeat_interleave(H)
+            visible = there[None, :] & (j[None, :] < P + length - (S - 1 - s)[:, None])
+            sees = visible[:, at].clone() if prefix is not None or n == 0 else torch.zeros(S * H, dtype=torch.bool)
+            if prefix is not None or n == 0:  # the token adds nothing but its NaN
+                visible[:, at] = False
+                rows[at] = 0.0
+            q = torch.cat([x.ql, x.qp], dim=-1)[n * S:(n + 1) * S].double().reshape(S * H, ROW)
+            ref, A, ref_lse, Z, vmax, L = R.attend(q, rows, rows[:, :LAT], visible, SCALE)
+            got, got_lse = o[n * S:(n + 1) * S].reshape(S * H, LAT), lse[n * S:(n + 1) * S].reshape(S * H)
+            assert torch.isnan(got[sees, 7]).all(), f"token {at} of sequence {n}: {got[sees, 7]}"
+            keep = [c for c in range(LAT) if c != 7]
+            R.check(got[:, keep], got_lse, (ref[:, keep], A[:, keep], ref_lse, Z, vmax, L), BF, ROW, f"token {at} seq {n}")
+            if not sees.all():
+                r = ~sees
+                R.check(got[r], got_lse[r], (ref[r], A[r], ref_lse[r], Z[r], vmax[r], L), BF, ROW, f"token {at} seq {n}, unseen")
