@@ -739,3 +739,24 @@ def test_decode_infinite_values_that_are_seen(value, wide, H, S, prefix):
             if not sees.all():
                 r = ~sees
                 R.check(got[r], got_lse[r], (ref[r], A[r], ref_lse[r], Z[r], vmax[r], L), BF, ROW, f"token {at} seq {n}, unseen")
+
+
+@pytest.mark.parametrize("cu_q,cu_k,keys", [([-5, 1 << 30], [50, 0], 0), ([-5, 1 << 30], [0, 1 << 30], 50), ([0, 25], [-3, 50], 50),
+                                            ([0, 1 << 31 - 1], [1 << 30, 1 << 30], 0), ([0, 20], [0, -1], 0)])
+def test_prefill_offsets_outside_leave_the_rest_alone(cu_q, cu_k, keys):
+    """cu_seqlens past the tensors, or falling: clamped, every row of the 20 queries is written, with zeros and -inf where no
+    key is left, and nothing around the outputs is."""
+    x = Expanded([20], [50], 2, BF, "dense")
+    o, lse = x.run()
+    q, k, v, pe = (t.to(DEV) for t in (x.q, x.k, x.v, x.pe))
+    wide = torch.full((20 + 300, 4, HEAD + 16), 3.0, dtype=BF, device=DEV)
+    lines = torch.full((20 + 300, 2), 5.0, device=DEV)
+    kda355.latent_prefill(q, k, v, pe, _i32(cu_q), _i32(cu_k), out=wide[150:170, 1:3, 8:8 + HEAD], lse=lines[150:170])
+    got, got_lse = wide[150:170, 1:3, 8:8 + HEAD].clone(), lines[150:170].clone()
+    if keys:
+        assert torch.equal(got, o) and torch.equal(got_lse, lse)
+    else:
+        assert (got == 0).all() and (got_lse == -float("inf")).all()
+    wide[150:170, 1:3, 8:8 + HEAD] = 3.0
+    lines[150:170] = 5.0
+    assert (wide == 3.0).all() and (lines == 5.0).all()

@@ -416,3 +416,57 @@ def test_a_page_size_that_is_written_again_counts_anew():
         d.same(book)
         assert d.lens.tolist() == book.lens
     assert not any(isinstance(part, torch.Tensor) for key in kda355.pages._seen for part in key)
+
+
+def test_captured_steps_move_the_contents():
+    """A step of drop, fork and compact recorded once and replayed: after every replay the pages hold what the plain form's
+    moves leave, bit for bit, and the lengths agree."""
+    rng = random.Random(13)
+    book, pools = _make(rng, 12, 6, 8, 80, 40)
+    for r in range(8, 12):
+        for g in book.table[r]:
+            if g >= 0:
+                book.refs[g] -= 1
+        book.table[r], book.lens[r] = [-1] * 6, 0
+    book.free = [p for p in range(80) if book.refs[p] == 0]
+    book.num = len(book.free)
+    book.free += [-1] * (80 - book.num)
+    d = _Device(book)
+    parents, children = _i32([0, 1, 2, 3]), _i32([8, 9, 10, 11])
+    want = [_bits(t).cpu().clone() for t in pools]
+
+    def step():
+        kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, children, 8)
+        kda355.fork_pages(pools, d.table, d.lens, d.refs, d.free, d.num, parents, children, 8)
+        kda355.compact_pages(pools, d.table, d.refs, d.free, d.num)
+
+    def compare(what):
+        book.moves = []
+        book.release(children.tolist())
+        book.fork(parents.tolist(), children.tolist())
+        book.compact()
+        for w in want:
+            for s, t in book.moves:
+                w[t] = w[s]
+        d.same(book)
+        assert d.lens.tolist() == book.lens, what
+        for t, w in zip(pools, want):
+            assert torch.equal(_bits(t).cpu(), w), what
+        return len(book.moves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()  # the first pass outside the capture
+    torch.cuda.current_stream().wait_stream(side)
+    moved = compare("eager")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(5):
+        parents.copy_(_i32([(i + 1) % 8, (i + 3) % 8, (i + 6) % 8, 2]))
+        graph.replay()
+        torch.cuda.synchronize()
+        moved += compare(f"replay {i}")
+        (torch.randn(64, 64, device=DEV) @ torch.randn(64, 64, device=DEV)).sum().item()
+    assert moved > 12  # (forks of part-filled pages and moved pages in more than one replay)
