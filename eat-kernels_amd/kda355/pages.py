@@ -182,7 +182,11 @@ def fork_pages(pools, block_table, seq_lens, ref_counts, free_pages, num_free, p
 
 def free_pages(block_table, seq_lens, ref_counts, free_pages, num_free, rows, page_size):
     """The sequences rows[i] (int32 [n], all different) give up the pages of their tokens: their table rows become holes and
-    their lengths 0; pages that nobody holds any more go onto the stack, the highest first (the lowest is taken next)."""
+    their lengths 0; pages that nobody holds any more go onto the stack, the highest first (the lowest is taken next).
+
+    Only the ceil(length / page_size) first entries of a row are given up.  Entries after them become holes without being given
+    up, and their pages would stay counted as held: where pages are reserved ahead of the tokens, or tokens were taken back,
+    raise the lengths to cover them first (seq_lens[rows] = width * page_size covers a whole row; holes in it are skipped)."""
     dev, pages, stride, count, width, size, _ = _check("free_pages", page_size, (), block_table, ref_counts, free_pages, num_free,
                                                        seq_lens, rows=rows)
     _launch("free_pages", dev, [], rows.numel(), rows.data_ptr(), 0, 0,

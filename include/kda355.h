@@ -427,7 +427,8 @@ int kda355_copy_rows_launch(const KdaPagesArgs* args, kda355_stream_t stream);
    Pairs outside [0, rows) are skipped; children must differ from one another and from every parent. */
 int kda355_fork_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 /* Sequences src[i] (all different) give up the pages of their seq_lens tokens; rows become holes, lengths 0.  Pages that
-   nobody holds any more go onto the stack, the highest first. */
+   nobody holds any more go onto the stack, the highest first.  Entries past the tokens become holes without being given up:
+   where pages are reserved ahead, raise seq_lens to cover them first (holes among them are skipped). */
 int kda355_free_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 /* With L pages held: the i-th held page at or above L moves into the i-th free one below L, in every pool; tables, counts
    and the stack (pages - 1 down to L, so that L is taken next) follow. */

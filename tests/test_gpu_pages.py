@@ -470,3 +470,27 @@ def test_captured_steps_move_the_contents():
         moved += compare(f"replay {i}")
         (torch.randn(64, 64, device=DEV) @ torch.randn(64, 64, device=DEV)).sum().item()
     assert moved > 12  # (forks of part-filled pages and moved pages in more than one replay)
+
+
+@pytest.mark.parametrize("rows,width,pages", [(6, 5, 60), (70, 9, 5000), (300, 40, 9000)])
+def test_free_gives_up_reserved_pages_that_the_length_covers(rows, width, pages):
+    """Pages reserved past a sequence's tokens are given up with it when its length is raised to cover them first."""
+    rng = random.Random(rows)
+    size = 16
+    perm = list(range(pages))
+    rng.shuffle(perm)
+    table, lens, refs = [], [], [0] * pages
+    for r in range(rows):
+        n = rng.randrange(1, width + 1)
+        own = [perm.pop() for _ in range(n)]
+        for g in own:
+            refs[g] = 1
+        table.append(own + [-1] * (width - n))
+        lens.append(rng.randrange(n * size + 1))  # anything from no token to all pages full
+    free = [p for p in range(pages) if not refs[p]]
+    d = _Device(Book(table, lens, refs, free + [-1] * (pages - len(free)), len(free), size))
+    which = _i32(list(range(rows)))
+    d.lens[which.long()] = width * size
+    kda355.free_pages(d.table, d.lens, d.refs, d.free, d.num, which, size)
+    assert (d.table == -1).all() and (d.lens == 0).all() and (d.refs == 0).all()
+    assert d.num.tolist() == [pages] and sorted(d.free.tolist()) == list(range(pages))
