@@ -16,14 +16,15 @@
 // 32x32x16 with one fragment for both row tiles.
 // With one row tile a group (RT = 1) a score wave has rows 16 (w % 2) .. + 15 of it and everything of a row is there once.
 //
-// Bound: with many rows of few sequences the two products, 576 and 512 cycles of a SIMD's matrix core a tile; a step takes about 1900,
-// with LDS (160 KiB read and written a step) and the instructions of the longer kind of wave behind them.  16 sequences of 6000 to
-// 9900 tokens, 8 draft tokens, 96 heads: 248 us, 0.86 PFLOP/s; 64 sequences of 32 heads behind 32768 shared tokens: 163 us, 0.91
-// PFLOP/s.  With a row tile or two a sequence HBM: 64 ragged sequences, 64 heads, 128 us, 4.3 TB/s.  One sequence of 4097 tokens, 12
-// heads: 13.9 us from a graph, 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5
-// the join.
-// Eight waves of one kind with the value dimensions split: 141 / 296 / 234 us instead of 142 / 260 / 227; four of one kind, one a SIMD,
-// pipelined: 142 / 276 / 264 (64 ragged, drafts, shared prefix).
+// Bound: with many rows of few sequences the step itself.  The two products are 576 and 512 cycles of a SIMD's matrix core a tile, a step
+// takes about 2200 (busy cycles of a CU over the units it walks): scores, maxima across lanes, weights through LDS and a barrier
+// follow one another, so the matrix cores are busy 48 % and LDS 33 % of the time.  16 sequences of 6000 to 9900 tokens, 8 draft tokens,
+// 96 heads: 234 us, 0.91 PFLOP/s; 64 sequences of 32 heads behind 32768 shared tokens: 159 us, 0.93 PFLOP/s (both after some 200 passes
+// without a pause; the first 20 after one take 291 and 197, with the clock that the card then allows).  With a row tile or two a
+// sequence HBM: 64 ragged sequences, 64 heads, 126 to 135 us, 4.3 TB/s.  One sequence of 4097 tokens, 12 heads: 13.9 us from a graph,
+// 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5 the join.
+// Other forms, each against this one as it stood then (64 ragged, drafts, shared prefix): eight waves of one kind with the value
+// dimensions split 141 / 296 / 234 us against 142 / 260 / 227; four of one kind, one a SIMD, pipelined 142 / 276 / 264.
 #include <type_traits>
 
 #include "attend.h"
@@ -56,7 +57,7 @@ struct Plan {
     Groups own, pre;       // of a sequence's rows; of all rows of the batch, for the prefix (no groups: no prefix)
     int grid;
     float per_wg;          // 1 / grid
-    int64_t pre_slots;     // workspace: prefix parts, then the sequences'
+    int64_t pre_slots;     // workspace: prefix parts, then the sequences' (64 KiB a slot of 32 rows)
     uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift, x < 2^31
 };
 __device__ __forceinline__ uint32_t page_of(const Plan& p, uint32_t tok) { return (uint32_t)((uint64_t)tok * p.page_mul >> p.page_shift); }
@@ -757,9 +758,9 @@ int check_decode_sizes(const KdaLatentDecodeArgs* a) {
 Plan plan_of(const KdaLatentDecodeArgs* a) {
     Plan p;
     const int cus = a->num_cus ? a->num_cus : 256;
-    // Groups of 64 rows read the keys least often.  Of 32 rows, and with a kernel for one row tile, whose steps are shorter (about 1400
-    // cycles instead of 2000), where even tables full of tokens leave workgroups over: 8 sequences of 12 heads behind 2000 shared
-    // tokens 15.2 us instead of 17.1.
+    // Groups of 64 rows read the keys least often.  Of 32 rows, and with a kernel for one row tile, whose steps take about two thirds
+    // of the time, where even tables full of tokens leave workgroups over: 8 sequences of 12 heads behind 2000 shared tokens 15.2 us
+    // instead of 17.1.
     const int64_t rows = (int64_t)a->S * a->H, own = a->B * (((int64_t)a->table_width * a->page_size + BN - 1) / BN + LEAD);
     const int64_t pre = ((int64_t)a->prefix_width * a->page_size + BN - 1) / BN;
     auto plan = [&](int most) {

@@ -6,13 +6,15 @@
 // a tile, the next tile's loads under way while this one is computed.  Per wave and tile: scores 24 MFMAs, running softmax
 // in registers, values 16 MFMAs (attend.h has the layouts).
 //
-// Bound: the matrix cores (40 MFMAs of 32 cycles a wave and tile, two waves a SIMD), and while they run the card's power.  8192
-// causal tokens of 32 heads: 639 us, 1.08 of the 1.22 PFLOP/s that a large library product reaches; the matrix cores are busy 62 % of
-// the cycles, LDS reads (4 cycles for 1 KiB, no conflicts) 31 %, and with fewer waits the clock falls as much as the cycles (operands
-// read 8 steps ahead: 10 % fewer cycles, the same time).  64 rows a wave, one wave a SIMD: 680 us, a wave issues an instruction every
-// 5.6 cycles at best.  Six prompts of 1 to 2048 tokens with up to 8191 before them: 160 us, a tile of 128 rows as fast as above, but
-// a quarter of the tiles has few rows and the last 25 us few workgroups.  77 rows of 16 heads over 1277 keys: 15.4 us, of which
-// 4.5 join the pieces and 4.8 go by in a piece's three tiles, one after the other; most of the rest is the start.
+// Bound: the matrix cores (40 MFMAs of 32 cycles a wave and tile, two waves a SIMD), and while they run the card's power: the clock
+// stands at 1.75 GHz where a kernel bound by HBM keeps 2.3 to 2.4.  8192 causal tokens of 32 heads: 639 to 686 us on different cards,
+// 1.00 to 1.08 of the 1.22 PFLOP/s that a large library product reaches (754 in the first 20 passes after a pause); the matrix cores are
+// busy 62 % of the cycles, LDS reads (4 cycles for 1 KiB, no conflicts) 31 %, and with fewer waits the clock falls as much as the cycles
+// (operands read 8 steps ahead: 10 % fewer cycles, the same time).  64 rows a wave, one wave a SIMD: 680 us against 651 then, a wave
+// issues an instruction every 5.6 cycles at best.  Six prompts of 1 to 2048 tokens with up to 8191 before them: 161 us (207 soon
+// after a pause), a tile of 128 rows as fast as above, but a quarter of the tiles has few rows, and their waves without any row do the
+// matrix steps of the others (17 % of all here); the last 25 us have few workgroups.  77 rows of 16 heads over 1277 keys: 15.4 us,
+// of which 4.5 join the pieces and 4.8 go by in a piece's three tiles, one after the other; most of the rest is the start.
 #include <type_traits>
 
 #include "attend.h"

@@ -37,7 +37,8 @@ _cus = {}
 
 # A decode step makes dozens of these calls, each of a few microseconds on the GPU.  What the checks look at (types, devices,
 # shapes, strides) comes back call after call, so every entry keeps what it found for it: the checked sizes and strides, packed as
-# the C struct's bytes.  The addresses are the call's own.
+# the C struct's bytes.  The addresses are the call's own.  (Host time of a call whose sizes were not there before: latent_prefill
+# 18 us instead of 12, latent_append 9.7 instead of 5.1, latent_gather 8.8 instead of 5.0.)
 _MOST = 4096  # kept at a time, per entry
 
 
@@ -173,10 +174,10 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
     heads.  cu_seqlens_q / cu_seqlens_k int32 [N + 1] on the device; the queries are the last tokens of their sequences, so
     with `causal` query i of Lq sees keys j <= i + Lk - Lq.  Returns out [Tq, H, 128]; `lse` (fp32 [Tq, H]) receives the
     logarithms of the softmax sums, for joining with the attention over other keys.  A query that sees no key gets zeros and
-    -inf, and keys it does not see never reach it, whatever they hold.
+    -inf, and keys it does not see never reach it, whatever they hold; rows of no sequence are not written.
 
-    workspace: uint8 tensor of latent_prefill_workspace_bytes(...); by default one is taken from torch's allocator for the
-    call.  Calls that may overlap need workspaces of their own."""
+    workspace: uint8 tensor of latent_prefill_workspace_bytes(...) (up to 136 MB); by default one is taken from torch's
+    allocator for the call.  Calls that may overlap need workspaces of their own."""
     scale, causal = SCALE if scale is None else float(scale), bool(causal)  # (what is kept is keyed by their values)
     try:
         key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype,
@@ -248,8 +249,9 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
     prefix_table (int32 [width]) and prefix_len (int32 [1]) name the pages of a prefix that all B sequences share and see in
     front of their own tokens; it is read once for the whole batch.  block_table and seq_lens then hold what follows it.
 
-    workspace: uint8 tensor of latent_decode_workspace_bytes(...); by default one is taken from torch's allocator for the
-    call.  Calls that may overlap need workspaces of their own."""
+    workspace: uint8 tensor of latent_decode_workspace_bytes(...) (17 MB for one sequence, 42 MB for 64 of 64 heads, 303 MB
+    for 128 of 8 tokens and 128 heads); by default one is taken from torch's allocator for the call.  Calls that may overlap
+    need workspaces of their own."""
     scale = SCALE if scale is None else float(scale)  # (what is kept is keyed by its value)
     try:
         key = (q_latent.shape, q_latent.stride(), q_latent.dtype, q_latent.device, q_pe.shape, q_pe.stride(), q_pe.dtype,

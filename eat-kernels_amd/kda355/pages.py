@@ -197,7 +197,8 @@ def free_pages(block_table, seq_lens, ref_counts, free_pages, num_free, rows, pa
 def compact_pages(pools, block_table, ref_counts, free_pages, num_free):
     """Moves the held pages to the start of every pool: with L pages held, the i-th held page at or above L goes into the
     i-th free one below L.  block_table, ref_counts and the stack (L is taken next) follow.  Afterwards pages L and up hold
-    nothing: the pools can be cut there."""
+    nothing: the pools can be cut there.  Lists of pages kept elsewhere are not rewritten: keep the pages of a shared prefix as a
+    row of block_table and pass that row to latent_decode."""
     pools = _sequence(pools)
     dev, pages, stride, rows, width, _, ps = _check("compact_pages", 1, pools, block_table, ref_counts, free_pages, num_free)
     ws = torch.empty(2 * pages + 2, dtype=torch.int32, device=dev)

@@ -307,7 +307,8 @@ int kda355_prefill_launch_noalloc(const KdaPrefillArgs* args, kda355_stream_t st
  * With its lengths Lq and Lk and KDA355_LATENT_CAUSAL, query i sees keys j <= i + Lk - Lq (the queries are the last
  * tokens); without, all of them.  z = scale (q[:128] . k + q[128:] . k_pe);  out = softmax(z) v;  lse = log sum e^z.  A
  * query that sees no key gets zeros and an lse of -inf.  Keys that a query does not see never reach its output, whatever
- * they hold.  Sums and softmax statistics are fp32.
+ * they hold.  Rows of no sequence are not written.  Sums and softmax statistics are fp32; weights are rounded to the type for
+ * their product with the values.  Scores z have to stay within +-2^24.
  */
 typedef struct KdaLatentPrefillArgs {
     const void* q;       /* [Tq, H, 192], strides in elements */
@@ -329,7 +330,9 @@ typedef struct KdaLatentPrefillArgs {
     int32_t num_cus;     /* CUs to fill (0: 256) */
 } KdaLatentPrefillArgs;
 
-/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL. */
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL.  Room for every cut of the
+   keys that the lengths on the device may ask for: 66560 bytes for each of up to 8 num_cus parts of 128 rows, 136 MB with 256
+   CUs however long the prompt (less where few rows and keys cannot be cut so far: 0.5 MB for 100 rows of 4 heads over 300 keys). */
 int64_t kda355_latent_prefill_workspace_bytes(const KdaLatentPrefillArgs* args);
 int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* args, kda355_stream_t stream);
 
@@ -340,7 +343,7 @@ int kda355_latent_prefill_launch(const KdaLatentPrefillArgs* args, kda355_stream
  * to [0, table_width * page_size].
  * With prefix_table, every sequence first sees the prefix_len[0] tokens of those pages (all S tokens see all of them),
  * then its own; the prefix is read once for all rows.  A row that sees nothing gets zeros and an lse of -inf.  scale must be
- * positive, B * S * H below 2^29.
+ * positive, B * S * H below 2^29.  Precision and range of the scores as above.
  */
 typedef struct KdaLatentDecodeArgs {
     const void* q_latent;        /* [B * S, H, 512], strides in elements */
@@ -362,7 +365,9 @@ typedef struct KdaLatentDecodeArgs {
     uint32_t flags;              /* 0 */
 } KdaLatentDecodeArgs;
 
-/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL. */
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL.  65792 bytes for 32 rows of a
+   part: num_cus parts and one for each group of up to 64 rows of a sequence, and num_cus more with a prefix.  With 256 CUs 17 MB
+   for one sequence of 12 heads, 42 MB for 64 of 64 heads, 303 MB for 128 x 8 tokens of 128 heads, 842 MB for 512 x 8 of 96. */
 int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArgs* args);
 int kda355_latent_decode_launch(const KdaLatentDecodeArgs* args, kda355_stream_t stream);
 
@@ -377,7 +382,7 @@ typedef struct KdaLatentTokensArgs {
     void* cache;                 /* [pages, page_size, 576] */
     const int64_t* slots;        /* append: [T] */
     const int32_t* block_table;  /* gather: [N, table_width] */
-    const int32_t* cu;           /* gather: [N + 1] on the device, clamped to [0, T] */
+    const int32_t* cu;           /* gather: [N + 1] on the device, not decreasing; rows outside [0, T) are skipped */
     void* out;                   /* gather: [T, 576], row stride out_row */
     int64_t latent_row, pe_row, out_row, page_stride, pages, table_stride, T;
     int32_t page_size, table_width, N, reserved;
@@ -431,7 +436,8 @@ int kda355_fork_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
    where pages are reserved ahead, raise seq_lens to cover them first (holes among them are skipped). */
 int kda355_free_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 /* With L pages held: the i-th held page at or above L moves into the i-th free one below L, in every pool; tables, counts
-   and the stack (pages - 1 down to L, so that L is taken next) follow. */
+   and the stack (pages - 1 down to L, so that L is taken next) follow.  Lists of pages kept elsewhere are not rewritten: keep
+   the pages of a shared prefix as a row of block_table. */
 int kda355_compact_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ misc */
