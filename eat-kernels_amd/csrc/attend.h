@@ -35,6 +35,13 @@ struct Bf16 {
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) { return f2bf2(x, y); }
     static __device__ __forceinline__ float up(uint16_t x) { return bf2f(x); }
+    // eight 4-bit codes times a power of two (a float of its exponent), each rounded to the type; NaN where the scale is (255)
+    static __device__ __forceinline__ u32x4 from4(uint32_t codes, float scale) {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+    }
 };
 struct Fp16 {
     static constexpr float B = 9.f, SLACK = 6.f;
@@ -49,6 +56,12 @@ struct Fp16 {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2_t));
     }
     static __device__ __forceinline__ float up(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+    static __device__ __forceinline__ u32x4 from4(uint32_t codes, float scale) {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
+    }
 };
 
 // ------------------------------------------------------------------------------------------------ LDS
@@ -72,6 +85,10 @@ __device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2" ::"s"(__builtin_amdgcn_readfirstlane(lds - OFFSET)),
                  "v"(src), "n"(OFFSET)
                  : "memory");
+}
+// 64 lanes x 4 bytes, lane l's to lds + 4 l
+__device__ __forceinline__ void load_words(uint32_t lds, uint64_t src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory");
 }
 __device__ __forceinline__ u32x4 tile_rsrc(const void* base, uint32_t size) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);

@@ -27,16 +27,13 @@
 // dimensions split 141 / 296 / 234 us against 142 / 260 / 227; four of one kind, one a SIMD, pipelined 142 / 276 / 264.
 #include <type_traits>
 
-#include "attend.h"
+#include "latent.h"
 
 namespace kda355 {
 namespace {
 
-constexpr int LAT = KDA355_LATENT_DIM, ROW = KDA355_LATENT_ROW, PE = KDA355_LATENT_PE;
-constexpr int ROW_BYTES = ROW * 2, LAT_BYTES = LAT * 2, PE_BYTES = PE * 2;
 constexpr int SCORE_WAVES = 4, VALUE_WAVES = 4, THREADS = (SCORE_WAVES + VALUE_WAVES) * 64;
-constexpr int BN = 32, BUFS = 4;                        // keys of a tile, tiles in LDS
-constexpr int LOADS = 10;                               // of a value wave a tile: 8 of latent rows, positional parts, page numbers
+constexpr int BN = 32;                                  // keys of a tile
 constexpr int MAX_ROWS = 64;                            // query rows of a group
 // The cut is by cost: beginning a sequence (lengths, queries, page numbers and first tile one after the other) takes about as
 // long as LEAD tiles, which stand in front of every sequence's own; a run is MIN_RUN of these units at least.  Measured: 64
@@ -58,17 +55,14 @@ struct Plan {
     int grid;
     float per_wg;          // 1 / grid
     int64_t pre_slots;     // workspace: prefix parts, then the sequences' (64 KiB a slot of 32 rows)
-    uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift, x < 2^31
+    PageOf page;
 };
-__device__ __forceinline__ uint32_t page_of(const Plan& p, uint32_t tok) { return (uint32_t)((uint64_t)tok * p.page_mul >> p.page_shift); }
-__device__ const uint4 zero_row[ROW_BYTES / 16] = {};  // what a token that is not there reads
 
 // ------------------------------------------------------------------------------------------------ who does what
 struct Cut {
     uint32_t own, pre, run;  // units of all sequences, tiles of the prefix; units of a workgroup
     uint32_t pre_runs, pre_wgs, own_wgs;
 };
-__device__ __forceinline__ int tokens_of(int len, int width, int page_size) { return min(max(len, 0), width * page_size); }
 __device__ __forceinline__ uint32_t tiles_of(int tokens) { return ((uint32_t)tokens + BN - 1) / BN; }
 __device__ __forceinline__ uint32_t units_of(int tokens) { return tokens ? tiles_of(tokens) + LEAD : 0; }
 __device__ __forceinline__ uint32_t cdiv(uint32_t x, uint32_t y) { return x / y + (x % y != 0); }
@@ -130,18 +124,25 @@ __device__ __forceinline__ At sequence_of(const Lengths& lens, uint32_t u) {
 // order: with this turn the former touch all 16 places of 256 bytes, and so do the latter.  (A turn that serves the former alone
 // and weights without their turn: 35 % more LDS cycles, 1 % more time.)
 __device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) << 1; }
-constexpr int BLOCK = 1024, TILE_PE = BN * LAT_BYTES, TILE_BYTES = TILE_PE + BN * PE_BYTES;
-constexpr int LDS_P = BUFS * TILE_BYTES;             // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
-constexpr int LDS_MAX = LDS_P + 2 * 4096;            // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
-constexpr int LDS_FLAG = LDS_MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
-constexpr int LDS_THERE = LDS_FLAG + 64;             // is the token there [tile % 4][32] bytes
-constexpr int LDS_PAGES = LDS_THERE + 4 * BN;        // page numbers [value wave][tile % 4][64]
-constexpr int LDS_BYTES = LDS_PAGES + VALUE_WAVES * 4 * 256;
-static_assert(LDS_BYTES <= 160 * 1024, "");
+constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
+template <bool Q4>
+struct Lds {
+    // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: latent rows of three tiles (one
+    // read for scores, one for values, one being written), positional parts of five, and codes and scales of three as they came.
+    static constexpr int BUFS = Q4 ? 3 : 4, PES = Q4 ? 5 : 4, RAWS = Q4 ? 3 : 0, THERES = Q4 ? 8 : 4;
+    static constexpr int LAT_STEP = Q4 ? LAT_TILE : LAT_TILE + PE_TILE, PE_STEP = Q4 ? PE_TILE : LAT_STEP;
+    static constexpr int PE0 = Q4 ? BUFS * LAT_STEP : LAT_TILE;
+    static constexpr int RAW = Q4 ? PE0 + PES * PE_STEP : BUFS * LAT_STEP, RAW_WAVE = 8 * (LAT / 2) + 256;  // 8 tokens' codes, scales
+    static constexpr int P = RAW + RAWS * VALUE_WAVES * RAW_WAVE;  // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
+    static constexpr int MAX = P + 2 * 4096;             // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
+    static constexpr int FLAG = MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
+    static constexpr int THERE = FLAG + 64;              // is the token there [tile % THERES][32] bytes
+    static constexpr int PAGES = THERE + THERES * BN;    // page numbers [value wave][tile % 4][64]
+    static constexpr int BYTES = PAGES + VALUE_WAVES * 4 * 256;
+    static constexpr int LOADS = Q4 ? 5 : 10;            // of a value wave a tile: codes 2, scales | 8 of latent rows; positional parts, page numbers
+    static_assert(BYTES <= 160 * 1024 && RAW % 1024 == 0 && P % 1024 == 0, "");
+};
 
-__device__ __forceinline__ uint64_t of_lane(uint64_t x, int l) {
-    return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), l) << 32 | (uint32_t)__shfl((int)(uint32_t)x, l);
-}
 template <int I>
 using Int = std::integral_constant<int, I>;
 // the four lane groups of 16 joined
@@ -153,9 +154,11 @@ __device__ __forceinline__ float join_groups(float x, F f) {
     return f(__uint_as_float(b.x), __uint_as_float(b.y));
 }
 
-template <typename T, int RT>
+template <typename T, int RT, bool Q4>
 __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
-    __shared__ __align__(1024) unsigned char sm[LDS_BYTES];
+    typedef Lds<Q4> L;
+    constexpr int CACHE_ROW = Q4 ? ROW4 : ROW_BYTES;
+    __shared__ __align__(1024) unsigned char sm[L::BYTES];
     const uint32_t lds = lds_offset(sm);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int c = lane & 31, half = lane >> 5;
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const Lengths lens(a);
     // ---- what does not depend on the lengths, while they come
     const float sc = a.scale * 1.44269504088896f;
-    const int64_t page_bytes = a.page_stride * 2;
+    const int64_t page_bytes = Q4 ? a.page_stride : a.page_stride * 2;
     const char* const cache = static_cast<const char*>(a.cache);
     const bool scores = w < SCORE_WAVES;
     const int rw = w & 1, kh = w >> 1 & 1;  // a score wave's rows 16 RT rw .. (16 RT of them) and keys 16 kh ..
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     if (scores) {
         const int t = 16 * kh + c16;
         ra[0] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
-        ra[1] = TILE_PE + t * PE_BYTES + ((quad ^ swz8(t)) << 4);
+        ra[1] = t * PE_BYTES + ((quad ^ swz8(t)) << 4);
     } else {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -185,6 +188,9 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             ra[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
         }
     }
+
+    auto lat_at = [&](uint32_t tile) { return lds + tile % L::BUFS * L::LAT_STEP; };        // a tile's latent rows
+    auto pe_at = [&](uint32_t tile) { return lds + L::PE0 + tile % L::PES * L::PE_STEP; };  // and positional parts
 
     uint32_t own = 0;
     for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
@@ -239,12 +245,12 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         const uint32_t n_tiles = stop - t0;
         // A tile's weights are relative to a past maximum of their rows, which is raised only when some row of a wave exceeds it
         // by SLACK (the result is the same for any reference): after the fact, at the start of the next step.
-        auto flags = [&](uint32_t tile) { return *reinterpret_cast<const u32x4*>(sm + LDS_FLAG + (tile & 1) * 16); };
+        auto flags = [&](uint32_t tile) { return *reinterpret_cast<const u32x4*>(sm + L::FLAG + (tile & 1) * 16); };
         auto any = [](u32x4 fl) { return __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]) != 0; };
         // the new reference of the group's row r after `tile`, by its own scores alone; returns the factor of what is there
         auto raise = [&](uint32_t tile, int r, float& m) {
-            const float m0 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + r * 4);
-            const float m1 = *reinterpret_cast<const float*>(sm + LDS_MAX + (tile & 1) * 512 + (MAX_ROWS + r) * 4);
+            const float m0 = *reinterpret_cast<const float*>(sm + L::MAX + (tile & 1) * 512 + r * 4);
+            const float m1 = *reinterpret_cast<const float*>(sm + L::MAX + (tile & 1) * 512 + (MAX_ROWS + r) * 4);
             const float mx = fmaxf(m0, m1), mn = mx - m > T::B + T::SLACK ? mx - T::B : m, f = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             return f;
@@ -252,12 +258,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         if (scores) {
             // ================================================================ score waves
             const int row0 = r0 + 16 * RT * rw + c16;  // this lane's rows: row0, and with two row tiles row0 + 16
-            // The queries come through the LDS of tiles t0 + 2 and t0 + 3, a row tile in each, laid out like keys, half of a wave's
+            // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: t0 + 1 and t0 + 2), a row tile in each, laid out like keys, half of a wave's
             // rows by it and half by the other wave that has them (rows past the end repeat the last one).  (Straight into registers,
             // 64 bytes of 16 rows at a time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of
             // 64 heads; 1900 and 4800 so.)
             int mine[RT];
-            const uint32_t qb = lds + (t0 + 2 + (RT > 1 ? rw : 0)) % BUFS * TILE_BYTES;
+            const uint32_t qt = t0 + (Q4 ? 1 : 2) + (RT > 1 ? rw : 0), qb = lat_at(qt);
+            const uint32_t qpe = Q4 ? lds + L::P + (RT > 1 ? rw : 0) * PE_TILE : pe_at(qt);
             const bool some = n_tiles && row0 - c16 < r1;
             auto half_of = [&](int x) { return RT > 1 ? x : rw; };  // of the row tile: where rows row0 + 16 x stand
             {
@@ -276,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 }
                 if (some) {
                     const uint32_t block = qb + (4 * half_of(x0) + at0 / 4) * (4 * BLOCK);
-                    const uint32_t pe_block = qb + TILE_PE + (16 * half_of(x0) + at0) * PE_BYTES;
+                    const uint32_t pe_block = qpe + (16 * half_of(x0) + at0) * PE_BYTES;
 #pragma unroll
                     for (int i = 0; i < 2 * RT; ++i) {
                         const int t = at0 + 4 * i + (me >> 4);
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             if (some)
 #pragma unroll
                 for (int x = 0; x < RT; ++x) {
-                    const uint32_t at = qb + ra[0] + (half_of(x) - kh) * (16 * LAT_BYTES), pat = qb + ra[1] + (half_of(x) - kh) * (16 * PE_BYTES);
+                    const uint32_t at = qb + ra[0] + (half_of(x) - kh) * (16 * LAT_BYTES), pat = qpe + ra[1] + (half_of(x) - kh) * (16 * PE_BYTES);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
 #pragma unroll
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     p0[r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], sc, -mo[x]));
                     sum[x] += p0[r];
                 }
-                *reinterpret_cast<u32x2*>(sm + LDS_P + (tile & 1) * 4096 + (2 * (RT > 1 ? rw : 0) + kh) * 1024 + half_of(x) * 512 + c16 * 32 +
+                *reinterpret_cast<u32x2*>(sm + L::P + (tile & 1) * 4096 + (2 * (RT > 1 ? rw : 0) + kh) * 1024 + half_of(x) * 512 + c16 * 32 +
                                           (quad ^ (c16 >> 3) << 1) * 8) =
                     u32x2{T::pack(p0[0], p0[1]), T::pack(p0[2], p0[3])};
             };
@@ -338,13 +345,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             };
             u32x4 fl = {};
             for (uint32_t tile = t0; tile < stop; ++tile) {
-                const uint32_t tb = lds + (tile % BUFS) * TILE_BYTES;
+                const uint32_t tb = lat_at(tile), tp = pe_at(tile);
                 const int k0 = (int)(tile * BN);
                 if (tile > t0) fl = flags(tile - 1);
-                const int there8 = *(sm + LDS_THERE + (tile % BUFS) * BN + c);
+                const int there8 = *(sm + L::THERE + (tile % L::THERES) * BN + c);
                 // ---- 18 steps for both halves of the rows, in two chains each, the operands read five steps ahead
                 auto key = [&](int i) {
-                    return i < 16 ? lds_read16(((tb + ra[0]) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tb + ra[1]) ^ ((i - 16) << 6));
+                    return i < 16 ? lds_read16(((tb + ra[0]) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tp + ra[1]) ^ ((i - 16) << 6));
                 };
                 f32x4 z[RT][2] = {};
                 u32x4 kf[6];
@@ -378,11 +385,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 for (int x = 0; x < RT; ++x) {
                     mx[x] = fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3]));
                     mx[x] = join_groups(mx[x], [](float p, float q) { return fmaxf(p, q); }) * sc;
-                    *reinterpret_cast<float*>(sm + LDS_MAX + (tile & 1) * 512 + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = mx[x];  // (the groups' values agree)
+                    *reinterpret_cast<float*>(sm + L::MAX + (tile & 1) * 512 + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = mx[x];  // (the groups' values agree)
                     weights(tile, x);
                 }
                 const bool up = __builtin_amdgcn_ballot_w64(fmaxf(mx[0] - mo[0], mx[RT - 1] - mo[RT - 1]) > T::B + T::SLACK) != 0;
-                *reinterpret_cast<int*>(sm + LDS_FLAG + (tile & 1) * 16 + w * 4) = up;
+                *reinterpret_cast<int*>(sm + L::FLAG + (tile & 1) * 16 + w * 4) = up;
                 lds_barrier();  // the tile's weights; the next tile is whole
             }
             if (n_tiles) settle(stop - 1, flags(stop - 1));
@@ -390,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
             for (int x = 0; x < RT; ++x) {
                 l[x] = join_groups(l[x], [](float p, float q) { return p + q; });
-                if (quad == 0) *reinterpret_cast<float*>(sm + LDS_MAX + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = l[x];
+                if (quad == 0) *reinterpret_cast<float*>(sm + L::MAX + (MAX_ROWS * kh + 16 * RT * rw + 16 * x + c16) * 4) = l[x];
             }
             lds_barrier();
             lds_barrier();  // the value waves have read it
@@ -401,43 +408,66 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // ---- loads
         const uint32_t pages = (uint32_t)min(a.pages, (int64_t)1 << 31);
         const u32x4 table_rsrc = tile_rsrc(table, (uint32_t)width * 4);  // entries past the table read as zeros (and are past `last`)
-        const uint32_t pages_at = lds + LDS_PAGES + vw * 1024;
+        const uint32_t pages_at = lds + L::PAGES + vw * 1024;
         int me = lane;  // (computed anew for every segment: the score waves have no registers for what follows from it)
         asm volatile("" : "+v"(me));
         const int own8 = 8 * vw + (me & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
         auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane(pages_at + (tile & 3) * 256)),
-                         "v"(page_of(p, tile * BN + own8) * 4), "s"(table_rsrc)
+                         "v"(p.page(tile * BN + own8) * 4), "s"(table_rsrc)
                          : "memory");
         };
         // where the next tile to be brought stands: this lane's pieces of 4 + 4 tokens and of the positional parts, found in
         // steps that can be spread: the page, the address of the lane's token, the addresses for the lane's pieces
-        uint64_t at_latent[2], at_pe;
+        uint64_t at_latent[2], at_pe, at_scales;
         auto find_page = [&](uint32_t tile) {
             return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 3) * 256 + lane * 4);
         };
         auto find_token = [&](uint32_t tile, int page) {
             const uint32_t tok = tile * BN + own8;
             const bool in = tok < (uint32_t)last && (uint32_t)page < pages;  // in the tokens that the group sees, no hole
-            *(sm + LDS_THERE + (tile % BUFS) * BN + own8) = in;
+            *(sm + L::THERE + (tile % L::THERES) * BN + own8) = in;
             uint64_t at = (uint64_t)cache + (uint32_t)page * (uint64_t)page_bytes +
-                          (uint64_t)(tok - page_of(p, tok) * (uint32_t)a.page_size) * ROW_BYTES;
+                          (uint64_t)(tok - p.page(tok) * (uint32_t)a.page_size) * CACHE_ROW;
             asm volatile("" : "+v"(at));  // (a choice of two, not a branch)
             return in ? at : (uint64_t)zero_row;
         };
         const uint32_t piece4[2] = {(uint32_t)((me & 15) ^ turn(8 * vw + (me >> 4))) << 4,
                                     (uint32_t)((me & 15) ^ turn(8 * vw + 4 + (me >> 4))) << 4};
-        const uint32_t piece8 = LAT_BYTES + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
-        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + piece4[x]; };
+        const uint32_t piece8 = (Q4 ? PE4 : LAT_BYTES) + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
+        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + (Q4 ? (me & 15) << 4 : piece4[x]); };
         auto find_pe = [&](uint64_t at) { at_pe = of_lane(at, me >> 3) + piece8; };
+        auto find_scales = [&](uint64_t at) { at_scales = of_lane(at, me >> 2 & 7) + (SCALES4 + (me & 3) * 4); };
+        auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile % 3 * VALUE_WAVES + vw) * L::RAW_WAVE; };
         auto bring = [&](uint32_t tile, auto i) {  // load i of 9: four of 4 tokens, four of 4 more, the positional parts
             constexpr int I = decltype(i)::value;
-            const uint32_t base = lds + (tile % BUFS) * TILE_BYTES;
-            if constexpr (I < 8)
-                load_block<(I & 3) * 256>(base + (2 * vw + (I >> 2)) * (4 * BLOCK) + (I & 3) * BLOCK, at_latent[I >> 2]);
-            else
-                load_block<0>(base + TILE_PE + 8 * vw * PE_BYTES, at_pe);
+            if constexpr (I == 8)
+                load_block<0>(pe_at(tile) + 8 * vw * PE_BYTES, at_pe);
+            else if constexpr (!Q4)
+                load_block<(I & 3) * 256>(lat_at(tile) + (2 * vw + (I >> 2)) * (4 * BLOCK) + (I & 3) * BLOCK, at_latent[I >> 2]);
+            else if constexpr (I < 2)
+                load_block<0>(raw_at(tile) + I * BLOCK, at_latent[I]);  // of 4: codes of 4 tokens and of 4 more, the scales
+            else if constexpr (I == 2)
+                load_words(raw_at(tile) + 2 * BLOCK, at_scales);
+        };
+        // A tile from 4 bits: lane l has values 8 l .. + 7 of each of the wave's tokens, which are a dword of codes and, as 16 bits, the
+        // token's piece l.  Reads and writes of 64 lanes touch every bank equally.
+        uint32_t code[4], scale[4];  // (two pairs of tokens)
+        const uint32_t to4 = vw * (8 * BLOCK) + (me >> 4) * BLOCK + (((me & 15) ^ turn(8 * vw)) << 4);
+        auto read_raw = [&](uint32_t tile, int pair) {  // the wave's tokens 2 pair, 2 pair + 1
+            const uint32_t from = raw_at(tile);
+#pragma unroll
+            for (int r = 2 * pair; r < 2 * pair + 2; ++r) {
+                code[r & 3] = *(__attribute__((address_space(3))) const uint32_t*)(lds_byte*)(uintptr_t)(from + me * 4 + r * (LAT / 2));
+                scale[r & 3] = *(__attribute__((address_space(3))) const uint8_t*)(lds_byte*)(uintptr_t)(from + 2 * BLOCK + (me >> 2) + r * 16);
+            }
+        };
+        auto widen = [&](uint32_t tile, int pair) {
+#pragma unroll
+            for (int r = 2 * pair; r < 2 * pair + 2; ++r)
+                *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)(((lat_at(tile) + to4) ^ ((r & 3) << 6)) + (r >> 2) * (4 * BLOCK) + (r & 3) * 256) =
+                    T::from4(code[r & 3], __uint_as_float(scale[r & 3] << 23));
         };
 
         f32x16 acc[RT][4] = {};  // [row tile][32 values]
@@ -445,12 +475,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
         for (int r = 0; r < RT; ++r) mo[r] = M_START;
         bool special = false;
-        // One step: `tile` added, the value waves' loads of tile + 3 (past the end: zeros) and the addresses of tile + 4 between
-        // the products.  LAST: nothing is brought.
+        // One step: `tile` added, the value waves' loads of tile + AHEAD (past the end: zeros) and the addresses of the one after
+        // it between the products.  From 4 bits: tile + 2 widened, and the addresses found just before (to save registers).  LAST: nothing is brought.
+        constexpr uint32_t AHEAD = Q4 ? 5 : 3;
         auto step = [&](uint32_t tile, auto last_) {
             constexpr bool LAST = decltype(last_)::value;
             const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
-            const uint32_t vb = lds + (tile % BUFS) * TILE_BYTES, pb = lds + LDS_P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
+            const uint32_t vb = lat_at(tile), pb = lds + L::P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
             auto value = [&](int k, int d) {
                 const u32x2 v0 = lds_read_tr(((vb + ra[0]) ^ (d << 6)) + k * 16 * BLOCK);
                 const u32x2 v1 = lds_read_tr(((vb + ra[1]) ^ (d << 6)) + k * 16 * BLOCK);
@@ -464,7 +495,10 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
 #pragma unroll
             for (int d = 0; d < 4; ++d) vf[d] = value(0, d);
-            if constexpr (!LAST) page = find_page(tile + 4);
+            if constexpr (!LAST) {
+                page = find_page(tile + (Q4 ? AHEAD : AHEAD + 1));
+                if constexpr (Q4) read_raw(tile + 2, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
             if (any(fl)) {
 #pragma unroll
@@ -500,7 +534,19 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                             for (int r = 0; r < RT; ++r) pn[r] = weight(1, r);
                     }
-                    if constexpr (!LAST) {  // (what an address is taken from is needed no more)
+                    if constexpr (!LAST && Q4) {
+                        if (k == 0) {
+                            if (d < 3) read_raw(tile + 2, d + 1);
+                            widen(tile + 2, d);
+                            if (d == 1) at = find_token(tile + AHEAD, page);
+                            if (d == 3) find_latent(at, 0);
+                        } else {  // (the codes' place is free: they are in registers)
+                            if (d == 0) bring(tile + AHEAD, Int<0>{}), find_scales(at);
+                            if (d == 1) bring(tile + AHEAD, Int<2>{}), find_latent(at, 1);
+                            if (d == 2) bring(tile + AHEAD, Int<1>{}), find_pe(at);
+                            if (d == 3) bring(tile + AHEAD, Int<8>{}), load_pages(tile + AHEAD + 3);
+                        }
+                    } else if constexpr (!LAST) {  // (what an address is taken from is needed no more)
                         if (k == 0) {
                             if (d == 0) bring(tile + 3, Int<0>{});
                             if (d == 1) bring(tile + 3, Int<1>{}), at = find_token(tile + 4, page);
@@ -520,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
-                wait_loads<LOADS>();
+                wait_loads<Q4 ? 2 * L::LOADS : L::LOADS>();
                 lds_barrier();  // the next tile's weights; the tile after it is whole
             }
         };
@@ -531,23 +577,48 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             auto find_tile = [&](uint32_t tile) {
                 const uint64_t at = find_token(tile, find_page(tile));
                 find_latent(at, 0), find_latent(at, 1), find_pe(at);
+                if constexpr (Q4) find_scales(at);
             };
-            auto whole_tile = [&](uint32_t tile) {
-                find_tile(tile);
+            auto bring_tile = [&](uint32_t tile) {
                 bring(tile, Int<0>{}), bring(tile, Int<1>{}), bring(tile, Int<2>{}), bring(tile, Int<3>{}), bring(tile, Int<4>{});
                 bring(tile, Int<5>{}), bring(tile, Int<6>{}), bring(tile, Int<7>{}), bring(tile, Int<8>{});
             };
+            auto whole_tile = [&](uint32_t tile) {
+                find_tile(tile);
+                bring_tile(tile);
+            };
             whole_tile(t0);
             whole_tile(t0 + 1);
-            load_pages(t0 + 4);
-            wait_loads<LOADS>();
-            lds_barrier();  // the first tile, the queries
-            lds_barrier();  // the queries are in registers
-            // while the first tile's scores are computed: tile t0 + 2, and where t0 + 3 stands
-            whole_tile(t0 + 2);
-            find_tile(t0 + 3);
-            load_pages(t0 + 5);
-            wait_loads<LOADS>();
+            if constexpr (Q4) {
+                auto widen_tile = [&](uint32_t tile) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) read_raw(tile, i), widen(tile, i);
+                };
+                whole_tile(t0 + 2);
+#pragma unroll
+                for (int i = 4; i < 7; ++i) load_pages(t0 + i);
+                wait_loads<2 * 4 + 3>();
+                widen_tile(t0);
+                lds_barrier();  // the first tile, the queries
+                lds_barrier();  // the queries are in registers
+                // while the first tile's scores are computed: the second tile, what comes after the third
+                wait_loads<4 + 3>();
+                widen_tile(t0 + 1);
+                whole_tile(t0 + 3);
+                load_pages(t0 + 7);
+                wait_loads<L::LOADS>();  // the page numbers of t0 + 4 .. 6
+                whole_tile(t0 + 4);
+            } else {
+                load_pages(t0 + 4);
+                wait_loads<L::LOADS>();
+                lds_barrier();  // the first tile, the queries
+                lds_barrier();  // the queries are in registers
+                // while the first tile's scores are computed: tile t0 + 2, and where t0 + 3 stands
+                whole_tile(t0 + 2);
+                find_tile(t0 + 3);
+                load_pages(t0 + 5);
+                wait_loads<L::LOADS>();
+            }
             lds_barrier();  // the first tile's weights; the second tile is whole
             for (uint32_t tile = t0; tile + 1 < stop; ++tile) step(tile, std::false_type{});
             step(stop - 1, std::true_type{});
@@ -564,8 +635,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             for (int j = max(first & ~(BN - 1), (int)(t0 * BN)); j < min(last, (int)(stop * BN)); ++j) {
                 const int page = table[j / a.page_size];
                 if (page < 0 || page >= a.pages) continue;
-                const uint16_t* vr = reinterpret_cast<const uint16_t*>(cache + page * page_bytes) + (int64_t)(j % a.page_size) * ROW +
-                                     128 * vw + 4 * half;
+                const char* row = cache + page * page_bytes + (int64_t)(j % a.page_size) * CACHE_ROW;
+                auto value = [&](int i) -> uint16_t {
+                    if constexpr (!Q4) return reinterpret_cast<const uint16_t*>(row)[i];
+                    const uint32_t b = *reinterpret_cast<const uint8_t*>(row + SCALES4 + i / GROUP);
+                    const uint32_t both = T::from4(*reinterpret_cast<const uint8_t*>(row + i / 2), __uint_as_float(b << 23))[0];
+                    return (uint16_t)(both >> (i & 1) * 16);
+                };
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int i = r0 + 32 * r + c;
@@ -574,7 +650,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     for (int d = 0; d < 4; ++d)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float x = T::up(vr[32 * d + 8 * (e >> 2) + (e & 3)]);
+                            const float x = T::up(value(128 * vw + 4 * half + 32 * d + 8 * (e >> 2) + (e & 3)));
                             if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] = NAN;
                         }
                 }
@@ -587,8 +663,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         float ls[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r)
-            ls[r] = *reinterpret_cast<const float*>(sm + LDS_MAX + (r * 32 + c) * 4) +
-                    *reinterpret_cast<const float*>(sm + LDS_MAX + (MAX_ROWS + r * 32 + c) * 4);
+            ls[r] = *reinterpret_cast<const float*>(sm + L::MAX + (r * 32 + c) * 4) +
+                    *reinterpret_cast<const float*>(sm + L::MAX + (MAX_ROWS + r * 32 + c) * 4);
         lds_barrier();  // free for the next segment
         if (whole) {
 #pragma unroll
@@ -735,10 +811,6 @@ __global__ void __launch_bounds__(SPLIT ? 1024 : 256) join_kernel(KdaLatentDecod
     }
 }
 
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-// rows of 16-byte pieces: aligned base, strides in multiples of 8 elements
-bool rows16(const void* p, int64_t s0, int64_t s1 = 0) { return aligned(p, 16) && s0 % 8 == 0 && s1 % 8 == 0; }
-
 int check_decode_sizes(const KdaLatentDecodeArgs* a) {
     KDA_CHECK_ARG(a != nullptr, "latent_decode: null args");
     KDA_CHECK_ARG(a->B >= 0 && a->S >= 1 && a->H >= 1 && a->page_size >= 1 && a->table_width >= 0 && a->prefix_width >= 0 &&
@@ -772,10 +844,7 @@ Plan plan_of(const KdaLatentDecodeArgs* a) {
     p.grid = cus > p.own.groups + p.pre.groups ? cus : p.own.groups + p.pre.groups;
     p.per_wg = 1.f / p.grid;
     p.pre_slots = p.pre.groups ? p.grid : 0;
-    int bits = 0;  // 2^bits >= page_size: page_mul page_size = 2^(31 + bits) + e, e < 2^bits, so the quotient is exact
-    while ((1ll << bits) < a->page_size) ++bits;
-    p.page_shift = 31 + bits;
-    p.page_mul = (uint32_t)(((1ull << p.page_shift) + a->page_size - 1) / a->page_size);
+    p.page = PageOf::by(a->page_size);
     return p;
 }
 
@@ -792,7 +861,9 @@ extern "C" int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArg
     return SLOTS + (p.pre_slots * (p.pre.rows / 32) + own * (p.own.rows / 32)) * SLOT_TILE;
 }
 
-extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
+namespace {
+template <bool Q4>
+int decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
     if (const int rc = check_decode_sizes(a)) return rc;
     KDA_CHECK_ARG(a->dtype == KDA355_DTYPE_BF16 || a->dtype == KDA355_DTYPE_FP16, "latent_decode: dtype %d", a->dtype);
     KDA_CHECK_ARG(a->flags == 0, "latent_decode: unknown flags 0x%x", a->flags);
@@ -806,7 +877,8 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     KDA_CHECK_ARG(rows16(a->q_latent, a->ql_row, a->ql_head) && rows16(a->q_pe, a->qp_row, a->qp_head) &&
                       rows16(a->out, a->out_row, a->out_head),
                   "latent_decode: q and out rows must be 16-byte aligned");
-    KDA_CHECK_ARG(rows16(a->cache, a->page_stride) && a->page_stride >= (int64_t)a->page_size * ROW,
+    KDA_CHECK_ARG((Q4 ? aligned(a->cache, 16) && a->page_stride % 16 == 0 : rows16(a->cache, a->page_stride)) &&
+                      a->page_stride >= (int64_t)a->page_size * (Q4 ? ROW4 : ROW),
                   "latent_decode: cache pages must be dense and 16-byte aligned");
     KDA_CHECK_ARG(a->scale > 0.f, "latent_decode: scale must be positive");
     const int64_t need = kda355_latent_decode_workspace_bytes(a);
@@ -819,9 +891,9 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     auto launch = [&](auto type) {
         typedef decltype(type) T;
         if (p.own.rows > 32 || p.pre.rows > 32)  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
-            launch_kernel((decode_kernel<T, 2>), dim3(p.grid), dim3(THREADS), s, *a, p);
+            launch_kernel((decode_kernel<T, 2, Q4>), dim3(p.grid), dim3(THREADS), s, *a, p);
         else
-            launch_kernel((decode_kernel<T, 1>), dim3(p.grid), dim3(THREADS), s, *a, p);
+            launch_kernel((decode_kernel<T, 1, Q4>), dim3(p.grid), dim3(THREADS), s, *a, p);
         if (few)
             launch_kernel((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), s, *a, p);
         else
@@ -835,3 +907,7 @@ extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_
     }
     return 0;
 }
+}  // namespace
+
+extern "C" int kda355_latent_decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) { return decode_launch<false>(a, stream); }
+extern "C" int kda355_latent4_decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) { return decode_launch<true>(a, stream); }

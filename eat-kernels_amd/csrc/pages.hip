@@ -5,7 +5,7 @@
 // The bookkeeping is deterministic: ranks come from scans in index order, reference counts from commutative integer
 // updates.  Parts that need an order over all pages run in one workgroup (a scan over 4096 pages is one step of it); what
 // follows from their result (table rows, page copies) runs over the whole chip in a second launch.
-#include "common.h"
+#include "pages.h"
 
 namespace kda355 {
 namespace {
@@ -14,10 +14,8 @@ constexpr int ROW = KDA355_LATENT_ROW, LAT = KDA355_LATENT_DIM;
 constexpr int ROW_Q = ROW / 8, LAT_Q = LAT / 8;  // 16-byte pieces of a cache row, of its latent part
 constexpr int TOK_THREADS = 192, TOKENS = 8, PIECES = TOKENS * ROW_Q / TOK_THREADS;  // 3 pieces a thread
 static_assert(PIECES * TOK_THREADS == TOKENS * ROW_Q, "");
-constexpr int SCAN_THREADS = 1024;
 constexpr int COPY_THREADS = 256, COPY_PER = 4;   // 16 KiB a workgroup
 constexpr int MAX_PAIRS = 1 << 23;                // rows of a launch: 256 threads each, below 2^32 in all
-constexpr int FREED = INT32_MIN;                  // count of a page freed in this call, until the stack has it
 constexpr int MOST_HOLDERS = 1 << 30;             // no count reaches it
 
 // ------------------------------------------------------------------------------------------------ token rows
@@ -120,35 +118,6 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_rows_kernel(KdaPagesArgs a)
     copy_segment(a.pool[blockIdx.z], a.src[blockIdx.x], a.dst[blockIdx.x], blockIdx.y);
 }
 
-// ------------------------------------------------------------------------------------------------ scans
-// exclusive prefix sum over the workgroup's threads; total in every thread
-__device__ __forceinline__ int block_scan(int x, int* sw, int& total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int s = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(s, d);
-        if (lane >= d) s += y;
-    }
-    __syncthreads();  // sw free again
-    if (lane == 63) sw[w] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < SCAN_THREADS / 64; ++i) {
-        const int v = sw[i];
-        if (i < w) before += v;
-        total += v;
-    }
-    return before + s - x;
-}
-
-// words that another thread of the workgroup wrote in this launch: past the vector L1
-__device__ __forceinline__ int load_fresh(const int32_t* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // ------------------------------------------------------------------------------------------------ fork
 __device__ __forceinline__ int row_len(const KdaPagesArgs& a, int row) {
     const int64_t most = (int64_t)a.table_width * a.page_size;
@@ -244,33 +213,6 @@ __global__ void __launch_bounds__(COPY_THREADS) free_rows_kernel(KdaPagesArgs a)
     }
     __syncthreads();  // every thread has read the length
     if (threadIdx.x == 0) a.seq_lens[r] = 0;
-}
-
-__global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a) {
-    __shared__ int sw[SCAN_THREADS / 64];
-    int top = a.num_free[0];
-    top = top < 0 ? 0 : top > a.pages ? a.pages : top;
-    for (int hi = a.pages; hi > 0; hi -= 4 * SCAN_THREADS) {  // four pages a thread, the highest first
-        int mine[4], count = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int p = hi - 1 - 4 * (int)threadIdx.x - k;
-            mine[k] = p >= 0 && a.ref_counts[p] == FREED;
-            count += mine[k];
-        }
-        int total;
-        int at = top + block_scan(count, sw, total);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (mine[k]) {
-                const int p = hi - 1 - 4 * (int)threadIdx.x - k;
-                a.ref_counts[p] = 0;
-                if (at < a.pages) a.free_pages[at] = p;
-                ++at;
-            }
-        top += total;
-    }
-    if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
 }
 
 // The same in one workgroup and one launch, where there is little to give up: what each page loses is counted in LDS, so that no
@@ -391,15 +333,6 @@ __global__ void __launch_bounds__(COPY_THREADS) compact_move_kernel(KdaPagesArgs
             const int page = *e;
             if (page >= 0 && page < a.pages) *e = a.workspace[page];
         }
-}
-
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-int launched(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return 0;
-    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
-    return KDA355_ELAUNCH;
 }
 
 int check_tokens(const KdaLatentTokensArgs* a, const char* what) {

@@ -119,7 +119,17 @@ class KdaLatentTokensArgs(ctypes.Structure):
         ("latent", P), ("k_pe", P), ("cache", P), ("slots", P), ("block_table", P), ("cu", P), ("out", P),
         ("latent_row", I64), ("pe_row", I64), ("out_row", I64), ("page_stride", I64), ("pages", I64),
         ("table_stride", I64), ("T", I64),
-        ("page_size", I32), ("table_width", I32), ("N", I32), ("reserved", I32),
+        ("page_size", I32), ("table_width", I32), ("N", I32), ("dtype", I32),
+    ]
+
+
+class KdaLatentWeightsArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_latent", P), ("q_pe", P), ("cache", P), ("block_table", P), ("seq_lens", P), ("lse", P), ("weights", P),
+        ("ql_row", I64), ("ql_head", I64), ("qp_row", I64), ("qp_head", I64), ("weights_row", I64),
+        ("page_stride", I64), ("pages", I64), ("table_stride", I64),
+        ("B", I32), ("S", I32), ("H", I32), ("page_size", I32), ("table_width", I32), ("dtype", I32),
+        ("cache_bits", I32), ("num_cus", I32), ("scale", F32), ("flags", U32),
     ]
 
 
@@ -138,6 +148,22 @@ class KdaPagesArgs(ctypes.Structure):
         ("rows", I32), ("table_width", I32), ("pages", I32), ("page_size", I32),
     ]
 
+
+class KdaEvictLayer(ctypes.Structure):
+    _fields_ = [("cache", P), ("token_bytes", I64), ("page_stride", I64), ("weights", P), ("weights_row", I64)]
+
+
+class KdaEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("layer", KdaEvictLayer * MAX_POOLS), ("num_layers", I32), ("n", I32),
+        ("src", P), ("block_table", P), ("seq_lens", P), ("ref_counts", P), ("free_pages", P), ("num_free", P),
+        ("workspace", P), ("workspace_bytes", I64), ("table_stride", I64),
+        ("rows", I32), ("table_width", I32), ("pages", I32), ("page_size", I32),
+        ("keep", I32), ("recent", I32), ("flags", U32), ("reserved", I32),
+    ]
+
+
+EVICT_MORE = 1  # KDA355_EVICT_MORE
 
 _lib = None
 _noalloc = None
@@ -165,12 +191,16 @@ def lib():
         L.kda355_prefill_launch.restype = ctypes.c_int
         for name, args in (("latent_prefill", KdaLatentPrefillArgs), ("latent_decode", KdaLatentDecodeArgs),
                            ("latent_append", KdaLatentTokensArgs), ("latent_gather", KdaLatentTokensArgs),
+                           ("latent4_append", KdaLatentTokensArgs), ("latent4_gather", KdaLatentTokensArgs),
+                           ("latent4_decode", KdaLatentDecodeArgs), ("latent_weights", KdaLatentWeightsArgs),
+                           ("evict_tokens", KdaEvictArgs),
                            ("copy_rows", KdaPagesArgs), ("fork_pages", KdaPagesArgs), ("free_pages", KdaPagesArgs),
                            ("compact_pages", KdaPagesArgs)):
             f = getattr(L, f"kda355_{name}_launch")
             f.argtypes = [ctypes.POINTER(args), P]
             f.restype = ctypes.c_int
-        for name, args in (("latent_prefill", KdaLatentPrefillArgs), ("latent_decode", KdaLatentDecodeArgs)):
+        for name, args in (("latent_prefill", KdaLatentPrefillArgs), ("latent_decode", KdaLatentDecodeArgs),
+                           ("evict_tokens", KdaEvictArgs)):
             f = getattr(L, f"kda355_{name}_workspace_bytes")
             f.argtypes = [ctypes.POINTER(args)]
             f.restype = I64
@@ -224,7 +254,9 @@ def exported_symbols():
     return ["kda355_recurrent_launch", "kda355_spec_commit_launch", "kda355_decode_launch", "kda355_prefill_plan",
             "kda355_prefill_workspace_bytes", "kda355_prefill_launch", "kda355_prefill_launch_noalloc",
             "kda355_latent_prefill_workspace_bytes", "kda355_latent_prefill_launch", "kda355_latent_decode_workspace_bytes", "kda355_latent_decode_launch",
-            "kda355_latent_append_launch", "kda355_latent_gather_launch", "kda355_copy_rows_launch",
+            "kda355_latent_append_launch", "kda355_latent_gather_launch", "kda355_latent4_append_launch",
+            "kda355_latent4_gather_launch", "kda355_latent4_decode_launch", "kda355_latent_weights_launch", "kda355_copy_rows_launch",
+            "kda355_evict_tokens_workspace_bytes", "kda355_evict_tokens_launch",
             "kda355_fork_pages_launch", "kda355_free_pages_launch", "kda355_compact_pages_launch",
             "kda355_last_error", "kda355_version"]
 

@@ -3,13 +3,16 @@ layers of a hybrid model.  No counterpart in the reference, which holds KDA laye
 
 Every token leaves one latent vector of 512 values and a positional part of 64 that all heads share (rotated or not, as the
 model has it).  A cache is [pages, page_size, 576] bf16 or fp16: token rows (latent | positional part) dense within a page,
-any page stride; page numbers outside the cache are holes whose tokens take no part.
+any page stride; page numbers outside the cache are holes whose tokens take no part.  Or it is [pages, page_size, 400]
+uint8, with the latent values in 4 bits: 256 bytes of codes, 16 scales, and the positional part in the 16-bit type of the
+calls' other tensors, which then has to be the same in all calls for this cache.
 
     latent_append(latent, k_pe, cache, slots)                              # token rows into their pages
     rows = latent_gather(cache, block_table, cu_seqlens, out)              # and back, dense
     o = latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k)          # expanded form, packed sequences
     o = latent_decode(q_latent, q_pe, cache, block_table, seq_lens)        # absorbed form, S tokens a sequence
     o = latent_decode(..., prefix_table=pages, prefix_len=n)               # the same behind one shared prefix
+    latent_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights)  # what that step gave every cached token
 
 The expanded form takes keys and values as the up-projection leaves them (views with any token and head stride), the
 absorbed form queries that carry the key up-projection, and returns outputs in the latent space.  The default scale is
@@ -30,6 +33,7 @@ from .recurrent import _need
 
 LATENT, PE, HEAD = 512, 64, 128
 ROW = LATENT + PE
+ROW_4BIT = LATENT // 2 + LATENT // 32 + 2 * PE  # codes, scales of 32 values, the positional part: bytes of a uint8 cache's rows
 SCALE = (HEAD + PE) ** -0.5
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _cus = {}
@@ -107,16 +111,21 @@ def _table(name, t, device):
 
 
 def _cache(cache, dtype, device):
-    """(pages, page_size, page stride) of a cache."""
+    """(pages, page_size, page stride in elements, bits of a latent value) of a cache in `dtype` or in 4 bits."""
+    bits = 4 if isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8 else 16
+    if bits == 4:
+        dtype, row = torch.uint8, ROW_4BIT
+    else:
+        row = ROW
     if not isinstance(cache, torch.Tensor) or cache.dtype is not dtype or cache.device != device:
         _need("cache", cache, dtype, device)
     sh, st = cache.shape, cache.stride()
-    if len(sh) != 3 or sh[2] != ROW or sh[0] < 1 or sh[1] < 1:
-        raise ValueError(f"kda355: cache must be [pages, page_size, {ROW}], got {list(sh)}")
+    if len(sh) != 3 or sh[2] != row or sh[0] < 1 or sh[1] < 1:
+        raise ValueError(f"kda355: cache must be [pages, page_size, {row}], got {list(sh)}")
     pages, size, _ = sh
-    if st[2] != 1 or (size > 1 and st[1] != ROW):
+    if st[2] != 1 or (size > 1 and st[1] != row):
         raise ValueError("kda355: cache must be dense within a page")
-    return pages, size, st[0] if pages > 1 else size * ROW
+    return pages, size, st[0] if pages > 1 else size * row, bits
 
 
 def _workspace(need, workspace, device):
@@ -141,7 +150,7 @@ def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-_prefill_seen, _decode_seen, _append_seen, _gather_seen = {}, {}, {}, {}
+_prefill_seen, _decode_seen, _append_seen, _gather_seen, _weights_seen = {}, {}, {}, {}, {}
 _PTR2, _PTR7, _PTR8, _PTR10 = (struct.Struct(f"{n}Q") for n in (2, 7, 8, 10))
 
 
@@ -208,13 +217,13 @@ def latent_prefill_workspace_bytes(N, H, Tq, Tk, *, num_cus=256):
 
 
 def _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, prefix_table, prefix_len):
-    """(device, dtype, out shape, bytes of workspace, struct bytes behind the pointers)."""
+    """(device, dtype, out shape, bytes of workspace, struct bytes behind the pointers, C entry)."""
     dev, dt = _first("q_latent", q_latent)
     if q_latent.dim() != 3 or q_latent.shape[2] != LATENT:
         raise ValueError(f"kda355: q_latent must be [B * S, H, {LATENT}], got {list(q_latent.shape)}")
     T, H = q_latent.shape[0], q_latent.shape[1]
     strides = _rows("q_latent", q_latent, (T, H, LATENT), dt, dev) + _rows("q_pe", q_pe, (T, H, PE), dt, dev)
-    pages, size, page_stride = _cache(cache, dt, dev)
+    pages, size, page_stride, bits = _cache(cache, dt, dev)
     table_stride = _table("block_table", block_table, dev)
     B = block_table.shape[0]
     _index("seq_lens", seq_lens, (B,), dev)
@@ -236,12 +245,12 @@ def _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, 
     a = _lib.KdaLatentDecodeArgs(*[None] * 10, *strides, page_stride, pages, table_stride, 0, B, S, H, size, block_table.shape[1],
                                  width, _DTYPES[dt], _num_cus(dev), scale, 0)
     a.workspace_bytes = need = _bytes_needed("latent_decode", a)
-    return dev, dt, (T, H, LATENT), need, bytes(a)[_PTR10.size:]
+    return dev, dt, (T, H, LATENT), need, bytes(a)[_PTR10.size:], "latent_decode" if bits == 16 else "latent4_decode"
 
 
 def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, out=None, lse=None, prefix_table=None,
                   prefix_len=None, workspace=None):
-    """The absorbed form over the paged cache: q_latent [B * S, H, 512] and q_pe [B * S, H, 64], S tokens a sequence (row
+    """The absorbed form over the paged cache (16 or 4 bits): q_latent [B * S, H, 512] and q_pe [B * S, H, 64], S tokens a sequence (row
     n * S + s), block_table int32 [B, width], seq_lens int32 [B] the cached tokens of each sequence, its S new ones among
     them (token s sees j < seq_lens[n] - (S - 1 - s)).  Returns out [B * S, H, 512] in the latent space; `lse` (fp32
     [B * S, H]) as in latent_prefill.
@@ -264,7 +273,7 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
     if plan is None:
         plan = _keep(_decode_seen, key, _plan_decode(q_latent, q_pe, cache, block_table, seq_lens, scale, out, lse, prefix_table,
                                                      prefix_len))
-    dev, dt, shape, need, tail = plan
+    dev, dt, shape, need, tail, entry = plan
     if out is None:
         out = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=dt, device=dev)  # (0.4 us less than empty)
     ws = _workspace(need, workspace, dev)
@@ -272,7 +281,7 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
                         0 if prefix_table is None else prefix_table.data_ptr(),
                         0 if prefix_len is None else prefix_len.data_ptr(),
                         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr()) + tail)
-    rc = _lib.LAUNCH["latent_decode"](args, _stream(dev))
+    rc = _lib.LAUNCH[entry](args, _stream(dev))
     if rc:
         _lib.check(rc, "latent_decode")
     return out
@@ -286,7 +295,11 @@ def latent_decode_workspace_bytes(B, S, H, page_size, table_width, prefix_width=
 
 def latent_append(latent, k_pe, cache, slots):
     """cache row slots[t] (= page * page_size + offset, int64 [T]) <- latent [T, 512] | k_pe [T, 64]; slots outside the cache
-    (padding: -1) are skipped.  The cache is written in place and returned."""
+    (padding: -1) are skipped.  The cache is written in place and returned.
+
+    Into a uint8 cache 32 consecutive latent values are rounded to codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) of one
+    power of two: with a the largest size among them, 2^(floor(log2 a) - 2), and the next power where a is over 7 of it; to the
+    nearest code, ties to the even one.  A group with an infinite value or a NaN reads as NaN throughout."""
     try:
         key = (latent.shape, latent.stride(), latent.dtype, latent.device, k_pe.shape, k_pe.stride(), k_pe.dtype, k_pe.device,
                cache.shape, cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
@@ -297,13 +310,13 @@ def latent_append(latent, k_pe, cache, slots):
         dev, dt = _first("latent", latent)
         T = latent.shape[0] if latent.dim() else 0
         strides = _rows("latent", latent, (T, LATENT), dt, dev) + _rows("k_pe", k_pe, (T, PE), dt, dev)
-        pages, size, page_stride = _cache(cache, dt, dev)
+        pages, size, page_stride, bits = _cache(cache, dt, dev)
         _index("slots", slots, (T,), dev, torch.int64)
-        a = _lib.KdaLatentTokensArgs(*[None] * 7, *strides, 0, page_stride, pages, 0, T, size, 0, 0, 0)
-        plan = _keep(_append_seen, key, (dev, bytes(a)[_PTR7.size:]))
-    dev, tail = plan
+        a = _lib.KdaLatentTokensArgs(*[None] * 7, *strides, 0, page_stride, pages, 0, T, size, 0, 0, _DTYPES[dt])
+        plan = _keep(_append_seen, key, (dev, bytes(a)[_PTR7.size:], "latent_append" if bits == 16 else "latent4_append"))
+    dev, tail, entry = plan
     args = _PTR7.pack(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), 0, 0, 0) + tail
-    rc = _lib.LAUNCH["latent_append"](args, _stream(dev))
+    rc = _lib.LAUNCH[entry](args, _stream(dev))
     if rc:
         _lib.check(rc, "latent_append")
     return cache
@@ -320,19 +333,74 @@ def latent_gather(cache, block_table, cu_seqlens, out):
     except (AttributeError, TypeError):  # something that is no tensor: the checks say what
         key = plan = None
     if plan is None:
-        dev, dt = _first("cache", cache)
-        pages, size, page_stride = _cache(cache, dt, dev)
+        dev, dt = _first("out", out) if isinstance(cache, torch.Tensor) and cache.dtype is torch.uint8 else _first("cache", cache)
+        pages, size, page_stride, bits = _cache(cache, dt, dev)
         table_stride = _table("block_table", block_table, dev)
         N = block_table.shape[0]
         _index("cu_seqlens", cu_seqlens, (N + 1,), dev)
         T = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() else 0
         o_st = _rows("out", out, (T, ROW), dt, dev)
         a = _lib.KdaLatentTokensArgs(*[None] * 7, 0, 0, *o_st, page_stride, pages, table_stride, T, size, block_table.shape[1], N,
-                                     0)
-        plan = _keep(_gather_seen, key, (dev, bytes(a)[_PTR7.size:]))
-    dev, tail = plan
+                                     _DTYPES[dt])
+        plan = _keep(_gather_seen, key, (dev, bytes(a)[_PTR7.size:], "latent_gather" if bits == 16 else "latent4_gather"))
+    dev, tail, entry = plan
     args = _PTR7.pack(0, 0, cache.data_ptr(), 0, block_table.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr()) + tail
-    rc = _lib.LAUNCH["latent_gather"](args, _stream(dev))
+    rc = _lib.LAUNCH[entry](args, _stream(dev))
     if rc:
         _lib.check(rc, "latent_gather")
     return out
+
+
+def _plan_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, scale):
+    """(device, struct bytes behind the pointers)"""
+    dev, dt = _first("q_latent", q_latent)
+    if q_latent.dim() != 3 or q_latent.shape[2] != LATENT:
+        raise ValueError(f"kda355: q_latent must be [B * S, H, {LATENT}], got {list(q_latent.shape)}")
+    T, H = q_latent.shape[0], q_latent.shape[1]
+    strides = _rows("q_latent", q_latent, (T, H, LATENT), dt, dev) + _rows("q_pe", q_pe, (T, H, PE), dt, dev)
+    pages, size, page_stride, bits = _cache(cache, dt, dev)
+    table_stride = _table("block_table", block_table, dev)
+    B, width = block_table.shape
+    _index("seq_lens", seq_lens, (B,), dev)
+    if T % B or T < B if B else T:
+        raise ValueError(f"kda355: {T} rows of q_latent are not B x S for B = {B}")
+    _index("lse", lse, (T, H), dev, torch.float32)
+    if not isinstance(weights, torch.Tensor) or weights.dtype is not torch.float32 or weights.device != dev:
+        _need("weights", weights, torch.float32, dev)
+    sh, st = weights.shape, weights.stride()
+    if len(sh) != 2 or sh[0] != B or sh[1] < width * size or (sh[1] > 1 and st[1] != 1):
+        raise ValueError(f"kda355: weights must be [{B}, >= {width * size}] with dense rows, got {list(sh)}")
+    row = st[0] if B > 1 else sh[1]
+    if row < sh[1]:
+        raise ValueError("kda355: rows of weights overlap")
+    a = _lib.KdaLatentWeightsArgs(*[None] * 7, *strides, row, page_stride, pages, table_stride, B, max(1, T // B) if B else 1, H, size,
+                                  width, _DTYPES[dt], bits, _num_cus(dev), scale, 0)
+    return dev, bytes(a)[_PTR7.size:]
+
+
+def latent_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, scale=None):
+    """weights[n, j] += what a step of latent_decode gave token j of sequence n: the sum over the S * H rows that see it of their
+    softmax weights e^(z - lse).  The arguments are the step's, lse (fp32 [B * S, H]) is what it left; behind a shared prefix
+    only the sequences' own tokens are written.  weights is fp32 [B, >= width * page_size] with dense rows, written in place and
+    returned; tokens in holes and places past the tokens stay as they are.
+
+    Kept from step to step this is the accumulated attention weight that evict_tokens goes by: clear the row of a sequence that
+    begins anew, copy it (copy_rows) where one is forked."""
+    scale = SCALE if scale is None else float(scale)  # (what is kept is keyed by its value)
+    try:
+        key = (q_latent.shape, q_latent.stride(), q_latent.dtype, q_latent.device, q_pe.shape, q_pe.stride(), q_pe.dtype,
+               q_pe.device, cache.shape, cache.stride(), cache.dtype, cache.device, block_table.shape, block_table.stride(),
+               block_table.dtype, block_table.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, lse.shape,
+               lse.stride(), lse.dtype, lse.device, weights.shape, weights.stride(), weights.dtype, weights.device, scale)
+        plan = _weights_seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        plan = _keep(_weights_seen, key, _plan_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, scale))
+    dev, tail = plan
+    args = _PTR7.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                      lse.data_ptr(), weights.data_ptr()) + tail
+    rc = _lib.LAUNCH["latent_weights"](args, _stream(dev))
+    if rc:
+        _lib.check(rc, "latent_weights")
+    return weights

@@ -18,7 +18,7 @@ registered ops with mutation annotations and fake implementations instead of opa
                        (kda/mi350x/benchmark/vllm_reference/kda.py:488-502).
   spec_commit          copies each sequence's accepted per-token state into its pool row.
   latent_*             latent attention and its paged cache (kda355/latent.py), `out` given by the caller.
-  copy_rows, fork_pages, free_pages, compact_pages
+  copy_rows, fork_pages, free_pages, compact_pages, evict_tokens
                        pages of a cache (kda355/pages.py).
 
 Every op is implemented for the CUDA dispatch key only and calls the HIP kernels of libkda355.so; on CPU tensors the
@@ -82,6 +82,9 @@ SCHEMAS = {
         "latent_append(Tensor latent, Tensor k_pe, Tensor(a!) cache, Tensor slots) -> ()",
     "latent_gather":
         "latent_gather(Tensor cache, Tensor block_table, Tensor cu_seqlens, Tensor(a!) out) -> ()",
+    "latent_weights":
+        "latent_weights(Tensor q_latent, Tensor q_pe, Tensor cache, Tensor block_table, Tensor seq_lens, Tensor lse, "
+        "Tensor(a!) weights, float? scale=None) -> ()",
     "copy_rows":
         "copy_rows(Tensor(a!)[] pools, Tensor src, Tensor dst) -> ()",
     "fork_pages":
@@ -93,6 +96,10 @@ SCHEMAS = {
     "compact_pages":
         "compact_pages(Tensor(a!)[] pools, Tensor(b!) block_table, Tensor(c!) ref_counts, Tensor(d!) free_pages, "
         "Tensor(e!) num_free) -> ()",
+    "evict_tokens":
+        "evict_tokens(Tensor(a!)[] pools, Tensor(b!)[] weights, Tensor(c!) block_table, Tensor(d!) seq_lens, "
+        "Tensor(e!) ref_counts, Tensor(f!) free_pages, Tensor(g!) num_free, Tensor rows, int keep, int recent, "
+        "int page_size) -> ()",
 }
 
 
@@ -249,6 +256,10 @@ def _latent_gather_op(cache, block_table, cu_seqlens, out):
     _latent.latent_gather(cache, block_table, cu_seqlens, out)
 
 
+def _latent_weights_op(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, scale=None):
+    _latent.latent_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, scale)
+
+
 _IMPLS = {
     "fused_kda_decode": _fused_kda_decode,
     "fused_kda_prefill": _fused_kda_prefill,
@@ -260,10 +271,12 @@ _IMPLS = {
     "latent_decode": _latent_decode_op,
     "latent_append": _latent_append_op,
     "latent_gather": _latent_gather_op,
+    "latent_weights": _latent_weights_op,
     "copy_rows": _pages.copy_rows,
     "fork_pages": _pages.fork_pages,
     "free_pages": _pages.free_pages,
     "compact_pages": _pages.compact_pages,
+    "evict_tokens": _pages.evict_tokens,
 }
 
 

@@ -1,5 +1,5 @@
-"""Pages of a cache (host side of kda355_{copy_rows, fork_pages, free_pages, compact_pages}_launch): sequences forked, freed
-and compacted on the device, with the copies in every layer's pool.  No counterpart in the reference (its caller manages
+"""Pages of a cache (host side of kda355_{copy_rows, fork_pages, free_pages, compact_pages, evict_tokens}_launch): sequences
+forked, freed, compacted and cut to a budget of tokens on the device, with the copies in every layer's pool.  No counterpart in the reference (its caller manages
 slots on the host).
 
 The bookkeeping is five int32 tensors that the caller keeps on the device:
@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from .latent import _index, _keep, _stream, _table
+from .recurrent import _need
 
 
 def _sequence(pools):
@@ -210,3 +211,85 @@ def compact_pages(pools, block_table, ref_counts, free_pages, num_free):
     half = pages // 2
     if half and len(flat) > most:
         _copy(dev, flat[most:], half, at + 4 * pages, at + 4 * (pages + half))
+
+
+_LAYER = struct.Struct("=5q")
+_EVICT = struct.Struct("=2i7Q2q6iIi")
+assert _LAYER.size * _lib.MAX_POOLS + _EVICT.size == ctypes.sizeof(_lib.KdaEvictArgs)
+
+
+def _check_evict(pools, weights, block_table, seq_lens, ref_counts, free_pages, num_free, rows, keep, recent, page_size):
+    """(device, table stride, rows, width, pages, [(token bytes, page stride, weights stride)], bytes of workspace of each call)"""
+    dev, pages, stride, count, width = _book(block_table, ref_counts, free_pages, num_free)
+    _index("seq_lens", seq_lens, (count,), dev)
+    n = rows.numel() if isinstance(rows, torch.Tensor) else 0
+    _index("rows", rows, (n,), dev)
+    if len(pools) != len(weights) or not pools:
+        raise ValueError(f"kda355: {len(pools)} pools and {len(weights)} weights: one of each for every layer")
+    pool_dev, found = _pools(pools, pages)
+    if pool_dev != dev:
+        raise TypeError(f"kda355: pools must be on {dev}, got {pool_dev}")
+    layers = []
+    for i, (t, p, w) in enumerate(zip(pools, found, weights)):
+        if p is None or t.dim() < 2 or t.shape[1] != page_size:
+            raise ValueError(f"kda355: pool {i} must be [pages, {page_size}, ...], got {list(t.shape)}")
+        if not isinstance(w, torch.Tensor) or w.dtype is not torch.float32 or w.device != dev:
+            _need(f"weights {i}", w, torch.float32, dev)
+        sh, st = w.shape, w.stride()
+        if len(sh) != 2 or sh[0] != count or sh[1] < width * page_size or (sh[1] > 1 and st[1] != 1):
+            raise ValueError(f"kda355: weights {i} must be [{count}, >= {width * page_size}] with dense rows, got {list(sh)}")
+        row = st[0] if count > 1 else sh[1]
+        if row < sh[1]:
+            raise ValueError(f"kda355: rows of weights {i} overlap")
+        layers.append((p[0] // page_size, p[1], row))
+    need = []
+    for i in range(0, len(layers), _lib.MAX_POOLS):
+        a = _lib.KdaEvictArgs(num_layers=len(layers[i:i + _lib.MAX_POOLS]), n=n, rows=count, table_width=width, pages=pages,
+                              page_size=page_size, keep=keep, recent=recent)
+        need.append(_lib.lib().kda355_evict_tokens_workspace_bytes(ctypes.byref(a)))
+        if need[-1] < 0:
+            _lib.check(int(need[-1]), "evict_tokens")
+    return dev, stride, count, width, pages, layers, need
+
+
+def evict_tokens(pools, weights, block_table, seq_lens, ref_counts, free_pages, num_free, rows, keep, recent, page_size):
+    """Cuts the sequences rows[i] (int32 [n] rows of block_table) that are longer than `keep` tokens to `keep`, in every layer:
+    pools[l] is [pages, page_size, ...] with token rows of a multiple of 16 bytes, weights[l] fp32 [rows, >= width * page_size]
+    what latent_weights added up for the layer.
+
+    The `recent` last tokens stay, and so do all up to the end of the sequence's last page that others hold too.  Of the tokens
+    between, those with the largest weights of the layer stay, as many as make `keep` in all (ties: the lower index; a NaN is
+    larger than any number).  With left = keep - recent, the i-th place below left whose token goes is filled by the i-th staying
+    token from left on; the recent ones follow in order.  Layers choose on their own, so that place j is another token in each.
+    Weights move along, and those of the places that became free are 0.  Pages behind the first ceil(keep / page_size) are given
+    up as in free_pages; pages reserved ahead of the tokens move down in the table behind the kept ones.
+
+    A sequence stays as it is where one of its pages is a hole, or where shared pages and recent tokens are more than `keep`.
+    Rows outside the table are skipped; a row that is given twice is taken once."""
+    pools, weights = _sequence(pools), _sequence(weights)
+    keep, recent, page_size = int(keep), int(recent), int(page_size)  # (what is kept is keyed by their values)
+    try:
+        key = (keep, recent) + _key("evict_tokens", page_size, pools, (block_table, seq_lens, ref_counts, free_pages, num_free, rows, *weights))
+        plan = _seen.get(key)
+    except (AttributeError, TypeError):  # something that is no tensor: the checks say what
+        key = plan = None
+    if plan is None:
+        plan = _keep(_seen, key, _check_evict(pools, weights, block_table, seq_lens, ref_counts, free_pages, num_free, rows, keep,
+                                              recent, page_size))
+    dev, stride, count, width, total, layers, need = plan
+    n = rows.numel()
+    if n == 0:
+        return
+    ws = torch.empty(max(need), dtype=torch.uint8, device=dev)
+    books = (rows.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ref_counts.data_ptr(), free_pages.data_ptr(),
+             num_free.data_ptr(), ws.data_ptr())
+    for c, first in enumerate(range(0, len(layers), _lib.MAX_POOLS)):
+        some = layers[first:first + _lib.MAX_POOLS]
+        args = b"".join([_LAYER.pack(t.data_ptr(), y[0], y[1], w.data_ptr(), y[2])
+                         for t, w, y in zip(pools[first:], weights[first:], some)])
+        more = _lib.EVICT_MORE if first + len(some) < len(layers) else 0
+        args += bytes(_LAYER.size * (_lib.MAX_POOLS - len(some))) + _EVICT.pack(
+            len(some), n, *books, need[c], stride, count, width, total, page_size, keep, recent, more, 0)
+        rc = _lib.LAUNCH["evict_tokens"](args, _stream(dev))
+        if rc:
+            _lib.check(rc, "evict_tokens")

@@ -294,10 +294,17 @@ int kda355_prefill_launch_noalloc(const KdaPrefillArgs* args, kda355_stream_t st
  *
  * Cache: [pages, page_size, 576] in 16-bit elements, the token rows (latent | positional part) dense within a page, any
  * page stride.  Page numbers outside [0, pages) are holes: their tokens are never read and take no part.
+ *
+ * A cache in 4 bits: [pages, page_size, 400] bytes.  A row is 256 bytes of codes (value 2 i in the low half of byte i), 16 scale
+ * bytes of 32 consecutive values each, and the positional part in 16 bits.  A code is a sign (8) and one of 0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6; a scale byte b stands for 2^(b - 127), 255 for NaN (a NaN group).  Readers round code x scale to their 16-bit type: with
+ * what kda355_latent4_append_launch writes for that type the products are numbers of it.
  */
 #define KDA355_LATENT_DIM 512
 #define KDA355_LATENT_PE 64
 #define KDA355_LATENT_ROW 576
+#define KDA355_LATENT_ROW_4BIT 400
+#define KDA355_LATENT_GROUP 32
 #define KDA355_DTYPE_BF16 0
 #define KDA355_DTYPE_FP16 1
 #define KDA355_LATENT_CAUSAL 1u
@@ -370,6 +377,33 @@ typedef struct KdaLatentDecodeArgs {
    for one sequence of 12 heads, 42 MB for 64 of 64 heads, 303 MB for 128 x 8 tokens of 128 heads, 842 MB for 512 x 8 of 96. */
 int64_t kda355_latent_decode_workspace_bytes(const KdaLatentDecodeArgs* args);
 int kda355_latent_decode_launch(const KdaLatentDecodeArgs* args, kda355_stream_t stream);
+/* The same over a cache in 4 bits: page_stride is in bytes, everything else (the workspace too) as above. */
+int kda355_latent4_decode_launch(const KdaLatentDecodeArgs* args, kda355_stream_t stream);
+
+/*
+ * What the cached tokens were given by an attention step of the absorbed form: weights[n, j] += sum over the S * H rows of
+ * sequence n that see token j of e^(z - lse[row]), z as above.  lse is what the step left (NULL is refused): with a shared prefix
+ * its weights count in lse, and only the sequence's own tokens are written.  Rows with an lse of -inf give nothing, tokens in holes
+ * get nothing, weights past the tokens stay as they are.  Sums are fp32, in an order that the sizes alone decide.
+ */
+typedef struct KdaLatentWeightsArgs {
+    const void* q_latent;        /* [B * S, H, 512], strides in elements */
+    const void* q_pe;            /* [B * S, H, 64] */
+    const void* cache;           /* [pages, page_size, 576] in 16 bits or [pages, page_size, 400] bytes */
+    const int32_t* block_table;  /* [B, table_width], row stride table_stride */
+    const int32_t* seq_lens;     /* [B], clamped to [0, table_width * page_size] */
+    const float* lse;            /* [B * S, H] dense */
+    float* weights;              /* [B, table_width * page_size], row stride weights_row */
+    int64_t ql_row, ql_head, qp_row, qp_head, weights_row;
+    int64_t page_stride, pages, table_stride;  /* page_stride: 16-bit elements, bytes of a cache in 4 bits */
+    int32_t B, S, H, page_size, table_width, dtype;
+    int32_t cache_bits;          /* 16 or 4 */
+    int32_t num_cus;             /* CUs to fill (0: 256) */
+    float scale;                 /* positive */
+    uint32_t flags;              /* 0 */
+} KdaLatentWeightsArgs;
+
+int kda355_latent_weights_launch(const KdaLatentWeightsArgs* args, kda355_stream_t stream);
 
 /*
  * Token rows into pages and back.  append: cache row slots[t] (page * page_size + offset) <- latent[t] | k_pe[t]; slots
@@ -385,11 +419,19 @@ typedef struct KdaLatentTokensArgs {
     const int32_t* cu;           /* gather: [N + 1] on the device, not decreasing; rows outside [0, T) are skipped */
     void* out;                   /* gather: [T, 576], row stride out_row */
     int64_t latent_row, pe_row, out_row, page_stride, pages, table_stride, T;
-    int32_t page_size, table_width, N, reserved;
+    int32_t page_size, table_width, N;
+    int32_t dtype;               /* of latent, k_pe and out; looked at for caches in 4 bits only */
 } KdaLatentTokensArgs;
 
 int kda355_latent_append_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
 int kda355_latent_gather_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
+/*
+ * The same with a cache in 4 bits (page_stride in bytes).  append: with a the largest |x| of 32 values, the scale is 2^e,
+ * e = floor(log2 a) - 2, and 1 more where a > 7 x 2^e, in [-125, 125] (bf16) or [-23, 13] (fp16); a value becomes the nearest
+ * code x 2^e, ties to the even code, at most 6 x 2^e, and is off by at most a / 5.  A group with an infinite value or a NaN reads as NaN throughout.
+ */
+int kda355_latent4_append_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
+int kda355_latent4_gather_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ pages of a cache */
 
@@ -439,6 +481,48 @@ int kda355_free_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
    and the stack (pages - 1 down to L, so that L is taken next) follow.  Lists of pages kept elsewhere are not rewritten: keep
    the pages of a shared prefix as a row of block_table. */
 int kda355_compact_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream);
+
+/*
+ * Sequences src[i] cut to `keep` tokens in every layer.  Of a sequence of len > keep tokens stay: the `recent` last; the fixed ones, all
+ * up to the end of its last page with a reference count above 1; and of the others (from there to len - recent) the
+ * keep - recent - fixed with the largest weights of the layer (a NaN is larger than any number, -0 is 0, ties go to the lower index).  With left = keep -
+ * recent, the i-th token below `left` that goes gives its place to the i-th token that stays at or above it, in both the cache
+ * and the weights; the recent ones follow in order.  Weights of places keep .. len - 1 become 0.  Pages behind the first
+ * ceil(keep / page_size) are given up, those that nobody holds any more go onto the stack, the highest first; table entries past
+ * the tokens (pages reserved ahead) move down behind the kept ones.
+ *
+ * A sequence stays as it is where len <= keep, an entry of its tokens' pages is a hole, or fixed > keep - recent.  Rows outside
+ * [0, rows) are skipped, a row that is given twice is taken once.  Results do not depend on timing.
+ */
+typedef struct KdaEvictLayer {
+    void* cache;                 /* [pages, page_size] tokens of token_bytes, dense within a page */
+    int64_t token_bytes;         /* a multiple of 16 */
+    int64_t page_stride;         /* bytes, a multiple of 16 */
+    float* weights;              /* [rows, table_width * page_size] */
+    int64_t weights_row;         /* elements */
+} KdaEvictLayer;
+
+typedef struct KdaEvictArgs {
+    KdaEvictLayer layer[KDA355_MAX_POOLS];
+    int32_t num_layers, n;       /* n: rows given */
+    const int32_t* src;          /* [n] */
+    int32_t* block_table;        /* books as above */
+    int32_t* seq_lens;
+    int32_t* ref_counts;
+    int32_t* free_pages;
+    int32_t* num_free;
+    void* workspace;             /* kda355_evict_tokens_workspace_bytes(args), 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t table_stride;
+    int32_t rows, table_width, pages, page_size;
+    int32_t keep, recent;        /* keep >= 1, 0 <= recent <= keep */
+    uint32_t flags;              /* KDA355_EVICT_MORE: more layers follow in another call, the books stay as they are */
+    int32_t reserved;
+} KdaEvictArgs;
+#define KDA355_EVICT_MORE 1u
+
+int64_t kda355_evict_tokens_workspace_bytes(const KdaEvictArgs* args);
+int kda355_evict_tokens_launch(const KdaEvictArgs* args, kda355_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ misc */
 
