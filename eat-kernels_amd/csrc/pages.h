@@ -38,16 +38,17 @@ __device__ __forceinline__ int load_fresh(const int32_t* p) {
 }
 
 // ------------------------------------------------------------------------------------------------ stack
-__global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a) {
-    __shared__ int sw[SCAN_THREADS / 64];
-    int top = a.num_free[0];
-    top = top < 0 ? 0 : top > a.pages ? a.pages : top;
-    for (int hi = a.pages; hi > 0; hi -= 4 * SCAN_THREADS) {  // four pages a thread, the highest first
+// The pages marked FREED, the highest first, by one workgroup.  FRESH: it marked them itself.
+template <bool FRESH>
+__device__ __forceinline__ void push_freed(int32_t* ref_counts, int32_t* free_pages, int32_t* num_free, int pages, int* sw) {
+    int top = num_free[0];
+    top = top < 0 ? 0 : top > pages ? pages : top;
+    for (int hi = pages; hi > 0; hi -= 4 * SCAN_THREADS) {  // four pages a thread
         int mine[4], count = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int p = hi - 1 - 4 * (int)threadIdx.x - k;
-            mine[k] = p >= 0 && a.ref_counts[p] == FREED;
+            mine[k] = p >= 0 && (FRESH ? load_fresh(ref_counts + p) : ref_counts[p]) == FREED;
             count += mine[k];
         }
         int total;
@@ -56,13 +57,18 @@ __global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a)
         for (int k = 0; k < 4; ++k)
             if (mine[k]) {
                 const int p = hi - 1 - 4 * (int)threadIdx.x - k;
-                a.ref_counts[p] = 0;
-                if (at < a.pages) a.free_pages[at] = p;
+                ref_counts[p] = 0;
+                if (at < pages) free_pages[at] = p;
                 ++at;
             }
         top += total;
     }
-    if (threadIdx.x == 0) a.num_free[0] = top < a.pages ? top : a.pages;
+    if (threadIdx.x == 0) num_free[0] = top < pages ? top : pages;
+}
+
+__global__ void __launch_bounds__(SCAN_THREADS) free_push_kernel(KdaPagesArgs a) {
+    __shared__ int sw[SCAN_THREADS / 64];
+    push_freed<false>(a.ref_counts, a.free_pages, a.num_free, a.pages, sw);
 }
 
 // ------------------------------------------------------------------------------------------------ host
