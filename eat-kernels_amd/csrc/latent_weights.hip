@@ -5,7 +5,8 @@
 // would be 4 bytes a row and token where a cache row is 400 or 1152 for all rows.  Keys stand still: a wave keeps 32 of them in
 // registers as operand rows (16x16x32 instructions; from 4 bits widened as they come), the query rows pass through LDS in tiles of 16,
 // and a lane adds up its row of every tile for its 4 + 4 keys.  One sum across the 16 lanes of a key at the end; no two workgroups
-// write the same token, so the order of a sum depends on the sizes alone.
+// write the same token, so the order of a sum depends on the sizes alone.  Two workgroups a CU, each with an equal run of units of 128
+// keys through the sequences; up to 64 query rows stay in LDS from one unit of a sequence to the next, more come three tiles ahead.
 #include "latent.h"
 
 namespace kda355 {
@@ -15,101 +16,133 @@ constexpr int WAVES = 4, THREADS = WAVES * 64;
 constexpr int KEYS = 32, UNIT = WAVES * KEYS;  // keys of a wave, of a workgroup
 constexpr int RT = 16;                         // query rows of a tile
 constexpr int STEPS = ROW / 32;                // matrix instructions of 16 keys and a tile
-constexpr int Q_LAT = RT * LAT_BYTES, Q_TILE = Q_LAT + RT * PE_BYTES;
+constexpr int Q_LAT = RT * LAT_BYTES, Q_LSE = Q_LAT + RT * PE_BYTES, Q_TILE = Q_LSE + 256, RING = 4;  // tiles in LDS
+constexpr int Q_LOADS = RT / WAVES + 1;        // of a wave a tile
+constexpr int AHEAD = 5;                       // operands read before they are needed
 
 struct Plan {
-    PageOf page;
+    PageOf page, head;  // head: row / H
     int grid;
+    bool dense;         // the rows of a sequence are one head stride apart throughout
 };
 
 __device__ __forceinline__ uint32_t units_of(int tokens) { return ((uint32_t)tokens + UNIT - 1) / UNIT; }
-struct At { int n; uint32_t before; };
-// the sequence that holds unit u of all (n = B: none), and the units before it
-__device__ __forceinline__ At sequence_of(const KdaLatentWeightsArgs& a, uint32_t u) {
+struct Run { uint32_t first, end; int n; uint32_t before; };
+// This workgroup's units [first, end) of all, the sequence that holds the first one, and the units before that sequence.
+__device__ __forceinline__ Run run_of(const KdaLatentWeightsArgs& a) {
     const int lane = threadIdx.x & 63;
-    uint32_t before = 0;
+    auto load = [&](int n) { return n < a.B ? units_of(tokens_of(a.seq_lens[n], a.table_width, a.page_size)) : 0u; };
+    const uint32_t mine = load(lane);  // (loaded once where there are no more sequences)
+    uint32_t all = mine;
+    for (int n = lane + 64; n < a.B; n += 64) all += load(n);
+    all = __builtin_amdgcn_readlane(scan_wave((int)all), 63);
+    const uint32_t b = xcd_task(blockIdx.x, gridDim.x);  // neighbours read the same queries: on one XCD
+    Run r = {(uint32_t)((uint64_t)b * all / gridDim.x), (uint32_t)((uint64_t)(b + 1) * all / gridDim.x), a.B, 0};
     for (int n0 = 0; n0 < a.B; n0 += 64) {
-        const int n = n0 + lane;
-        const uint32_t t = n < a.B ? units_of(tokens_of(a.seq_lens[n], a.table_width, a.page_size)) : 0u;
-        const uint32_t s = (uint32_t)scan_wave((int)t);
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + s > u);
+        const uint32_t t = n0 ? load(n0 + lane) : mine, s = (uint32_t)scan_wave((int)t);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(r.before + s > r.first);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            return {n0 + l, before + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(t, l)};
+            r.n = n0 + l;
+            r.before += __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(t, l);
+            break;
         }
-        before += __builtin_amdgcn_readlane(s, 63);
+        r.before += __builtin_amdgcn_readlane(s, 63);
     }
-    return {a.B, before};
+    return r;
 }
 
-// A key's operand of step i: 8 values of a lane quarter.  In 16 bits values 32 i + 8 quad ..; from 4 bits, where 16 bytes are the 32 values of
-// one scale, step 4 j + e has values 128 j + 32 quad + 8 e ... (the order of the contraction is free).  Returns the 16-byte piece of a query row.
+// Latent row b of a tile stands at 1024 b, its piece p at place (p % 16) ^ turn(b) of each 16.  16-byte reads go 16 lanes at a time, lanes 0
+// .. 3, 12 .. 15, 20 .. 23 and 24 .. 27 of 32 and the others: with these turns they touch all 16 places.
 template <bool Q4>
-__device__ __forceinline__ int piece_of(int i, int quad) {
-    if (i >= 16) return 4 * (i - 16) + quad;  // of the positional part
-    return Q4 ? 16 * (i >> 2) + 4 * quad + (i & 3) : 4 * i + quad;
-}
+__device__ __forceinline__ int turn(int b) { return (b & 3) << 2 | (Q4 ? b >> 2 & 3 : (b >> 3 & 1) << 1); }
 
 template <typename T, bool Q4>
 __global__ void __launch_bounds__(THREADS, 2) weights_kernel(KdaLatentWeightsArgs a, Plan p) {
-    __shared__ __align__(1024) unsigned char sm[2 * Q_TILE];
+    static_assert(2 * RING * Q_TILE <= 160 * 1024, "");
+    __shared__ __align__(1024) unsigned char sm[RING * Q_TILE];
     const uint32_t lds = lds_offset(sm);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int c = lane & 15, quad = lane >> 4;
     const int rows = a.S * a.H, tiles = (rows + RT - 1) / RT;
     constexpr int CACHE_ROW = Q4 ? ROW4 : ROW_BYTES;
     const int64_t page_bytes = Q4 ? a.page_stride : a.page_stride * 2;
+    // A key's operand of step i < 16 has of a lane quarter values 32 i + 8 quad .., from 4 bits, where 16 bytes are the 32 values of one scale,
+    // 128 (i / 4) + 32 quad + 8 (i % 4) .. (the order of the contraction is free): piece 4 i + quad of a query row, or 16 (i / 4) + 4 quad +
+    // i % 4.  Steps 16 and 17: pieces quad and 4 + quad of its positional part.
+    const uint32_t at_latent = c * LAT_BYTES + (((Q4 ? quad << 2 : quad) ^ turn<Q4>(c)) << 4), at_pe = Q_LAT + c * PE_BYTES + ((quad ^ swz8(c)) << 4);
+    const Run run = run_of(a);
+    int n = run.n, held = -1;  // held: the sequence whose query rows are all in LDS
+    uint32_t before = run.before;
+    int tokens = 0;
+    uint32_t units = 0;
 
-    for (uint32_t u = blockIdx.x;; u += gridDim.x) {
-        const At at = sequence_of(a, u);
-        if (at.n >= a.B) return;
-        const int n = __builtin_amdgcn_readfirstlane(at.n);
-        const int tokens = __builtin_amdgcn_readfirstlane(tokens_of(a.seq_lens[n], a.table_width, a.page_size));
-        const int k0 = __builtin_amdgcn_readfirstlane((int)((u - at.before) * UNIT) + KEYS * w);
+    for (uint32_t u = run.first; u < run.end; ++u) {
+        while (n < a.B) {  // (sequences without tokens have no units)
+            tokens = __builtin_amdgcn_readfirstlane(tokens_of(a.seq_lens[n], a.table_width, a.page_size));
+            units = units_of(tokens);
+            if (u < before + units) break;
+            before += units;
+            ++n;
+        }
+        n = __builtin_amdgcn_readfirstlane(n);
+        const int k0 = __builtin_amdgcn_readfirstlane((int)((u - before) * UNIT) + KEYS * w);
 
-        // ---- query rows: latent row b of a tile at 1024 b, its piece p at place (p % 16) ^ swz16(b) of each 16, positional parts as rows of 8
+        // ---- query rows
+        const char* const ql = static_cast<const char*>(a.q_latent) + n * (int64_t)a.S * a.ql_row * 2;
+        const char* const qp = static_cast<const char*>(a.q_pe) + n * (int64_t)a.S * a.qp_row * 2;
         auto bring = [&](int tile) {
-            const uint32_t to = lds + (tile & 1) * Q_TILE;
+            const uint32_t to = lds + tile % RING * Q_TILE;
+            const int first = tile * RT;
+            uint64_t row[RT / WAVES];  // of the wave's latent rows
+            int64_t pe;                // to the lane's row of positional parts
+            if (p.dense) {
+#pragma unroll
+                for (int i = 0; i < RT / WAVES; ++i)
+                    row[i] = (uint64_t)ql + (uint64_t)(uint32_t)min(first + w * (RT / WAVES) + i, rows - 1) * (uint64_t)(2 * a.ql_head);
+                pe = min(first + 8 * (w & 1) + (lane >> 3), rows - 1) * (2 * a.qp_head);
+            } else {
+                auto at = [&](int r, int64_t stride, int64_t head) {
+                    r = min(r, rows - 1);
+                    const uint32_t s = p.head(r);
+                    return 2 * (s * stride + (r - (int)s * a.H) * head);
+                };
+#pragma unroll
+                for (int i = 0; i < RT / WAVES; ++i) row[i] = (uint64_t)ql + at(first + w * (RT / WAVES) + i, a.ql_row, a.ql_head);
+                pe = at(first + 8 * (w & 1) + (lane >> 3), a.qp_row, a.qp_head);
+            }
 #pragma unroll
             for (int i = 0; i < RT / WAVES; ++i) {
-                const int b = w * (RT / WAVES) + i, r = min(tile * RT + b, rows - 1), s = r / a.H, h = r - s * a.H;
-                const uint16_t* row = static_cast<const uint16_t*>(a.q_latent) + (n * (int64_t)a.S + s) * a.ql_row + h * a.ql_head;
-                load_block<0>(to + b * LAT_BYTES, (uint64_t)row + (((lane & 48) | ((lane & 15) ^ swz16(b))) << 4));
+                const int b = w * (RT / WAVES) + i;
+                load_block_from(to + b * LAT_BYTES, row[i], ((lane & 48) | ((lane & 15) ^ turn<Q4>(b))) << 4);
             }
-            if (w < 2) {
-                const int b = 8 * w + (lane >> 3), r = min(tile * RT + b, rows - 1), s = r / a.H, h = r - s * a.H;
-                const uint16_t* row = static_cast<const uint16_t*>(a.q_pe) + (n * (int64_t)a.S + s) * a.qp_row + h * a.qp_head;
-                load_block<0>(to + Q_LAT + 8 * w * PE_BYTES, (uint64_t)row + (((lane & 7) ^ swz8(b)) << 4));
-            }
+            if (w < 2)
+                load_block<0>(to + Q_LAT + 8 * w * PE_BYTES, (uint64_t)qp + pe + (((lane & 7) ^ swz8(8 * w + (lane >> 3))) << 4));
+            else  // the rows' log-sums, by both others: a compiler's load would be waited for with everything that is under way
+                load_words(to + Q_LSE, (uint64_t)(a.lse + n * (int64_t)rows + min(first + c, rows - 1)));
         };
-        auto lse_of = [&](int tile) {  // of the lane's row; -inf: it gives nothing
-            const int r = tile * RT + c;
-            return r < rows ? a.lse[n * (int64_t)rows + r] : -INFINITY;
-        };
-        bring(0);
-        float lse = lse_of(0);
-
         // ---- keys
         u32x4 kf[2][STEPS];
         bool there[2];
+        uint64_t from[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             const int key = k0 + 16 * y + c;
             const uint32_t pg = p.page((uint32_t)key);
             const int page = key < tokens ? a.block_table[n * a.table_stride + pg] : -1;
             there[y] = page >= 0 && page < a.pages;
-            uint64_t from = (uint64_t)a.cache + page * page_bytes + (int64_t)((uint32_t)key - pg * (uint32_t)a.page_size) * CACHE_ROW;
-            asm volatile("" : "+v"(from));  // (a choice of two, not a branch)
-            const char* row = reinterpret_cast<const char*>(there[y] ? from : (uint64_t)zero_row);
+            from[y] = (uint64_t)a.cache + page * page_bytes + (int64_t)((uint32_t)key - pg * (uint32_t)a.page_size) * CACHE_ROW;
+            asm volatile("" : "+v"(from[y]));  // (a choice of two, not a branch)
+            from[y] = there[y] ? from[y] : (uint64_t)zero_row;
+        }
+        u32x4 scales[2], codes[2][4];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const char* row = reinterpret_cast<const char*>(from[y]);
             if constexpr (Q4) {
-                const u32x4 scales = *reinterpret_cast<const u32x4*>(row + SCALES4);
+                scales[y] = *reinterpret_cast<const u32x4*>(row + SCALES4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const u32x4 codes = *reinterpret_cast<const u32x4*>(row + 64 * j + 16 * quad);
-                    const float scale = __uint_as_float((scales[j] >> 8 * quad & 255u) << 23);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kf[y][4 * j + e] = T::from4(codes[e], scale);
-                }
+                for (int j = 0; j < 4; ++j) codes[y][j] = *reinterpret_cast<const u32x4*>(row + 64 * j + 16 * quad);
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) kf[y][i] = *reinterpret_cast<const u32x4*>(row + 64 * i + 16 * quad);
@@ -118,49 +151,79 @@ __global__ void __launch_bounds__(THREADS, 2) weights_kernel(KdaLatentWeightsArg
             for (int i = 0; i < 2; ++i)
                 kf[y][16 + i] = *reinterpret_cast<const u32x4*>(row + (Q4 ? PE4 : LAT_BYTES) + 64 * i + 16 * quad);
         }
-        // of key 16 y + 4 quad + r: is it there
-        uint32_t mine = 0;
+        // what lane c < 8 adds to: key 16 (c / 4) + 4 quad + c % 4
+        uint32_t mine = 0;  // of key 16 y + 4 quad + r: is it there
 #pragma unroll
         for (int y = 0; y < 2; ++y) mine |= ((uint32_t)__builtin_amdgcn_ballot_w64(there[y]) >> 4 * quad & 15u) << 4 * y;
-        wait_loads<0>();
-        __syncthreads();
-
-        float sum[2][4] = {};
-        for (int tile = 0; tile < tiles; ++tile) {
-            const uint32_t from = lds + (tile & 1) * Q_TILE;
-            float next = -INFINITY;
-            if (tile + 1 < tiles) {
-                bring(tile + 1);
-                next = lse_of(tile + 1);
-            }
-            f32x4 z[2][2] = {};
-            auto query = [&](int i) {
-                const int piece = piece_of<Q4>(i, quad);
-                if (i >= 16) return lds_read16(from + Q_LAT + c * PE_BYTES + ((piece ^ swz8(c)) << 4));
-                return lds_read16(from + c * LAT_BYTES + (piece >> 4) * 256 + (((piece & 15) ^ swz16(c)) << 4));
-            };
+        float* const at = a.weights + n * a.weights_row + k0 + 16 * (c >> 2) + 4 * quad + (c & 3);
+        const bool writes = c < 8 && (mine >> c & 1);
+        const float old = writes ? *at : 0.f;
+        // (query rows after the keys' loads: what waits for these does not wait for those)
+        const bool stay = tiles <= RING;
+        if (!stay || held != n) {
+            for (int t = 0; t < min(tiles, stay ? RING : RING - 1); ++t) bring(t);
+            held = stay ? n : -1;
+        }
+        if constexpr (Q4) {
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const u32x4 q = query(i);
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) z[y][i & 1] = T::mfma16(kf[y][i], q, z[y][i & 1]);
-            }
-            const int row = tile * RT + c, left = tokens - (a.S - 1 - row / a.H) - k0 - 4 * quad;  // keys that the row sees, from the lane's first on
+                for (int j = 0; j < 4; ++j) {
+                    const float scale = __uint_as_float((scales[y][j] >> 8 * quad & 255u) << 23);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const f32x4 s = z[y][0] + z[y][1];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    // the difference first: it is small where the weight counts, and so is its rounding
-                    const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -lse) * 1.44269504088896f);
-                    if ((mine >> (4 * y + r) & 1) && 16 * y + r < left && lse != -INFINITY) sum[y][r] += e;
+                    for (int e = 0; e < 4; ++e) kf[y][4 * j + e] = T::from4(codes[y][j][e], scale);
                 }
-            }
-            lse = next;
+        }
+        // every row sees all 32 keys: no masks
+        const bool plain = k0 + KEYS <= tokens - (a.S - 1) && __builtin_amdgcn_ballot_w64(mine != 255u) == 0;
+        if (stay) {
             wait_loads<0>();
             __syncthreads();
         }
-        // ---- the 16 rows of a key's lanes; lane c < 8 writes key 16 (c / 4) + 4 quad + c % 4
+
+        float sum[2][4] = {};
+        for (int tile = 0; tile < tiles; ++tile) {
+            if (!stay) {
+                if (tile + RING - 2 < tiles) wait_loads<(RING - 2) * Q_LOADS>(); else wait_loads<0>();
+                lds_barrier();  // the tile is whole; all have read the one before it
+            }
+            if (!stay && tile + RING - 1 < tiles) bring(tile + RING - 1);
+            const uint32_t from = lds + tile % RING * Q_TILE;
+            const float lse = *reinterpret_cast<const float*>(sm + tile % RING * Q_TILE + Q_LSE + c * 4);
+            f32x4 z[2][2] = {};
+            auto query = [&](int i) {
+                if (i >= 16) return lds_read16((from + at_pe) ^ (i - 16) << 6);
+                return lds_read16(((from + at_latent) ^ (i & 3) << (Q4 ? 4 : 6)) + (i >> 2) * 256);
+            };
+            u32x4 q[AHEAD + 1];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) q[i] = query(i);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + AHEAD < STEPS) q[(i + AHEAD) % (AHEAD + 1)] = query(i + AHEAD);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) z[y][i & 1] = T::mfma16(kf[y][i], q[i % (AHEAD + 1)], z[y][i & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const int row = tile * RT + c;
+            const bool alive = row < rows && lse != -INFINITY;
+            auto add = [&](bool all) {
+                const int left = all ? 0 : tokens - (a.S - 1 - (int)p.head(row)) - k0 - 4 * quad;  // keys that the row sees, from the lane's first on
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const f32x4 s = z[y][0] + z[y][1];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        // the difference first: it is small where the weight counts, and so is its rounding
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale, -lse) * 1.44269504088896f);
+                        if (alive && (all || ((mine >> (4 * y + r) & 1) && 16 * y + r < left))) sum[y][r] += e;
+                    }
+                }
+            };
+            if (plain) add(true); else add(false);
+        }
+        // ---- the 16 rows of a key's lanes
         float out = 0.f;
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -169,10 +232,8 @@ __global__ void __launch_bounds__(THREADS, 2) weights_kernel(KdaLatentWeightsArg
                 const float s = sum16(sum[y][r]);
                 if (c == 4 * y + r) out = s;
             }
-        if (c < 8 && (mine >> c & 1)) {
-            float* x = a.weights + n * a.weights_row + k0 + 16 * (c >> 2) + 4 * quad + (c & 3);
-            *x += out;
-        }
+        if (writes) *at = old + out;
+        if (!stay || u + 1 == before + units) __syncthreads();  // the query rows are read
     }
 }
 
@@ -189,8 +250,8 @@ extern "C" int kda355_latent_weights_launch(const KdaLatentWeightsArgs* a, kda35
     KDA_CHECK_ARG((int64_t)a->S * a->H < (1ll << 29) && (int64_t)a->B * a->S * a->H < (1ll << 29) && a->B < (1 << 22),
                   "latent_weights: B * S * H is too large");
     const int64_t span = (int64_t)a->table_width * a->page_size;
-    KDA_CHECK_ARG(span < (1ll << 31) - UNIT, "latent_weights: a table spans 2^31 tokens or more");
-    KDA_CHECK_ARG(a->B * (span / UNIT + 1) < (1ll << 31), "latent_weights: the tables span 2^38 tokens or more");
+    KDA_CHECK_ARG(span < (1ll << 31) - 256, "latent_weights: a table spans 2^31 tokens or more");
+    KDA_CHECK_ARG(a->B * (span / 128 + 1) < (1ll << 31), "latent_weights: the tables span 2^38 tokens or more");
     KDA_CHECK_ARG(a->dtype == KDA355_DTYPE_BF16 || a->dtype == KDA355_DTYPE_FP16, "latent_weights: dtype %d", a->dtype);
     KDA_CHECK_ARG(a->cache_bits == 16 || a->cache_bits == 4, "latent_weights: cache_bits %d", a->cache_bits);
     KDA_CHECK_ARG(a->flags == 0, "latent_weights: unknown flags 0x%x", a->flags);
@@ -209,6 +270,8 @@ extern "C" int kda355_latent_weights_launch(const KdaLatentWeightsArgs* a, kda35
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     Plan p;
     p.page = PageOf::by(a->page_size);
+    p.head = PageOf::by(a->H);
+    p.dense = a->S == 1 || (a->ql_row == a->H * a->ql_head && a->qp_row == a->H * a->qp_head);
     const int64_t most = a->B * ((span + UNIT - 1) / UNIT), fill = 2 * (a->num_cus ? a->num_cus : 256);
     p.grid = (int)(most < fill ? most : fill);
     auto launch = [&](auto type) {
