@@ -86,6 +86,13 @@ __device__ __forceinline__ void load_block(uint32_t lds, uint64_t src) {
                  "v"(src), "n"(OFFSET)
                  : "memory");
 }
+// the same from a wave's address and a lane's offset (s_nop 4: see load_to_lds)
+__device__ __forceinline__ void load_block_from(uint32_t lds, uint64_t base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_words_from(uint32_t lds, uint64_t base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base) : "memory");
+}
 // 64 lanes x 4 bytes, lane l's to lds + 4 l
 __device__ __forceinline__ void load_words(uint32_t lds, uint64_t src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory");

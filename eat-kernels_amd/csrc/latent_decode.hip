@@ -42,6 +42,8 @@ constexpr uint32_t LEAD = 8, MIN_RUN = 3;
 // workspace: the cut for the second kernel (run, runs of the prefix), then slots, of 32 rows: accumulators, (m, l) of each row
 constexpr int SLOTS = 256, SLOT_ACC = 65536, SLOT_TILE = SLOT_ACC + 256;
 
+__device__ const uint4 zero_rows4[8 * ROW4 / 16] = {};  // what 8 tokens that are not there read, in 4 bits
+
 struct Groups {
     int rows, groups;  // rows of a group, groups
     static Groups of(int64_t n, int most) {
@@ -127,20 +129,20 @@ __device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) 
 constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
 template <bool Q4>
 struct Lds {
-    // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: latent rows of three tiles (one
-    // read for scores, one for values, one being written), positional parts of five, and codes and scales of three as they came.
-    static constexpr int BUFS = Q4 ? 3 : 4, PES = Q4 ? 5 : 4, RAWS = Q4 ? 3 : 0, THERES = Q4 ? 8 : 4;
-    static constexpr int LAT_STEP = Q4 ? LAT_TILE : LAT_TILE + PE_TILE, PE_STEP = Q4 ? PE_TILE : LAT_STEP;
-    static constexpr int PE0 = Q4 ? BUFS * LAT_STEP : LAT_TILE;
-    static constexpr int RAW = Q4 ? PE0 + PES * PE_STEP : BUFS * LAT_STEP, RAW_WAVE = 8 * (LAT / 2) + 256;  // 8 tokens' codes, scales
-    static constexpr int P = RAW + RAWS * VALUE_WAVES * RAW_WAVE;  // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
+    // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: latent rows of two tiles widened (a
+    // value wave reads only what it widened itself), and codes, scales and positional parts of six tiles as they came.  A token's
+    // 16-byte piece p of codes stands at p ^ (t % 16), its scales at 256 (t / 8) + 16 (t % 8).
+    static constexpr int BUFS = Q4 ? 2 : 4, RAWS = Q4 ? 6 : 0, THERES = Q4 ? 8 : 4, PAGE_RING = Q4 ? 8 : 4;
+    static constexpr int LAT_STEP = Q4 ? LAT_TILE : LAT_TILE + PE_TILE, RAW = BUFS * LAT_STEP;
+    static constexpr int RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + VALUE_WAVES * 256, RAW_TILE = RAW_PE + PE_TILE;
+    static constexpr int P = RAW + RAWS * RAW_TILE;      // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
     static constexpr int MAX = P + 2 * 4096;             // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
     static constexpr int FLAG = MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
     static constexpr int THERE = FLAG + 64;              // is the token there [tile % THERES][32] bytes
-    static constexpr int PAGES = THERE + THERES * BN;    // page numbers [value wave][tile % 4][64]
-    static constexpr int BYTES = PAGES + VALUE_WAVES * 4 * 256;
+    static constexpr int PAGES = THERE + THERES * BN;    // page numbers [value wave][tile % PAGE_RING][64]
+    static constexpr int BYTES = PAGES + VALUE_WAVES * PAGE_RING * 256;
     static constexpr int LOADS = Q4 ? 5 : 10;            // of a value wave a tile: codes 2, scales | 8 of latent rows; positional parts, page numbers
-    static_assert(BYTES <= 160 * 1024 && RAW % 1024 == 0 && P % 1024 == 0, "");
+    static_assert(BYTES <= 160 * 1024 && RAW % 1024 == 0 && P % 1024 == 0 && RAW_TILE % 1024 == 0, "");
 };
 
 template <int I>
@@ -154,7 +156,7 @@ __device__ __forceinline__ float join_groups(float x, F f) {
     return f(__uint_as_float(b.x), __uint_as_float(b.y));
 }
 
-template <typename T, int RT, bool Q4>
+template <typename T, int RT, bool Q4, bool EVEN>
 __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
     typedef Lds<Q4> L;
     constexpr int CACHE_ROW = Q4 ? ROW4 : ROW_BYTES;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     uint32_t ra[2];
     if (scores) {
         const int t = 16 * kh + c16;
-        ra[0] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
+        ra[0] = Q4 ? t * SCALES4 + ((quad ^ c16) << 4) : (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
         ra[1] = t * PE_BYTES + ((quad ^ swz8(t)) << 4);
     } else {
 #pragma unroll
@@ -189,8 +191,9 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         }
     }
 
-    auto lat_at = [&](uint32_t tile) { return lds + tile % L::BUFS * L::LAT_STEP; };        // a tile's latent rows
-    auto pe_at = [&](uint32_t tile) { return lds + L::PE0 + tile % L::PES * L::PE_STEP; };  // and positional parts
+    auto lat_at = [&](uint32_t tile) { return lds + tile % L::BUFS * L::LAT_STEP; };  // a tile's latent rows
+    auto raw_at = [&](uint32_t tile) { return lds + L::RAW + tile % 6 * L::RAW_TILE; };  // what came of it in 4 bits
+    auto pe_at = [&](uint32_t tile) { return Q4 ? raw_at(tile) + L::RAW_PE : lat_at(tile) + LAT_TILE; };  // its positional parts
 
     uint32_t own = 0;
     for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
@@ -258,13 +261,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         if (scores) {
             // ================================================================ score waves
             const int row0 = r0 + 16 * RT * rw + c16;  // this lane's rows: row0, and with two row tiles row0 + 16
-            // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: t0 + 1 and t0 + 2), a row tile in each, laid out like keys, half of a wave's
+            // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: of both widened tiles), a row tile in each, laid out like keys, half of a wave's
             // rows by it and half by the other wave that has them (rows past the end repeat the last one).  (Straight into registers,
             // 64 bytes of 16 rows at a time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of
             // 64 heads; 1900 and 4800 so.)
             int mine[RT];
-            const uint32_t qt = t0 + (Q4 ? 1 : 2) + (RT > 1 ? rw : 0), qb = lat_at(qt);
-            const uint32_t qpe = Q4 ? lds + L::P + (RT > 1 ? rw : 0) * PE_TILE : pe_at(qt);
+            const uint32_t qt = (Q4 ? 0 : t0 + 2) + (RT > 1 ? rw : 0), qb = lat_at(qt);
+            const uint32_t qpe = Q4 ? lds + L::P + qt * PE_TILE : pe_at(qt);
             const bool some = n_tiles && row0 - c16 < r1;
             auto half_of = [&](int x) { return RT > 1 ? x : rw; };  // of the row tile: where rows row0 + 16 x stand
             {
@@ -307,9 +310,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             if (some)
 #pragma unroll
                 for (int x = 0; x < RT; ++x) {
+                    // Step i of the scores takes values 32 i + 8 quad .., from 4 bits, where a lane reads all 32 of a scale, 128 (i / 4) +
+                    // 32 quad + 8 (i % 4) .. (the order of the contraction is free).
+                    const int row = 16 * half_of(x) + c16;
+                    const uint32_t at4 = qb + (row >> 2) * (4 * BLOCK) + (row & 3) * 256 + ((quad << 2 ^ turn(row)) << 4);
                     const uint32_t at = qb + ra[0] + (half_of(x) - kh) * (16 * LAT_BYTES), pat = qpe + ra[1] + (half_of(x) - kh) * (16 * PE_BYTES);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
+                    for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((Q4 ? at4 ^ ((i & 3) << 4) : at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) q[x][16 + i] = lds_read16(pat ^ (i << 6));
                 }
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             };
             u32x4 fl = {};
             for (uint32_t tile = t0; tile < stop; ++tile) {
-                const uint32_t tb = lat_at(tile), tp = pe_at(tile);
+                const uint32_t tb = Q4 ? raw_at(tile) : lat_at(tile), tp = pe_at(tile);
                 const int k0 = (int)(tile * BN);
                 if (tile > t0) fl = flags(tile - 1);
                 const int there8 = *(sm + L::THERE + (tile % L::THERES) * BN + c);
@@ -354,17 +361,34 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     return i < 16 ? lds_read16(((tb + ra[0]) ^ ((i & 3) << 6)) + (i >> 2) * BLOCK) : lds_read16((tp + ra[1]) ^ ((i - 16) << 6));
                 };
                 f32x4 z[RT][2] = {};
-                u32x4 kf[6];
+                if constexpr (Q4) {
+                    u32x4 codes[4], pe[2];
 #pragma unroll
-                for (int i = 0; i < 5; ++i) kf[i] = key(i);
-                __builtin_amdgcn_sched_barrier(0);
-                settle(tile - 1, fl);
+                    for (int j = 0; j < 4; ++j) codes[j] = lds_read16((tb + ra[0]) ^ (j << 6));
+                    const u32x4 scales = lds_read16(tb + L::RAW_SCALES + (2 * kh + (c16 >> 3)) * 256 + (c16 & 7) * 16);
 #pragma unroll
-                for (int i = 0; i < 18; ++i) {
+                    for (int i = 0; i < 2; ++i) pe[i] = lds_read16((tp + ra[1]) ^ (i << 6));
                     __builtin_amdgcn_sched_barrier(0);
-                    if (i + 5 < 18) kf[(i + 5) % 6] = key(i + 5);
+                    settle(tile - 1, fl);
 #pragma unroll
-                    for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf[i % 6], q[y][i], z[y][i & 1]);
+                    for (int i = 0; i < 18; ++i) {
+                        const u32x4 kf = i < 16 ? T::from4(codes[i >> 2][i & 3], __uint_as_float((scales[i >> 2] >> 8 * quad & 255u) << 23)) : pe[i & 1];
+#pragma unroll
+                        for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf, q[y][i], z[y][i & 1]);
+                    }
+                } else {
+                    u32x4 kf[6];
+#pragma unroll
+                    for (int i = 0; i < 5; ++i) kf[i] = key(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                    settle(tile - 1, fl);
+#pragma unroll
+                    for (int i = 0; i < 18; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i + 5 < 18) kf[(i + 5) % 6] = key(i + 5);
+#pragma unroll
+                        for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf[i % 6], q[y][i], z[y][i & 1]);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -408,13 +432,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // ---- loads
         const uint32_t pages = (uint32_t)min(a.pages, (int64_t)1 << 31);
         const u32x4 table_rsrc = tile_rsrc(table, (uint32_t)width * 4);  // entries past the table read as zeros (and are past `last`)
-        const uint32_t pages_at = lds + L::PAGES + vw * 1024;
+        const uint32_t pages_at = lds + L::PAGES + vw * (L::PAGE_RING * 256);
         int me = lane;  // (computed anew for every segment: the score waves have no registers for what follows from it)
         asm volatile("" : "+v"(me));
         const int own8 = 8 * vw + (me & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
         auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
-                             __builtin_amdgcn_readfirstlane(pages_at + (tile & 3) * 256)),
+                             __builtin_amdgcn_readfirstlane(pages_at + tile % L::PAGE_RING * 256)),
                          "v"(p.page(tile * BN + own8) * 4), "s"(table_rsrc)
                          : "memory");
         };
@@ -422,7 +446,16 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // steps that can be spread: the page, the address of the lane's token, the addresses for the lane's pieces
         uint64_t at_latent[2], at_pe, at_scales;
         auto find_page = [&](uint32_t tile) {
-            return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + (tile & 3) * 256 + lane * 4);
+            return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + tile % L::PAGE_RING * 256 + (EVEN ? 0 : lane * 4));
+        };
+        // EVEN: the wave's 8 tokens stand in one page in a row, so one address and fixed offsets lead to all of them.  (Tokens past the
+        // last are read as they are: no row sees them.)
+        auto find_rows = [&](uint32_t tile, int page) {
+            const uint32_t tok = tile * BN + 8 * vw, pg = __builtin_amdgcn_readfirstlane(page);
+            const bool there = tok < (uint32_t)last && pg < pages;
+            *(sm + L::THERE + (tile % L::THERES) * BN + own8) = there && tile * BN + own8 < (uint32_t)last;
+            const uint64_t at = (uint64_t)cache + pg * (uint64_t)page_bytes + (uint64_t)(tok - p.page(tok) * (uint32_t)a.page_size) * CACHE_ROW;
+            return there ? at : (uint64_t)zero_rows4;
         };
         auto find_token = [&](uint32_t tile, int page) {
             const uint32_t tok = tile * BN + own8;
@@ -433,13 +466,19 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             asm volatile("" : "+v"(at));  // (a choice of two, not a branch)
             return in ? at : (uint64_t)zero_row;
         };
-        const uint32_t piece4[2] = {(uint32_t)((me & 15) ^ turn(8 * vw + (me >> 4))) << 4,
-                                    (uint32_t)((me & 15) ^ turn(8 * vw + 4 + (me >> 4))) << 4};
+        auto place = [&](int t) { return (uint32_t)((me & 15) ^ (Q4 ? t & 15 : turn(t))) << 4; };
+        const uint32_t piece4[2] = {place(8 * vw + (me >> 4)), place(8 * vw + 4 + (me >> 4))};
         const uint32_t piece8 = (Q4 ? PE4 : LAT_BYTES) + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
-        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + (Q4 ? (me & 15) << 4 : piece4[x]); };
+        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + piece4[x]; };
         auto find_pe = [&](uint64_t at) { at_pe = of_lane(at, me >> 3) + piece8; };
+        const uint32_t off4[4] = {(uint32_t)(me >> 4) * ROW4 + piece4[0], (uint32_t)(4 + (me >> 4)) * ROW4 + piece4[1],
+                                  (uint32_t)(me >> 2 & 7) * ROW4 + SCALES4 + (me & 3) * 4, (uint32_t)(me >> 3) * ROW4 + piece8};
+        auto bring_even = [&](uint32_t tile, uint64_t at, int i) {
+            if (i < 2) load_block_from(raw_at(tile) + (2 * vw + i) * BLOCK, at, off4[i]);
+            if (i == 2) load_words_from(raw_at(tile) + L::RAW_SCALES + vw * 256, at, off4[2]);
+            if (i == 3) load_block_from(pe_at(tile) + 8 * vw * PE_BYTES, at, off4[3]);
+        };
         auto find_scales = [&](uint64_t at) { at_scales = of_lane(at, me >> 2 & 7) + (SCALES4 + (me & 3) * 4); };
-        auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile % 3 * VALUE_WAVES + vw) * L::RAW_WAVE; };
         auto bring = [&](uint32_t tile, auto i) {  // load i of 9: four of 4 tokens, four of 4 more, the positional parts
             constexpr int I = decltype(i)::value;
             if constexpr (I == 8)
@@ -447,27 +486,29 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             else if constexpr (!Q4)
                 load_block<(I & 3) * 256>(lat_at(tile) + (2 * vw + (I >> 2)) * (4 * BLOCK) + (I & 3) * BLOCK, at_latent[I >> 2]);
             else if constexpr (I < 2)
-                load_block<0>(raw_at(tile) + I * BLOCK, at_latent[I]);  // of 4: codes of 4 tokens and of 4 more, the scales
+                load_block<0>(raw_at(tile) + (2 * vw + I) * BLOCK, at_latent[I]);  // of 4: codes of 4 tokens and of 4 more, the scales
             else if constexpr (I == 2)
-                load_words(raw_at(tile) + 2 * BLOCK, at_scales);
+                load_words(raw_at(tile) + L::RAW_SCALES + vw * 256, at_scales);
         };
-        // A tile from 4 bits: lane l has values 8 l .. + 7 of each of the wave's tokens, which are a dword of codes and, as 16 bits, the
-        // token's piece l.  Reads and writes of 64 lanes touch every bank equally.
-        uint32_t code[4], scale[4];  // (two pairs of tokens)
-        const uint32_t to4 = vw * (8 * BLOCK) + (me >> 4) * BLOCK + (((me & 15) ^ turn(8 * vw)) << 4);
-        auto read_raw = [&](uint32_t tile, int pair) {  // the wave's tokens 2 pair, 2 pair + 1
+        // A tile's values 128 vw .. + 127 from 4 bits, 4 tokens at a time: token t = i % 4 + 4 (l / 16) + 16 (i / 4), of which lane l has a
+        // dword of codes and, as 16 bits, the piece l % 16.  Reads and writes of 64 lanes touch every bank equally.
+        const int pl = me & 15, ml = me >> 4;
+        const uint32_t from_codes = ml * (4 * SCALES4) + (((4 * vw + (pl >> 2)) ^ ml << 2) << 4) + (pl & 3) * 4;
+        const uint32_t from_scales = L::RAW_SCALES + (ml >> 1) * 256 + (ml & 1) * 64 + 4 * vw + (pl >> 2);
+        const uint32_t to_values = ml * (4 * BLOCK) + vw * BLOCK + ((pl ^ (ml >> 1) << 1) << 4);
+        uint32_t code[8], scale[8];
+        auto read_raw = [&](uint32_t tile) {
             const uint32_t from = raw_at(tile);
 #pragma unroll
-            for (int r = 2 * pair; r < 2 * pair + 2; ++r) {
-                code[r & 3] = *(__attribute__((address_space(3))) const uint32_t*)(lds_byte*)(uintptr_t)(from + me * 4 + r * (LAT / 2));
-                scale[r & 3] = *(__attribute__((address_space(3))) const uint8_t*)(lds_byte*)(uintptr_t)(from + 2 * BLOCK + (me >> 2) + r * 16);
+            for (int i = 0; i < 8; ++i) {
+                code[i] = *(__attribute__((address_space(3))) const uint32_t*)(lds_byte*)(uintptr_t)(((from + from_codes) ^ ((i & 3) << 4)) + (i & 3) * SCALES4 +
+                                                                                                (i >> 2) * (16 * SCALES4));
+                scale[i] = *(__attribute__((address_space(3))) const uint8_t*)(lds_byte*)(uintptr_t)(from + from_scales + (i & 3) * 16 + (i >> 2) * 512);
             }
         };
-        auto widen = [&](uint32_t tile, int pair) {
-#pragma unroll
-            for (int r = 2 * pair; r < 2 * pair + 2; ++r)
-                *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)(((lat_at(tile) + to4) ^ ((r & 3) << 6)) + (r >> 2) * (4 * BLOCK) + (r & 3) * 256) =
-                    T::from4(code[r & 3], __uint_as_float(scale[r & 3] << 23));
+        auto widen = [&](uint32_t tile, int i) {
+            *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)(((lat_at(tile) + to_values) ^ ((i & 3) << 6)) + (i & 3) * 256 + (i >> 2) * (16 * BLOCK)) =
+                T::from4(code[i], __uint_as_float(scale[i] << 23));
         };
 
         f32x16 acc[RT][4] = {};  // [row tile][32 values]
@@ -476,8 +517,9 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         for (int r = 0; r < RT; ++r) mo[r] = M_START;
         bool special = false;
         // One step: `tile` added, the value waves' loads of tile + AHEAD (past the end: zeros) and the addresses of the one after
-        // it between the products.  From 4 bits: tile + 2 widened, and the addresses found just before (to save registers).  LAST: nothing is brought.
-        constexpr uint32_t AHEAD = Q4 ? 5 : 3;
+        // it between the products.  From 4 bits: the next tile's values widened, and addresses found just before
+        // they are used (to save registers).  LAST: nothing is brought.
+        constexpr uint32_t AHEAD = Q4 ? 6 : 3;
         auto step = [&](uint32_t tile, auto last_) {
             constexpr bool LAST = decltype(last_)::value;
             const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
@@ -489,16 +531,17 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             };
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
+            if constexpr (!LAST && Q4) {
+                read_raw(tile + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             u32x4 vf[4], pf[RT];
             int page = 0;
 #pragma unroll
             for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
 #pragma unroll
             for (int d = 0; d < 4; ++d) vf[d] = value(0, d);
-            if constexpr (!LAST) {
-                page = find_page(tile + (Q4 ? AHEAD : AHEAD + 1));
-                if constexpr (Q4) read_raw(tile + 2, 0);
-            }
+            if constexpr (!LAST) page = find_page(tile + (Q4 ? AHEAD : AHEAD + 1));
             __builtin_amdgcn_sched_barrier(0);
             if (any(fl)) {
 #pragma unroll
@@ -535,16 +578,18 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                             for (int r = 0; r < RT; ++r) pn[r] = weight(1, r);
                     }
                     if constexpr (!LAST && Q4) {
-                        if (k == 0) {
-                            if (d < 3) read_raw(tile + 2, d + 1);
-                            widen(tile + 2, d);
-                            if (d == 1) at = find_token(tile + AHEAD, page);
-                            if (d == 3) find_latent(at, 0);
-                        } else {  // (the codes' place is free: they are in registers)
-                            if (d == 0) bring(tile + AHEAD, Int<0>{}), find_scales(at);
-                            if (d == 1) bring(tile + AHEAD, Int<2>{}), find_latent(at, 1);
-                            if (d == 2) bring(tile + AHEAD, Int<1>{}), find_pe(at);
-                            if (d == 3) bring(tile + AHEAD, Int<8>{}), load_pages(tile + AHEAD + 3);
+                        widen(tile + 1, 4 * k + d);
+                        if constexpr (EVEN) {
+                            if (k == 0 && d == 1) at = find_rows(tile + AHEAD, page);
+                            if (k == 1) bring_even(tile + AHEAD, at, d);
+                            if (k == 1 && d == 3) load_pages(tile + AHEAD + 8);
+                        } else {
+                        if (k == 0 && d == 1) at = find_token(tile + AHEAD, page);
+                        if (k == 0 && d == 3) find_latent(at, 0);
+                        if (k == 1 && d == 0) bring(tile + AHEAD, Int<0>{}), find_scales(at);
+                        if (k == 1 && d == 1) bring(tile + AHEAD, Int<2>{}), find_latent(at, 1);
+                        if (k == 1 && d == 2) bring(tile + AHEAD, Int<1>{}), find_pe(at);
+                        if (k == 1 && d == 3) bring(tile + AHEAD, Int<8>{}), load_pages(tile + AHEAD + 8);
                         }
                     } else if constexpr (!LAST) {  // (what an address is taken from is needed no more)
                         if (k == 0) {
@@ -566,13 +611,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
-                wait_loads<Q4 ? 2 * L::LOADS : L::LOADS>();
+                wait_loads<Q4 ? 4 * L::LOADS : L::LOADS>();
                 lds_barrier();  // the next tile's weights; the tile after it is whole
             }
         };
         if (n_tiles) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_pages(t0 + i);
+            for (int i = 0; i < L::PAGE_RING; ++i) load_pages(t0 + i);
             wait_loads<0>();
             auto find_tile = [&](uint32_t tile) {
                 const uint64_t at = find_token(tile, find_page(tile));
@@ -582,32 +627,33 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             auto bring_tile = [&](uint32_t tile) {
                 bring(tile, Int<0>{}), bring(tile, Int<1>{}), bring(tile, Int<2>{}), bring(tile, Int<3>{}), bring(tile, Int<4>{});
                 bring(tile, Int<5>{}), bring(tile, Int<6>{}), bring(tile, Int<7>{}), bring(tile, Int<8>{});
+                if constexpr (Q4) load_pages(tile + L::PAGE_RING);
             };
             auto whole_tile = [&](uint32_t tile) {
+                if constexpr (EVEN) {
+                    const uint64_t at = find_rows(tile, find_page(tile));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bring_even(tile, at, i);
+                    load_pages(tile + L::PAGE_RING);
+                    return;
+                }
                 find_tile(tile);
                 bring_tile(tile);
             };
             whole_tile(t0);
             whole_tile(t0 + 1);
             if constexpr (Q4) {
-                auto widen_tile = [&](uint32_t tile) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) read_raw(tile, i), widen(tile, i);
-                };
                 whole_tile(t0 + 2);
-#pragma unroll
-                for (int i = 4; i < 7; ++i) load_pages(t0 + i);
-                wait_loads<2 * 4 + 3>();
-                widen_tile(t0);
+                wait_loads<2 * L::LOADS>();
                 lds_barrier();  // the first tile, the queries
                 lds_barrier();  // the queries are in registers
-                // while the first tile's scores are computed: the second tile, what comes after the third
-                wait_loads<4 + 3>();
-                widen_tile(t0 + 1);
-                whole_tile(t0 + 3);
-                load_pages(t0 + 7);
-                wait_loads<L::LOADS>();  // the page numbers of t0 + 4 .. 6
-                whole_tile(t0 + 4);
+                // while the first tile's scores are computed: its values, and what comes after the third tile
+                read_raw(t0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) widen(t0, i);
+#pragma unroll
+                for (int i = 3; i < 6; ++i) whole_tile(t0 + i);
+                wait_loads<4 * L::LOADS>();
             } else {
                 load_pages(t0 + 4);
                 wait_loads<L::LOADS>();
@@ -890,10 +936,11 @@ int decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
     const bool few = (int64_t)join * tiles * 16 <= p.grid;  // blocks of rows and values: likely many parts each
     auto launch = [&](auto type) {
         typedef decltype(type) T;
-        if (p.own.rows > 32 || p.pre.rows > 32)  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
-            launch_kernel((decode_kernel<T, 2, Q4>), dim3(p.grid), dim3(THREADS), s, *a, p);
+        const bool two = p.own.rows > 32 || p.pre.rows > 32;  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
+        if (Q4 && a->page_size % 8 == 0)
+            launch_kernel(two ? decode_kernel<T, 2, Q4, Q4> : decode_kernel<T, 1, Q4, Q4>, dim3(p.grid), dim3(THREADS), s, *a, p);
         else
-            launch_kernel((decode_kernel<T, 1, Q4>), dim3(p.grid), dim3(THREADS), s, *a, p);
+            launch_kernel(two ? decode_kernel<T, 2, Q4, false> : decode_kernel<T, 1, Q4, false>, dim3(p.grid), dim3(THREADS), s, *a, p);
         if (few)
             launch_kernel((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), s, *a, p);
         else

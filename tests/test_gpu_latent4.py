@@ -1,6 +1,6 @@
-"""The latent cache in 4 bits: rows rounded into pages and read back, bit for bit against a plain form, and attention over them:
-against float64 (tolerances of latent_ref) and, since the widened rows are numbers of the 16-bit type and both kernels cut and add up
-alike, bit for bit against the same call over the widened cache."""
+"""The latent cache in 4 bits: rows rounded into pages and read back, bit for bit against a plain form, and attention over them against
+float64 (tolerances of latent_ref; the widened rows are numbers of the 16-bit type).  Where values are not finite: what is not
+finite in the outputs against the same call over the widened cache, which has tests of its own."""
 import random
 
 import pytest
@@ -9,7 +9,7 @@ import torch
 import kda355
 import latent4_ref as Q
 import latent_ref as R
-from latent_ref import LAT, PE, ROW
+from latent_ref import LAT, PE, ROW, SCALE
 from test_gpu_latent import DECODE, Absorbed, _i32, _randn
 
 pytestmark = pytest.mark.gpu
@@ -152,17 +152,29 @@ def _run4(x, wide=False, workspace=None, scale=None, cache=None):
     return o, lse
 
 
-def _check4(x, what="", plain=True, **kw):
+def _check4(x, what="", **kw):
     o, lse = _run4(x, **kw)
-    o16, lse16 = x.run()
-    _same(o, o16)
-    _same(lse, lse16)
-    if plain:
-        S, H = x.S, x.H
-        oc, lc = o.cpu(), lse.cpu()
-        for n, ref in enumerate(R.decode(x.ql, x.qp, x.cache, x.table, x.lens, S, prefix_table=x.prefix_table, prefix_len=x.prefix or 0)):
-            R.check(oc[n * S:(n + 1) * S].reshape(S * H, LAT), lc[n * S:(n + 1) * S].reshape(S * H), ref, x.dtype, ROW, f"{what} seq {n}")
+    S, H = x.S, x.H
+    oc, lc = o.cpu(), lse.cpu()
+    for n, ref in enumerate(R.decode(x.ql, x.qp, x.cache, x.table, x.lens, S, prefix_table=x.prefix_table, prefix_len=x.prefix or 0)):
+        R.check(oc[n * S:(n + 1) * S].reshape(S * H, LAT), lc[n * S:(n + 1) * S].reshape(S * H), ref, x.dtype, ROW, f"{what} seq {n}")
     return o, lse
+
+
+def _like_the_widened(x, o, lse):
+    """What is not finite stands where the call over the widened cache has it; the rest is near that: both are off from the exact
+    result by latent_ref's tolerance at most, whose weights add up to one and so A to the largest value."""
+    o16, lse16 = x.run()
+    u, f = torch.finfo(x.dtype).eps / 2, 2.0 ** -24
+    size = x.cache.double().nan_to_num(0, 0, 0).abs()
+    Z = SCALE * torch.cat([x.ql, x.qp], dim=-1).double().abs().sum(dim=-1).max() * size.max()
+    L = x.table.shape[1] * x.size + (x.prefix or 0)
+    for a, b, tol in ((o, o16, 2 * (2 * u + (2 * ROW * Z + 2 * L + 9) * f) * size.max()), (lse, lse16, 2 * (ROW * Z + L + 16 + 4 * Z) * f)):
+        a, b = a.cpu().double(), b.cpu().double()
+        for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(kind(a), kind(b))
+        fine = torch.isfinite(a)
+        assert ((a - b).abs()[fine] <= tol).all()
 
 
 IDS = [f"{len(c[0])}seq-{max(c[0])}-S{c[1]}-H{c[2]}-p{c[3]}" for c in DECODE]
@@ -177,7 +189,7 @@ def test_decode_lengths(lens, S, H, size, dtype):
 @pytest.mark.parametrize("lens,S,H,size", DECODE, ids=IDS)
 def test_decode_lengths_in_wide_tables(lens, S, H, size):
     """Tables with room for many more tokens: groups of 64 rows."""
-    _check4(_narrow(Absorbed(lens, S, H, size, BF)).widen(), plain=False)
+    _check4(_narrow(Absorbed(lens, S, H, size, BF)).widen())
 
 
 @pytest.mark.parametrize("n", [1, 31, 32, 33, 64, 65, 96, 97, 128, 129, 160, 161, 192, 193, 224, 225, 256, 257, 300])
@@ -185,8 +197,8 @@ def test_decode_lengths_in_wide_tables(lens, S, H, size):
 def test_decode_tiles_of_a_run(n, H):
     """Runs of one tile, of two, ...: every fill of the rings that the tiles pass through, in one workgroup's run and in several."""
     x = _narrow(Absorbed([n, n + 2000], 1, H, 16, BF))
-    _check4(x, plain=False)
-    _check4(x.widen(), plain=False)
+    _check4(x)
+    _check4(x.widen())
 
 
 @pytest.mark.parametrize("lens,S,H,size", [([400, 90], 1, 12, 64), ([130, 77, 1], 4, 16, 16), ([513], 1, 128, 100)])
@@ -198,7 +210,7 @@ def test_decode_views(lens, S, H, size):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("H", [8, 64, 128])
 def test_decode_long(dtype, H):
-    _check4(_narrow(Absorbed([9000, 3333], 1, H, 64, dtype)), plain=H == 8)
+    _check4(_narrow(Absorbed([9000, 3333], 1, H, 64, dtype)))
 
 
 @pytest.mark.parametrize("H", [4, 40, 128])
@@ -248,9 +260,7 @@ def test_decode_later_draft_tokens_do_not_matter(kind, H, S, widen):
         assert torch.equal(o[a:b], o2[a:b]) and torch.equal(lse[a:b], lse2[a:b])
         assert torch.isnan(o2[b]).any(dim=-1).all()
     x.cache = Q.values(cache.cpu(), HF)
-    o3, lse3 = x.run()
-    _same(o2, o3)
-    _same(lse2, lse3)
+    _like_the_widened(x, o2, lse2)
 
 
 @pytest.mark.parametrize("at", [3, 33, 60, 66, 97, 100, 103])
@@ -266,9 +276,8 @@ def test_decode_values_past_the_end_of_the_type(at, H, S, prefix):
     x.cache = Q.values(x.bytes.cpu(), HF)
     for _ in range(2):
         o, lse = _run4(x)
-        o16, lse16 = x.run()
-        _same(o, o16)
-        _same(lse, lse16)
+        assert not torch.isfinite(o).all()
+        _like_the_widened(x, o, lse)
         x.widen()
 
 
@@ -282,7 +291,7 @@ def test_decode_prefix(lens, S, H, size, prefix, dtype):
 
 @pytest.mark.parametrize("lens,S,H,size,prefix", [([1, 33, 64, 100], 1, 12, 16, 2000), ([5, 300], 3, 40, 64, 129), ([40, 7], 8, 96, 7, 300)])
 def test_decode_prefix_in_wide_tables(lens, S, H, size, prefix):
-    _check4(_narrow(Absorbed(lens, S, H, size, BF, prefix=prefix)).widen(), plain=False)
+    _check4(_narrow(Absorbed(lens, S, H, size, BF, prefix=prefix)).widen())
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -292,7 +301,7 @@ def test_decode_any(seed):
     lens = [rng.choice([0, 1, S, rng.randint(1, 2500)]) for _ in range(rng.choice([1, 3, 20, 66]))]
     x = Absorbed(lens, S, H, rng.choice([1, 3, 16, 64, 272]), rng.choice([BF, HF]), prefix=rng.choice([None, 40, 1111]), seed=seed)
     x = _narrow(x)
-    _check4(x.widen() if rng.random() < 0.5 else x, plain=False)
+    _check4(x.widen() if rng.random() < 0.5 else x)
 
 
 def test_decode_far_offsets():
