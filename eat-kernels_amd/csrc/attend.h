@@ -35,6 +35,11 @@ struct Bf16 {
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) { return f2bf2(x, y); }
     static __device__ __forceinline__ float up(uint16_t x) { return bf2f(x); }
+    // the codes in byte BYTE
+    template <int BYTE>
+    static __device__ __forceinline__ uint32_t pair4(uint32_t codes, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, BYTE));
+    }
     // eight 4-bit codes times a power of two (a float of its exponent), each rounded to the type; NaN where the scale is (255)
     static __device__ __forceinline__ u32x4 from4(uint32_t codes, float scale) {
         return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
@@ -56,6 +61,10 @@ struct Fp16 {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2_t));
     }
     static __device__ __forceinline__ float up(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+    template <int BYTE>
+    static __device__ __forceinline__ uint32_t pair4(uint32_t codes, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, BYTE));
+    }
     static __device__ __forceinline__ u32x4 from4(uint32_t codes, float scale) {
         return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
@@ -109,6 +118,15 @@ __device__ __forceinline__ void wait_loads() {  // all but the N youngest loads 
 
 __device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
     return *(__attribute__((address_space(3))) const u32x4*)(lds_byte*)(uintptr_t)at;
+}
+__device__ __forceinline__ void lds_write16(uint32_t at, u32x4 x) {
+    *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)at = x;
+}
+// transposed read of bytes: of 16 lanes, lane i gives the address of 8; lane i receives column i of the 8 x 16 matrix whose row r are the
+// bytes at lanes 2 r and 2 r + 1
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2 lds_read_tr8(uint32_t at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(lds_byte*)(uintptr_t)at));
 }
 // transposed read: of 16 lanes, lane i gives the address of 4 elements; lane i receives element i % 4.. column i of the
 // 4 x 16 matrix whose row r are the elements at lanes 4 r .. 4 r + 3

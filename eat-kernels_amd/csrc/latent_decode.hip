@@ -126,16 +126,21 @@ __device__ __forceinline__ At sequence_of(const Lengths& lens, uint32_t u) {
 // order: with this turn the former touch all 16 places of 256 bytes, and so do the latter.  (A turn that serves the former alone
 // and weights without their turn: 35 % more LDS cycles, 1 % more time.)
 __device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) << 1; }
+// From 4 bits 16-byte reads of 16 tokens' same piece (and, by the other lanes, its neighbour p ^ 1) and transposed reads of 8 tokens'
+// pieces p and p ^ 1 both touch all 16 places.
+__device__ __forceinline__ int turn4(int t) { return ((t & 7) ^ (t & 8) >> 1) << 1 | (t >> 3 & 1); }
 constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
 template <bool Q4>
 struct Lds {
-    // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: latent rows of two tiles widened (a
-    // value wave reads only what it widened itself), and codes, scales and positional parts of six tiles as they came.  A token's
-    // 16-byte piece p of codes stands at p ^ (t % 16), its scales at 256 (t / 8) + 16 (t % 8).
-    static constexpr int BUFS = Q4 ? 2 : 4, RAWS = Q4 ? 6 : 0, THERES = Q4 ? 8 : 4, PAGE_RING = Q4 ? 8 : 4;
-    static constexpr int LAT_STEP = Q4 ? LAT_TILE : LAT_TILE + PE_TILE, RAW = BUFS * LAT_STEP;
-    static constexpr int RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + VALUE_WAVES * 256, RAW_TILE = RAW_PE + PE_TILE;
-    static constexpr int P = RAW + RAWS * RAW_TILE;      // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
+    // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: codes, scales and positional parts of
+    // eight tiles as they came, and the scales of two once more for the values: SPREAD bytes a token, 8 equal ones a scale.  A token's
+    // 16-byte piece p of codes stands at p ^ turn4(t), its scales at 256 (t / 8) + 16 (t % 8).  The queries come through the first 64 KiB,
+    // which the first three tiles of a segment (slots 5 .. 7) leave free.
+    static constexpr int THERES = Q4 ? 8 : 4, PAGE_RING = Q4 ? 8 : 4;
+    static constexpr int SPREAD = 144, SPREAD_TILE = BN * SPREAD;
+    static constexpr int RAW = 10240, RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + VALUE_WAVES * 256, RAW_TILE = RAW_PE + PE_TILE;
+    static_assert(2 * SPREAD_TILE <= RAW && RAW + 5 * RAW_TILE >= 2 * LAT_TILE, "");
+    static constexpr int P = Q4 ? RAW + 8 * RAW_TILE : 4 * (LAT_TILE + PE_TILE);  // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
     static constexpr int MAX = P + 2 * 4096;             // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
     static constexpr int FLAG = MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
     static constexpr int THERE = FLAG + 64;              // is the token there [tile % THERES][32] bytes
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     uint32_t ra[2];
     if (scores) {
         const int t = 16 * kh + c16;
-        ra[0] = Q4 ? t * SCALES4 + ((quad ^ c16) << 4) : (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
+        ra[0] = Q4 ? t * SCALES4 + ((quad ^ turn4(c16)) << 4) : (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
         ra[1] = t * PE_BYTES + ((quad ^ swz8(t)) << 4);
     } else {
 #pragma unroll
@@ -191,9 +196,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         }
     }
 
-    auto lat_at = [&](uint32_t tile) { return lds + tile % L::BUFS * L::LAT_STEP; };  // a tile's latent rows
-    auto raw_at = [&](uint32_t tile) { return lds + L::RAW + tile % 6 * L::RAW_TILE; };  // what came of it in 4 bits
+    uint32_t t0 = 0;  // the segment's first tile
+    auto lat_at = [&](uint32_t tile) { return lds + tile % 4 * (LAT_TILE + PE_TILE); };            // a tile's latent rows
+    auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile - t0 + 5) % 8 * L::RAW_TILE; };  // what came of it in 4 bits
     auto pe_at = [&](uint32_t tile) { return Q4 ? raw_at(tile) + L::RAW_PE : lat_at(tile) + LAT_TILE; };  // its positional parts
+    auto spread_at = [&](uint32_t tile) { return lds + (tile & 1) * L::SPREAD_TILE; };
 
     uint32_t own = 0;
     for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
@@ -215,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     while (u < end) {
         // ---- the segment: key tiles [t0, t1) of one key sequence, for rows [r0, r1) of the batch
         int n = 0, tokens, r0, r1;
-        uint32_t t0, t1, whole;
+        uint32_t t1, whole;
         const int32_t* table;
         int width;
         if (prefix) {
@@ -261,13 +268,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         if (scores) {
             // ================================================================ score waves
             const int row0 = r0 + 16 * RT * rw + c16;  // this lane's rows: row0, and with two row tiles row0 + 16
-            // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: of both widened tiles), a row tile in each, laid out like keys, half of a wave's
+            // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: the first 64 KiB and the weights'), a row tile in each, laid out like keys, half of a wave's
             // rows by it and half by the other wave that has them (rows past the end repeat the last one).  (Straight into registers,
             // 64 bytes of 16 rows at a time and every row twice, 4900 cycles until the first tile was there, and 10800 in 64 sequences of
             // 64 heads; 1900 and 4800 so.)
             int mine[RT];
-            const uint32_t qt = (Q4 ? 0 : t0 + 2) + (RT > 1 ? rw : 0), qb = lat_at(qt);
-            const uint32_t qpe = Q4 ? lds + L::P + qt * PE_TILE : pe_at(qt);
+            const uint32_t qx = RT > 1 ? rw : 0, qb = Q4 ? lds + qx * LAT_TILE : lat_at(t0 + 2 + qx);
+            const uint32_t qpe = Q4 ? lds + L::P + qx * PE_TILE : pe_at(t0 + 2 + qx);
             const bool some = n_tiles && row0 - c16 < r1;
             auto half_of = [&](int x) { return RT > 1 ? x : rw; };  // of the row tile: where rows row0 + 16 x stand
             {
@@ -370,11 +377,22 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     for (int i = 0; i < 2; ++i) pe[i] = lds_read16((tp + ra[1]) ^ (i << 6));
                     __builtin_amdgcn_sched_barrier(0);
                     settle(tile - 1, fl);
+                    {  // two of the key's scales (rows' halves share the 16), each 8 times, for the values
+                        const uint32_t two = quad & 2 ? scales[2 * rw + 1] : scales[2 * rw], first = 0x01010101u * (2 * (quad & 1));
+                        const uint32_t x = __builtin_amdgcn_perm(two, two, first), y = __builtin_amdgcn_perm(two, two, first + 0x01010101u);
+                        lds_write16(spread_at(tile) + (16 * kh + c16) * L::SPREAD + (8 * rw + 2 * quad) * 8, u32x4{x, x, y, y});
+                    }
+                    auto key4 = [&](int i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
+                        const uint32_t s4 = scales[i >> 2 & 3];
+                        return i < 16 ? T::from4(codes[i >> 2 & 3][i & 3], __uint_as_float(__builtin_amdgcn_alignbit(s4, s4, 8 * quad + 9))) : pe[i & 1];
+                    };
+                    u32x4 kf[2] = {key4(0)};
 #pragma unroll
                     for (int i = 0; i < 18; ++i) {
-                        const u32x4 kf = i < 16 ? T::from4(codes[i >> 2][i & 3], __uint_as_float((scales[i >> 2] >> 8 * quad & 255u) << 23)) : pe[i & 1];
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i + 1 < 18) kf[(i + 1) & 1] = key4(i + 1);
 #pragma unroll
-                        for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf, q[y][i], z[y][i & 1]);
+                        for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf[i & 1], q[y][i], z[y][i & 1]);
                     }
                 } else {
                     u32x4 kf[6];
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             asm volatile("" : "+v"(at));  // (a choice of two, not a branch)
             return in ? at : (uint64_t)zero_row;
         };
-        auto place = [&](int t) { return (uint32_t)((me & 15) ^ (Q4 ? t & 15 : turn(t))) << 4; };
+        auto place = [&](int t) { return (uint32_t)((me & 15) ^ (Q4 ? turn4(t & 15) : turn(t))) << 4; };
         const uint32_t piece4[2] = {place(8 * vw + (me >> 4)), place(8 * vw + 4 + (me >> 4))};
         const uint32_t piece8 = (Q4 ? PE4 : LAT_BYTES) + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
         auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + piece4[x]; };
@@ -490,36 +508,15 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             else if constexpr (I == 2)
                 load_words(raw_at(tile) + L::RAW_SCALES + vw * 256, at_scales);
         };
-        // A tile's values 128 vw .. + 127 from 4 bits, 4 tokens at a time: token t = i % 4 + 4 (l / 16) + 16 (i / 4), of which lane l has a
-        // dword of codes and, as 16 bits, the piece l % 16.  Reads and writes of 64 lanes touch every bank equally.
-        const int pl = me & 15, ml = me >> 4;
-        const uint32_t from_codes = ml * (4 * SCALES4) + (((4 * vw + (pl >> 2)) ^ ml << 2) << 4) + (pl & 3) * 4;
-        const uint32_t from_scales = L::RAW_SCALES + (ml >> 1) * 256 + (ml & 1) * 64 + 4 * vw + (pl >> 2);
-        const uint32_t to_values = ml * (4 * BLOCK) + vw * BLOCK + ((pl ^ (ml >> 1) << 1) << 4);
-        uint32_t code[8], scale[8];
-        auto read_raw = [&](uint32_t tile) {
-            const uint32_t from = raw_at(tile);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                code[i] = *(__attribute__((address_space(3))) const uint32_t*)(lds_byte*)(uintptr_t)(((from + from_codes) ^ ((i & 3) << 4)) + (i & 3) * SCALES4 +
-                                                                                                (i >> 2) * (16 * SCALES4));
-                scale[i] = *(__attribute__((address_space(3))) const uint8_t*)(lds_byte*)(uintptr_t)(from + from_scales + (i & 3) * 16 + (i >> 2) * 512);
-            }
-        };
-        auto widen = [&](uint32_t tile, int i) {
-            *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)(((lat_at(tile) + to_values) ^ ((i & 3) << 6)) + (i & 3) * 256 + (i >> 2) * (16 * BLOCK)) =
-                T::from4(code[i], __uint_as_float(scale[i] << 23));
-        };
-
-        f32x16 acc[RT][4] = {};  // [row tile][32 values]
+        // [row tile][32 values]: from 16 bits values 32 d + i, from 4 bits 64 (d / 2) + 2 i + d % 2, i = (e & 3) + 8 (e >> 2) + 4 half
+        f32x16 acc[RT][4] = {};
         float mo[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) mo[r] = M_START;
         bool special = false;
         // One step: `tile` added, the value waves' loads of tile + AHEAD (past the end: zeros) and the addresses of the one after
-        // it between the products.  From 4 bits: the next tile's values widened, and addresses found just before
-        // they are used (to save registers).  LAST: nothing is brought.
-        constexpr uint32_t AHEAD = Q4 ? 6 : 3;
+        // it between the products.  LAST: nothing is brought.
+        constexpr uint32_t AHEAD = 3;
         auto step = [&](uint32_t tile, auto last_) {
             constexpr bool LAST = decltype(last_)::value;
             const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
@@ -531,17 +528,13 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             };
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
-            if constexpr (!LAST && Q4) {
-                read_raw(tile + 1);
-                __builtin_amdgcn_sched_barrier(0);
-            }
             u32x4 vf[4], pf[RT];
             int page = 0;
 #pragma unroll
             for (int r = 0; r < RT; ++r) pf[r] = weight(0, r);
 #pragma unroll
             for (int d = 0; d < 4; ++d) vf[d] = value(0, d);
-            if constexpr (!LAST) page = find_page(tile + (Q4 ? AHEAD : AHEAD + 1));
+            if constexpr (!LAST) page = find_page(tile + AHEAD + 1);
             __builtin_amdgcn_sched_barrier(0);
             if (any(fl)) {
 #pragma unroll
@@ -577,21 +570,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                             for (int r = 0; r < RT; ++r) pn[r] = weight(1, r);
                     }
-                    if constexpr (!LAST && Q4) {
-                        widen(tile + 1, 4 * k + d);
-                        if constexpr (EVEN) {
-                            if (k == 0 && d == 1) at = find_rows(tile + AHEAD, page);
-                            if (k == 1) bring_even(tile + AHEAD, at, d);
-                            if (k == 1 && d == 3) load_pages(tile + AHEAD + 8);
-                        } else {
-                        if (k == 0 && d == 1) at = find_token(tile + AHEAD, page);
-                        if (k == 0 && d == 3) find_latent(at, 0);
-                        if (k == 1 && d == 0) bring(tile + AHEAD, Int<0>{}), find_scales(at);
-                        if (k == 1 && d == 1) bring(tile + AHEAD, Int<2>{}), find_latent(at, 1);
-                        if (k == 1 && d == 2) bring(tile + AHEAD, Int<1>{}), find_pe(at);
-                        if (k == 1 && d == 3) bring(tile + AHEAD, Int<8>{}), load_pages(tile + AHEAD + 8);
-                        }
-                    } else if constexpr (!LAST) {  // (what an address is taken from is needed no more)
+                    if constexpr (!LAST) {  // (what an address is taken from is needed no more)
                         if (k == 0) {
                             if (d == 0) bring(tile + 3, Int<0>{});
                             if (d == 1) bring(tile + 3, Int<1>{}), at = find_token(tile + 4, page);
@@ -611,7 +590,102 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
-                wait_loads<Q4 ? 4 * L::LOADS : L::LOADS>();
+                wait_loads<L::LOADS>();
+                lds_barrier();  // the next tile's weights; the tile after it is whole
+            }
+        };
+        // The same from 4 bits.  A transposed read of bytes gives a lane 8 tokens' codes of values 2 m and 2 m + 1 (m = l % 32 of 64 values), and
+        // another, of the scales spread, their scales: eight conversions and eight exchanges of halves make one operand of even values and
+        // one of odd ones, without a detour through LDS (which, as 16-bit tiles written and read back transposed, took as long as
+        // everything else: a step 2500 cycles with one row tile and 2850 with two).
+        const int tk = 8 * half + (c16 >> 1), pc = quad & 1;  // of 16 tokens the one whose bytes this lane reads; of two pieces the one
+        const uint32_t at_codes = tk * SCALES4 + (((4 * vw + pc) ^ turn4(tk)) << 4) + (c16 & 1) * 8, at_spread = tk * L::SPREAD + (4 * vw + pc) * 8;
+        constexpr uint32_t AHEAD4 = 7;
+        auto step4 = [&](uint32_t tile, auto last_) {
+            constexpr bool LAST = decltype(last_)::value;
+            const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
+            const uint32_t pb = lds + L::P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
+            const uint32_t cb = raw_at(tile) + at_codes, sb = spread_at(tile) + at_spread;
+            auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
+            const u32x4 fl = flags(tile);
+            u32x2 codes[4], scales[4];  // [16-token step][64 values]
+            u32x4 pf[2][RT];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                codes[g] = lds_read_tr8((cb ^ (g & 1) << 5) + (g >> 1) * (16 * SCALES4));
+                scales[g] = lds_read_tr8(sb + (g & 1) * 16 + (g >> 1) * (16 * L::SPREAD));
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) pf[0][r] = weight(0, r);
+            int page = 0;
+            if constexpr (!LAST) page = find_page(tile + AHEAD4);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) pf[1][r] = weight(1, r);
+            __builtin_amdgcn_sched_barrier(0);
+            if (any(fl)) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    if (RT > 1 && !__builtin_amdgcn_readfirstlane(fl[r] | fl[r + 2])) continue;
+                    const float f = raise(tile, 32 * r + c, mo[r]);
+                    if (tile != t0)  // (nothing is there yet)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                }
+                lds_barrier();  // the weights anew
+#pragma unroll
+                for (int r = 0; r < RT; ++r) pf[0][r] = weight(0, r), pf[1][r] = weight(1, r);
+            }
+            u32x4 vf[2][2];  // [group % 2][even, odd]
+            auto widen = [&](int g) {
+                uint32_t x[8];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
+                    const uint32_t s4 = scales[g][i], c4 = codes[g][i];
+                    x[4 * i] = T::template pair4<0>(c4, __uint_as_float(s4 << 23));
+                    x[4 * i + 1] = T::template pair4<1>(c4, __uint_as_float(s4 << 15));
+                    x[4 * i + 2] = T::template pair4<2>(c4, __uint_as_float(s4 << 7));
+                    x[4 * i + 3] = T::template pair4<3>(c4, __uint_as_float(s4 >> 1));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    vf[g & 1][0][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+                    vf[g & 1][1][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+                }
+                if (mixed)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        special |= nonfinite<T>(vf[g & 1][i]);
+                        vf[g & 1][i] = finite_part<T>(vf[g & 1][i]);
+                    }
+            };
+            uint64_t at = 0;
+            widen(0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[r][2 * (g & 1) + i] = T::mfma(vf[g & 1][i], pf[g >> 1][r], acc[r][2 * (g & 1) + i]);
+                if (g < 3) widen(g + 1);
+                if constexpr (!LAST) {
+                    if constexpr (EVEN) {
+                        if (g == 0) at = find_rows(tile + AHEAD4, page);
+                        if (g == 1) bring_even(tile + AHEAD4, at, 0);
+                        if (g == 2) bring_even(tile + AHEAD4, at, 1), bring_even(tile + AHEAD4, at, 2);
+                        if (g == 3) bring_even(tile + AHEAD4, at, 3);
+                    } else {
+                        if (g == 0) at = find_token(tile + AHEAD4, page), find_latent(at, 0), find_latent(at, 1);
+                        if (g == 1) bring(tile + AHEAD4, Int<0>{}), find_scales(at), find_pe(at);
+                        if (g == 2) bring(tile + AHEAD4, Int<1>{}), bring(tile + AHEAD4, Int<2>{});
+                        if (g == 3) bring(tile + AHEAD4, Int<8>{});
+                    }
+                    if (g == 3) load_pages(tile + AHEAD4 + 8);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!LAST) {
+                wait_loads<5 * L::LOADS>();
                 lds_barrier();  // the next tile's weights; the tile after it is whole
             }
         };
@@ -647,13 +721,10 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 wait_loads<2 * L::LOADS>();
                 lds_barrier();  // the first tile, the queries
                 lds_barrier();  // the queries are in registers
-                // while the first tile's scores are computed: its values, and what comes after the third tile
-                read_raw(t0);
+                // while the first tile's scores are computed: what comes after the third tile
 #pragma unroll
-                for (int i = 0; i < 8; ++i) widen(t0, i);
-#pragma unroll
-                for (int i = 3; i < 6; ++i) whole_tile(t0 + i);
-                wait_loads<4 * L::LOADS>();
+                for (int i = 3; i < 7; ++i) whole_tile(t0 + i);
+                wait_loads<5 * L::LOADS>();
             } else {
                 load_pages(t0 + 4);
                 wait_loads<L::LOADS>();
@@ -666,8 +737,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 wait_loads<L::LOADS>();
             }
             lds_barrier();  // the first tile's weights; the second tile is whole
-            for (uint32_t tile = t0; tile + 1 < stop; ++tile) step(tile, std::false_type{});
-            step(stop - 1, std::true_type{});
+            auto any_step = [&](uint32_t tile, auto last_) {
+                if constexpr (Q4) step4(tile, last_); else step(tile, last_);
+            };
+            for (uint32_t tile = t0; tile + 1 < stop; ++tile) any_step(tile, std::false_type{});
+            any_step(stop - 1, std::true_type{});
             wait_loads<0>();  // what was brought past the end
         } else {
             lds_barrier();
@@ -682,23 +756,40 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 const int page = table[j / a.page_size];
                 if (page < 0 || page >= a.pages) continue;
                 const char* row = cache + page * page_bytes + (int64_t)(j % a.page_size) * CACHE_ROW;
-                auto value = [&](int i) -> uint16_t {
-                    if constexpr (!Q4) return reinterpret_cast<const uint16_t*>(row)[i];
-                    const uint32_t b = *reinterpret_cast<const uint8_t*>(row + SCALES4 + i / GROUP);
-                    const uint32_t both = T::from4(*reinterpret_cast<const uint8_t*>(row + i / 2), __uint_as_float(b << 23))[0];
-                    return (uint16_t)(both >> (i & 1) * 16);
-                };
+                int my = half;  // (addresses found here: kept from before the loops they would take their registers)
+                asm volatile("" : "+v"(my));
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int i = r0 + 32 * r + c;
                     const bool seen = i < r1 && j < sees(min(i, r1 - 1));
+                    auto give = [&](float& x, uint32_t value) {
+                        if (seen && !(fabsf(T::up((uint16_t)value)) < INFINITY)) x = NAN;
+                    };
+                    if constexpr (Q4) {
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
+                        for (int d = 0; d < 2; ++d)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float x = T::up(value(128 * vw + 4 * half + 32 * d + 8 * (e >> 2) + (e & 3)));
-                            if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] = NAN;
-                        }
+                            for (int e = 0; e < 4; ++e) {  // 8 values in a row
+                                const int at = 128 * vw + 64 * d + 16 * e + 8 * my;
+                                const uint32_t b = *reinterpret_cast<const uint8_t*>(row + SCALES4 + at / GROUP);
+                                const u32x4 x = T::from4(*reinterpret_cast<const uint32_t*>(row + at / 2), __uint_as_float(b << 23));
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    float even = acc[r][2 * d][4 * e + k], odd = acc[r][2 * d + 1][4 * e + k];
+                                    give(even, x[k]), give(odd, x[k] >> 16);
+                                    acc[r][2 * d][4 * e + k] = even, acc[r][2 * d + 1][4 * e + k] = odd;
+                                }
+                            }
+                    } else {
+                        const uint16_t* vr = reinterpret_cast<const uint16_t*>(row) + 128 * vw + 4 * half;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float x = T::up(vr[32 * d + 8 * (e >> 2) + (e & 3)]);
+                                if (seen && !(fabsf(x) < INFINITY)) acc[r][d][e] = NAN;
+                            }
+                    }
                 }
             }
         }
@@ -720,6 +811,17 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 const float inv = ls[r] > 0.f ? 1.f / ls[r] : 0.f;
                 const int t = i / a.H, h = i - t * a.H;
                 uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 128 * vw + 4 * half;
+                if constexpr (Q4) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            u32x4 x;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[j] = ls[r] == 0.f ? 0u : T::pack(acc[r][2 * b][e + j] * inv, acc[r][2 * b + 1][e + j] * inv);
+                            *reinterpret_cast<u32x4*>(o + 4 * half + 64 * b + 4 * e) = x;
+                        }
+                } else
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -740,6 +842,17 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             for (int r = 0; r < RT; ++r) {
                 if (r0 + 32 * r + c >= r1) break;
                 char* o = out + r * SLOT_TILE + vw * 16384 + lane * 16;
+                if constexpr (Q4) {  // as the other form leaves them: a lane's 8 values in a row are two lanes' four
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            f32x16 &x = acc[r][2 * b], &y = acc[r][2 * b + 1];
+                            char* to = out + r * SLOT_TILE + vw * 16384 + c * 16 + ((2 * b + (e >> 1)) * 4 + 2 * (e & 1) + half) * 1024;
+                            *reinterpret_cast<f32x4*>(to) = f32x4{x[4 * e], y[4 * e], x[4 * e + 1], y[4 * e + 1]};
+                            *reinterpret_cast<f32x4*>(to + 512) = f32x4{x[4 * e + 2], y[4 * e + 2], x[4 * e + 3], y[4 * e + 3]};
+                        }
+                } else
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
