@@ -32,7 +32,12 @@
 namespace kda355 {
 namespace {
 
-constexpr int SCORE_WAVES = 4, VALUE_WAVES = 4, THREADS = (SCORE_WAVES + VALUE_WAVES) * 64;
+constexpr int SCORE_WAVES = 4;
+// Value waves: 4, and 8 from 4 bits with one row tile, where a wave's conversions, one after the other, are the longest way through a step.
+template <int RT, bool Q4>
+constexpr int VALUE_WAVES = Q4 && RT == 1 ? 8 : 4;
+template <int RT, bool Q4>
+constexpr int THREADS = (SCORE_WAVES + VALUE_WAVES<RT, Q4>) * 64;
 constexpr int BN = 32;                                  // keys of a tile
 constexpr int MAX_ROWS = 64;                            // query rows of a group
 // The cut is by cost: beginning a sequence (lengths, queries, page numbers and first tile one after the other) takes about as
@@ -130,23 +135,23 @@ __device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) 
 // pieces p and p ^ 1 both touch all 16 places.
 __device__ __forceinline__ int turn4(int t) { return ((t & 7) ^ (t & 8) >> 1) << 1 | (t >> 3 & 1); }
 constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
-template <bool Q4>
+template <bool Q4, int VW>
 struct Lds {
     // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: codes, scales and positional parts of
-    // eight tiles as they came, and the scales of two once more for the values: SPREAD bytes a token, 8 equal ones a scale.  A token's
-    // 16-byte piece p of codes stands at p ^ turn4(t), its scales at 256 (t / 8) + 16 (t % 8).  The queries come through the first 64 KiB,
-    // which the first three tiles of a segment (slots 5 .. 7) leave free.
+    // eight tiles as they came, and of every value wave the scales of its values once more, 8 equal bytes each.  A token's 16-byte piece p of
+    // codes stands at p ^ turn4(t), its scales at 256 (t / 8) + 16 (t % 8).  The queries come through the first 64 KiB, which the first
+    // three tiles of a segment (slots 5 .. 7) leave free.
     static constexpr int THERES = Q4 ? 8 : 4, PAGE_RING = Q4 ? 8 : 4;
-    static constexpr int SPREAD = 144, SPREAD_TILE = BN * SPREAD;
-    static constexpr int RAW = 10240, RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + VALUE_WAVES * 256, RAW_TILE = RAW_PE + PE_TILE;
-    static_assert(2 * SPREAD_TILE <= RAW && RAW + 5 * RAW_TILE >= 2 * LAT_TILE, "");
+    static constexpr int SPREAD = LAT / GROUP / VW * 8;  // bytes a token
+    static constexpr int RAW = VW * BN * SPREAD, RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + 4 * 256, RAW_TILE = RAW_PE + PE_TILE;
+    static_assert(RAW + 5 * RAW_TILE >= 2 * LAT_TILE, "");
     static constexpr int P = Q4 ? RAW + 8 * RAW_TILE : 4 * (LAT_TILE + PE_TILE);  // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
     static constexpr int MAX = P + 2 * 4096;             // a tile's maxima [tile % 2][score wave][32], at the end the sums of rows
     static constexpr int FLAG = MAX + 2 * SCORE_WAVES * 128;  // does the wave's tile raise the maximum [tile % 2][score wave]
     static constexpr int THERE = FLAG + 64;              // is the token there [tile % THERES][32] bytes
     static constexpr int PAGES = THERE + THERES * BN;    // page numbers [value wave][tile % PAGE_RING][64]
-    static constexpr int BYTES = PAGES + VALUE_WAVES * PAGE_RING * 256;
-    static constexpr int LOADS = Q4 ? 5 : 10;            // of a value wave a tile: codes 2, scales | 8 of latent rows; positional parts, page numbers
+    static constexpr int BYTES = PAGES + VW * PAGE_RING * 256;
+    static constexpr int LOADS = !Q4 ? 10 : VW == 8 ? 3 : 5;  // of a value wave a tile: 8 of latent rows | 2 of codes, scales; positional parts, page numbers
     static_assert(BYTES <= 160 * 1024 && RAW % 1024 == 0 && P % 1024 == 0 && RAW_TILE % 1024 == 0, "");
 };
 
@@ -162,8 +167,9 @@ __device__ __forceinline__ float join_groups(float x, F f) {
 }
 
 template <typename T, int RT, bool Q4, bool EVEN>
-__global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
-    typedef Lds<Q4> L;
+__global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) decode_kernel(KdaLatentDecodeArgs a, Plan p) {
+    constexpr int VW = VALUE_WAVES<RT, Q4>, DIMS = LAT / VW, DV = DIMS / 32;  // values of a value wave, accumulators of 32
+    typedef Lds<Q4, VW> L;
     constexpr int CACHE_ROW = Q4 ? ROW4 : ROW_BYTES;
     __shared__ __align__(1024) unsigned char sm[L::BYTES];
     const uint32_t lds = lds_offset(sm);
@@ -178,7 +184,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     const char* const cache = static_cast<const char*>(a.cache);
     const bool scores = w < SCORE_WAVES;
     const int rw = w & 1, kh = w >> 1 & 1;  // a score wave's rows 16 RT rw .. (16 RT of them) and keys 16 kh ..
-    const int vw = w & 3;                   // a value wave's 128 values
+    const int vw = w & (VW - 1);            // a value wave's DIMS values (waves SCORE_WAVES .. : in any order)
+    const int tw = VW == 8 ? vw >> 1 : vw;  // it brings of tokens 8 tw .. + 7
     const int c16 = lane & 15, quad = lane >> 4;
     // LDS read addresses within a tile.  Of a score wave: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step, latent and
     // positional; of a value wave: values as operand rows (key 8 half + e of a 16-key step is element e), e < 4 and from 4 on.
@@ -200,7 +207,6 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
     auto lat_at = [&](uint32_t tile) { return lds + tile % 4 * (LAT_TILE + PE_TILE); };            // a tile's latent rows
     auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile - t0 + 5) % 8 * L::RAW_TILE; };  // what came of it in 4 bits
     auto pe_at = [&](uint32_t tile) { return Q4 ? raw_at(tile) + L::RAW_PE : lat_at(tile) + LAT_TILE; };  // its positional parts
-    auto spread_at = [&](uint32_t tile) { return lds + (tile & 1) * L::SPREAD_TILE; };
 
     uint32_t own = 0;
     for (int n = lane; n < a.B; n += 64) own += units_of(lens.of_lane(n));
@@ -358,8 +364,19 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 for (int x = 0; x < RT; ++x) l[x] += sum[x];
             };
             u32x4 fl = {};
+            // from 4 bits: the lane's part of its key, read a tile ahead
+            u32x4 codes[4], scales, pe[2];
+            auto fetch = [&](uint32_t tile) {
+                const uint32_t tb = raw_at(tile);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) codes[j] = lds_read16((tb + ra[0]) ^ (j << 6));
+                scales = lds_read16(tb + L::RAW_SCALES + (2 * kh + (c16 >> 3)) * 256 + (c16 & 7) * 16);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) pe[i] = lds_read16((tb + L::RAW_PE + ra[1]) ^ (i << 6));
+            };
+            if (Q4 && n_tiles) fetch(t0);
             for (uint32_t tile = t0; tile < stop; ++tile) {
-                const uint32_t tb = Q4 ? raw_at(tile) : lat_at(tile), tp = pe_at(tile);
+                const uint32_t tb = lat_at(tile), tp = pe_at(tile);
                 const int k0 = (int)(tile * BN);
                 if (tile > t0) fl = flags(tile - 1);
                 const int there8 = *(sm + L::THERE + (tile % L::THERES) * BN + c);
@@ -369,19 +386,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 };
                 f32x4 z[RT][2] = {};
                 if constexpr (Q4) {
-                    u32x4 codes[4], pe[2];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) codes[j] = lds_read16((tb + ra[0]) ^ (j << 6));
-                    const u32x4 scales = lds_read16(tb + L::RAW_SCALES + (2 * kh + (c16 >> 3)) * 256 + (c16 & 7) * 16);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) pe[i] = lds_read16((tp + ra[1]) ^ (i << 6));
-                    __builtin_amdgcn_sched_barrier(0);
                     settle(tile - 1, fl);
-                    {  // two of the key's scales (rows' halves share the 16), each 8 times, for the values
-                        const uint32_t two = quad & 2 ? scales[2 * rw + 1] : scales[2 * rw], first = 0x01010101u * (2 * (quad & 1));
-                        const uint32_t x = __builtin_amdgcn_perm(two, two, first), y = __builtin_amdgcn_perm(two, two, first + 0x01010101u);
-                        lds_write16(spread_at(tile) + (16 * kh + c16) * L::SPREAD + (8 * rw + 2 * quad) * 8, u32x4{x, x, y, y});
-                    }
                     auto key4 = [&](int i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
                         const uint32_t s4 = scales[i >> 2 & 3];
                         return i < 16 ? T::from4(codes[i >> 2 & 3][i & 3], __uint_as_float(__builtin_amdgcn_alignbit(s4, s4, 8 * quad + 9))) : pe[i & 1];
@@ -394,6 +399,8 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
 #pragma unroll
                         for (int y = 0; y < RT; ++y) z[y][i & 1] = T::mfma16(kf[i & 1], q[y][i], z[y][i & 1]);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(tile + 1);
                 } else {
                     u32x4 kf[6];
 #pragma unroll
@@ -453,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         const uint32_t pages_at = lds + L::PAGES + vw * (L::PAGE_RING * 256);
         int me = lane;  // (computed anew for every segment: the score waves have no registers for what follows from it)
         asm volatile("" : "+v"(me));
-        const int own8 = 8 * vw + (me & 7);  // the wave brings tokens 8 w .. + 7; this lane finds the address of one
+        const int own8 = 8 * tw + (me & 7);  // this lane finds the address of one token
         auto load_pages = [&](uint32_t tile) {  // the page numbers of the wave's tokens
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane(pages_at + tile % L::PAGE_RING * 256)),
@@ -469,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
         // EVEN: the wave's 8 tokens stand in one page in a row, so one address and fixed offsets lead to all of them.  (Tokens past the
         // last are read as they are: no row sees them.)
         auto find_rows = [&](uint32_t tile, int page) {
-            const uint32_t tok = tile * BN + 8 * vw, pg = __builtin_amdgcn_readfirstlane(page);
+            const uint32_t tok = tile * BN + 8 * tw, pg = __builtin_amdgcn_readfirstlane(page);
             const bool there = tok < (uint32_t)last && pg < pages;
             *(sm + L::THERE + (tile % L::THERES) * BN + own8) = there && tile * BN + own8 < (uint32_t)last;
             const uint64_t at = (uint64_t)cache + pg * (uint64_t)page_bytes + (uint64_t)(tok - p.page(tok) * (uint32_t)a.page_size) * CACHE_ROW;
@@ -485,31 +492,33 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             return in ? at : (uint64_t)zero_row;
         };
         auto place = [&](int t) { return (uint32_t)((me & 15) ^ (Q4 ? turn4(t & 15) : turn(t))) << 4; };
-        const uint32_t piece4[2] = {place(8 * vw + (me >> 4)), place(8 * vw + 4 + (me >> 4))};
-        const uint32_t piece8 = (Q4 ? PE4 : LAT_BYTES) + (((me & 7) ^ swz8(8 * vw + (me >> 3))) << 4);
-        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * x + (me >> 4)) + piece4[x]; };
+        const int four = VW == 8 ? vw & 1 : 0;  // with 8 value waves: of the 8 tokens the 4 whose codes the wave brings; beside them scales or positional parts
+        const uint32_t piece4[2] = {place(8 * tw + 4 * four + (me >> 4)), place(8 * tw + 4 + (me >> 4))};
+        const uint32_t piece8 = (Q4 ? PE4 : LAT_BYTES) + (((me & 7) ^ swz8(8 * tw + (me >> 3))) << 4);
+        auto find_latent = [&](uint64_t at, int x) { at_latent[x] = of_lane(at, 4 * (x + four) + (me >> 4)) + piece4[x]; };
         auto find_pe = [&](uint64_t at) { at_pe = of_lane(at, me >> 3) + piece8; };
-        const uint32_t off4[4] = {(uint32_t)(me >> 4) * ROW4 + piece4[0], (uint32_t)(4 + (me >> 4)) * ROW4 + piece4[1],
+        const uint32_t off4[4] = {(uint32_t)(4 * four + (me >> 4)) * ROW4 + piece4[0], (uint32_t)(4 + (me >> 4)) * ROW4 + piece4[1],
                                   (uint32_t)(me >> 2 & 7) * ROW4 + SCALES4 + (me & 3) * 4, (uint32_t)(me >> 3) * ROW4 + piece8};
         auto bring_even = [&](uint32_t tile, uint64_t at, int i) {
-            if (i < 2) load_block_from(raw_at(tile) + (2 * vw + i) * BLOCK, at, off4[i]);
-            if (i == 2) load_words_from(raw_at(tile) + L::RAW_SCALES + vw * 256, at, off4[2]);
-            if (i == 3) load_block_from(pe_at(tile) + 8 * vw * PE_BYTES, at, off4[3]);
+            if (i == 0 || (i == 1 && VW == 4)) load_block_from(raw_at(tile) + (2 * tw + four + i) * BLOCK, at, off4[i]);
+            if (i == 2 && !four) load_words_from(raw_at(tile) + L::RAW_SCALES + tw * 256, at, off4[2]);
+            if (i == 3 && (VW == 4 || four)) load_block_from(pe_at(tile) + 8 * tw * PE_BYTES, at, off4[3]);
         };
         auto find_scales = [&](uint64_t at) { at_scales = of_lane(at, me >> 2 & 7) + (SCALES4 + (me & 3) * 4); };
         auto bring = [&](uint32_t tile, auto i) {  // load i of 9: four of 4 tokens, four of 4 more, the positional parts
             constexpr int I = decltype(i)::value;
-            if constexpr (I == 8)
-                load_block<0>(pe_at(tile) + 8 * vw * PE_BYTES, at_pe);
-            else if constexpr (!Q4)
+            if constexpr (I == 8) {
+                if (VW == 4 || four) load_block<0>(pe_at(tile) + 8 * tw * PE_BYTES, at_pe);
+            } else if constexpr (!Q4)
                 load_block<(I & 3) * 256>(lat_at(tile) + (2 * vw + (I >> 2)) * (4 * BLOCK) + (I & 3) * BLOCK, at_latent[I >> 2]);
-            else if constexpr (I < 2)
-                load_block<0>(raw_at(tile) + (2 * vw + I) * BLOCK, at_latent[I]);  // of 4: codes of 4 tokens and of 4 more, the scales
-            else if constexpr (I == 2)
-                load_words(raw_at(tile) + L::RAW_SCALES + vw * 256, at_scales);
+            else if constexpr (I == 0 || (I == 1 && VW == 4))
+                load_block<0>(raw_at(tile) + (2 * tw + four + I) * BLOCK, at_latent[I]);  // of 4 bits: codes of 4 tokens and of 4 more, the scales
+            else if constexpr (I == 2) {
+                if (!four) load_words(raw_at(tile) + L::RAW_SCALES + tw * 256, at_scales);
+            }
         };
         // [row tile][32 values]: from 16 bits values 32 d + i, from 4 bits 64 (d / 2) + 2 i + d % 2, i = (e & 3) + 8 (e >> 2) + 4 half
-        f32x16 acc[RT][4] = {};
+        f32x16 acc[RT][DV] = {};
         float mo[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) mo[r] = M_START;
@@ -595,32 +604,76 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
             }
         };
         // The same from 4 bits.  A transposed read of bytes gives a lane 8 tokens' codes of values 2 m and 2 m + 1 (m = l % 32 of 64 values), and
-        // another, of the scales spread, their scales: eight conversions and eight exchanges of halves make one operand of even values and
-        // one of odd ones, without a detour through LDS (which, as 16-bit tiles written and read back transposed, took as long as
-        // everything else: a step 2500 cycles with one row tile and 2850 with two).
+        // another, of the scales written out 8 times, their scales: eight conversions and eight exchanges of halves make one operand of even
+        // values and one of odd ones.  A step multiplies what the step before made and makes the next tile's, so that no read of LDS is waited
+        // for but the weights'.
         const int tk = 8 * half + (c16 >> 1), pc = quad & 1;  // of 16 tokens the one whose bytes this lane reads; of two pieces the one
-        const uint32_t at_codes = tk * SCALES4 + (((4 * vw + pc) ^ turn4(tk)) << 4) + (c16 & 1) * 8, at_spread = tk * L::SPREAD + (4 * vw + pc) * 8;
+        const uint32_t at_codes = tk * SCALES4 + (((DV * vw + pc) ^ turn4(tk)) << 4) + (c16 & 1) * 8;
+        constexpr int NB = DV / 2, G = 2 * NB;  // blocks of 64 values, groups of a tile: [16 tokens][64 values]
+        const uint32_t spread = lds + vw * (BN * L::SPREAD), at_spread = spread + tk * L::SPREAD + pc * 8;
+        // lane l spreads the scales of token l / 2: with 4 value waves two of the wave's four, with 8 one of two
+        const uint32_t at_scale = L::RAW_SCALES + (lane >> 4) * 256 + (lane >> 1 & 7) * 16 + DV * vw + (lane & 1) * NB;
+        u32x4 vf[G][2];  // [group][even, odd]
+        uint32_t scale;
+        u32x2 code[G];
+        auto read_codes = [&](uint32_t tile) {
+            const uint32_t from = raw_at(tile);
+            if constexpr (NB == 2)
+                scale = *(__attribute__((address_space(3))) const uint16_t*)(lds_byte*)(uintptr_t)(from + at_scale);
+            else
+                scale = *(__attribute__((address_space(3))) const uint8_t*)(lds_byte*)(uintptr_t)(from + at_scale);
+#pragma unroll
+            for (int g = 0; g < G; ++g) code[g] = lds_read_tr8(((from + at_codes) ^ (g % NB) << 5) + g / NB * (16 * SCALES4));
+        };
+        u32x2 scale8[G];
+        auto spread_scales = [&] {
+            const uint32_t x = __builtin_amdgcn_perm(scale, scale, 0u), y = __builtin_amdgcn_perm(scale, scale, 0x01010101u);
+            if constexpr (NB == 2)
+                lds_write16(spread + lane * 16, u32x4{x, x, y, y});
+            else
+                *(__attribute__((address_space(3))) u32x2*)(lds_byte*)(uintptr_t)(spread + lane * 8) = u32x2{x, x};
+#pragma unroll
+            for (int g = 0; g < G; ++g) scale8[g] = lds_read_tr8(at_spread + g % NB * 16 + g / NB * (16 * L::SPREAD));
+        };
+        auto widen = [&](int g, bool mixed) {
+            uint32_t x[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
+                const uint32_t s4 = scale8[g][i], c4 = code[g][i];
+                x[4 * i] = T::template pair4<0>(c4, __uint_as_float(s4 << 23));
+                x[4 * i + 1] = T::template pair4<1>(c4, __uint_as_float(s4 << 15));
+                x[4 * i + 2] = T::template pair4<2>(c4, __uint_as_float(s4 << 7));
+                x[4 * i + 3] = T::template pair4<3>(c4, __uint_as_float(s4 >> 1));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                vf[g][0][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+                vf[g][1][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+            }
+            if (mixed)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    special |= nonfinite<T>(vf[g][i]);
+                    vf[g][i] = finite_part<T>(vf[g][i]);
+                }
+        };
+        auto is_mixed = [&](uint32_t tile) { return (int)(tile * BN + BN) > first; };  // some row does not see some token of the tile
         constexpr uint32_t AHEAD4 = 7;
         auto step4 = [&](uint32_t tile, auto last_) {
             constexpr bool LAST = decltype(last_)::value;
-            const bool mixed = (int)(tile * BN + BN) > first;  // some row does not see some token of the tile
             const uint32_t pb = lds + L::P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
-            const uint32_t cb = raw_at(tile) + at_codes, sb = spread_at(tile) + at_spread;
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
-            u32x2 codes[4], scales[4];  // [16-token step][64 values]
             u32x4 pf[2][RT];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                codes[g] = lds_read_tr8((cb ^ (g & 1) << 5) + (g >> 1) * (16 * SCALES4));
-                scales[g] = lds_read_tr8(sb + (g & 1) * 16 + (g >> 1) * (16 * L::SPREAD));
-            }
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) pf[0][r] = weight(0, r);
+                for (int r = 0; r < RT; ++r) pf[k][r] = weight(k, r);
             int page = 0;
-            if constexpr (!LAST) page = find_page(tile + AHEAD4);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) pf[1][r] = weight(1, r);
+            if constexpr (!LAST) {
+                page = find_page(tile + AHEAD4);
+                read_codes(tile + 1);
+            }
             __builtin_amdgcn_sched_barrier(0);
             if (any(fl)) {
 #pragma unroll
@@ -629,64 +682,45 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     const float f = raise(tile, 32 * r + c, mo[r]);
                     if (tile != t0)  // (nothing is there yet)
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) acc[r][d] *= f;
+                        for (int d = 0; d < DV; ++d) acc[r][d] *= f;
                 }
                 lds_barrier();  // the weights anew
 #pragma unroll
-                for (int r = 0; r < RT; ++r) pf[0][r] = weight(0, r), pf[1][r] = weight(1, r);
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) pf[k][r] = weight(k, r);
             }
-            u32x4 vf[2][2];  // [group % 2][even, odd]
-            auto widen = [&](int g) {
-                uint32_t x[8];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
-                    const uint32_t s4 = scales[g][i], c4 = codes[g][i];
-                    x[4 * i] = T::template pair4<0>(c4, __uint_as_float(s4 << 23));
-                    x[4 * i + 1] = T::template pair4<1>(c4, __uint_as_float(s4 << 15));
-                    x[4 * i + 2] = T::template pair4<2>(c4, __uint_as_float(s4 << 7));
-                    x[4 * i + 3] = T::template pair4<3>(c4, __uint_as_float(s4 >> 1));
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    vf[g & 1][0][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
-                    vf[g & 1][1][j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
-                }
-                if (mixed)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        special |= nonfinite<T>(vf[g & 1][i]);
-                        vf[g & 1][i] = finite_part<T>(vf[g & 1][i]);
-                    }
-            };
+            const bool mixed = is_mixed(tile + 1);
             uint64_t at = 0;
-            widen(0);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < G; ++g) {
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[r][2 * (g & 1) + i] = T::mfma(vf[g & 1][i], pf[g >> 1][r], acc[r][2 * (g & 1) + i]);
-                if (g < 3) widen(g + 1);
+                    for (int r = 0; r < RT; ++r) acc[r][2 * (g % NB) + i] = T::mfma(vf[g][i], pf[g / NB][r], acc[r][2 * (g % NB) + i]);
                 if constexpr (!LAST) {
+                    if (g == 0) spread_scales();
                     if constexpr (EVEN) {
                         if (g == 0) at = find_rows(tile + AHEAD4, page);
                         if (g == 1) bring_even(tile + AHEAD4, at, 0);
-                        if (g == 2) bring_even(tile + AHEAD4, at, 1), bring_even(tile + AHEAD4, at, 2);
-                        if (g == 3) bring_even(tile + AHEAD4, at, 3);
+                        if (g == G / 2) bring_even(tile + AHEAD4, at, 1), bring_even(tile + AHEAD4, at, 2);
+                        if (g == G - 1) bring_even(tile + AHEAD4, at, 3);
                     } else {
                         if (g == 0) at = find_token(tile + AHEAD4, page), find_latent(at, 0), find_latent(at, 1);
                         if (g == 1) bring(tile + AHEAD4, Int<0>{}), find_scales(at), find_pe(at);
-                        if (g == 2) bring(tile + AHEAD4, Int<1>{}), bring(tile + AHEAD4, Int<2>{});
-                        if (g == 3) bring(tile + AHEAD4, Int<8>{});
+                        if (g == G / 2) bring(tile + AHEAD4, Int<1>{});
+                        if (g == G - 1) bring(tile + AHEAD4, Int<2>{}), bring(tile + AHEAD4, Int<8>{});
                     }
-                    if (g == 3) load_pages(tile + AHEAD4 + 8);
+                    if (g == G - 1) load_pages(tile + AHEAD4 + 8);
+                    if (g > 0) widen(g - 1, mixed);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
-                wait_loads<5 * L::LOADS>();
-                lds_barrier();  // the next tile's weights; the tile after it is whole
+                widen(G - 1, mixed);
+                wait_loads<4 * L::LOADS>();
+                lds_barrier();  // the next tile's weights; the two tiles after it are whole
             }
         };
         if (n_tiles) {
@@ -720,11 +754,16 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 whole_tile(t0 + 2);
                 wait_loads<2 * L::LOADS>();
                 lds_barrier();  // the first tile, the queries
-                lds_barrier();  // the queries are in registers
-                // while the first tile's scores are computed: what comes after the third tile
+                wait_loads<L::LOADS>();
+                lds_barrier();  // the queries are in registers; the second tile is whole
+                // while the first tile's scores are computed: its values, and what comes after the third tile
+                read_codes(t0);
+                spread_scales();
 #pragma unroll
                 for (int i = 3; i < 7; ++i) whole_tile(t0 + i);
-                wait_loads<5 * L::LOADS>();
+#pragma unroll
+                for (int g = 0; g < G; ++g) widen(g, is_mixed(t0));
+                wait_loads<4 * L::LOADS>();
             } else {
                 load_pages(t0 + 4);
                 wait_loads<L::LOADS>();
@@ -767,10 +806,10 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                     };
                     if constexpr (Q4) {
 #pragma unroll
-                        for (int d = 0; d < 2; ++d)
+                        for (int d = 0; d < DV / 2; ++d)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {  // 8 values in a row
-                                const int at = 128 * vw + 64 * d + 16 * e + 8 * my;
+                                const int at = DIMS * vw + 64 * d + 16 * e + 8 * my;
                                 const uint32_t b = *reinterpret_cast<const uint8_t*>(row + SCALES4 + at / GROUP);
                                 const u32x4 x = T::from4(*reinterpret_cast<const uint32_t*>(row + at / 2), __uint_as_float(b << 23));
 #pragma unroll
@@ -810,10 +849,10 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 if (i >= r1) break;
                 const float inv = ls[r] > 0.f ? 1.f / ls[r] : 0.f;
                 const int t = i / a.H, h = i - t * a.H;
-                uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + 128 * vw + 4 * half;
+                uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_row + h * a.out_head + DIMS * vw + 4 * half;
                 if constexpr (Q4) {
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < DV / 2; ++b)
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) {
                             u32x4 x;
@@ -844,11 +883,11 @@ __global__ void __launch_bounds__(THREADS, 2) decode_kernel(KdaLatentDecodeArgs 
                 char* o = out + r * SLOT_TILE + vw * 16384 + lane * 16;
                 if constexpr (Q4) {  // as the other form leaves them: a lane's 8 values in a row are two lanes' four
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < DV / 2; ++b)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             f32x16 &x = acc[r][2 * b], &y = acc[r][2 * b + 1];
-                            char* to = out + r * SLOT_TILE + vw * 16384 + c * 16 + ((2 * b + (e >> 1)) * 4 + 2 * (e & 1) + half) * 1024;
+                            char* to = out + r * SLOT_TILE + vw * (DIMS * 128) + c * 16 + ((2 * b + (e >> 1)) * 4 + 2 * (e & 1) + half) * 1024;
                             *reinterpret_cast<f32x4*>(to) = f32x4{x[4 * e], y[4 * e], x[4 * e + 1], y[4 * e + 1]};
                             *reinterpret_cast<f32x4*>(to + 512) = f32x4{x[4 * e + 2], y[4 * e + 2], x[4 * e + 3], y[4 * e + 3]};
                         }
@@ -1050,10 +1089,11 @@ int decode_launch(const KdaLatentDecodeArgs* a, kda355_stream_t stream) {
     auto launch = [&](auto type) {
         typedef decltype(type) T;
         const bool two = p.own.rows > 32 || p.pre.rows > 32;  // (one row tile: one sequence of 4097 tokens, 12 heads 14.0 us, with two 15.4)
+        const dim3 threads(two ? THREADS<2, Q4> : THREADS<1, Q4>);
         if (Q4 && a->page_size % 8 == 0)
-            launch_kernel(two ? decode_kernel<T, 2, Q4, Q4> : decode_kernel<T, 1, Q4, Q4>, dim3(p.grid), dim3(THREADS), s, *a, p);
+            launch_kernel(two ? decode_kernel<T, 2, Q4, Q4> : decode_kernel<T, 1, Q4, Q4>, dim3(p.grid), threads, s, *a, p);
         else
-            launch_kernel(two ? decode_kernel<T, 2, Q4, false> : decode_kernel<T, 1, Q4, false>, dim3(p.grid), dim3(THREADS), s, *a, p);
+            launch_kernel(two ? decode_kernel<T, 2, Q4, false> : decode_kernel<T, 1, Q4, false>, dim3(p.grid), threads, s, *a, p);
         if (few)
             launch_kernel((join_kernel<T, true>), dim3(join, tiles * 16), dim3(1024), s, *a, p);
         else
