@@ -4,13 +4,15 @@
 // token from above, and the recent ones follow in order.
 //
 // 1. A workgroup a (sequence, layer): the weight of the last one that stays, by its bits from the top, 11 at a time over a histogram in LDS;
-//    then the places and tokens of the pairs by ranks in index order, and the weights moved; few pairs' rows at once.
+//    then the places and tokens of the pairs by ranks in index order, and the weights moved; few pairs' rows at once.  Long sequences by a
+//    workgroup for 8192 tokens, with a launch for each digit, one for the parts' counts and one for the lists; the weights go with the rows.
 // 2. The pairs' rows: no place of a pair is read by another, so all at once.
 // 3. The recent rows.  Where they move by their own number or more, all at once.  Else in place: their new places are other recent rows' old
 //    ones, so a workgroup takes a strip of columns and walks down, reading a step's rows before it writes any of them (a row moves
 //    down, so what is read later has not been written).  Beside it, for few table entries, the books.
 // 4. For many entries: table rows, lengths and counts, then what nobody holds any more onto the stack.
-// All are bound by memory or, for few tokens, by their launches.
+// The rows are bound by memory (2 and 3 for 800 MB: 180 us, 4.5 TB/s), the rest by the latency of its steps: 1 takes 13 us for one sequence
+// of 4160 tokens, 18 for 64 in 4 layers, 39 for 131072 and 100001 in 7.
 #include "pages.h"
 
 namespace kda355 {
@@ -21,7 +23,8 @@ constexpr int PAIRS = 64;                        // of a workgroup at a time
 constexpr int MOVE_THREADS = 256;
 constexpr int STRIP = 8, SHIFT_ROWS = 4;         // 16-byte pieces of a strip, rows of a thread at a time
 constexpr int FEW = 128;                         // pairs that the first kernel moves itself
-constexpr int WAVES = SCAN_THREADS / 64, BINS = 2048, SOME = 16 * 1024, ROW_PAGES = 2048;
+constexpr int WAVES = SCAN_THREADS / 64, BINS = 2048, ROW_PAGES = 2048;
+constexpr int PART_KEYS = 8, PART = PART_KEYS * SCAN_THREADS, AT_ONCE = 1024;  // of a thread, of a workgroup; (sequence, layer)s in one run of the parts
 constexpr int BOOK_ENTRIES = 4096, BOOK_PAGES = 16 * 1024;  // up to so many table entries and pages the books take one workgroup
 
 struct Plan {
@@ -30,9 +33,13 @@ struct Plan {
     int tail;         // pages that hold the recent tokens, at most
     int strips;       // workgroups of a sequence and layer in the third kernel
     int books;        // the books beside it
+    int parts;        // workgroups that select for a sequence and layer, 0: one
+    int first, rows;  // with parts: sequences of this run of them
 };
 // workspace: the lengths of the sequences that are cut, -1 for others [n]; pairs of (sequence, layer) [n][layers]; the pages from the
-// first recent token's on [n][tail] (the books change the table); places and tokens of the pairs [n][layers][2][most]
+// first recent token's on [n][tail] (the books change the table); places and tokens of the pairs [n][layers][2][most];
+// with parts: the tokens that stay for being held elsewhere [n], and of a run of sequences histograms [rows][layers][3][BINS] and counts
+// of the parts [rows][layers][parts][4]
 __device__ __forceinline__ int32_t* lens_of(const KdaEvictArgs& a) { return static_cast<int32_t*>(a.workspace); }
 __device__ __forceinline__ int32_t* pairs_of(const KdaEvictArgs& a, int i, int l) { return lens_of(a) + a.n + i * a.num_layers + l; }
 __device__ __forceinline__ int32_t* tail_of(const KdaEvictArgs& a, const Plan& p, int i) {
@@ -40,6 +47,13 @@ __device__ __forceinline__ int32_t* tail_of(const KdaEvictArgs& a, const Plan& p
 }
 __device__ __forceinline__ int32_t* lists_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {
     return tail_of(a, p, a.n) + ((int64_t)i * a.num_layers + l) * 2 * p.most;
+}
+__device__ __forceinline__ int32_t* fixed_of(const KdaEvictArgs& a, const Plan& p) { return lists_of(a, p, a.n, 0); }
+__device__ __forceinline__ int32_t* hist_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {  // i: of the run
+    return fixed_of(a, p) + a.n + ((int64_t)i * a.num_layers + l) * 3 * BINS;
+}
+__device__ __forceinline__ int32_t* counts_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {
+    return hist_of(a, p, p.rows, 0) + ((int64_t)i * a.num_layers + l) * 4 * p.parts;
 }
 __device__ __forceinline__ char* token_in(const KdaEvictArgs& a, const KdaEvictLayer& y, int page, int j) {
     return static_cast<char*>(y.cache) + page * y.page_stride + (int64_t)(j % a.page_size) * y.token_bytes;
@@ -75,44 +89,29 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 
 __device__ __forceinline__ int below(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
 
-// The keys of the tokens before the recent ones: wave w has a run of them, in rounds of 64 in index order, so that ranks take one exchange
-// between the waves.  R > 0: in registers, up to 1024 R of them; R = 0: read anew (from L2) wherever they are needed.
+// The keys of tokens from .. stop - 1, up to 1024 R of them, in registers: wave w has a run of them, in rounds of 64 in index order, so that
+// ranks take one exchange between the waves.
 template <int R>
 struct Keys {
-    const float* weights;
     int first, end, rounds;  // of this wave
-    uint32_t k[R ? R : 1];
-    __device__ __forceinline__ Keys(const float* w, int stop) : weights(w) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        rounds = ((stop + 63) / 64 + WAVES - 1) / WAVES;
-        first = wave * rounds * 64 + lane;
+    uint32_t k[R];
+    __device__ __forceinline__ Keys(const float* weights, int from, int stop) {
+        rounds = ((stop - from + 63) / 64 + WAVES - 1) / WAVES;
+        first = from + (threadIdx.x >> 6) * rounds * 64 + (threadIdx.x & 63);
         end = stop;
-        if constexpr (R > 0) {
-            float x[R];
+        float x[R];
 #pragma unroll
-            for (int r = 0; r < R; ++r) x[r] = weights[max(min(first + r * 64, end - 1), 0)];  // (no branches; `weights` has a first one)
+        for (int r = 0; r < R; ++r) x[r] = weights[max(min(first + r * 64, end - 1), 0)];  // (no branches; `weights` has a first one)
 #pragma unroll
-            for (int r = 0; r < R; ++r) k[r] = key_of(x[r]);
-        }
+        for (int r = 0; r < R; ++r) k[r] = key_of(x[r]);
     }
     // f(position, key, is it a candidate: at or after `fixed`) for all rounds, in order
     template <typename F>
     __device__ __forceinline__ void each(int fixed, F f) const {
-        auto there = [&](int j) { return j < end && j >= fixed; };
-        if constexpr (R > 0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (r < rounds) f(first + r * 64, k[r], there(first + r * 64));
-        } else {
-            constexpr int U = 16;  // in flight (131072 keys: 10 to 15 us a pass)
-            for (int r0 = 0; r0 < rounds; r0 += U) {
-                float x[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) x[u] = weights[min(first + (r0 + u) * 64, end - 1)];  // (no branches)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r0 + u < rounds) f(first + (r0 + u) * 64, key_of(x[u]), there(first + (r0 + u) * 64));
-            }
+        for (int r = 0; r < R; ++r) {
+            const int j = first + r * 64;
+            if (r < rounds) f(j, k[r], j < end && j >= fixed);
         }
     }
 };
@@ -132,44 +131,120 @@ __device__ __forceinline__ int before_wave(int x, int* sw, int& total) {
     return before;
 }
 
+// tokens of the row in slot i, -1 where nothing is to be cut
+__device__ __forceinline__ int length_of(const KdaEvictArgs& a, int row) {
+    int len = -1;
+    if (row >= 0 && row < a.rows) len = (int)min((int64_t)a.seq_lens[row], (int64_t)a.table_width * a.page_size);
+    return len <= a.keep ? -1 : len;
+}
+// The tokens that stay for being held elsewhere into flags[0], whether there is a hole or the row was given before into flags[1] (zeros
+// before, a barrier after); the pages of the recent tokens, if `tail`; the first pages into `pages`, if there is such a list.
+__device__ __forceinline__ void look(const KdaEvictArgs& a, const Plan& p, int i, int row, int len, int* flags, bool tail, int* pages) {
+    const int used = (len + a.page_size - 1) / a.page_size, from = (len - a.recent) / a.page_size;
+    int fixed = 0, bad = 0;
+    for (int j = threadIdx.x; j < used; j += SCAN_THREADS) {
+        const int page = a.block_table[row * a.table_stride + j];
+        if (page < 0 || page >= a.pages) bad = 1;
+        else if (a.ref_counts[page] > 1) fixed = (j + 1) * a.page_size;
+        if (tail && j >= from) tail_of(a, p, i)[j - from] = page;
+        if (pages && j < ROW_PAGES) pages[j] = page;
+    }
+    for (int j = threadIdx.x; j < i; j += SCAN_THREADS) bad |= a.src[j] == row;
+    if (fixed) atomicMax(&flags[0], fixed);
+    if (bad) flags[1] = 1;
+}
+
+// The stay-th largest key, digit by digit from the top: 11 bits, 11 and 10.
+struct Last {
+    uint32_t prefix;  // its digits so far; ~0 if none stays (not even a NaN, of which `stay` = 0 do)
+    int stay;         // how many with these digits stay
+    bool all;         // whether all do
+    __device__ __forceinline__ explicit Last(int n) : prefix(n > 0 ? 0u : ~0u), stay(n), all(false) {}
+    static __device__ __forceinline__ int shift(int digit) { return digit == 0 ? 21 : digit == 1 ? 10 : 0; }
+    // histogram of a digit over the keys with the digits before it
+    __device__ __forceinline__ void count(int* hist, int digit, uint32_t k, bool there) const {
+        const uint32_t mask = digit == 0 ? 0u : ~0u << shift(digit - 1);
+        if (there && (k & mask) == prefix) atomicAdd(&hist[k >> shift(digit) & (digit < 2 ? 2047 : 1023)], 1);
+    }
+    // the digit from the histogram, which is cleared; found: 3 words in LDS
+    __device__ __forceinline__ void pick(int* hist, int digit, int* found, int* sw) {
+        const int t = threadIdx.x;
+        int total;
+        __syncthreads();
+        // the largest digits first: thread t has 2047 - 2 t and 2046 - 2 t
+        const int hi = hist[BINS - 1 - 2 * t], lo = hist[BINS - 2 - 2 * t];
+        const int before = block_scan(hi + lo, sw, total);
+        if (before < stay && stay <= before + hi + lo) {
+            const bool upper = stay <= before + hi;
+            found[0] = upper ? BINS - 1 - 2 * t : BINS - 2 - 2 * t;
+            found[1] = stay - before - (upper ? 0 : hi);
+            found[2] = upper ? hi : lo;
+        }
+        hist[BINS - 1 - 2 * t] = hist[BINS - 2 - 2 * t] = 0;
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << shift(digit);
+        stay = found[1];
+        all = stay == found[2];
+    }
+    // f(position, is it a hole: a place below left whose token goes, is it a mover: a token from left on that stays, their ballots); ties:
+    // tokens with the key before this wave's
+    template <int R, typename F>
+    __device__ __forceinline__ void marks(const Keys<R>& keys, int fixed, int left, int ties, F f) const {
+        keys.each(fixed, [&](int j, uint32_t k, bool there) {
+            bool stays = there && k >= prefix;
+            if (!all) {  // the first `stay` of those with the key stay
+                const bool tie = there && k == prefix;
+                const uint64_t tied = __builtin_amdgcn_ballot_w64(tie);
+                if (tie) stays = ties + below(tied) < stay;
+                ties += __popcll(tied);
+            }
+            const bool hole = there && !stays && j < left, mover = stays && j >= left;
+            f(j, hole, mover, __builtin_amdgcn_ballot_w64(hole), __builtin_amdgcn_ballot_w64(mover));
+        });
+    }
+};
+// The recent weights where they go, zeros behind them, by one workgroup; late: the first 4 x 1024.
+__device__ __forceinline__ void shift_weights(const KdaEvictArgs& a, const Plan& p, float* weights, int len, const float (&late)[4]) {
+    const int end = len - a.recent, tid = threadIdx.x;
+    for (int k0 = 0; k0 < a.recent; k0 += 4 * SCAN_THREADS) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = k0 + u * SCAN_THREADS + tid;
+            x[u] = k0 == 0 ? late[u] : k < a.recent ? weights[end + k] : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = k0 + u * SCAN_THREADS + tid;
+            if (k < a.recent) weights[p.left + k] = x[u];
+        }
+        __syncthreads();
+    }
+    for (int j = a.keep + tid; j < len; j += SCAN_THREADS) weights[j] = 0.f;
+}
+
 template <int R>
 __global__ void __launch_bounds__(SCAN_THREADS) select_kernel(KdaEvictArgs a, Plan p) {
     __shared__ int hist[BINS];
     __shared__ int sw[WAVES];
-    __shared__ int flags[6];  // fixed; is there a hole or was the row given before; digit, rank in it, keys with it; keys gathered
+    __shared__ int flags[5];  // of `look`; of `pick`
     __shared__ char* at[2][PAIRS];
     __shared__ int few[2][FEW];  // the first pairs
-    __shared__ uint32_t some[R ? 1 : SOME];
     __shared__ int pages[ROW_PAGES];  // the first of the row's
     const int i = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
     const int row = a.src[i];
     const KdaEvictLayer y = a.layer[l];
-    if (tid < 6) flags[tid] = 0;
+    if (tid < 5) flags[tid] = 0;
     hist[tid] = hist[tid + SCAN_THREADS] = 0;
-    int len = -1;
-    if (row >= 0 && row < a.rows) len = (int)min((int64_t)a.seq_lens[row], (int64_t)a.table_width * a.page_size);
-    if (len <= a.keep) len = -1;
-    const int end = len - a.recent;  // candidates [fixed, end), `stay` of them stay
+    const int len = length_of(a, row), end = len - a.recent;  // candidates [fixed, end)
     float* const weights = y.weights + (len < 0 ? 0 : row) * y.weights_row;
-    const Keys<R> keys(weights, len < 0 ? 0 : end);
+    const Keys<R> keys(weights, 0, len < 0 ? 0 : end);
     float late[4];  // the first recent ones, for the end
 #pragma unroll
     for (int u = 0; u < 4; ++u) late[u] = weights[len < 0 ? 0 : min(end + u * SCAN_THREADS + tid, len - 1)];
     __syncthreads();
-    if (len >= 0) {
-        const int used = (len + a.page_size - 1) / a.page_size, tail = end / a.page_size;
-        int fixed = 0, bad = 0;
-        for (int j = tid; j < used; j += SCAN_THREADS) {
-            const int page = a.block_table[row * a.table_stride + j];
-            if (page < 0 || page >= a.pages) bad = 1;
-            else if (a.ref_counts[page] > 1) fixed = (j + 1) * a.page_size;
-            if (l == 0 && j >= tail) tail_of(a, p, i)[j - tail] = page;
-            if (j < ROW_PAGES) pages[j] = page;
-        }
-        for (int j = tid; j < i; j += SCAN_THREADS) bad |= a.src[j] == row;
-        if (fixed) atomicMax(&flags[0], fixed);
-        if (bad) flags[1] = 1;
-    }
+    if (len >= 0) look(a, p, i, row, len, flags, l == 0, pages);
     __syncthreads();
     const int fixed = flags[0];
     const bool cut = len >= 0 && !flags[1] && fixed <= p.left;
@@ -178,79 +253,29 @@ __global__ void __launch_bounds__(SCAN_THREADS) select_kernel(KdaEvictArgs a, Pl
         if (tid == 0) *pairs_of(a, i, l) = 0;
         return;
     }
-    int stay = p.left - fixed, total;
-    // ---- the key of the last one that stays, how many with this key stay, and whether all with it do
-    uint32_t prefix = ~0u;  // none stays: not even a NaN, of which `stay` = 0 do
-    bool all = false;
-    if (stay > 0) {
-        prefix = 0;
-        auto pick = [&](uint32_t shift) {  // the digit of the stay-th largest key from the histogram, which is cleared
-            __syncthreads();
-            // the largest digits first: thread t has 2047 - 2 t and 2046 - 2 t
-            const int hi = hist[BINS - 1 - 2 * tid], lo = hist[BINS - 2 - 2 * tid];
-            const int before = block_scan(hi + lo, sw, total);
-            if (before < stay && stay <= before + hi + lo) {
-                const bool upper = stay <= before + hi;
-                flags[2] = upper ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid;
-                flags[3] = stay - before - (upper ? 0 : hi);
-                flags[4] = upper ? hi : lo;
-            }
-            hist[BINS - 1 - 2 * tid] = hist[BINS - 2 - 2 * tid] = 0;
-            __syncthreads();
-            prefix |= (uint32_t)flags[2] << shift;
-            stay = flags[3];
-            all = stay == flags[4];
-        };
-        auto count = [&](uint32_t k, bool there, uint32_t mask, uint32_t shift, uint32_t bins) {
-            if (there && (k & mask) == prefix) atomicAdd(&hist[k >> shift & bins], 1);
-        };
-        keys.each(fixed, [&](int, uint32_t k, bool there) { count(k, there, 0, 21, 2047); });
-        pick(21);
-        if (R == 0 && flags[4] <= SOME) {  // the other digits over the keys that have the first one, gathered in LDS
-            keys.each(fixed, [&](int, uint32_t k, bool there) {
-                if (there && (k & ~0u << 21) == prefix) some[atomicAdd(&flags[5], 1)] = k;
-            });
-            __syncthreads();
-            const int n = flags[5];
-            for (int j = tid; j < n; j += SCAN_THREADS) count(some[j], true, ~0u << 21, 10, 2047);
-            pick(10);
-            for (int j = tid; j < n; j += SCAN_THREADS) count(some[j], true, ~0u << 10, 0, 1023);
-        } else {
-            keys.each(fixed, [&](int, uint32_t k, bool there) { count(k, there, ~0u << 21, 10, 2047); });
-            pick(10);
-            keys.each(fixed, [&](int, uint32_t k, bool there) { count(k, there, ~0u << 10, 0, 1023); });
+    int total;
+    Last last(p.left - fixed);
+    if (last.stay > 0)
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+            keys.each(fixed, [&](int, uint32_t k, bool there) { last.count(hist, d, k, there); });
+            last.pick(hist, d, flags + 2, sw);
         }
-        pick(0);
-    }
-    // ---- places below left whose token goes, tokens from left on that stay, in index order
+    // ---- holes and movers, in index order
     int32_t* const places = lists_of(a, p, i, l);
     int32_t* const tokens = places + p.most;
     int ties = 0;
-    if (!all) {  // the first `stay` of those with the key stay
-        keys.each(fixed, [&](int, uint32_t k, bool there) { ties += __popcll(__builtin_amdgcn_ballot_w64(there && k == prefix)); });
+    if (!last.all) {
+        keys.each(fixed, [&](int, uint32_t k, bool there) { ties += __popcll(__builtin_amdgcn_ballot_w64(there && k == last.prefix)); });
         ties = before_wave(ties, sw, total);
     }
     int holes = 0, movers = 0;
-    auto marks = [&](auto f) {  // f(position, is it a hole, is it a mover, their ballots)
-        int t = ties;
-        keys.each(fixed, [&](int j, uint32_t k, bool there) {
-            bool stays = there && k >= prefix;
-            if (!all) {
-                const bool tie = there && k == prefix;
-                const uint64_t tied = __builtin_amdgcn_ballot_w64(tie);
-                if (tie) stays = t + below(tied) < stay;
-                t += __popcll(tied);
-            }
-            const bool hole = there && !stays && j < p.left, mover = stays && j >= p.left;
-            f(j, hole, mover, __builtin_amdgcn_ballot_w64(hole), __builtin_amdgcn_ballot_w64(mover));
-        });
-    };
-    marks([&](int, bool, bool, uint64_t h, uint64_t m) { holes += __popcll(h), movers += __popcll(m); });
+    last.marks(keys, fixed, p.left, ties, [&](int, bool, bool, uint64_t h, uint64_t m) { holes += __popcll(h), movers += __popcll(m); });
     int pairs;
     holes = before_wave(holes, sw, pairs);
     movers = before_wave(movers, sw, total);  // (as many)
     const bool few_pairs = pairs <= FEW;
-    marks([&](int j, bool hole, bool mover, uint64_t h, uint64_t m) {
+    last.marks(keys, fixed, p.left, ties, [&](int j, bool hole, bool mover, uint64_t h, uint64_t m) {
         if (hole) (few_pairs ? few[0] : places)[holes + below(h)] = j;
         if (mover) (few_pairs ? few[1] : tokens)[movers + below(m)] = j;
         holes += __popcll(h), movers += __popcll(m);
@@ -287,37 +312,133 @@ __global__ void __launch_bounds__(SCAN_THREADS) select_kernel(KdaEvictArgs a, Pl
         }
     }
     __syncthreads();
-    for (int k0 = 0; k0 < a.recent; k0 += 4 * SCAN_THREADS) {
-        float x[4];
+    shift_weights(a, p, weights, len, late);
+}
+
+// The same of more tokens, by a workgroup for 8192 of each (sequence, layer): what a row's pages say, the histograms of three digits, the
+// counts of each part, the lists.
+__global__ void __launch_bounds__(SCAN_THREADS) look_kernel(KdaEvictArgs a, Plan p) {
+    __shared__ int flags[2];
+    const int i = p.first + blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
+    int32_t* const hist = hist_of(a, p, blockIdx.x, l);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int k = k0 + u * SCAN_THREADS + tid;
-            x[u] = k0 == 0 ? late[u] : k < a.recent ? weights[end + k] : 0.f;
-        }
-        __syncthreads();
+    for (int k = 0; k < 3 * BINS; k += SCAN_THREADS) hist[k + tid] = 0;
+    if (tid == 0) *pairs_of(a, i, l) = 0;
+    if (l) return;
+    if (tid < 2) flags[tid] = 0;
+    const int row = a.src[i], len = length_of(a, row);
+    __syncthreads();
+    if (len >= 0) look(a, p, i, row, len, flags, true, nullptr);
+    __syncthreads();
+    if (tid) return;
+    lens_of(a)[i] = len >= 0 && !flags[1] && flags[0] <= p.left ? len : -1;
+    fixed_of(a, p)[i] = flags[0];
+}
+
+// PASS 0 to 2: the histogram of a digit.  3: the part's counts.  4: its lists.
+template <int PASS>
+__global__ void __launch_bounds__(SCAN_THREADS) part_kernel(KdaEvictArgs a, Plan p) {
+    __shared__ int hist[BINS];
+    __shared__ int sw[WAVES];
+    __shared__ int found[3], earlier[3];  // of `pick`; the parts before this one: tokens with the key, holes, movers
+    const int i = p.first + blockIdx.y, l = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int len = lens_of(a)[i], from = blockIdx.x * PART, end = len - a.recent;
+    if (len < 0 || from >= end) return;
+    const KdaEvictLayer y = a.layer[l];
+    const Keys<PART_KEYS> keys(y.weights + a.src[i] * y.weights_row, from, min(end, from + PART));
+    const int fixed = fixed_of(a, p)[i];
+    int32_t* const hists = hist_of(a, p, blockIdx.y, l);
+    int x[3][2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int k = k0 + u * SCAN_THREADS + tid;
-            if (k < a.recent) weights[p.left + k] = x[u];
+    for (int d = 0; d < 3 && d < PASS; ++d) x[d][0] = hists[d * BINS + tid], x[d][1] = hists[d * BINS + SCAN_THREADS + tid];
+    Last last(p.left - fixed);
+    if (last.stay > 0) {
+#pragma unroll
+        for (int d = 0; d < 3 && d < PASS; ++d) {
+            hist[tid] = x[d][0], hist[tid + SCAN_THREADS] = x[d][1];
+            last.pick(hist, d, found, sw);
         }
-        __syncthreads();
+        if constexpr (PASS < 3) {
+            if (PASS == 0) hist[tid] = hist[tid + SCAN_THREADS] = 0;
+            __syncthreads();
+            keys.each(fixed, [&](int, uint32_t k, bool there) { last.count(hist, PASS, k, there); });
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < BINS; k += SCAN_THREADS)
+                if (hist[k + tid]) atomicAdd(hists + PASS * BINS + k + tid, hist[k + tid]);
+        }
     }
-    for (int j = a.keep + tid; j < len; j += SCAN_THREADS) weights[j] = 0.f;
+    if constexpr (PASS < 3) return;
+    // with the key below left and from it on; lighter ones below left, heavier ones from it on
+    int32_t* const counts = counts_of(a, p, blockIdx.y, l);
+    if constexpr (PASS == 3) {
+        int n[4] = {}, total[4];
+        keys.each(fixed, [&](int j, uint32_t k, bool there) {
+            const bool low = j < p.left;
+            n[0] += __popcll(__builtin_amdgcn_ballot_w64(there && k == last.prefix && low));
+            n[1] += __popcll(__builtin_amdgcn_ballot_w64(there && k == last.prefix && !low));
+            n[2] += __popcll(__builtin_amdgcn_ballot_w64(there && k < last.prefix && low));
+            n[3] += __popcll(__builtin_amdgcn_ballot_w64(there && k > last.prefix && !low));
+        });
+#pragma unroll
+        for (int k = 0; k < 4; ++k) before_wave(n[k], sw, total[k]);
+        if (tid < 4) counts[4 * blockIdx.x + tid] = tid == 0 ? total[0] : tid == 1 ? total[1] : tid == 2 ? total[2] : total[3];
+        return;
+    }
+    // ---- the parts before this one
+    if (tid < 64) {
+        int ties = 0, holes = 0, movers = 0;
+        for (int c0 = 0; c0 < (int)blockIdx.x; c0 += 64) {
+            int n[4] = {};
+            if (c0 + lane < (int)blockIdx.x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) n[k] = counts[4 * (c0 + lane) + k];
+            int sum = n[0] + n[1];
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int v = __shfl_up(sum, d);
+                if (lane >= d) sum += v;
+            }
+            const int left = last.stay - (ties + sum - n[0] - n[1]);  // of those with the key may stay from this part on
+            const int low = max(0, min(left, n[0])), high = max(0, min(left - n[0], n[1]));
+            holes += n[2] + n[0] - low, movers += n[3] + high;
+            ties += __shfl(sum, 63);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) holes += __shfl_xor(holes, d), movers += __shfl_xor(movers, d);
+        if (tid == 0) earlier[0] = ties, earlier[1] = holes, earlier[2] = movers;
+    }
+    int total, pairs, ties = 0, holes = 0, movers = 0;
+    keys.each(fixed, [&](int, uint32_t k, bool there) { ties += __popcll(__builtin_amdgcn_ballot_w64(there && k == last.prefix)); });
+    ties = before_wave(ties, sw, total) + earlier[0];
+    last.marks(keys, fixed, p.left, ties, [&](int, bool, bool, uint64_t h, uint64_t m) { holes += __popcll(h), movers += __popcll(m); });
+    holes = before_wave(holes, sw, pairs) + earlier[1];
+    movers = before_wave(movers, sw, total) + earlier[2];
+    int32_t* const places = lists_of(a, p, i, l);
+    int32_t* const tokens = places + p.most;
+    if (tid == 0 && from + PART >= end) *pairs_of(a, i, l) = earlier[1] + pairs;
+    last.marks(keys, fixed, p.left, ties, [&](int j, bool hole, bool mover, uint64_t h, uint64_t m) {
+        if (hole) places[holes + below(h)] = j;
+        if (mover) tokens[movers + below(m)] = j;
+        holes += __popcll(h), movers += __popcll(m);
+    });
 }
 
 __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(KdaEvictArgs a, Plan p) {
     __shared__ char* at[2][PAIRS];
     const int i = blockIdx.y, l = blockIdx.z;
     const int pairs = *pairs_of(a, i, l);
-    if (pairs <= FEW) return;
+    if (!p.parts && pairs <= FEW) return;
     const int32_t* lists = lists_of(a, p, i, l);
     const KdaEvictLayer y = a.layer[l];
     const int row = a.src[i], pieces = (int)(y.token_bytes / 16);
+    float* const weights = y.weights + row * y.weights_row;
     for (int first = blockIdx.x * PAIRS; first < pairs; first += gridDim.x * PAIRS) {
         const int count = min(pairs - first, PAIRS);
         __syncthreads();
         for (int k = threadIdx.x; k < 2 * PAIRS; k += MOVE_THREADS)
             if (k % PAIRS < count) at[k / PAIRS][k % PAIRS] = token_at(a, y, row, lists[(int64_t)(k / PAIRS) * p.most + first + k % PAIRS]);
+        if (p.parts && (int)threadIdx.x < count) weights[lists[first + threadIdx.x]] = weights[lists[(int64_t)p.most + first + threadIdx.x]];
         __syncthreads();
         copy_tokens<MOVE_THREADS>(at, count, pieces);
     }
@@ -366,7 +487,23 @@ __global__ void __launch_bounds__(SCAN_THREADS) shift_kernel(KdaEvictArgs a, Pla
     // The places are below keep: their pages stay where they are in the table, unlike those of the tokens.
     auto token = [&](int k) { return token_in(a, y, tail[(end + k) / a.page_size - first_page], end + k); };
     auto place = [&](int k) { return token_at(a, y, row, p.left + k); };
-    if (len - a.keep >= a.recent) {
+    if (p.parts) {  // the weights
+        float* const weights = y.weights + row * y.weights_row;
+        const int first = blockIdx.x * SCAN_THREADS + tid, step = p.strips * SCAN_THREADS;
+        if (end >= a.keep) {  // no place is another one's token
+            for (int k = first; k < a.recent; k += step) {
+                weights[p.left + k] = weights[end + k];
+                weights[end + k] = 0.f;
+            }
+            for (int j = a.keep + first; j < end; j += step) weights[j] = 0.f;
+        } else if (blockIdx.x == 0) {
+            float late[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) late[u] = weights[min(end + u * SCAN_THREADS + tid, len - 1)];
+            shift_weights(a, p, weights, len, late);
+        }
+    }
+    if (end >= a.keep) {
         for (int first = blockIdx.x * PAIRS; first < a.recent; first += p.strips * PAIRS) {
             const int count = min(a.recent - first, PAIRS);
             __syncthreads();
@@ -411,6 +548,12 @@ Plan plan_of(const KdaEvictArgs* a) {
     const int64_t goes = span - a->keep;  // no more tokens go from below `left` than go in all
     p.most = (int)(goes <= 0 ? 0 : goes < p.left ? goes : p.left);
     p.tail = (int)((a->recent + a->page_size - 1) / a->page_size + 1);
+    // More candidates than a workgroup has registers for: by parts.  (One workgroup that read them anew for each digit: 124 us for sequences of
+    // 131072 and 100001 tokens in 7 layers; the six launches of the parts 39.  For 256 times 4000 one launch takes 18 us and six would not.)
+    const int64_t candidates = span - a->recent;
+    p.parts = candidates <= 16 * SCAN_THREADS ? 0 : (int)((candidates + PART - 1) / PART);
+    const int at_once = AT_ONCE / (a->num_layers > 0 ? a->num_layers : 1);
+    p.first = 0, p.rows = at_once < 1 ? 1 : at_once < a->n ? at_once : a->n;
     return p;
 }
 
@@ -423,7 +566,8 @@ extern "C" int64_t kda355_evict_tokens_workspace_bytes(const KdaEvictArgs* a) {
     if (const int rc = check_evict(a)) return rc;
     const int64_t lists = (int64_t)a->n * a->num_layers;
     const Plan p = plan_of(a);
-    return 4 * (a->n * (1 + (int64_t)p.tail) + lists * (1 + 2 * (int64_t)p.most));
+    const int64_t parts = p.parts ? a->n + (int64_t)p.rows * a->num_layers * (3 * BINS + 4 * (int64_t)p.parts) : 0;
+    return 4 * (a->n * (1 + (int64_t)p.tail) + lists * (1 + 2 * (int64_t)p.most) + parts);
 }
 
 extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t stream) {
@@ -454,15 +598,26 @@ extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t
     const int64_t fill = 4096 / lists + 1;  // workgroups of a sequence and layer
     const auto some = [](int64_t x, int64_t y) { return (int)(x < y ? x : y); };
     const auto cdiv = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    // the candidates: at most all tokens but the recent ones
-    const int64_t most = span - a->recent;
-    launch_kernel(most <= 4 * SCAN_THREADS ? select_kernel<4> : most <= 16 * SCAN_THREADS ? select_kernel<16> : select_kernel<0>,
-                  dim3(a->n, a->num_layers), dim3(SCAN_THREADS), s, *a, p);
-    if (p.most > FEW)
+    if (p.parts) {
+        const int at_once = p.rows;
+        for (; p.first < a->n; p.first += at_once) {
+            const dim3 grid(p.parts, some(at_once, a->n - p.first), a->num_layers), threads(SCAN_THREADS);
+            launch_kernel(look_kernel, dim3(grid.y, grid.z), threads, s, *a, p);
+            launch_kernel(part_kernel<0>, grid, threads, s, *a, p);
+            launch_kernel(part_kernel<1>, grid, threads, s, *a, p);
+            launch_kernel(part_kernel<2>, grid, threads, s, *a, p);
+            launch_kernel(part_kernel<3>, grid, threads, s, *a, p);
+            launch_kernel(part_kernel<4>, grid, threads, s, *a, p);
+        }
+    } else
+        launch_kernel(span - a->recent <= 4 * SCAN_THREADS ? select_kernel<4> : select_kernel<16>, dim3(a->n, a->num_layers), dim3(SCAN_THREADS), s,
+                      *a, p);
+    if (p.most > (p.parts ? 0 : FEW))
         launch_kernel(move_kernel, dim3(some(cdiv(p.most, PAIRS), fill), a->n, a->num_layers), dim3(MOVE_THREADS), s, *a, p);
     const bool last = !(a->flags & KDA355_EVICT_MORE);
     const int strips = (int)cdiv(pieces, STRIP), parts = some(cdiv(a->recent, PAIRS), fill / 4 + 1);
     p.strips = a->recent == 0 ? 0 : strips > parts ? strips : parts;
+    if (p.parts) p.strips = p.strips > (p.parts + 3) / 4 ? p.strips : (p.parts + 3) / 4;  // (the weights are left to them)
     p.books = last && (int64_t)a->n * a->table_width <= BOOK_ENTRIES && a->pages <= BOOK_PAGES;
     if (p.strips + p.books)
         launch_kernel(shift_kernel, dim3(p.strips + p.books, p.strips ? a->n : 1, p.strips ? a->num_layers : 1), dim3(SCAN_THREADS), s, *a, p);

@@ -164,10 +164,10 @@ def test_weights_refusals():
 class Budget:
     """Sequences on scattered pages with their books; pools and weights whose values name their place."""
 
-    def __init__(self, lens, size, layers=1, seed=0, token=(16,), dtype=torch.int32, spare=3, reserve=0, shared=(), ties=0.3):
+    def __init__(self, lens, size, layers=1, seed=0, token=(16,), dtype=torch.int32, spare=3, reserve=0, shared=(), ties=0.3, span=0):
         rng = random.Random(seed)
         self.size, need = size, [-(-n // size) for n in lens]
-        width = max([1] + need) + reserve + 1
+        width = max(max([1] + need) + reserve + 1, -(-span // size))
         pages = sum(need) + len(lens) * reserve + spare
         perm = list(range(pages))
         rng.shuffle(perm)
@@ -358,6 +358,30 @@ def test_evict_long(n):
         at = lambda j: t[j // 272] * 272 + j % 272  # noqa: E731
         assert torch.equal(pools[0].cpu().view(-1, 4)[at(torch.arange(keep))], flat[at(place)])
         assert d["seq_lens"].tolist()[0] == keep
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_evict_any_in_wide_tables(seed):
+    """Tables with room for more tokens than a workgroup selects from: the sequences are short, or end behind the first 8192 tokens."""
+    rng = random.Random(seed)
+    size = rng.choice([16, 64, 100])
+    lens = [rng.randint(0, rng.choice([700, 1500])) for _ in range(rng.choice([1, 2, 9]))] + [rng.choice([8190, 8200, 9500])]
+    shared = [(n, 0, min(2, lens[n] // size, lens[0] // size)) for n in range(1, len(lens)) if rng.random() < 0.3]
+    x = Budget(lens, size, rng.choice([1, 2]), seed=seed, token=(4,), reserve=rng.choice([0, 2]), shared=shared, span=40000,
+               ties=rng.choice([0.1, 1.0]))
+    if seed % 2:
+        x.mass[0][:, 1:900:5], x.mass[0][0, 2:900:7] = NAN, -INF
+    keep = rng.randint(1, max(lens)) if seed % 4 else max(lens) - 9
+    rows = list(range(len(lens)))
+    rng.shuffle(rows)
+    x.check(rows + rows[:1], keep, rng.randint(0, keep))
+
+
+def test_evict_many_rows_in_wide_tables():
+    """More sequences and layers than one run of the selecting workgroups takes."""
+    lens = [20 + n % 60 for n in range(47)]
+    x = Budget(lens, 16, 24, seed=3, token=(4,), span=20000)
+    assert x.check(list(range(47)), 40, 11) == [min(n, 40) for n in lens]
 
 
 def test_evict_captured():
