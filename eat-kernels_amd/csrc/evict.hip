@@ -9,8 +9,9 @@
 // 2. The pairs' rows: no place of a pair is read by another, so all at once.
 // 3. The recent rows.  Where they move by their own number or more, all at once.  Else in place: their new places are other recent rows' old
 //    ones, so a workgroup takes a strip of columns and walks down, reading a step's rows before it writes any of them (a row moves
-//    down, so what is read later has not been written).  Beside it, for few table entries, the books.
-// 4. For many entries: table rows, lengths and counts, then what nobody holds any more onto the stack.
+//    down, so what is read later has not been written).  Beside them the books: table rows, lengths and counts, and for few of them what
+//    nobody holds any more onto the stack.
+// 4. For many: that.
 // The rows are bound by memory (2 and 3 for 800 MB: 180 us, 4.5 TB/s), the rest by the latency of its steps: 1 takes 13 us for one sequence
 // of 4160 tokens, 18 for 64 in 4 layers, 39 for 131072 and 100001 in 7.
 #include "pages.h"
@@ -27,12 +28,13 @@ constexpr int WAVES = SCAN_THREADS / 64, BINS = 2048, ROW_PAGES = 2048;
 constexpr int PART_KEYS = 8, PART = PART_KEYS * SCAN_THREADS, AT_ONCE = 1024;  // of a thread, of a workgroup; (sequence, layer)s in one run of the parts
 constexpr int BOOK_ENTRIES = 4096, BOOK_PAGES = 16 * 1024;  // up to so many table entries and pages the books take one workgroup
 
+enum { ROWS = 1, ALL };
 struct Plan {
     int left;         // keep - recent
     int most;         // pairs of a sequence and layer
     int tail;         // pages that hold the recent tokens, at most
     int strips;       // workgroups of a sequence and layer in the third kernel
-    int books;        // the books beside it
+    int books;        // the books beside it: none, by a workgroup for each sequence, all by one
     int parts;        // workgroups that select for a sequence and layer, 0: one
     int first, rows;  // with parts: sequences of this run of them
 };
@@ -465,14 +467,13 @@ __device__ __forceinline__ void book(const KdaEvictArgs& a, int i) {
     if (threadIdx.x == 0) a.seq_lens[row] = a.keep;
 }
 
-__global__ void __launch_bounds__(MOVE_THREADS) books_kernel(KdaEvictArgs a) { book(a, blockIdx.x); }
-
 __global__ void __launch_bounds__(SCAN_THREADS) shift_kernel(KdaEvictArgs a, Plan p) {
     __shared__ int sw[WAVES];
     __shared__ char* at[2][PAIRS];
     const int i = blockIdx.y, l = blockIdx.z, tid = threadIdx.x;
-    if ((int)blockIdx.x == p.strips) {  // the books, by one workgroup
-        if (i || l) return;
+    if ((int)blockIdx.x == p.strips) {  // the books
+        if (l || (i && p.books == ALL)) return;
+        if (p.books == ROWS) return book(a, i);
         for (int k = 0; k < a.n; ++k) book(a, k);
         __syncthreads();
         push_freed<true>(a.ref_counts, a.free_pages, a.num_free, a.pages, sw);
@@ -618,11 +619,10 @@ extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t
     const int strips = (int)cdiv(pieces, STRIP), parts = some(cdiv(a->recent, PAIRS), fill / 4 + 1);
     p.strips = a->recent == 0 ? 0 : strips > parts ? strips : parts;
     if (p.parts) p.strips = p.strips > (p.parts + 3) / 4 ? p.strips : (p.parts + 3) / 4;  // (the weights are left to them)
-    p.books = last && (int64_t)a->n * a->table_width <= BOOK_ENTRIES && a->pages <= BOOK_PAGES;
-    if (p.strips + p.books)
-        launch_kernel(shift_kernel, dim3(p.strips + p.books, p.strips ? a->n : 1, p.strips ? a->num_layers : 1), dim3(SCAN_THREADS), s, *a, p);
-    if (last && !p.books) {
-        launch_kernel(books_kernel, dim3(a->n), dim3(MOVE_THREADS), s, *a);
+    p.books = !last ? 0 : (int64_t)a->n * a->table_width <= BOOK_ENTRIES && a->pages <= BOOK_PAGES ? ALL : ROWS;
+    if (p.strips || p.books)
+        launch_kernel(shift_kernel, dim3(p.strips + (p.books != 0), a->n, p.strips ? a->num_layers : 1), dim3(SCAN_THREADS), s, *a, p);
+    if (p.books == ROWS) {
         KdaPagesArgs b = {};
         b.ref_counts = a->ref_counts, b.free_pages = a->free_pages, b.num_free = a->num_free, b.pages = a->pages;
         launch_kernel(free_push_kernel, dim3(1), dim3(SCAN_THREADS), s, b);
