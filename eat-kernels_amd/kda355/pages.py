@@ -265,7 +265,7 @@ def evict_tokens(pools, weights, block_table, seq_lens, ref_counts, free_pages, 
     up as in free_pages; pages reserved ahead of the tokens move down in the table behind the kept ones.
 
     A sequence stays as it is where one of its pages is a hole, or where shared pages and recent tokens are more than `keep`.
-    Rows outside the table are skipped; a row that is given twice is taken once."""
+    Rows outside the table are skipped; a row that is given twice is taken once.  No two layers may have the same memory."""
     pools, weights = _sequence(pools), _sequence(weights)
     keep, recent, page_size = int(keep), int(recent), int(page_size)  # (what is kept is keyed by their values)
     try:
@@ -280,6 +280,8 @@ def evict_tokens(pools, weights, block_table, seq_lens, ref_counts, free_pages, 
     n = rows.numel()
     if n == 0:
         return
+    if len({t.data_ptr() for t in pools}) < len(pools) or len({w.data_ptr() for w in weights}) < len(weights):
+        raise ValueError("kda355: evict_tokens: a pool or its weights are given twice: layers are cut at the same time")
     ws = torch.empty(max(need), dtype=torch.uint8, device=dev)
     books = (rows.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), ref_counts.data_ptr(), free_pages.data_ptr(),
              num_free.data_ptr(), ws.data_ptr())

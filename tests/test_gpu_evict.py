@@ -441,7 +441,7 @@ def test_evict_refusals():
                dict(w=[m[:1] for m in mass]), dict(w=[m.t() for m in mass]), dict(w=[m[:1].expand(2, W) for m in mass]),
                dict(p=[q[:3] for q in pools]), dict(p=[q[:, ::2] for q in pools]), dict(p=[q[..., :3] for q in pools]),
                dict(p=[torch.zeros(len(x.refs), 16, 2, dtype=torch.int32, device=DEV)] * 2), dict(p=[q.view(len(x.refs), -1) for q in pools]),
-               dict(seq_lens=d["seq_lens"][:1]), dict(free_pages=d["free_pages"][:2]), dict(num_free=d["free_pages"]), dict(r=rows[None])):
+               dict(p=pools[:1] * 2), dict(w=mass[:1] * 2), dict(seq_lens=d["seq_lens"][:1]), dict(free_pages=d["free_pages"][:2]), dict(num_free=d["free_pages"]), dict(r=rows[None])):
         with pytest.raises(ValueError):
             call(**kw)
     for kw in (dict(w=[m.half() for m in mass]), dict(w=[m.cpu() for m in mass]), dict(p=[q.cpu() for q in pools]), dict(r=rows.long()),
