@@ -142,6 +142,29 @@ def test_weights_in_wide_tables():
     _check_weights(x, 4)
 
 
+def test_weights_far_offsets():
+    """Pages beyond 2^32 bytes of the cache; on another stream, with the weights of one row far from the next one's."""
+    pages, size = 90000, 128  # 4.6 GB
+    x = Absorbed([700, 90], 2, 20, size, BF)
+    _, _, lse = _check_weights(x, 4)
+    W = x.table.shape[1] * size
+    want = _weights(x, 4, lse, torch.zeros(2, W))
+    cache = torch.empty(pages, size, 400, dtype=torch.uint8, device=DEV)
+    to = [pages - 1 - 3 * i for i in range(x.bytes.shape[0])]
+    assert min(to) * size * 400 > 1 << 32
+    cache[to] = x.bytes
+    table = torch.where(x.table >= 0, torch.tensor(to)[x.table.clamp(min=0).long()].int(), x.table)
+    far = torch.empty((1 << 30) + W + 64, device=DEV)  # row 1 begins 2^32 + 256 bytes behind row 0
+    weights = far.as_strided((2, W), ((1 << 30) + 64, 1)).zero_()
+    args = (x.ql.to(DEV), x.qp.to(DEV), cache, table.to(DEV), _i32(x.lens), lse.to(DEV), weights)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kda355.latent_weights(*args)
+    side.synchronize()
+    assert torch.equal(weights.cpu(), want)
+
+
 def test_weights_refusals():
     x = _narrow(Absorbed([20, 5], 1, 4, 16, BF))
     ql, qp, table, lens = x.ql.to(DEV), x.qp.to(DEV), x.table.to(DEV), _i32(x.lens)
@@ -384,12 +407,38 @@ def test_evict_many_rows_in_wide_tables():
     assert x.check(list(range(47)), 40, 11) == [min(n, 40) for n in lens]
 
 
-def test_evict_captured():
+def test_evict_far_offsets():
+    """Pages beyond 2^32 bytes of the pool, on another stream."""
+    pages, size = 90000, 128  # 4.6 GB
+    x = Budget([700, 300, 129], size, 1, token=(400,), dtype=torch.uint8)
+    for keep, recent in ((260, 30), (128, 100), (600, 500)):
+        pools, mass, d = x.run([0, 1, 2], keep, recent)
+        to = [pages - 1 - 3 * i for i in range(len(x.refs))]
+        assert min(to) * size * 400 > 1 << 32
+        cache = torch.empty(pages, size, 400, dtype=torch.uint8, device=DEV)
+        cache[to] = x.pools[0].to(DEV)
+        table = _i32([[to[g] if g >= 0 else -1 for g in row] for row in x.table])
+        refs = torch.zeros(pages, dtype=torch.int32, device=DEV)
+        refs[to] = _i32(x.refs)
+        free, num, lens = torch.full((pages,), -1, dtype=torch.int32, device=DEV), _i32([0]), _i32(x.lens)
+        w, rows = x.mass[0].to(DEV), _i32([0, 1, 2])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            kda355.evict_tokens([cache], [w], table, lens, refs, free, num, rows, keep, recent, size)
+        side.synchronize()
+        assert torch.equal(cache[to], pools[0]) and torch.equal(w, mass[0]) and torch.equal(lens, d["seq_lens"])
+        assert torch.equal(refs[to], d["ref_counts"]) and int(num) == int(d["num_free"]) - x.num
+        assert table.tolist() == [[to[g] if g >= 0 else -1 for g in row] for row in d["block_table"].tolist()]
+
+
+@pytest.mark.parametrize("span", [0, 20000])
+def test_evict_captured(span):
     """One graph, replayed over other lengths, tables and weights; every replay against the eager call."""
-    xs = [Budget(lens, 16, 2, seed=s, token=(4,), spare=40 - sum(-(-n // 16) for n in lens), reserve=0)
+    xs = [Budget(lens, 16, 2, seed=s, token=(4,), spare=40 - sum(-(-n // 16) for n in lens), reserve=0, span=span)
           for s, lens in enumerate(([100, 40, 7], [3, 200, 60], [150, 2, 133]))]
     width = max(len(x.table[0]) for x in xs)
-    pools, mass, d = Budget([16 * (width - 1)] * 3, 16, 2, token=(4,), spare=40 - 3 * (width - 1)).device()
+    pools, mass, d = Budget([150] * 3, 16, 2, token=(4,), spare=40 - 30, span=16 * width).device()
     rows = _i32([2, 0, 1])
 
     def step():
