@@ -138,11 +138,11 @@ constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
 template <bool Q4, int VW>
 struct Lds {
     // A cache in 16 bits: latent rows and positional parts of four tiles, side by side.  In 4 bits: codes, scales and positional parts of
-    // eight tiles as they came, and of every value wave the scales of its values once more, 8 equal bytes each.  A token's 16-byte piece p of
+    // eight tiles as they came, and of every value wave the scales of its values once more, in 32 bits.  A token's 16-byte piece p of
     // codes stands at p ^ turn4(t), its scales at 256 (t / 8) + 16 (t % 8).  The queries come through the first 64 KiB, which the first
     // three tiles of a segment (slots 5 .. 7) leave free.
     static constexpr int THERES = Q4 ? 8 : 4, PAGE_RING = Q4 ? 8 : 4;
-    static constexpr int SPREAD = LAT / GROUP / VW * 8;  // bytes a token
+    static constexpr int SPREAD = LAT / GROUP / VW * 4;  // bytes a token
     static constexpr int RAW = VW * BN * SPREAD, RAW_SCALES = BN * SCALES4, RAW_PE = RAW_SCALES + 4 * 256, RAW_TILE = RAW_PE + PE_TILE;
     static_assert(RAW + 5 * RAW_TILE >= 2 * LAT_TILE, "");
     static constexpr int P = Q4 ? RAW + 8 * RAW_TILE : 4 * (LAT_TILE + PE_TILE);  // weights: [tile % 2][row tile][16-key step][row][key ^ (row & 8)] 16 bits
@@ -603,14 +603,14 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 lds_barrier();  // the next tile's weights; the tile after it is whole
             }
         };
-        // The same from 4 bits.  A transposed read of bytes gives a lane 8 tokens' codes of values 2 m and 2 m + 1 (m = l % 32 of 64 values), and
-        // another, of the scales written out 8 times, their scales: eight conversions and eight exchanges of halves make one operand of even
-        // values and one of odd ones.  A step multiplies what the step before made and makes the next tile's, so that no read of LDS is waited
-        // for but the weights'.
+        // The same from 4 bits.  A transposed read of bytes gives a lane 8 tokens' codes of values 2 m and 2 m + 1 (m = l % 32 of 64 values):
+        // eight conversions and eight exchanges of halves make one operand of even values and one of odd ones.  The scales the wave writes out
+        // first, as the conversion takes them (64 ragged sequences of 32 heads 62.5 us; 65.3 with 7 shifts for 8 bytes of a transposed read).  A
+        // step multiplies what the step before made and makes the next tile's, so that no read of LDS is waited for but the weights'.
         const int tk = 8 * half + (c16 >> 1), pc = quad & 1;  // of 16 tokens the one whose bytes this lane reads; of two pieces the one
         const uint32_t at_codes = tk * SCALES4 + (((DV * vw + pc) ^ turn4(tk)) << 4) + (c16 & 1) * 8;
         constexpr int NB = DV / 2, G = 2 * NB;  // blocks of 64 values, groups of a tile: [16 tokens][64 values]
-        const uint32_t spread = lds + vw * (BN * L::SPREAD), at_spread = spread + tk * L::SPREAD + pc * 8;
+        const uint32_t spread = lds + vw * (BN * L::SPREAD), at_spread = spread + pc * (BN * 4) + half * 32;  // [32 values][token]
         // lane l spreads the scales of token l / 2: with 4 value waves two of the wave's four, with 8 one of two
         const uint32_t at_scale = L::RAW_SCALES + (lane >> 4) * 256 + (lane >> 1 & 7) * 16 + DV * vw + (lane & 1) * NB;
         u32x4 vf[G][2];  // [group][even, odd]
@@ -625,25 +625,27 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
 #pragma unroll
             for (int g = 0; g < G; ++g) code[g] = lds_read_tr8(((from + at_codes) ^ (g % NB) << 5) + g / NB * (16 * SCALES4));
         };
-        u32x2 scale8[G];
+        u32x4 scales[2][2];  // of 8 tokens, for two groups
         auto spread_scales = [&] {
-            const uint32_t x = __builtin_amdgcn_perm(scale, scale, 0u), y = __builtin_amdgcn_perm(scale, scale, 0x01010101u);
-            if constexpr (NB == 2)
-                lds_write16(spread + lane * 16, u32x4{x, x, y, y});
-            else
-                *(__attribute__((address_space(3))) u32x2*)(lds_byte*)(uintptr_t)(spread + lane * 8) = u32x2{x, x};
+            auto* to = (__attribute__((address_space(3))) uint32_t*)(lds_byte*)(uintptr_t)(spread + (lane & 1) * (NB * BN * 4) + (lane >> 1) * 4);
+            to[0] = scale << 23;
+            if (NB == 2) to[BN] = (scale & 0xff00u) << 15;
+            asm volatile("" ::: "memory");
+        };
+        auto read_scales = [&](int g) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) scale8[g] = lds_read_tr8(at_spread + g % NB * 16 + g / NB * (16 * L::SPREAD));
+            for (int i = 0; i < 2; ++i) scales[g & 1][i] = lds_read16(at_spread + g % NB * (2 * BN * 4) + g / NB * 64 + i * 16);
         };
         auto widen = [&](int g, bool mixed) {
             uint32_t x[8];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {  // (the exponent in place: the conversion looks at nothing else of the scale)
-                const uint32_t s4 = scale8[g][i], c4 = code[g][i];
-                x[4 * i] = T::template pair4<0>(c4, __uint_as_float(s4 << 23));
-                x[4 * i + 1] = T::template pair4<1>(c4, __uint_as_float(s4 << 15));
-                x[4 * i + 2] = T::template pair4<2>(c4, __uint_as_float(s4 << 7));
-                x[4 * i + 3] = T::template pair4<3>(c4, __uint_as_float(s4 >> 1));
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t c4 = code[g][i];
+                const u32x4 s4 = scales[g & 1][i];
+                x[4 * i] = T::template pair4<0>(c4, __uint_as_float(s4[0]));
+                x[4 * i + 1] = T::template pair4<1>(c4, __uint_as_float(s4[1]));
+                x[4 * i + 2] = T::template pair4<2>(c4, __uint_as_float(s4[2]));
+                x[4 * i + 3] = T::template pair4<3>(c4, __uint_as_float(s4[3]));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -701,6 +703,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                     for (int r = 0; r < RT; ++r) acc[r][2 * (g % NB) + i] = T::mfma(vf[g][i], pf[g / NB][r], acc[r][2 * (g % NB) + i]);
                 if constexpr (!LAST) {
                     if (g == 0) spread_scales();
+                    read_scales(g);
                     if constexpr (EVEN) {
                         if (g == 0) at = find_rows(tile + AHEAD4, page);
                         if (g == 1) bring_even(tile + AHEAD4, at, 0);
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
 #pragma unroll
                 for (int i = 3; i < 7; ++i) whole_tile(t0 + i);
 #pragma unroll
-                for (int g = 0; g < G; ++g) widen(g, is_mixed(t0));
+                for (int g = 0; g < G; ++g) read_scales(g), widen(g, is_mixed(t0));
                 wait_loads<4 * L::LOADS>();
             } else {
                 load_pages(t0 + 4);
