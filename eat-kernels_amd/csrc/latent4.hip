@@ -1,4 +1,5 @@
-// Token rows of the latent cache in 4 bits: into pages and back (gfx950).  Both move bytes: bound by HBM, small calls by a launch.
+// Token rows of the latent cache in 4 bits: into pages and back (gfx950).  Both move bytes: bound by HBM (65769 rows read and widened
+// 19 us, 5.3 TB/s, of which the caches take a part; 6614 written 5.6), small calls by a launch (3.5 and 4.6).
 //
 // A row's 16-bit form is 72 pieces of 16 bytes, a lane each: four lanes hold the 32 values of a scale, find the largest among
 // them through DPP and write a dword of codes each.  The scale is a power of two, so that scaling is exact and the conversion is one

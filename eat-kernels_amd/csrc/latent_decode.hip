@@ -23,6 +23,14 @@
 // without a pause; the first 20 after one take 291 and 197, with the clock that the card then allows).  With a row tile or two a
 // sequence HBM: 64 ragged sequences, 64 heads, 126 to 135 us, 4.3 TB/s.  One sequence of 4097 tokens, 12 heads: 13.9 us from a graph,
 // 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5 the join.
+// A cache in 4 bits (Q4) stays in 4 bits in LDS (13 KiB a tile, eight tiles, brought seven ahead); both kinds of waves widen what they
+// multiply, in registers: a score wave its 16 keys between its products, a value wave the next tile's values while it multiplies this
+// one's.  Bound by the step: a wave has some 110 instructions for that in it beside its products, and the SIMD's two (three) waves' vector
+// instructions (46 %) and products (40 %) rarely run side by side.  The same three shapes: drafts 231 to 243 us, 64 sequences of 64 heads
+// behind 32768 tokens 359 to 367 (315 to 321 over 16 bits), and 64 ragged sequences of 32 heads 56 against 102 over 16 bits, 3.3 TB/s.
+// Forms before it: 16-bit tiles made in LDS by waves of their own 78 / 284 / 447 us, made by the value waves 69 / 261 / 396.  Two tiles a
+// step with one row tile: 62 against 64, and 12.0 against 10.3 for one sequence of 4097 tokens; the next tile's codes read a step earlier:
+// 256 against 244 for the drafts (registers spilled).
 // Other forms, each against this one as it stood then (64 ragged, drafts, shared prefix): eight waves of one kind with the value
 // dimensions split 141 / 296 / 234 us against 142 / 260 / 227; four of one kind, one a SIMD, pipelined 142 / 276 / 264.
 #include <type_traits>
@@ -33,7 +41,8 @@ namespace kda355 {
 namespace {
 
 constexpr int SCORE_WAVES = 4;
-// Value waves: 4, and 8 from 4 bits with one row tile, where a wave's conversions, one after the other, are the longest way through a step.
+// Value waves: 4, and 8 from 4 bits with one row tile, where a wave's conversions, one after the other, are the longest way through a step
+// (64 ragged sequences of 32 heads: 4 waves 70 us, 8 waves 64).
 template <int RT, bool Q4>
 constexpr int VALUE_WAVES = Q4 && RT == 1 ? 8 : 4;
 template <int RT, bool Q4>

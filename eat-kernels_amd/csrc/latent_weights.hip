@@ -7,6 +7,13 @@
 // and a lane adds up its row of every tile for its 4 + 4 keys.  One sum across the 16 lanes of a key at the end; no two workgroups
 // write the same token, so the order of a sum depends on the sizes alone.  Two workgroups a CU, each with an equal run of units of 128
 // keys through the sequences; up to 64 query rows stay in LDS from one unit of a sequence to the next, more come three tiles ahead.
+//
+// Bound: with many rows the products (matrix cores busy 40 %, LDS 21 % over the launch) and what does not run beside them.  16 sequences of
+// 6000 to 9900 tokens, 8 x 96 rows: 127 us steady, 0.88 PFLOP/s; timed without bringing the query rows 102, with rows that stay in L1 115,
+// without the exponentials 117, without either 92; some 15 go by before the first keys are there.  Eight waves a workgroup, which halves
+// the rows' way from L2, and a barrier for two tiles: 123, but 62 against 48 with few rows; with a barrier a tile 136.  The loads of rows
+// spread between the products: 134.  With few rows memory: 64 ragged sequences of 64 heads in 4 bits 48 us, 4.0 TB/s.  One sequence of 4097
+// tokens, 12 heads: 7.6 us, lengths, keys and queries one after the other.
 #include "latent.h"
 
 namespace kda355 {
