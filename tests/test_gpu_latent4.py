@@ -393,6 +393,49 @@ def test_captured_steps():
         assert torch.allclose(weights, got[3] + (got[3] - 0.5), rtol=1e-5, atol=1e-6)
 
 
+def test_pages_in_4_bits_forked_freed_and_compacted():
+    """The page bookkeeping takes a cache in 4 bits like any pool: a fork reads as its parent, and nothing changes for those that stay."""
+    size, H = 16, 10
+    x = _narrow(Absorbed([90, 33, 70, 0], 1, H, size, HF))
+    used = x.bytes.shape[0]
+    pages = used + 9
+    cache = torch.zeros(pages, size, 400, dtype=torch.uint8, device=DEV)
+    cache[:used] = x.bytes
+    need = [-(-n // size) for n in x.lens]
+    table = [[int(p) for p in x.table[n][:need[n]]] for n in range(4)]
+    held = sorted(p for row in table for p in row)
+    left = [p for p in range(pages) if p not in held]
+    width = max(need) + 1
+    table = _i32([row + [-1] * (width - len(row)) for row in table])
+    lens, num = _i32(x.lens), _i32([len(left)])
+    refs, free = _i32([int(p in held) for p in range(pages)]), _i32(left + [-1] * (pages - len(left)))
+    ql, qp = x.ql.to(DEV), x.qp.to(DEV)
+
+    def step(what):
+        """The rows of every sequence; the step over them within the tolerances.  (How a sequence is cut depends on those beside it.)"""
+        n = lens.tolist()
+        cu = [sum(n[:i]) for i in range(5)]
+        rows = torch.zeros(cu[4], ROW, dtype=HF, device=DEV)
+        kda355.latent_gather(cache, table, _i32(cu), rows)
+        out = kda355.latent_decode(ql, qp, cache, table, lens).cpu()
+        rows = [rows[cu[i]:cu[i + 1]].cpu() for i in range(4)]
+        for i in range(4):
+            q, k = torch.cat([ql[i], qp[i]], dim=-1).cpu().double(), rows[i].double()
+            R.check(out[i], None, R.attend(q, k, k[:, :LAT], torch.ones(H, n[i], dtype=torch.bool), R.SCALE), HF, ROW, f"{what} seq {i}")
+        return rows
+
+    before = step("before")
+    kda355.fork_pages([cache], table, lens, refs, free, num, _i32([0]), _i32([3]), size)
+    assert lens.tolist() == [90, 33, 70, 90]
+    after = step("forked")
+    assert all(torch.equal(a, b) for a, b in zip(after, before[:3] + before[:1]))
+    kda355.free_pages(table, lens, refs, free, num, _i32([0, 1]), size)
+    kda355.compact_pages([cache], table, refs, free, num)
+    assert lens.tolist() == [0, 0, 70, 90] and int(table.max()) == need[0] + need[2] - 1
+    last = step("compacted")
+    assert torch.equal(last[2], before[2]) and torch.equal(last[3], before[0])
+
+
 def test_refusals():
     x = _narrow(Absorbed([20, 5], 1, 4, 16, BF))
     ql, qp, table, lens = x.ql.to(DEV), x.qp.to(DEV), x.table.to(DEV), _i32(x.lens)
