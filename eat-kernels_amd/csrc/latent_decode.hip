@@ -670,8 +670,17 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         };
         auto is_mixed = [&](uint32_t tile) { return (int)(tile * BN + BN) > first; };  // some row does not see some token of the tile
         constexpr uint32_t AHEAD4 = 7;
-        auto step4 = [&](uint32_t tile, auto last_) {
-            constexpr bool LAST = decltype(last_)::value;
+        // the loads of all tiles up to `tile` have arrived, if those of tiles up to `issued` were the last
+        auto wait_tile = [&](uint32_t tile, uint32_t issued) {
+            const uint32_t left = tile < issued ? issued - tile : 0;
+            if (left == 0) wait_loads<0>();
+            else if (left == 1) wait_loads<L::LOADS>();
+            else if (left == 2) wait_loads<2 * L::LOADS>();
+            else if (left == 3) wait_loads<3 * L::LOADS>();
+            else wait_loads<4 * L::LOADS>();
+        };
+        auto step4 = [&](uint32_t tile, auto kind) {  // 0: with loads, 1: none are left, 2: the last one
+            constexpr bool LAST = decltype(kind)::value == 2, BRINGS = decltype(kind)::value == 0;
             const uint32_t pb = lds + L::P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
@@ -682,7 +691,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 for (int r = 0; r < RT; ++r) pf[k][r] = weight(k, r);
             int page = 0;
             if constexpr (!LAST) {
-                page = find_page(tile + AHEAD4);
+                if constexpr (BRINGS) page = find_page(tile + AHEAD4);
                 read_codes(tile + 1);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -713,25 +722,25 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 if constexpr (!LAST) {
                     if (g == 0) spread_scales();
                     read_scales(g);
-                    if constexpr (EVEN) {
+                    if constexpr (BRINGS && EVEN) {
                         if (g == 0) at = find_rows(tile + AHEAD4, page);
                         if (g == 1) bring_even(tile + AHEAD4, at, 0);
                         if (g == G / 2) bring_even(tile + AHEAD4, at, 1), bring_even(tile + AHEAD4, at, 2);
                         if (g == G - 1) bring_even(tile + AHEAD4, at, 3);
-                    } else {
+                    } else if constexpr (BRINGS) {
                         if (g == 0) at = find_token(tile + AHEAD4, page), find_latent(at, 0), find_latent(at, 1);
                         if (g == 1) bring(tile + AHEAD4, Int<0>{}), find_scales(at), find_pe(at);
                         if (g == G / 2) bring(tile + AHEAD4, Int<1>{});
                         if (g == G - 1) bring(tile + AHEAD4, Int<2>{}), bring(tile + AHEAD4, Int<8>{});
                     }
-                    if (g == G - 1) load_pages(tile + AHEAD4 + 8);
+                    if (BRINGS && g == G - 1) load_pages(tile + AHEAD4 + 8);
                     if (g > 0) widen(g - 1, mixed);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!LAST) {
                 widen(G - 1, mixed);
-                wait_loads<4 * L::LOADS>();
+                if constexpr (BRINGS) wait_loads<4 * L::LOADS>(); else wait_tile(tile + 3, stop - 1);
                 lds_barrier();  // the next tile's weights; the two tiles after it are whole
             }
         };
@@ -760,23 +769,38 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 find_tile(tile);
                 bring_tile(tile);
             };
-            whole_tile(t0);
-            whole_tile(t0 + 1);
             if constexpr (Q4) {
-                whole_tile(t0 + 2);
-                wait_loads<2 * L::LOADS>();
+                // Tiles past the end are not brought (64 ragged sequences of 32 heads 60.6 us, 62.6 with them; one sequence 14.6, 15.2), but with
+                // two row tiles and one address for 8 tokens, where steps without loads cost more than these do (drafts 252 us, 246 with them).
+                constexpr bool ENDS = RT == 1 || !EVEN;
+                const uint32_t end = ENDS ? stop - 1 : ~0u;
+                auto some_tile = [&](uint32_t tile) {
+                    if (tile <= end) whole_tile(tile);
+                };
+                whole_tile(t0);
+                some_tile(t0 + 1);
+                some_tile(t0 + 2);
+                wait_tile(t0, min(t0 + 2, end));
                 lds_barrier();  // the first tile, the queries
-                wait_loads<L::LOADS>();
-                lds_barrier();  // the queries are in registers; the second tile is whole
-                // while the first tile's scores are computed: its values, and what comes after the third tile
+                wait_tile(t0 + 1, min(t0 + 2, end));
+                lds_barrier();  // the queries are in registers; the second tile
+                // while the first tile's scores are computed: its values, and tiles t0 + 3 and on
                 read_codes(t0);
                 spread_scales();
-#pragma unroll
-                for (int i = 3; i < 7; ++i) whole_tile(t0 + i);
+#pragma unroll 1
+                for (uint32_t i = 3; i < AHEAD4; ++i) some_tile(t0 + i);
 #pragma unroll
                 for (int g = 0; g < G; ++g) read_scales(g), widen(g, is_mixed(t0));
-                wait_loads<4 * L::LOADS>();
+                wait_tile(t0 + 2, min(t0 + AHEAD4 - 1, end));
+                lds_barrier();  // the first tile's weights; the second tile is whole
+                uint32_t tile = t0;
+                for (; tile + (ENDS ? AHEAD4 : 1) < stop; ++tile) step4(tile, Int<0>{});
+                if constexpr (ENDS)
+                    for (; tile < end; ++tile) step4(tile, Int<1>{});
+                step4(tile, Int<2>{});
             } else {
+                whole_tile(t0);
+                whole_tile(t0 + 1);
                 load_pages(t0 + 4);
                 wait_loads<L::LOADS>();
                 lds_barrier();  // the first tile, the queries
@@ -786,13 +810,10 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 find_tile(t0 + 3);
                 load_pages(t0 + 5);
                 wait_loads<L::LOADS>();
+                lds_barrier();  // the first tile's weights; the second tile is whole
+                for (uint32_t tile = t0; tile + 1 < stop; ++tile) step(tile, std::false_type{});
+                step(stop - 1, std::true_type{});
             }
-            lds_barrier();  // the first tile's weights; the second tile is whole
-            auto any_step = [&](uint32_t tile, auto last_) {
-                if constexpr (Q4) step4(tile, last_); else step(tile, last_);
-            };
-            for (uint32_t tile = t0; tile + 1 < stop; ++tile) any_step(tile, std::false_type{});
-            any_step(stop - 1, std::true_type{});
             wait_loads<0>();  // what was brought past the end
         } else {
             lds_barrier();
