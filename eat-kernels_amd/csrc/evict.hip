@@ -26,7 +26,7 @@ constexpr int STRIP = 8, SHIFT_ROWS = 4;         // 16-byte pieces of a strip, r
 constexpr int FEW = 128;                         // pairs that the first kernel moves itself
 constexpr int WAVES = SCAN_THREADS / 64, BINS = 2048, ROW_PAGES = 2048;
 constexpr int PART_KEYS = 8, PART = PART_KEYS * SCAN_THREADS, AT_ONCE = 1024;  // of a thread, of a workgroup; (sequence, layer)s in one run of the parts
-constexpr int BOOK_ENTRIES = 4096, BOOK_PAGES = 16 * 1024;  // up to so many table entries and pages the books take one workgroup
+constexpr int BOOK_ROWS = 64, BOOK_ENTRIES = 4096, BOOK_PAGES = 16 * 1024;  // up to so many rows, table entries and pages the books take one workgroup
 
 enum { ROWS = 1, ALL };
 struct Plan {
@@ -446,25 +446,30 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(KdaEvictArgs a, Plan
     }
 }
 
-// A row's first pages stay, the rest of its tokens' pages go, entries past the tokens follow the first ones.
-__device__ __forceinline__ void book(const KdaEvictArgs& a, int i) {
-    const int len = lens_of(a)[i];
-    if (len < 0) return;
-    const int row = a.src[i];
-    const int used = (len + a.page_size - 1) / a.page_size, kept = (a.keep + a.page_size - 1) / a.page_size;
-    int32_t* table = a.block_table + row * a.table_stride;
-    for (int j = kept + threadIdx.x; j < used; j += blockDim.x) atomicCAS(a.ref_counts + table[j], 1, FREED);  // (none is held twice)
-    __syncthreads();
-    const int by = used - kept;
-    if (by > 0)
-        for (int j0 = kept; j0 < a.table_width; j0 += blockDim.x) {
-            const int j = j0 + threadIdx.x;
-            const int32_t next = j + by < a.table_width ? table[j + by] : -1;
+// A row's first pages stay, the rest of its tokens' pages go, entries past the tokens follow the first ones.  Of `count` rows from slot
+// `first` on by one workgroup, up to 16 at a time.  (24 rows of 2200 tokens in 7
+// layers, the launch with the recent rows: one after the other 18 us, so 9.)
+__device__ __forceinline__ void books(const KdaEvictArgs& a, int first, int count) {
+    int side = 1;  // rows at a time
+    while (side < 16 && side < count) side *= 2;
+    const int per = SCAN_THREADS / side, lane = threadIdx.x % per, kept = (a.keep + a.page_size - 1) / a.page_size;
+    for (int k = 0; k < count; k += side) {
+        const int i = first + min(k + (int)threadIdx.x / per, count - 1);
+        const int len = k + (int)threadIdx.x / per < count ? lens_of(a)[i] : -1, row = len < 0 ? 0 : a.src[i];
+        const int used = (len + a.page_size - 1) / a.page_size, by = len < 0 ? 0 : used - kept;
+        int32_t* table = a.block_table + row * a.table_stride;
+        for (int j = kept + lane; j < kept + by; j += per) atomicCAS(a.ref_counts + table[j], 1, FREED);  // (none is held twice)
+        __syncthreads();
+        for (int j0 = kept; j0 < a.table_width; j0 += per) {
+            const int j = j0 + lane;
+            const bool moves = by > 0 && j < a.table_width;
+            const int32_t next = moves && j + by < a.table_width ? table[j + by] : -1;
             __syncthreads();
-            if (j < a.table_width) table[j] = next;
+            if (moves) table[j] = next;
             __syncthreads();
         }
-    if (threadIdx.x == 0) a.seq_lens[row] = a.keep;
+        if (lane == 0 && len >= 0) a.seq_lens[row] = a.keep;
+    }
 }
 
 __global__ void __launch_bounds__(SCAN_THREADS) shift_kernel(KdaEvictArgs a, Plan p) {
@@ -473,8 +478,8 @@ __global__ void __launch_bounds__(SCAN_THREADS) shift_kernel(KdaEvictArgs a, Pla
     const int i = blockIdx.y, l = blockIdx.z, tid = threadIdx.x;
     if ((int)blockIdx.x == p.strips) {  // the books
         if (l || (i && p.books == ALL)) return;
-        if (p.books == ROWS) return book(a, i);
-        for (int k = 0; k < a.n; ++k) book(a, k);
+        if (p.books == ROWS) return books(a, i, 1);
+        books(a, 0, a.n);
         __syncthreads();
         push_freed<true>(a.ref_counts, a.free_pages, a.num_free, a.pages, sw);
         return;
@@ -619,7 +624,7 @@ extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t
     const int strips = (int)cdiv(pieces, STRIP), parts = some(cdiv(a->recent, PAIRS), fill / 4 + 1);
     p.strips = a->recent == 0 ? 0 : strips > parts ? strips : parts;
     if (p.parts) p.strips = p.strips > (p.parts + 3) / 4 ? p.strips : (p.parts + 3) / 4;  // (the weights are left to them)
-    p.books = !last ? 0 : (int64_t)a->n * a->table_width <= BOOK_ENTRIES && a->pages <= BOOK_PAGES ? ALL : ROWS;
+    p.books = !last ? 0 : a->n <= BOOK_ROWS && (int64_t)a->n * a->table_width <= BOOK_ENTRIES && a->pages <= BOOK_PAGES ? ALL : ROWS;
     if (p.strips || p.books)
         launch_kernel(shift_kernel, dim3(p.strips + (p.books != 0), a->n, p.strips ? a->num_layers : 1), dim3(SCAN_THREADS), s, *a, p);
     if (p.books == ROWS) {
