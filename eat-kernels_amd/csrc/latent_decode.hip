@@ -143,6 +143,8 @@ __device__ __forceinline__ int turn(int t) { return (t & 3) << 2 | (t >> 3 & 1) 
 // From 4 bits 16-byte reads of 16 tokens' same piece (and, by the other lanes, its neighbour p ^ 1) and transposed reads of 8 tokens'
 // pieces p and p ^ 1 both touch all 16 places.
 __device__ __forceinline__ int turn4(int t) { return ((t & 7) ^ (t & 8) >> 1) << 1 | (t >> 3 & 1); }
+// The queries' turn for that order: a lane quarter reads pieces 4 quad .. of 16 rows.
+__device__ __forceinline__ int turn_q4(int t) { return (t & 3) << 2 | (t >> 2 & 3); }
 constexpr int BLOCK = 1024, LAT_TILE = BN * LAT_BYTES, PE_TILE = BN * PE_BYTES;
 template <bool Q4, int VW>
 struct Lds {
@@ -212,9 +214,9 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         }
     }
 
-    uint32_t t0 = 0;  // the segment's first tile
+    uint32_t t0 = 0, t0_ = 0;  // the segment's first tile; the same, unknown to the compiler: addresses of the first tiles would be kept and spilled
     auto lat_at = [&](uint32_t tile) { return lds + tile % 4 * (LAT_TILE + PE_TILE); };            // a tile's latent rows
-    auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile - t0 + 5) % 8 * L::RAW_TILE; };  // what came of it in 4 bits
+    auto raw_at = [&](uint32_t tile) { return lds + L::RAW + (tile - t0_ + 5) % 8 * L::RAW_TILE; };  // what came of it in 4 bits
     auto pe_at = [&](uint32_t tile) { return Q4 ? raw_at(tile) + L::RAW_PE : lat_at(tile) + LAT_TILE; };  // its positional parts
 
     uint32_t own = 0;
@@ -268,6 +270,8 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         const uint32_t stop = max(t0, min(t1, last > 0 ? ((uint32_t)last + BN - 1) / BN : 0u));
 
         const uint32_t n_tiles = stop - t0;
+        t0_ = __builtin_amdgcn_readfirstlane(t0);
+        asm volatile("" : "+s"(t0_));
         // A tile's weights are relative to a past maximum of their rows, which is raised only when some row of a wave exceeds it
         // by SLACK (the result is the same for any reference): after the fact, at the start of the next step.
         auto flags = [&](uint32_t tile) { return *reinterpret_cast<const u32x4*>(sm + L::FLAG + (tile & 1) * 16); };
@@ -312,7 +316,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
 #pragma unroll
                     for (int i = 0; i < 2 * RT; ++i) {
                         const int t = at0 + 4 * i + (me >> 4);
-                        const uint64_t from = of_lane(latent, t) + (((me & 15) ^ turn(t)) << 4);
+                        const uint64_t from = of_lane(latent, t) + (((me & 15) ^ (Q4 ? turn_q4(t) : turn(t))) << 4);
                         const uint32_t to = block + i * (4 * BLOCK);
                         load_block<0>(to, from);
                         load_block<256>(to + BLOCK, from);
@@ -329,19 +333,23 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
             wait_loads<0>();
             lds_barrier();  // the first tile, the queries
             u32x4 q[RT][18] = {};
-            if (some)
+            if (some) {
+                int me = lane;
+                asm volatile("" : "+v"(me));
+                const int c16 = me & 15, quad = me >> 4;
 #pragma unroll
                 for (int x = 0; x < RT; ++x) {
                     // Step i of the scores takes values 32 i + 8 quad .., from 4 bits, where a lane reads all 32 of a scale, 128 (i / 4) +
                     // 32 quad + 8 (i % 4) .. (the order of the contraction is free).
                     const int row = 16 * half_of(x) + c16;
-                    const uint32_t at4 = qb + (row >> 2) * (4 * BLOCK) + (row & 3) * 256 + ((quad << 2 ^ turn(row)) << 4);
-                    const uint32_t at = qb + ra[0] + (half_of(x) - kh) * (16 * LAT_BYTES), pat = qpe + ra[1] + (half_of(x) - kh) * (16 * PE_BYTES);
+                    const uint32_t at4 = qb + (row >> 2) * (4 * BLOCK) + (row & 3) * 256 + ((quad << 2 ^ turn_q4(row)) << 4);
+                    const uint32_t at = qb + (row >> 2) * (4 * BLOCK) + (row & 3) * 256 + ((quad ^ turn(row)) << 4), pat = qpe + row * PE_BYTES + ((quad ^ swz8(row)) << 4);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) q[x][i] = lds_read16((Q4 ? at4 ^ ((i & 3) << 4) : at ^ ((i & 3) << 6)) + (i >> 2) * BLOCK);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) q[x][16 + i] = lds_read16(pat ^ (i << 6));
                 }
+            }
             lds_barrier();  // the queries are in registers
             float mo[RT], l[RT] = {}, sum[RT] = {};
 #pragma unroll
@@ -913,7 +921,10 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 if (r0 + 32 * r + c >= r1) break;
-                char* o = out + r * SLOT_TILE + vw * 16384 + lane * 16;
+                int my = lane;  // (addresses found here: kept from before the loops they would be spilled, and their reload waits for all stores)
+                asm volatile("" : "+v"(my));
+                const int c = my & 31, half = my >> 5;
+                char* o = out + r * SLOT_TILE + vw * 16384 + my * 16;
                 if constexpr (Q4) {  // as the other form leaves them: a lane's 8 values in a row are two lanes' four
 #pragma unroll
                     for (int b = 0; b < DV / 2; ++b)
