@@ -25,7 +25,8 @@ __device__ const uint4 zero_row[ROW_BYTES / 16] = {};  // what a token that is n
 __device__ __forceinline__ int tokens_of(int len, int width, int page_size) { return min(max(len, 0), width * page_size); }
 
 __device__ __forceinline__ uint64_t of_lane(uint64_t x, int l) {
-    return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), l) << 32 | (uint32_t)__shfl((int)(uint32_t)x, l);
+    return (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * l, (int)(uint32_t)(x >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_ds_bpermute(4 * l, (int)(uint32_t)x);
 }
 
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }

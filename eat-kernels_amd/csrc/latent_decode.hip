@@ -185,7 +185,6 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
     __shared__ __align__(1024) unsigned char sm[L::BYTES];
     const uint32_t lds = lds_offset(sm);
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int c = lane & 31, half = lane >> 5;
 
     asm volatile("" ::"s"(a.q_latent), "s"(a.ql_row), "s"(a.page_stride), "s"(a.B), "s"(p.grid));  // all arguments at once
     const Lengths lens(a);
@@ -197,22 +196,12 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
     const int rw = w & 1, kh = w >> 1 & 1;  // a score wave's rows 16 RT rw .. (16 RT of them) and keys 16 kh ..
     const int vw = w & (VW - 1);            // a value wave's DIMS values (waves SCORE_WAVES .. : in any order)
     const int tw = VW == 8 ? vw >> 1 : vw;  // it brings of tokens 8 tw .. + 7
-    const int c16 = lane & 15, quad = lane >> 4;
-    // LDS read addresses within a tile.  Of a score wave: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step, latent and
-    // positional; of a value wave: values as operand rows (key 8 half + e of a 16-key step is element e), e < 4 and from 4 on.
-    uint32_t ra[2];
-    if (scores) {
-        const int t = 16 * kh + c16;
-        ra[0] = Q4 ? t * SCALES4 + ((quad ^ turn4(c16)) << 4) : (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + ((quad ^ turn(t)) << 4);
-        ra[1] = t * PE_BYTES + ((quad ^ swz8(t)) << 4);
-    } else {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int t = 8 * half + 4 * x + (c16 >> 2);
-            const int e = 2 * (quad & 1) + ((c16 & 3) >> 1);
-            ra[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
-        }
-    }
+    // What follows from the lane, from 4 bits anew in every segment: kept, what the waves of one kind read would take the other kind's registers.
+    auto my_lane = [&] {
+        int l = lane;
+        if constexpr (Q4) asm volatile("" : "+v"(l));
+        return l;
+    };
 
     uint32_t t0 = 0, t0_ = 0;  // the segment's first tile; the same, unknown to the compiler: addresses of the first tiles would be kept and spilled
     auto lat_at = [&](uint32_t tile) { return lds + tile % 4 * (LAT_TILE + PE_TILE); };            // a tile's latent rows
@@ -286,6 +275,12 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         };
         if (scores) {
             // ================================================================ score waves
+            const int my = my_lane(), c16 = my & 15, quad = my >> 4, c = my & 31;
+            // LDS read addresses within a tile: key 16 kh + c16, dimensions 8 quad .. of a 32-dimension step, latent and positional
+            const int key_at = 16 * kh + c16;
+            const uint32_t ra[2] = {(uint32_t)(Q4 ? key_at * SCALES4 + ((quad ^ turn4(c16)) << 4)
+                                                  : (key_at >> 2) * (4 * BLOCK) + (key_at & 3) * 256 + ((quad ^ turn(key_at)) << 4)),
+                                    (uint32_t)(key_at * PE_BYTES + ((quad ^ swz8(key_at)) << 4))};
             const int row0 = r0 + 16 * RT * rw + c16;  // this lane's rows: row0, and with two row tiles row0 + 16
             // The queries come through the LDS of tiles t0 + 2 and t0 + 3 (from 4 bits: the first 64 KiB and the weights'), a row tile in each, laid out like keys, half of a wave's
             // rows by it and half by the other wave that has them (rows past the end repeat the last one).  (Straight into registers,
@@ -471,6 +466,15 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         }
 
         // ==================================================================== value waves
+        const int my = my_lane(), c16 = my & 15, quad = my >> 4, c = my & 31, half = my >> 5;
+        // LDS read addresses within a tile: values as operand rows (key 8 half + e of a 16-key step is element e), e < 4 and from 4 on
+        uint32_t ra[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int t = 8 * half + 4 * x + (c16 >> 2);
+            const int e = 2 * (quad & 1) + ((c16 & 3) >> 1);
+            ra[x] = (t >> 2) * (4 * BLOCK) + (t & 3) * 256 + vw * BLOCK + ((e ^ turn(t)) << 4) + (c16 & 1) * 8;
+        }
         // ---- loads
         const uint32_t pages = (uint32_t)min(a.pages, (int64_t)1 << 31);
         const u32x4 table_rsrc = tile_rsrc(table, (uint32_t)width * 4);  // entries past the table read as zeros (and are past `last`)
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         // steps that can be spread: the page, the address of the lane's token, the addresses for the lane's pieces
         uint64_t at_latent[2], at_pe, at_scales;
         auto find_page = [&](uint32_t tile) {
-            return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + tile % L::PAGE_RING * 256 + (EVEN ? 0 : lane * 4));
+            return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + tile % L::PAGE_RING * 256 + (EVEN ? 0 : my * 4));
         };
         // EVEN: the wave's 8 tokens stand in one page in a row, so one address and fixed offsets lead to all of them.  (Tokens past the
         // last are read as they are: no row sees them.)
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         constexpr int NB = DV / 2, G = 2 * NB;  // blocks of 64 values, groups of a tile: [16 tokens][64 values]
         const uint32_t spread = lds + vw * (BN * L::SPREAD), at_spread = spread + pc * (BN * 4) + half * 32;  // [32 values][token]
         // lane l spreads the scales of token l / 2: with 4 value waves two of the wave's four, with 8 one of two
-        const uint32_t at_scale = L::RAW_SCALES + (lane >> 4) * 256 + (lane >> 1 & 7) * 16 + DV * vw + (lane & 1) * NB;
+        const uint32_t at_scale = L::RAW_SCALES + (my >> 4) * 256 + (my >> 1 & 7) * 16 + DV * vw + (my & 1) * NB;
         u32x4 vf[G][2];  // [group][even, odd]
         uint32_t scale;
         u32x2 code[G];
@@ -644,7 +648,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         };
         u32x4 scales[2][2];  // of 8 tokens, for two groups
         auto spread_scales = [&] {
-            auto* to = (__attribute__((address_space(3))) uint32_t*)(lds_byte*)(uintptr_t)(spread + (lane & 1) * (NB * BN * 4) + (lane >> 1) * 4);
+            auto* to = (__attribute__((address_space(3))) uint32_t*)(lds_byte*)(uintptr_t)(spread + (my & 1) * (NB * BN * 4) + (my >> 1) * 4);
             to[0] = scale << 23;
             if (NB == 2) to[BN] = (scale & 0xff00u) << 15;
             asm volatile("" ::: "memory");
@@ -778,10 +782,8 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 bring_tile(tile);
             };
             if constexpr (Q4) {
-                // Tiles past the end are not brought (64 ragged sequences of 32 heads 60.6 us, 62.6 with them; one sequence 14.6, 15.2), but with
-                // two row tiles and one address for 8 tokens, where steps without loads cost more than these do (drafts 252 us, 246 with them).
-                constexpr bool ENDS = RT == 1 || !EVEN;
-                const uint32_t end = ENDS ? stop - 1 : ~0u;
+                // Tiles past the end are not brought (64 ragged sequences of 32 heads 60.6 us, 62.6 with them; one sequence 14.6, 15.2).
+                const uint32_t end = stop - 1;
                 auto some_tile = [&](uint32_t tile) {
                     if (tile <= end) whole_tile(tile);
                 };
@@ -802,9 +804,8 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 wait_tile(t0 + 2, min(t0 + AHEAD4 - 1, end));
                 lds_barrier();  // the first tile's weights; the second tile is whole
                 uint32_t tile = t0;
-                for (; tile + (ENDS ? AHEAD4 : 1) < stop; ++tile) step4(tile, Int<0>{});
-                if constexpr (ENDS)
-                    for (; tile < end; ++tile) step4(tile, Int<1>{});
+                for (; tile + AHEAD4 < stop; ++tile) step4(tile, Int<0>{});
+                for (; tile < end; ++tile) step4(tile, Int<1>{});
                 step4(tile, Int<2>{});
             } else {
                 whole_tile(t0);
