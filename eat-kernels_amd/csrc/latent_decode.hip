@@ -25,12 +25,13 @@
 // 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5 the join.
 // A cache in 4 bits (Q4) stays in 4 bits in LDS (13 KiB a tile, eight tiles, brought seven ahead); both kinds of waves widen what they
 // multiply, in registers: a score wave its 16 keys between its products, a value wave the next tile's values while it multiplies this
-// one's.  Bound by the step: a wave has some 110 instructions for that in it beside its products, and the SIMD's two (three) waves' vector
-// instructions (46 %) and products (40 %) rarely run side by side.  The same three shapes: drafts 231 to 243 us, 64 sequences of 64 heads
-// behind 32768 tokens 359 to 367 (315 to 321 over 16 bits), and 64 ragged sequences of 32 heads 56 against 102 over 16 bits, 3.3 TB/s.
+// one's.  Bound by the step: a wave has some 80 instructions for that in it beside its products, and the SIMD's two (three) waves' vector
+// instructions (46 %) and products (43 %) rarely run side by side.  The same three shapes: drafts 215 to 228 us, 64 sequences of 64 heads
+// behind 32768 tokens 328 to 332 (311 to 318 over 16 bits), and 64 ragged sequences of 32 heads 53 against 102 over 16 bits, 3.6 TB/s.
+// What a segment keeps from before the loops is spilled, and its reload waits for every load under way: addresses are found where they are
+// needed (drafts 246 us with the join before, 226 so).
 // Forms before it: 16-bit tiles made in LDS by waves of their own 78 / 284 / 447 us, made by the value waves 69 / 261 / 396.  Two tiles a
-// step with one row tile: 62 against 64, and 12.0 against 10.3 for one sequence of 4097 tokens; the next tile's codes read a step earlier:
-// 256 against 244 for the drafts (registers spilled).
+// step with one row tile: 62 against 64, and 12.0 against 10.3 for one sequence of 4097 tokens.
 // Other forms, each against this one as it stood then (64 ragged, drafts, shared prefix): eight waves of one kind with the value
 // dimensions split 141 / 296 / 234 us against 142 / 260 / 227; four of one kind, one a SIMD, pipelined 142 / 276 / 264.
 #include <type_traits>
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
         };
         // The same from 4 bits.  A transposed read of bytes gives a lane 8 tokens' codes of values 2 m and 2 m + 1 (m = l % 32 of 64 values):
         // eight conversions and eight exchanges of halves make one operand of even values and one of odd ones.  The scales the wave writes out
-        // first, as the conversion takes them (64 ragged sequences of 32 heads 62.5 us; 65.3 with 7 shifts for 8 bytes of a transposed read).  A
+        // first, as the conversion takes them (64 ragged sequences of 32 heads 62.5 us with the join; 65.3 with 7 shifts for 8 bytes of a transposed read).  A
         // step multiplies what the step before made and makes the next tile's, so that no read of LDS is waited for but the weights'.
         const int tk = 8 * half + (c16 >> 1), pc = quad & 1;  // of 16 tokens the one whose bytes this lane reads; of two pieces the one
         const uint32_t at_codes = tk * SCALES4 + (((DV * vw + pc) ^ turn4(tk)) << 4) + (c16 & 1) * 8;
