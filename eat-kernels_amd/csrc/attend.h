@@ -119,9 +119,6 @@ __device__ __forceinline__ void wait_loads() {  // all but the N youngest loads 
 __device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
     return *(__attribute__((address_space(3))) const u32x4*)(lds_byte*)(uintptr_t)at;
 }
-__device__ __forceinline__ void lds_write16(uint32_t at, u32x4 x) {
-    *(__attribute__((address_space(3))) u32x4*)(lds_byte*)(uintptr_t)at = x;
-}
 // transposed read of bytes: of 16 lanes, lane i gives the address of 8; lane i receives column i of the 8 x 16 matrix whose row r are the
 // bytes at lanes 2 r and 2 r + 1
 typedef int i32x2 __attribute__((ext_vector_type(2)));
