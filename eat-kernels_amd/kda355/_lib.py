@@ -7,6 +7,8 @@ from __future__ import annotations
 import ctypes
 from pathlib import Path
 
+import torch
+
 LIB_PATH = Path(__file__).resolve().parent / "libkda355.so"
 NOALLOC_LIB_PATH = Path(__file__).resolve().parent / "libkda355_noalloc.so"
 
@@ -222,6 +224,19 @@ class _Launches(dict):
 
 
 LAUNCH = _Launches()
+
+_device = torch._C._cuda_getDevice  # without current_device()'s look whether there is a GPU
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object (2 us)
+
+
+def launch(entry, args, device):
+    """entry(args, stream) with the tensors' device the current one, on its current stream.  The handle of a default stream is 0 on
+    every device and means the current device's: a kernel would run there, over another device's memory."""
+    index = device.index
+    if index == _device():
+        return entry(args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return entry(args, _raw_stream(index))
 
 
 def noalloc_lib():

@@ -151,6 +151,5 @@ def decode_batch(mixed_qkv, conv_state, conv_weight, gate, beta, out_gate, A_log
     a.norm_eps, a.lower_bound = float(norm_eps), float(lower_bound)
     a.flags = 0
     a.workspace = workspace.data_ptr() if workspace is not None else None
-    stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(_lib.lib().kda355_decode_launch(ctypes.byref(a), stream), "decode")
+    _lib.check(_lib.launch(_lib.lib().kda355_decode_launch, ctypes.byref(a), dev), "decode")
     return out

@@ -53,13 +53,6 @@ def _keep(seen, key, plan):
     return plan
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object (2 us)
-
-
-def _stream(device):
-    return _raw_stream(device.index)
-
-
 def _num_cus(device):
     n = _cus.get(device)
     if n is None:
@@ -205,7 +198,7 @@ def latent_prefill(q, k, v, k_pe, cu_seqlens_q, cu_seqlens_k, scale=None, causal
     args = (_PTR8.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pe.data_ptr(), out.data_ptr(),
                        0 if lse is None else lse.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()) + mid +
             _PTR2.pack(0 if ws is None else ws.data_ptr(), need) + tail)
-    rc = _lib.LAUNCH["latent_prefill"](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH["latent_prefill"], args, dev)
     if rc:
         _lib.check(rc, "latent_prefill")
     return out
@@ -281,7 +274,7 @@ def latent_decode(q_latent, q_pe, cache, block_table, seq_lens, scale=None, *, o
                         0 if prefix_table is None else prefix_table.data_ptr(),
                         0 if prefix_len is None else prefix_len.data_ptr(),
                         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if ws is None else ws.data_ptr()) + tail)
-    rc = _lib.LAUNCH[entry](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH[entry], args, dev)
     if rc:
         _lib.check(rc, "latent_decode")
     return out
@@ -316,7 +309,7 @@ def latent_append(latent, k_pe, cache, slots):
         plan = _keep(_append_seen, key, (dev, bytes(a)[_PTR7.size:], "latent_append" if bits == 16 else "latent4_append"))
     dev, tail, entry = plan
     args = _PTR7.pack(latent.data_ptr(), k_pe.data_ptr(), cache.data_ptr(), slots.data_ptr(), 0, 0, 0) + tail
-    rc = _lib.LAUNCH[entry](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH[entry], args, dev)
     if rc:
         _lib.check(rc, "latent_append")
     return cache
@@ -345,7 +338,7 @@ def latent_gather(cache, block_table, cu_seqlens, out):
         plan = _keep(_gather_seen, key, (dev, bytes(a)[_PTR7.size:], "latent_gather" if bits == 16 else "latent4_gather"))
     dev, tail, entry = plan
     args = _PTR7.pack(0, 0, cache.data_ptr(), 0, block_table.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr()) + tail
-    rc = _lib.LAUNCH[entry](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH[entry], args, dev)
     if rc:
         _lib.check(rc, "latent_gather")
     return out
@@ -400,7 +393,7 @@ def latent_weights(q_latent, q_pe, cache, block_table, seq_lens, lse, weights, s
     dev, tail = plan
     args = _PTR7.pack(q_latent.data_ptr(), q_pe.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
                       lse.data_ptr(), weights.data_ptr()) + tail
-    rc = _lib.LAUNCH["latent_weights"](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH["latent_weights"], args, dev)
     if rc:
         _lib.check(rc, "latent_weights")
     return weights

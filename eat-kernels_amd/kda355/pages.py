@@ -22,7 +22,7 @@ import struct
 import torch
 
 from . import _lib
-from .latent import _index, _keep, _stream, _table
+from .latent import _index, _keep, _table
 from .recurrent import _need
 
 
@@ -89,7 +89,7 @@ def _launch(name, dev, pools, n, src, dst, ws, book=(0, 0, 0, 0, 0), stride=0, r
                 _PACK.pack(count, n, src, dst, *book, ws, stride, rows, width, pages, size))
     except struct.error as e:
         raise ValueError(f"kda355: {name}: a size is out of range ({e})") from None
-    rc = _lib.LAUNCH[name](args, _stream(dev))
+    rc = _lib.launch(_lib.LAUNCH[name], args, dev)
     if rc:
         _lib.check(rc, name)
 
@@ -292,6 +292,6 @@ def evict_tokens(pools, weights, block_table, seq_lens, ref_counts, free_pages, 
         more = _lib.EVICT_MORE if first + len(some) < len(layers) else 0
         args += bytes(_LAYER.size * (_lib.MAX_POOLS - len(some))) + _EVICT.pack(
             len(some), n, *books, need[c], stride, count, width, total, page_size, keep, recent, more, 0)
-        rc = _lib.LAUNCH["evict_tokens"](args, _stream(dev))
+        rc = _lib.launch(_lib.LAUNCH["evict_tokens"], args, dev)
         if rc:
             _lib.check(rc, "evict_tokens")

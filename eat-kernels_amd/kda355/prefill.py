@@ -218,11 +218,10 @@ def _launch(meta, q, k, v, gt, bt, out, flags, scale, lower_bound, A_log=None, d
     a.scale, a.lower_bound = float(scale), float(lower_bound)
     a.flags = flags | (PF_CHUNK64 if getattr(meta, "chunk64", False) else 0)
     a.plan = ctypes.pointer(meta.plan)
-    stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
     if static:
-        _lib.check(_lib.noalloc_lib().kda355_prefill_launch_noalloc(ctypes.byref(a), stream), "prefill_noalloc")
+        _lib.check(_lib.launch(_lib.noalloc_lib().kda355_prefill_launch_noalloc, ctypes.byref(a), dev), "prefill_noalloc")
     else:
-        _lib.check(_lib.lib().kda355_prefill_launch(ctypes.byref(a), stream), "prefill")
+        _lib.check(_lib.launch(_lib.lib().kda355_prefill_launch, ctypes.byref(a), dev), "prefill")
 
 
 def _check_qkv(q, k, v):

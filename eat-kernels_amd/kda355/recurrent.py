@@ -31,10 +31,6 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
 def _need(name, t, dtype, device):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"kda355: {name} must be a tensor")
@@ -167,7 +163,7 @@ def fused_recurrent_kda(q, k, v, g=None, beta=None, scale=None, initial_state=No
     a.scale = float(D ** -0.5 if scale is None else scale)
     a.lower_bound = float(lower_bound)
     a.flags = flags
-    _lib.check(_lib.lib().kda355_recurrent_launch(ctypes.byref(a), _stream(dev)), "fused_recurrent_kda")
+    _lib.check(_lib.launch(_lib.lib().kda355_recurrent_launch, ctypes.byref(a), dev), "fused_recurrent_kda")
     return out, pool
 
 
@@ -189,5 +185,5 @@ def spec_commit(scratch, scratch_indices, pool, pool_indices, num_accepted_token
     a.scratch_slot_stride, a.scratch_slots, a.pool_slot_stride, a.pool_slots = sss, scratch.shape[0], pss, pool.shape[0]
     a.B, a.S, a.H = B, S, H
     a.flags = _lib.REC_SLOT0_RESERVED if slot0_reserved else 0
-    _lib.check(_lib.lib().kda355_spec_commit_launch(ctypes.byref(a), _stream(dev)), "spec_commit")
+    _lib.check(_lib.launch(_lib.lib().kda355_spec_commit_launch, ctypes.byref(a), dev), "spec_commit")
     return pool

@@ -8,6 +8,7 @@
  * hipStream_t, launches asynchronously on that stream and returns a status code.  Nothing here allocates device
  * memory, synchronizes, or keeps per-call global state, so every launch entry point is safe inside HIP-graph
  * capture and re-entrant across threads and streams.  bf16 / fp16 tensors are passed as `const void*`.
+ * The stream has to be one of the current device (hipSetDevice; stream 0 always is), and all pointers that device's.
  *
  * Status codes: 0 = launched; KDA355_EINVAL (-1) = invalid arguments (nothing launched, kda355_last_error()
  * names the argument); KDA355_ELAUNCH (-2) = the HIP launch failed.
