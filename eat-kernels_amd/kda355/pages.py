@@ -220,6 +220,9 @@ assert _LAYER.size * _lib.MAX_POOLS + _EVICT.size == ctypes.sizeof(_lib.KdaEvict
 
 def _check_evict(pools, weights, block_table, seq_lens, ref_counts, free_pages, num_free, rows, keep, recent, page_size):
     """(device, table stride, rows, width, pages, [(token bytes, page stride, weights stride)], bytes of workspace of each call)"""
+    for name, x in (("keep", keep), ("recent", recent), ("page_size", page_size)):
+        if not -1 << 31 <= x < 1 << 31:  # (the struct would take the low 32 bits)
+            raise ValueError(f"kda355: evict_tokens: {name}={x} does not fit in 32 bits")
     dev, pages, stride, count, width = _book(block_table, ref_counts, free_pages, num_free)
     _index("seq_lens", seq_lens, (count,), dev)
     n = rows.numel() if isinstance(rows, torch.Tensor) else 0

@@ -502,6 +502,17 @@ def test_evict_refusals():
     assert d["seq_lens"].tolist() == [20, 20]
 
 
+@pytest.mark.parametrize("keep,recent", [((1 << 32) + 20, 4), ((1 << 63) - 1, 4), (20, (1 << 32) + 4), (1 << 31, 1 << 31)])
+def test_evict_budgets_beyond_32_bits(keep, recent):
+    x = Budget([64, 30], 16, 2, token=(4,))
+    pools, mass, d = x.device()
+    for _ in range(2):  # (nothing is kept of a call that was refused)
+        with pytest.raises(ValueError, match="32 bits"):
+            kda355.evict_tokens(pools, mass, *d.values(), _i32([0, 1]), keep, recent, 16)
+    assert d["seq_lens"].tolist() == [64, 30]
+    assert x.check([0, 1], (1 << 29), 4) == [64, 30]
+
+
 # ================================================================================================ together
 @pytest.mark.parametrize("bits,dtype", [(16, BF), (4, BF), (4, HF)])
 def test_a_sequence_under_a_budget(bits, dtype):

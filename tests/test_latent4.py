@@ -2,6 +2,7 @@
 device call) and of the Python functions, the op schemas, the plain forms that the GPU tests go by."""
 import ctypes
 import subprocess
+import sys
 import tempfile
 
 import pytest
@@ -142,6 +143,17 @@ def test_cpu_tensors_raise():
                               torch.zeros(2, 32))
     with pytest.raises(TypeError):
         kda355.evict_tokens([cache], [torch.zeros(2, 32)], table, i32[:2], i32[:2], i32[:2], i32[:1], i32[:1], 20, 4, 16)
+
+
+@pytest.mark.parametrize("kw", [dict(keep=(1 << 32) + 20), dict(keep=sys.maxsize), dict(keep=-(1 << 40)), dict(keep=1 << 31, recent=1 << 31),
+                                dict(recent=(1 << 32) + 4), dict(size=(1 << 32) + 16)], ids=str)
+def test_evict_sizes_beyond_32_bits(kw):
+    """Refused before the tensors are looked at: the argument struct would take their low 32 bits."""
+    import kda355
+    i32 = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="32 bits"):
+        kda355.evict_tokens([torch.zeros(2, 16, 400, dtype=torch.uint8)], [torch.zeros(2, 32)], torch.zeros(2, 2, dtype=torch.int32), i32[:2],
+                            i32[:2], i32[:2], i32[:1], i32[:1], kw.get("keep", 20), kw.get("recent", 4), kw.get("size", 16))
 
 
 def test_ops_are_registered():
