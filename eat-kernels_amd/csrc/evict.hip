@@ -544,6 +544,7 @@ int check_evict(const KdaEvictArgs* a) {
                   "evict_tokens: rows=%d table_width=%d pages=%d page_size=%d", a->rows, a->table_width, a->pages, a->page_size);
     KDA_CHECK_ARG((int64_t)a->table_width * a->page_size < (1ll << 30), "evict_tokens: a table row spans 2^30 tokens or more");
     KDA_CHECK_ARG(a->keep >= 1 && a->recent >= 0 && a->recent <= a->keep, "evict_tokens: keep=%d recent=%d", a->keep, a->recent);
+    KDA_CHECK_ARG(a->n <= 65535 || (int64_t)a->table_width * a->page_size <= a->keep, "evict_tokens: %d rows in one call (at most 65535)", a->n);
     return 0;
 }
 
@@ -597,7 +598,6 @@ extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t
     const int64_t need = kda355_evict_tokens_workspace_bytes(a);
     KDA_CHECK_ARG(a->workspace && aligned(a->workspace, 16) && a->workspace_bytes >= need, "evict_tokens: needs %lld bytes of 16-byte aligned workspace",
                   (long long)need);
-    KDA_CHECK_ARG((int64_t)a->n <= 65535, "evict_tokens: %d rows in one call (at most 65535)", a->n);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     Plan p = plan_of(a);
     const int lists = a->n * a->num_layers;

@@ -494,6 +494,7 @@ int kda355_compact_pages_launch(const KdaPagesArgs* args, kda355_stream_t stream
  *
  * A sequence stays as it is where len <= keep, an entry of its tokens' pages is a hole, or fixed > keep - recent.  Rows outside
  * [0, rows) are skipped, a row that is given twice is taken once.  Results do not depend on timing.
+ * At most 65535 rows in one call (2^20 - 1 where the table holds no more than keep tokens: nothing can be cut), 2^30 tokens a table row.
  */
 typedef struct KdaEvictLayer {
     void* cache;                 /* [pages, page_size] tokens of token_bytes, dense within a page */
@@ -522,6 +523,7 @@ typedef struct KdaEvictArgs {
 } KdaEvictArgs;
 #define KDA355_EVICT_MORE 1u
 
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL for sizes that the launch refuses. */
 int64_t kda355_evict_tokens_workspace_bytes(const KdaEvictArgs* args);
 int kda355_evict_tokens_launch(const KdaEvictArgs* args, kda355_stream_t stream);
 

@@ -128,6 +128,19 @@ def test_evict_workspace():
     assert m.lib().kda355_evict_tokens_workspace_bytes(None) == m.EINVAL
 
 
+def test_evict_workspace_and_launch_take_the_same_rows():
+    """A size that the launch refuses has no workspace; where no row can be longer than the budget both take more rows."""
+    m = _lib()
+    L = m.lib()
+    assert L.kda355_evict_tokens_workspace_bytes(ctypes.byref(_evict_args(n=65535))) > 0
+    for n in (65536, (1 << 20) - 1):
+        assert L.kda355_evict_tokens_workspace_bytes(ctypes.byref(_evict_args(n=n))) == m.EINVAL
+        assert b"65535" in L.kda355_last_error()
+        assert L.kda355_evict_tokens_launch(ctypes.byref(_evict_args(n=n)), None) == m.EINVAL
+        a = _evict_args(n=n, keep=64)  # (the table's tokens)
+        assert L.kda355_evict_tokens_workspace_bytes(ctypes.byref(a)) > 0 and L.kda355_evict_tokens_launch(ctypes.byref(a), None) == 0
+
+
 def test_cpu_tensors_raise():
     import kda355
     pe, i32 = torch.zeros(4, 64).bfloat16(), torch.zeros(4, dtype=torch.int32)
