@@ -496,7 +496,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
             return *(__attribute__((address_space(3))) const int*)(lds_byte*)(uintptr_t)(pages_at + tile % L::PAGE_RING * 256 + (EVEN ? 0 : my * 4));
         };
         // EVEN: the wave's 8 tokens stand in one page in a row, so one address and fixed offsets lead to all of them.  (Tokens past the
-        // last are read as they are: no row sees them.)
+        // last are read as they are: no row sees them.  spread_scales takes their values out.)
         auto find_rows = [&](uint32_t tile, int page) {
             const uint32_t tok = tile * BN + 8 * tw, pg = __builtin_amdgcn_readfirstlane(page);
             const bool there = tok < (uint32_t)last && pg < pages;
@@ -648,7 +648,11 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
             for (int g = 0; g < G; ++g) code[g] = lds_read_tr8(((from + at_codes) ^ (g % NB) << 5) + g / NB * (16 * SCALES4));
         };
         u32x4 scales[2][2];  // of 8 tokens, for two groups
-        auto spread_scales = [&] {
+        // Of a page's places behind the tokens nobody knows what they hold, and in EVEN they come as they stand: scaled by 2^-127 they are
+        // finite, so that no walk for values that are not follows from them (one sequence of 4127 tokens, 12 heads: 14.3 us; 62 with the walk).
+        // Only a segment's last tile can have some: ENDS where it may be that one.  (In every step: drafts 234 us for 227.)
+        auto spread_scales = [&](uint32_t tile, auto ends) {
+            if (EVEN && decltype(ends)::value && (int)(tile * BN) + (my >> 1) >= last) scale = 0;
             auto* to = (__attribute__((address_space(3))) uint32_t*)(lds_byte*)(uintptr_t)(spread + (my & 1) * (NB * BN * 4) + (my >> 1) * 4);
             to[0] = scale << 23;
             if (NB == 2) to[BN] = (scale & 0xff00u) << 15;
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
             else wait_loads<4 * L::LOADS>();
         };
         auto step4 = [&](uint32_t tile, auto kind) {  // 0: with loads, 1: none are left, 2: the last one
-            constexpr bool LAST = decltype(kind)::value == 2, BRINGS = decltype(kind)::value == 0;
+            constexpr bool LAST = decltype(kind)::value == 2, BRINGS = decltype(kind)::value == 0;  // (then AHEAD4 tiles or more follow this one)
             const uint32_t pb = lds + L::P + (tile & 1) * 4096 + c * 32 + (half ^ (c >> 3 & 1)) * 16;
             auto weight = [&](int k, int r) { return lds_read16(pb + (2 * r + k) * 1024); };
             const u32x4 fl = flags(tile);
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
 #pragma unroll
                     for (int r = 0; r < RT; ++r) acc[r][2 * (g % NB) + i] = T::mfma(vf[g][i], pf[g / NB][r], acc[r][2 * (g % NB) + i]);
                 if constexpr (!LAST) {
-                    if (g == 0) spread_scales();
+                    if (g == 0) spread_scales(tile + 1, std::bool_constant<!BRINGS>{});
                     read_scales(g);
                     if constexpr (BRINGS && EVEN) {
                         if (g == 0) at = find_rows(tile + AHEAD4, page);
@@ -797,7 +801,7 @@ __global__ void __launch_bounds__((THREADS<RT, Q4>), (THREADS<RT, Q4> / 256)) de
                 lds_barrier();  // the queries are in registers; the second tile
                 // while the first tile's scores are computed: its values, and tiles t0 + 3 and on
                 read_codes(t0);
-                spread_scales();
+                spread_scales(t0, std::true_type{});
 #pragma unroll 1
                 for (uint32_t i = 3; i < AHEAD4; ++i) some_tile(t0 + i);
 #pragma unroll

@@ -294,6 +294,55 @@ def test_decode_prefix_in_wide_tables(lens, S, H, size, prefix):
     _check4(_narrow(Absorbed(lens, S, H, size, BF, prefix=prefix)).widen())
 
 
+def _tails(x, byte):
+    """The cache's rows, the places of pages behind the tokens of a sequence and of the prefix full of a byte."""
+    cache = x.bytes.clone()
+    ends = [(x.table[n], length) for n, length in enumerate(x.lens)]
+    if x.prefix is not None:
+        ends.append((x.prefix_table, x.prefix))
+    for pages, length in ends:
+        if length % x.size:
+            cache[int(pages[length // x.size]), length % x.size:] = byte
+    return cache
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens,S,H,size,prefix", [
+    ([1, 33, 64, 100, 7, 250, 18, 90], 1, 12, 16, 2001), ([5, 300, 1031], 3, 40, 64, 129), ([513, 1], 1, 128, 100, None), ([61], 8, 4, 8, None),
+    ([40, 7, 500], 8, 96, 7, 300), ([1025], 1, 64, 272, None)])
+def test_decode_what_stands_behind_the_tokens(lens, S, H, size, prefix, dtype):
+    """Places of a page that hold no token yet: NaN groups, products past the type's end, the largest finite ones.  The same bits."""
+    x = _narrow(Absorbed(lens, S, H, size, dtype, prefix=prefix))
+    for _ in range(2):
+        o, lse = _run4(x, cache=_tails(x, 0))
+        for byte in (255, 254, 200, 139, 1):
+            o2, lse2 = _run4(x, cache=_tails(x, byte))
+            assert torch.equal(o, o2) and torch.equal(lse, lse2), byte
+        x.widen()
+
+
+@pytest.mark.parametrize("n,S,H", [(4127, 1, 12), (4127, 1, 64), (31, 1, 4), (2079, 8, 96)])
+def test_decode_time_does_not_follow_what_stands_behind_the_tokens(n, S, H):
+    """Recycled pages hold anything.  Best times of calls in a row, a quarter for noise; the last tile has 31 tokens and a place behind
+    them, so that a walk through its tokens for what is not finite would be 31 dependent reads."""
+    x = _narrow(Absorbed([n], S, H, 64, BF))
+    args = [t.to(DEV) for t in (x.ql, x.qp)], x.table.to(DEV), _i32(x.lens)
+    caches = [_tails(x, 0), _tails(x, 255)]
+    best = [float("inf")] * 2
+    for _ in range(12):
+        for i, cache in enumerate(caches):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            kda355.latent_decode(*args[0], cache, *args[1:])
+            a.record()
+            for _ in range(20):
+                kda355.latent_decode(*args[0], cache, *args[1:])
+            b.record()
+            b.synchronize()
+            best[i] = min(best[i], a.elapsed_time(b) / 20 * 1e3)
+    print(f"[time] {best[0]:.1f} us over zeros, {best[1]:.1f} over NaN groups", flush=True)
+    assert best[1] < 1.25 * best[0]
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_decode_any(seed):
     rng = random.Random(seed)
