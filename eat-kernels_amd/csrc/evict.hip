@@ -25,7 +25,11 @@ constexpr int MOVE_THREADS = 256;
 constexpr int STRIP = 8, SHIFT_ROWS = 4;         // 16-byte pieces of a strip, rows of a thread at a time
 constexpr int FEW = 128;                         // pairs that the first kernel moves itself
 constexpr int WAVES = SCAN_THREADS / 64, BINS = 2048, ROW_PAGES = 2048;
-constexpr int PART_KEYS = 8, PART = PART_KEYS * SCAN_THREADS, AT_ONCE = 1024;  // of a thread, of a workgroup; (sequence, layer)s in one run of the parts
+constexpr int PART_KEYS = 8, PART = PART_KEYS * SCAN_THREADS;  // of a thread, of a workgroup
+// Pairs of so many (sequence, layer)s at once, and so many bytes of them (if not of a single sequence): a table's tokens, not the sequences',
+// set a list's length, and all lists of 256 rows that hold 131072 tokens in 24 layers would be 1.5 GiB.
+constexpr int AT_ONCE = 1024;
+constexpr int64_t LIST_BYTES = 128 << 20;
 constexpr int BOOK_ROWS = 64, BOOK_ENTRIES = 4096, BOOK_PAGES = 16 * 1024;  // up to so many rows, table entries and pages the books take one workgroup
 
 enum { ROWS = 1, ALL };
@@ -36,22 +40,22 @@ struct Plan {
     int strips;       // workgroups of a sequence and layer in the third kernel
     int books;        // the books beside it: none, by a workgroup for each sequence, all by one
     int parts;        // workgroups that select for a sequence and layer, 0: one
-    int first, rows;  // with parts: sequences of this run of them
+    int first, rows;  // sequences of this run
 };
 // workspace: the lengths of the sequences that are cut, -1 for others [n]; pairs of (sequence, layer) [n][layers]; the pages from the
-// first recent token's on [n][tail] (the books change the table); places and tokens of the pairs [n][layers][2][most];
-// with parts: the tokens that stay for being held elsewhere [n], and of a run of sequences histograms [rows][layers][3][BINS] and counts
-// of the parts [rows][layers][parts][4]
+// first recent token's on [n][tail] (the books change the table); of a run of sequences the places and tokens of the pairs
+// [rows][layers][2][most]; with parts: the tokens that stay for being held elsewhere [n], and of a run histograms [rows][layers][3][BINS]
+// and counts of the parts [rows][layers][parts][4]
 __device__ __forceinline__ int32_t* lens_of(const KdaEvictArgs& a) { return static_cast<int32_t*>(a.workspace); }
 __device__ __forceinline__ int32_t* pairs_of(const KdaEvictArgs& a, int i, int l) { return lens_of(a) + a.n + i * a.num_layers + l; }
 __device__ __forceinline__ int32_t* tail_of(const KdaEvictArgs& a, const Plan& p, int i) {
     return lens_of(a) + a.n + (int64_t)a.n * a.num_layers + (int64_t)i * p.tail;
 }
-__device__ __forceinline__ int32_t* lists_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {
+__device__ __forceinline__ int32_t* lists_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {  // i: of the run, from here on
     return tail_of(a, p, a.n) + ((int64_t)i * a.num_layers + l) * 2 * p.most;
 }
-__device__ __forceinline__ int32_t* fixed_of(const KdaEvictArgs& a, const Plan& p) { return lists_of(a, p, a.n, 0); }
-__device__ __forceinline__ int32_t* hist_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {  // i: of the run
+__device__ __forceinline__ int32_t* fixed_of(const KdaEvictArgs& a, const Plan& p) { return lists_of(a, p, p.rows, 0); }
+__device__ __forceinline__ int32_t* hist_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {
     return fixed_of(a, p) + a.n + ((int64_t)i * a.num_layers + l) * 3 * BINS;
 }
 __device__ __forceinline__ int32_t* counts_of(const KdaEvictArgs& a, const Plan& p, int i, int l) {
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) select_kernel(KdaEvictArgs a, Pl
     __shared__ char* at[2][PAIRS];
     __shared__ int few[2][FEW];  // the first pairs
     __shared__ int pages[ROW_PAGES];  // the first of the row's
-    const int i = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
+    const int i = p.first + blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
     const int row = a.src[i];
     const KdaEvictLayer y = a.layer[l];
     if (tid < 5) flags[tid] = 0;
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) select_kernel(KdaEvictArgs a, Pl
             last.pick(hist, d, flags + 2, sw);
         }
     // ---- holes and movers, in index order
-    int32_t* const places = lists_of(a, p, i, l);
+    int32_t* const places = lists_of(a, p, blockIdx.x, l);
     int32_t* const tokens = places + p.most;
     int ties = 0;
     if (!last.all) {
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) part_kernel(KdaEvictArgs a, Plan
     last.marks(keys, fixed, p.left, ties, [&](int, bool, bool, uint64_t h, uint64_t m) { holes += __popcll(h), movers += __popcll(m); });
     holes = before_wave(holes, sw, pairs) + earlier[1];
     movers = before_wave(movers, sw, total) + earlier[2];
-    int32_t* const places = lists_of(a, p, i, l);
+    int32_t* const places = lists_of(a, p, blockIdx.y, l);
     int32_t* const tokens = places + p.most;
     if (tid == 0 && from + PART >= end) *pairs_of(a, i, l) = earlier[1] + pairs;
     last.marks(keys, fixed, p.left, ties, [&](int j, bool hole, bool mover, uint64_t h, uint64_t m) {
@@ -428,10 +432,10 @@ __global__ void __launch_bounds__(SCAN_THREADS) part_kernel(KdaEvictArgs a, Plan
 
 __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(KdaEvictArgs a, Plan p) {
     __shared__ char* at[2][PAIRS];
-    const int i = blockIdx.y, l = blockIdx.z;
+    const int i = p.first + blockIdx.y, l = blockIdx.z;
     const int pairs = *pairs_of(a, i, l);
     if (!p.parts && pairs <= FEW) return;
-    const int32_t* lists = lists_of(a, p, i, l);
+    const int32_t* lists = lists_of(a, p, blockIdx.y, l);
     const KdaEvictLayer y = a.layer[l];
     const int row = a.src[i], pieces = (int)(y.token_bytes / 16);
     float* const weights = y.weights + row * y.weights_row;
@@ -559,8 +563,10 @@ Plan plan_of(const KdaEvictArgs* a) {
     // 131072 and 100001 tokens in 7 layers; the six launches of the parts 39.  For 256 times 4000 one launch takes 18 us and six would not.)
     const int64_t candidates = span - a->recent;
     p.parts = candidates <= 16 * SCAN_THREADS ? 0 : (int)((candidates + PART - 1) / PART);
-    const int at_once = AT_ONCE / (a->num_layers > 0 ? a->num_layers : 1);
-    p.first = 0, p.rows = at_once < 1 ? 1 : at_once < a->n ? at_once : a->n;
+    const int layers = a->num_layers > 0 ? a->num_layers : 1;
+    const int64_t fit = LIST_BYTES / (8 * (int64_t)layers * (p.most > 0 ? p.most : 1)), at_once = AT_ONCE / layers;
+    const int64_t rows = p.parts && at_once < fit ? at_once : fit;
+    p.first = 0, p.rows = (int)(rows < 1 ? 1 : rows < a->n ? rows : a->n);
     return p;
 }
 
@@ -571,10 +577,10 @@ using namespace kda355;
 
 extern "C" int64_t kda355_evict_tokens_workspace_bytes(const KdaEvictArgs* a) {
     if (const int rc = check_evict(a)) return rc;
-    const int64_t lists = (int64_t)a->n * a->num_layers;
     const Plan p = plan_of(a);
-    const int64_t parts = p.parts ? a->n + (int64_t)p.rows * a->num_layers * (3 * BINS + 4 * (int64_t)p.parts) : 0;
-    return 4 * (a->n * (1 + (int64_t)p.tail) + lists * (1 + 2 * (int64_t)p.most) + parts);
+    const int64_t run = (int64_t)p.rows * a->num_layers;
+    const int64_t parts = p.parts ? a->n + run * (3 * BINS + 4 * (int64_t)p.parts) : 0;
+    return 4 * (a->n * (1 + (int64_t)p.tail) + (int64_t)a->n * a->num_layers + run * 2 * p.most + parts);
 }
 
 extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t stream) {
@@ -600,26 +606,25 @@ extern "C" int kda355_evict_tokens_launch(const KdaEvictArgs* a, kda355_stream_t
                   (long long)need);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     Plan p = plan_of(a);
-    const int lists = a->n * a->num_layers;
-    const int64_t fill = 4096 / lists + 1;  // workgroups of a sequence and layer
+    const int64_t fill = 4096 / (a->n * a->num_layers) + 1;  // workgroups of a sequence and layer
     const auto some = [](int64_t x, int64_t y) { return (int)(x < y ? x : y); };
     const auto cdiv = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    if (p.parts) {
-        const int at_once = p.rows;
-        for (; p.first < a->n; p.first += at_once) {
-            const dim3 grid(p.parts, some(at_once, a->n - p.first), a->num_layers), threads(SCAN_THREADS);
+    for (; p.first < a->n; p.first += p.rows) {
+        const int rows = some(p.rows, a->n - p.first);
+        const dim3 threads(SCAN_THREADS);
+        if (p.parts) {
+            const dim3 grid(p.parts, rows, a->num_layers);
             launch_kernel(look_kernel, dim3(grid.y, grid.z), threads, s, *a, p);
             launch_kernel(part_kernel<0>, grid, threads, s, *a, p);
             launch_kernel(part_kernel<1>, grid, threads, s, *a, p);
             launch_kernel(part_kernel<2>, grid, threads, s, *a, p);
             launch_kernel(part_kernel<3>, grid, threads, s, *a, p);
             launch_kernel(part_kernel<4>, grid, threads, s, *a, p);
-        }
-    } else
-        launch_kernel(span - a->recent <= 4 * SCAN_THREADS ? select_kernel<4> : select_kernel<16>, dim3(a->n, a->num_layers), dim3(SCAN_THREADS), s,
-                      *a, p);
-    if (p.most > (p.parts ? 0 : FEW))
-        launch_kernel(move_kernel, dim3(some(cdiv(p.most, PAIRS), fill), a->n, a->num_layers), dim3(MOVE_THREADS), s, *a, p);
+        } else
+            launch_kernel(span - a->recent <= 4 * SCAN_THREADS ? select_kernel<4> : select_kernel<16>, dim3(rows, a->num_layers), threads, s, *a, p);
+        if (p.most > (p.parts ? 0 : FEW))
+            launch_kernel(move_kernel, dim3(some(cdiv(p.most, PAIRS), 4096 / (rows * a->num_layers) + 1), rows, a->num_layers), dim3(MOVE_THREADS), s, *a, p);
+    }
     const bool last = !(a->flags & KDA355_EVICT_MORE);
     const int strips = (int)cdiv(pieces, STRIP), parts = some(cdiv(a->recent, PAIRS), fill / 4 + 1);
     p.strips = a->recent == 0 ? 0 : strips > parts ? strips : parts;

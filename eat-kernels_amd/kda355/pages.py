@@ -268,7 +268,8 @@ def evict_tokens(pools, weights, block_table, seq_lens, ref_counts, free_pages, 
     up as in free_pages; pages reserved ahead of the tokens move down in the table behind the kept ones.
 
     A sequence stays as it is where one of its pages is a hole, or where shared pages and recent tokens are more than `keep`.
-    Rows outside the table are skipped; a row that is given twice is taken once.  No two layers may have the same memory."""
+    Rows outside the table are skipped; a row that is given twice is taken once.  No two layers may have the same memory.  At most 65535
+    rows; the workspace (up to some 160 MB, more only where one sequence's layers need it) comes from torch's allocator for the call."""
     pools, weights = _sequence(pools), _sequence(weights)
     keep, recent, page_size = int(keep), int(recent), int(page_size)  # (what is kept is keyed by their values)
     try:

@@ -523,7 +523,10 @@ typedef struct KdaEvictArgs {
 } KdaEvictArgs;
 #define KDA355_EVICT_MORE 1u
 
-/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL for sizes that the launch refuses. */
+/* Bytes of workspace for these sizes (pointers and strides are not looked at), or KDA355_EINVAL for sizes that the launch refuses.  At most
+   128 MiB of lists (8 bytes for each of min(keep - recent, table_width * page_size - keep) tokens of a layer; those of one sequence's layers
+   where they are more), 25 KiB and 16 bytes a part of 8192 tokens for 1024 (sequence, layer)s where a table row spans more than
+   recent + 16384 tokens, and the lengths, counts and pages of the recent tokens of all rows. */
 int64_t kda355_evict_tokens_workspace_bytes(const KdaEvictArgs* args);
 int kda355_evict_tokens_launch(const KdaEvictArgs* args, kda355_stream_t stream);
 

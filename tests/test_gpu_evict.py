@@ -407,6 +407,31 @@ def test_evict_many_rows_in_wide_tables():
     assert x.check(list(range(47)), 40, 11) == [min(n, 40) for n in lens]
 
 
+@pytest.mark.parametrize("layers,B,size,span,keep,recent", [(24, 130, 16, 16384, 7000, 30), (24, 47, 16, 20000, 400, 0),
+                                                            (3, 48, 272, 300000, 125000, 64)])
+def test_evict_in_runs(layers, B, size, span, keep, recent):
+    """More lists of pairs than are held at a time (100, 42 and 44 rows): a call is the calls for a few of its rows, one after the other,
+    but for the order in which pages come onto the stack.  Rows given twice stand in different runs."""
+    x = Budget([keep - 20 + (7 * n) % 500 for n in range(B)], size, layers, seed=layers, token=(4,), shared=[(9, 2, 1), (B - 1, 2, 1)])
+    width = span // size
+    outs = []
+    for parts in (1, 5):
+        pools, _, d = x.device()
+        g = torch.Generator(device=DEV).manual_seed(layers)
+        mass = [torch.rand(B, width * size, generator=g, device=DEV) for _ in range(layers)]
+        d["block_table"] = torch.cat([d["block_table"], _i32([[-1] * (width - d["block_table"].shape[1])] * B)], dim=1)
+        order = list(range(B)) + [0, B // 2]
+        step = -(-len(order) // parts)
+        for i in range(0, len(order), step):
+            kda355.evict_tokens(pools, mass, *d.values(), _i32(order[i:i + step]), keep, recent, size)
+        top = int(d["num_free"])
+        d["free_pages"][:top] = d["free_pages"][:top].sort().values
+        outs.append([*pools, *mass, *d.values()])
+        assert d["seq_lens"].tolist() == [min(n, keep) for n in x.lens]
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
 def test_evict_far_offsets():
     """Pages beyond 2^32 bytes of the pool, on another stream."""
     pages, size = 90000, 128  # 4.6 GB

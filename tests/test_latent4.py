@@ -128,6 +128,20 @@ def test_evict_workspace():
     assert m.lib().kda355_evict_tokens_workspace_bytes(None) == m.EINVAL
 
 
+@pytest.mark.parametrize("n,layers,width,keep,recent", [(256, 24, 2048, 32768, 512), (65535, 24, 256, 8192, 100), (1000, 7, 200, 6000, 0),
+                                                        (4, 24, 1 << 15, 1 << 20, 4096)])
+def test_evict_workspace_is_bounded(n, layers, width, keep, recent):
+    """Of the pairs that could move 128 MiB are held at a time, and those of one sequence's layers where they are more; 25 KiB and 16 bytes
+    a part for 1024 (sequence, layer)s of long tables; lengths, counts and pages of recent tokens for all."""
+    m = _lib()
+    L = m.lib()
+    a = _evict_args(n=n, num_layers=layers, table_width=width, page_size=64, pages=1 << 16, keep=keep, recent=recent)
+    need = L.kda355_evict_tokens_workspace_bytes(ctypes.byref(a))
+    pairs = 8 * layers * min(keep - recent, width * 64 - keep)
+    parts = 1024 * (25 * 1024 + 16 * (width // 128 + 1)) if width * 64 - recent > 16384 else 0
+    assert 4 * n < need <= max(128 << 20, pairs) + parts + 4 * n * (4 + recent // 64 + layers)
+
+
 def test_evict_workspace_and_launch_take_the_same_rows():
     """A size that the launch refuses has no workspace; where no row can be longer than the budget both take more rows."""
     m = _lib()
