@@ -292,7 +292,9 @@ def latent_append(latent, k_pe, cache, slots):
 
     Into a uint8 cache 32 consecutive latent values are rounded to codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) of one
     power of two: with a the largest size among them, 2^(floor(log2 a) - 2), and the next power where a is over 7 of it; to the
-    nearest code, ties to the even one.  A group with an infinite value or a NaN reads as NaN throughout."""
+    nearest code, ties to the even one.  The power stays within [-23, 13] for fp16 and [-125, 125] for bf16, so that what is read back is
+    a finite number of the type.  A value is off by at most a / 5, next to the type's largest ones (a > 57344 in fp16) by a / 4.  A
+    group with an infinite value or a NaN reads as NaN throughout."""
     try:
         key = (latent.shape, latent.stride(), latent.dtype, latent.device, k_pe.shape, k_pe.stride(), k_pe.dtype, k_pe.device,
                cache.shape, cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)

@@ -429,7 +429,9 @@ int kda355_latent_gather_launch(const KdaLatentTokensArgs* args, kda355_stream_t
 /*
  * The same with a cache in 4 bits (page_stride in bytes).  append: with a the largest |x| of 32 values, the scale is 2^e,
  * e = floor(log2 a) - 2, and 1 more where a > 7 x 2^e, in [-125, 125] (bf16) or [-23, 13] (fp16); a value becomes the nearest
- * code x 2^e, ties to the even code, at most 6 x 2^e, and is off by at most a / 5.  A group with an infinite value or a NaN reads as NaN throughout.
+ * code x 2^e, ties to the even code, at most 6 x 2^e, and is off by at most a / 5; by a / 4 where the upper limit holds e down (a > 57344 in
+ * fp16, 7 x 2^125 in bf16: the largest value reads back as 6 x 2^e), and by 2^-127 if that is more where bf16's lower limit holds it up (a <
+ * 2^-123).  A group with an infinite value or a NaN reads as NaN throughout.
  */
 int kda355_latent4_append_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);
 int kda355_latent4_gather_launch(const KdaLatentTokensArgs* args, kda355_stream_t stream);

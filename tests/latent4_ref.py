@@ -38,6 +38,17 @@ def rounded(latent, pe):
     return out
 
 
+def ends(dtype):
+    """[21, 512]: groups about the largest and the smallest numbers of the type, where the scale's exponent is held."""
+    info = torch.finfo(dtype)
+    top, step, rows = MOST[dtype], info.tiny * info.eps, []
+    for a in (info.max, 6.0 * 2.0 ** top, 6.5 * 2.0 ** top, 7.0 * 2.0 ** top, 7.0 * 2.0 ** top * (1 + info.eps), 7.75 * 2.0 ** top):
+        rows.append(a * torch.linspace(-1, 1, LAT, dtype=torch.float64))
+    for k in (1, 2, 3, 5, 7, 8, 11, 60, 64, 100, 127, 128, 250, 255, 1000):  # the largest is the k-th number
+        rows.append(step * torch.round(k * torch.linspace(-1, 1, LAT, dtype=torch.float64)))
+    return torch.stack(rows).to(dtype)
+
+
 def values(rows, dtype):
     """[..., 400] uint8 -> [..., 576] of the type"""
     size = torch.tensor(SIZES + [-s for s in SIZES], dtype=torch.float64)
@@ -117,4 +128,4 @@ def evict(pools, mass, table, lens, refs, free, num, rows, keep, recent, size):
     return num
 
 
-__all__ = ["ROW4", "GROUP", "LAT", "PE", "rounded", "values", "weights", "evict"]
+__all__ = ["ROW4", "GROUP", "LAT", "PE", "ends", "rounded", "values", "weights", "evict"]

@@ -61,6 +61,21 @@ def test_append_rounds(dtype):
     assert (cache.view(-1, 400)[T:] == 170).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_and_gather_at_the_ends_of_the_type(dtype):
+    latent = Q.ends(dtype)
+    T = len(latent)
+    pe = _randn(T, PE, dtype=dtype, seed=8)
+    cache = torch.zeros(T, 1, 400, dtype=torch.uint8, device=DEV)
+    kda355.latent_append(latent.to(DEV), pe.to(DEV), cache, torch.arange(T, device=DEV))
+    rows = Q.rounded(latent, pe)
+    assert torch.equal(cache.cpu()[:, 0], rows)
+    out = torch.empty(T, ROW, dtype=dtype, device=DEV)
+    kda355.latent_gather(cache, torch.arange(T, dtype=torch.int32, device=DEV)[None], _i32([0, T]), out)
+    assert torch.isfinite(out).all()
+    _same(out, Q.values(rows, dtype))
+
+
 @pytest.mark.parametrize("T,pages,size,dtype", [(1, 1, 1, BF), (7, 5, 3, HF), (8, 2, 16, BF), (9, 4, 7, BF), (100, 9, 16, HF)])
 def test_append_anywhere(T, pages, size, dtype):
     """Views of wider rows, pages apart, slots in any order and outside."""

@@ -204,3 +204,20 @@ def test_plain_rounding(dtype):
     assert ((y.double() - x.double()).abs().view(50, 16, 32).amax(dim=-1) <= top / 5).all()
     again = Q.values(Q.rounded(y, torch.zeros(50, 64).to(dtype)), dtype)[:, :512]
     assert torch.equal(again, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_plain_rounding_at_the_ends_of_the_type(dtype):
+    """The stated bounds where the scale's limits hold: a / 4 for the largest numbers, 2^-127 or a / 5 for the smallest; a / 5 just inside."""
+    top, x = Q.MOST[dtype], Q.ends(dtype)
+    y = Q.values(Q.rounded(x, torch.zeros(len(x), 64).to(dtype)), dtype)[:, :512]
+    assert torch.isfinite(y).all()
+    a = x.double().abs().view(-1, 16, 32).amax(dim=-1)
+    off = (y.double() - x.double()).abs().view(-1, 16, 32).amax(dim=-1)
+    held = a > 7 * 2.0 ** top
+    low = 2.0 ** -127 if dtype is torch.bfloat16 else 0.0
+    bound = torch.where(held, a / 4, torch.where(a < 2.0 ** -123, (a / 5).clamp(min=low), a / 5))
+    assert (off <= bound).all()
+    assert (off > a / 5)[held].any() and held[0, 0]  # (the bound of the others does not hold there)
+    if dtype is torch.bfloat16:
+        assert (off > a / 5)[a < 2.0 ** -123].any()
