@@ -383,6 +383,69 @@ def test_evict_long(n):
         assert d["seq_lens"].tolist()[0] == keep
 
 
+def _cut(w, n, fixed, keep, recent):
+    """Where the tokens of a row of n come from after a cut, by torch's stable sort."""
+    left = keep - recent
+    order = fixed + torch.sort(w[fixed:n - recent], descending=True, stable=True).indices[:left - fixed]
+    stays = torch.zeros(n - recent, dtype=torch.bool)
+    stays[:fixed], stays[order] = True, True
+    place = torch.arange(keep)
+    place[torch.nonzero(~stays[:left]).flatten()] = left + torch.nonzero(stays[left:]).flatten()
+    place[left:] = torch.arange(n - recent, n)
+    return place
+
+
+@pytest.mark.parametrize("n,kind", [(540000, "ties"), (600000, "few"), (1100000, "ties"), (700001, "heads"), (1000000, "none")])
+def test_evict_beyond_64_parts(n, kind):
+    """More parts of a sequence than a wave has lanes (540672 tokens): how many ties, places and movers stand before a part goes from one
+    64 of them to the next.  Ties alone; a few heavier tokens between them; all movers behind the first 64 parts; neighbouring numbers.  Rows
+    of other lengths beside it, one of them with shared pages, another left as it is; all books and both layers' rows and weights."""
+    size = 272
+    lens = [n, 9000, n // 3, 700]
+    x = Budget(lens, size, 2, token=(4,), seed=n, shared=[(2, 0, 5)], reserve=1)
+    g = torch.Generator().manual_seed(n + 1)
+    for w in x.mass:
+        W = w.shape[1]
+        if kind == "ties":
+            w[:] = (torch.rand(w.shape, generator=g) < 0.5).float()
+        elif kind == "few":
+            w[:] = 0.25
+            w[0, torch.randint(0, n, (500,), generator=g)] = 1.0
+            w[0, torch.randint(0, n, (500,), generator=g)] = 0.0
+        elif kind == "heads":
+            w[0] = torch.arange(W).float()
+        else:
+            w[0] = 1.0 + torch.randperm(W, generator=g) * 2.0 ** -23
+    for keep, recent in ((n // 2, n // 50), (n - 5000, 9000), (7 * size, 0)):
+        pools, mass, d = x.run([3, 0, 2, 1, 0], keep, recent)
+        after, table, refs, gone = list(lens), [list(r) for r in x.table], list(x.refs), []
+        for l in range(2):
+            want, rows = x.mass[l].clone(), x.pools[l].view(-1, 4).clone()
+            for r, length in enumerate(lens):
+                if length <= keep:
+                    continue
+                fixed = 5 * size if r in (0, 2) else 0
+                place = _cut(x.mass[l][r], length, fixed, keep, recent)
+                t = torch.tensor(x.table[r])
+                at = lambda j: t[j // size] * size + j % size  # noqa: E731
+                rows[at(torch.arange(keep))] = x.pools[l].view(-1, 4)[at(place)]
+                want[r, :keep] = x.mass[l][r][place]
+                want[r, keep:length] = 0
+            assert torch.equal(pools[l].cpu().view(-1, 4), rows)
+            assert torch.equal(mass[l].cpu(), want)
+        for r, length in enumerate(lens):
+            if length > keep:
+                kept, used = -(-keep // size), -(-length // size)
+                gone += table[r][kept:used]
+                table[r] = table[r][:kept] + table[r][used:] + [-1] * (used - kept)
+                after[r] = keep
+        for page in gone:
+            refs[page] = 0
+        free = x.free[:x.num] + sorted(gone, reverse=True)
+        assert d["seq_lens"].tolist() == after and d["block_table"].tolist() == table and d["ref_counts"].tolist() == refs
+        assert d["num_free"].tolist() == [len(free)] and d["free_pages"].tolist() == free + [-1] * (len(refs) - len(free))
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_evict_any_in_wide_tables(seed):
     """Tables with room for more tokens than a workgroup selects from: the sequences are short, or end behind the first 8192 tokens."""
