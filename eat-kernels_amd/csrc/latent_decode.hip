@@ -18,19 +18,22 @@
 //
 // Bound: with many rows of few sequences the step itself.  The two products are 576 and 512 cycles of a SIMD's matrix core a tile, a step
 // takes about 2200 (busy cycles of a CU over the units it walks): scores, maxima across lanes, weights through LDS and a barrier
-// follow one another, so the matrix cores are busy 48 % and LDS 33 % of the time.  16 sequences of 6000 to 9900 tokens, 8 draft tokens,
-// 96 heads: 234 us, 0.91 PFLOP/s; 64 sequences of 32 heads behind 32768 shared tokens: 159 us, 0.93 PFLOP/s (both after some 200 passes
-// without a pause; the first 20 after one take 291 and 197, with the clock that the card then allows).  With a row tile or two a
-// sequence HBM: 64 ragged sequences, 64 heads, 126 to 135 us, 4.3 TB/s.  One sequence of 4097 tokens, 12 heads: 13.9 us from a graph,
+// follow one another, so the matrix cores are busy 48 % and LDS 33 % of the time.  Calls with their join, one after the other on inputs that
+// change: 16 sequences of 6000 to 9900 tokens, 8 draft tokens, 96 heads (drafts, fp16) 221 to 232 us, 0.91 to 0.96 PFLOP/s; 64 sequences of
+// 32 heads behind 32768 shared tokens 156 us, 0.95 PFLOP/s, of 64 heads 324.  With a row tile or two a sequence HBM: 64 ragged sequences of
+// 64 heads 126 to 128 us, 4.3 TB/s, of 32 heads 109 to 115.  One sequence of 4097 tokens, 12 heads: 13.9 us from a graph,
 // 9.0 of it this kernel (lengths and cut 2.2, queries and first tile 2.0, three tiles and the end 3) and 4.5 the join.
 // A cache in 4 bits (Q4) stays in 4 bits in LDS (13 KiB a tile, eight tiles, brought seven ahead); both kinds of waves widen what they
 // multiply, in registers: a score wave its 16 keys between its products, a value wave the next tile's values while it multiplies this
 // one's.  Bound by the step: a wave has some 80 instructions for that in it beside its products, and the SIMD's two (three) waves' vector
-// instructions (46 %) and products (43 %) rarely run side by side.  The same three shapes: drafts 215 to 228 us, 64 sequences of 64 heads
-// behind 32768 tokens 328 to 332 (311 to 318 over 16 bits), and 64 ragged sequences of 32 heads 53 against 102 over 16 bits, 3.6 TB/s.
+// instructions (46 %) and products (43 %) rarely run side by side.  So many rows take as long as over 16 bits or a little longer: drafts 225
+// to 231 us, 32 heads behind the prefix 158 to 161, 64 heads 336 to 342; few rows less: 64 ragged sequences of 64 heads 84 to 92, of 32 heads
+// 62 to 72 (3.0 TB/s; this kernel alone, on a cache that stays in L3, 53 us and 3.6 TB/s).  Pages that are no multiple of 8 tokens (not EVEN:
+// an address a token): drafts 241, 64 heads behind the prefix 371, 32 heads ragged 73.
 // What a segment keeps from before the loops is spilled, and its reload waits for every load under way: addresses are found where they are
-// needed (drafts 246 us with the join before, 226 so).
-// Forms before it: 16-bit tiles made in LDS by waves of their own 78 / 284 / 447 us, made by the value waves 69 / 261 / 396.  Two tiles a
+// needed (drafts 246 us with the join before, 226 so).  Nothing is spilled in a vector register but by the form for two row tiles that is not
+// EVEN: 1 in bf16, 4 in fp16.
+// Forms before it (64 ragged sequences of 32 heads / drafts / 64 heads behind the prefix, without the join): 16-bit tiles made in LDS by waves of their own 78 / 284 / 447 us, made by the value waves 69 / 261 / 396.  Two tiles a
 // step with one row tile: 62 against 64, and 12.0 against 10.3 for one sequence of 4097 tokens.
 // Other forms, each against this one as it stood then (64 ragged, drafts, shared prefix): eight waves of one kind with the value
 // dimensions split 141 / 296 / 234 us against 142 / 260 / 227; four of one kind, one a SIMD, pipelined 142 / 276 / 264.

@@ -408,7 +408,7 @@ int kda355_latent_weights_launch(const KdaLatentWeightsArgs* args, kda355_stream
 
 /*
  * Token rows into pages and back.  append: cache row slots[t] (page * page_size + offset) <- latent[t] | k_pe[t]; slots
- * outside [0, pages * page_size) are skipped (two tokens of one slot: either may stay).  gather: out[cu[n] + j] <- token
+ * outside [0, pages * page_size) are skipped, those inside have to differ (of two tokens of one slot pieces of both may stay).  gather: out[cu[n] + j] <- token
  * j of sequence n, for j < cu[n + 1] - cu[n]; tokens of holes or past the table give zero rows.
  */
 typedef struct KdaLatentTokensArgs {
